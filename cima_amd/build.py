@@ -7,6 +7,9 @@ Produces, in ``cima_amd/lib/``:
   cima_dequant.hsaco    dequant-to-f16 and packed gather,
   cima_decode.hsaco     decode-step support (norm, RoPE, attention, argmax)
   cima_bnb4.hsaco       bitsandbytes NF4/FP4 dequant and decode GEMV
+  cima_paged.hsaco      paged KV cache: RoPE with append, page operations
+  cima_paged_attn.hsaco  attention of a batch over the paged cache
+  cima_sample.hsaco     row softmax, verification of drafted tokens
   libcima_hip.so      host C ABI (include/cima_hip.h), links libamdhip64
   libcima_synth.so    seeded synthetic weights + quantisers (include/cima_synth.h)
 
@@ -33,7 +36,8 @@ ARCH = "gfx950"
 SOURCES = {"gemv_a": ("gguf_gemv.hip", ["-DCIMA_GEMV_SET=0"]), "gemv_b": ("gguf_gemv.hip", ["-DCIMA_GEMV_SET=1"]),
            "gemv_c": ("gguf_gemv.hip", ["-DCIMA_GEMV_SET=2"]), "gemm": ("gguf_gemm.hip", []),
            "dequant": ("gguf_dequant.hip", []), "decode": ("decode_ops.hip", []),
-           "bnb4": ("bnb4.hip", []), "gemm_wide": ("gguf_gemm_wide.hip", [])}
+           "bnb4": ("bnb4.hip", []), "gemm_wide": ("gguf_gemm_wide.hip", []),
+           "paged": ("paged_ops.hip", []), "paged_attn": ("paged_attn.hip", []), "sample": ("sample_ops.hip", [])}
 HSACOS = {name: os.path.join(LIB, f"cima_{name}.hsaco") for name in SOURCES}
 GEMV_OBJECTS = ("gemv_a", "gemv_b", "gemv_c")
 LIBHIP = os.path.join(LIB, "libcima_hip.so")

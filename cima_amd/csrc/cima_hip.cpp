@@ -1,6 +1,6 @@
 // Host side of the C ABI declared in include/cima_hip.h.
 //
-// The library loads seven gfx950 code objects (kModuleFiles, built from the
+// The library loads eleven gfx950 code objects (kModuleFiles, built from the
 // .hip sources with hipcc --genco) through hipModuleLoad and launches their
 // kernels with hipModuleLaunchKernel -- the HIP counterpart of the
 // reference's CudaCtx (src/cuda.rs), which JIT-compiles kernels.cu with
@@ -111,7 +111,7 @@ struct cima_hip_ctx {
     int device = 0;
     int num_cu = 0;
     int max_lds = 0;  // bytes of LDS one workgroup may use
-    hipModule_t modules[8] = {};  // kModuleFiles
+    hipModule_t modules[11] = {};  // kModuleFiles
     bool loaded = false;
     hipStream_t own_stream = nullptr;
     hipStream_t stream = nullptr;
@@ -156,12 +156,15 @@ int launch(cima_hip_ctx* ctx, hipFunction_t f, unsigned grid, unsigned block, vo
 }
 
 // code objects: the GEMVs in three (format sets compiled in parallel),
-// the prefill GEMMs, dequant / gather, the decode-step kernels, and the
-// 256 x 256 prefill tiles (compiled beside the other GEMMs)
-enum { MOD_GEMM = 3, MOD_DEQUANT = 4, MOD_DECODE = 5, MOD_BNB4 = 6, MOD_GEMM_WIDE = 7, NUM_MODULES = 8 };
+// the prefill GEMMs, dequant / gather, the decode-step kernels, the
+// 256 x 256 prefill tiles (compiled beside the other GEMMs), the paged cache's
+// operations, its attention, and sampling
+enum { MOD_GEMM = 3, MOD_DEQUANT = 4, MOD_DECODE = 5, MOD_BNB4 = 6, MOD_GEMM_WIDE = 7, MOD_PAGED = 8,
+       MOD_PAGED_ATTN = 9, MOD_SAMPLE = 10, NUM_MODULES = 11 };
 const char* const kModuleFiles[NUM_MODULES] = {"cima_gemv_a.hsaco", "cima_gemv_b.hsaco", "cima_gemv_c.hsaco",
                                                "cima_gemm.hsaco",   "cima_dequant.hsaco", "cima_decode.hsaco",
-                                               "cima_bnb4.hsaco",   "cima_gemm_wide.hsaco"};
+                                               "cima_bnb4.hsaco",   "cima_gemm_wide.hsaco",
+                                               "cima_paged.hsaco",  "cima_paged_attn.hsaco", "cima_sample.hsaco"};
 
 // weights and X types whose 32 x 16 prefill tiles are built twice: _b16_ decodes
 // in one go, _b16l_ in parts (sk16_serial in gguf_gemm.hip)
@@ -195,6 +198,20 @@ const char* const kDecodeKernels[] = {
     "cima_attn_decode_d64_c128", "cima_attn_decode_d64_c256", "cima_attn_decode_d128_c64",
     "cima_attn_decode_d128_c128", "cima_attn_decode_d128_c256", "cima_argmax_f16", "cima_argmax_to_ids",
     "cima_pos_bump", "cima_attn_reduce_wide_d64", "cima_attn_reduce_wide_d128"};
+
+// the paged cache (cima_paged.hsaco), its attention (cima_paged_attn.hsaco) and
+// sampling (cima_sample.hsaco)
+const char* const kPagedKernels[] = {
+    "cima_rope_append_paged_d64", "cima_rope_append_paged_d128", "cima_kv_pages_copy", "cima_kv_pages_reserve",
+    "cima_kv_pages_fork", "cima_kv_pages_fork_copy", "cima_kv_pages_free", "cima_kv_pages_compact",
+    "cima_kv_pages_compact_move"};
+const char* const kPagedAttnKernels[] = {
+    "cima_attn_paged_prefix_d64_r1k4", "cima_attn_paged_prefix_d64_r2k2", "cima_attn_paged_prefix_d64_r4k1",
+    "cima_attn_paged_prefix_d64_r8k1", "cima_attn_paged_own_d64_k4", "cima_attn_paged_join_d64",
+    "cima_attn_paged_prefix_d128_r1k4", "cima_attn_paged_prefix_d128_r2k2", "cima_attn_paged_prefix_d128_r4k1",
+    "cima_attn_paged_prefix_d128_r8k1", "cima_attn_paged_own_d128_k4", "cima_attn_paged_join_d128"};
+const char* const kSampleKernels[] = {"cima_softmax_stats_f16", "cima_softmax_stats_f32", "cima_softmax_probs_f16",
+                                      "cima_softmax_probs_f32", "cima_verify_sums", "cima_verify_draw"};
 
 std::string default_code_dir() {
     Dl_info info;
@@ -638,6 +655,12 @@ int cima_hip_init(int device, const char* code_dir, cima_hip_ctx** out) {
             }
     for (const char* kn : kDecodeKernels)
         if (!rc) rc = add(MOD_DECODE, kn);
+    for (const char* kn : kPagedKernels)
+        if (!rc) rc = add(MOD_PAGED, kn);
+    for (const char* kn : kPagedAttnKernels)
+        if (!rc) rc = add(MOD_PAGED_ATTN, kn);
+    for (const char* kn : kSampleKernels)
+        if (!rc) rc = add(MOD_SAMPLE, kn);
     if (rc) {
         unload(ctx);
         delete ctx;
@@ -1573,6 +1596,344 @@ int cima_hip_decode_step(cima_hip_ctx* ctx, const cima_decoder* d) {
 }
 
 // ---------------------------------------------------------------- graphs
+
+// -------------------------------------------------------------- paged cache
+
+namespace {
+
+// most pages and slots the one-workgroup kernels look over (MAX_CHUNKS *
+// CH and MAX_SLOTS in paged_ops.hip)
+const int kMaxPages = 1 << 20, kMaxSlots = 4096;
+
+int kv_check(cima_hip_ctx* ctx, const cima_kv_pages* kv, const char* api) {
+    if (int rc = ready(ctx, api)) return rc;
+    if (!kv) return fail(CIMA_E_INVALID, "%s: null cache", api);
+    const bool pow2 = kv->page > 0 && (kv->page & (kv->page - 1)) == 0;
+    if (kv->n_planes <= 0 || kv->n_planes % 2 || kv->n_pages <= 0 || kv->n_pages > kMaxPages || kv->kv_heads <= 0 ||
+        !pow2 || kv->page < 16 || kv->page > 256 || !attn_dim_ok(kv->head_dim) || kv->max_seqs <= 0 ||
+        kv->max_seqs > kMaxSlots || kv->table_stride <= 0 || (long long)kv->table_stride * kv->page > 0x40000000LL ||
+        (long long)kv->kv_heads * kv->page * kv->head_dim > 0x10000000LL)
+        return fail(CIMA_E_INVALID,
+                    "%s: n_planes=%d n_pages=%d kv_heads=%d page=%d head_dim=%d max_seqs=%d table_stride=%d (planes in "
+                    "pairs, at most %d pages and %d slots, page a power of two from 16 to 256, head_dim 64 or 128, at "
+                    "most 2^30 positions a slot)",
+                    api, kv->n_planes, kv->n_pages, kv->kv_heads, kv->page, kv->head_dim, kv->max_seqs,
+                    kv->table_stride, kMaxPages, kMaxSlots);
+    if (kv->plane_elems % 8 ||
+        kv->plane_elems < (long long)kv->n_pages * kv->kv_heads * kv->page * kv->head_dim)
+        return fail(CIMA_E_INVALID, "%s: plane_elems=%lld is less than a plane or no multiple of 8", api,
+                    kv->plane_elems);
+    if (!kv->pool || !kv->refs || !kv->table || !kv->lens) return fail(CIMA_E_INVALID, "%s: null tensor in the cache", api);
+    if (!aligned(kv->pool, 16) || !aligned(kv->refs, 4) || !aligned(kv->table, 4) || !aligned(kv->lens, 4))
+        return fail(CIMA_E_INVALID, "%s: misaligned pool (16 B) or bookkeeping (4 B)", api);
+    return 0;
+}
+int kv_layer(const cima_kv_pages* kv, int layer, const char* api) {
+    if (layer < 0 || layer >= kv->n_planes / 2)
+        return fail(CIMA_E_INVALID, "%s: layer %d of %d", api, layer, kv->n_planes / 2);
+    return 0;
+}
+// 16-byte words of a page, and pieces of PIECE words that it is copied in
+// (paged_ops.hip)
+long long page_words(const cima_kv_pages* kv) { return (long long)kv->kv_heads * kv->page * kv->head_dim / 8; }
+int page_pieces(const cima_kv_pages* kv) { return (int)((page_words(kv) + 1023) / 1024); }
+// workgroups of the page copies: a piece each, at most eight to a CU
+unsigned copy_grid(const cima_hip_ctx* ctx, long long units) {
+    return (unsigned)std::max(1LL, std::min(units, 8LL * ctx->num_cu));
+}
+
+// kernel-argument mirror of AttnArgs in paged_attn.hip (same member order)
+struct PagedAttnArgs {
+    const void *q, *kp, *vp;
+    const int *table, *lens;
+    void* out;
+    float* acc;
+    void* ml;
+    int seqs, n_new, q_heads, kv_heads, page_shift, n_pages, table_stride;
+    int prefix_pages, prefix_slot, window;
+    int prefix_parts, own_parts, row_tiles;
+    float scale2;
+};
+
+// LDS of Tile<dim, wr, wk> in paged_attn.hip
+unsigned paged_attn_lds(int dim, int wr, int wk) {
+    const int kt = 32 * (wk == 1 ? 2 : 1) * wk, bytes = kt * dim * 2;
+    const int st = 2 * bytes * 3 <= 98304 ? 3 : 2;
+    return (unsigned)(st * 2 * bytes + 1024 * 4 + wr * wk * 32);
+}
+
+}  // namespace
+
+int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* qkv, void* q,
+                               int seqs, int n_new, int q_heads, float theta) {
+    const char* api = "cima_hip_rope_append_paged";
+    if (int rc = kv_check(ctx, kv, api)) return rc;
+    if (int rc = kv_layer(kv, layer, api)) return rc;
+    if (seqs < 0 || seqs > kv->max_seqs || n_new < 0 || q_heads <= 0 || (long long)seqs * n_new > 0x7fffffffLL ||
+        q_heads > 0xffff || !(theta == 0.f || (theta > 0.f && theta < INFINITY)))
+        return fail(CIMA_E_INVALID, "%s: seqs=%d (of %d) n_new=%d q_heads=%d theta=%g", api, seqs, kv->max_seqs, n_new,
+                    q_heads, theta);
+    if (seqs == 0 || n_new == 0) return 0;
+    if (!qkv || !q || !aligned(qkv, 16) || !aligned(q, 16))
+        return fail(CIMA_E_INVALID, "%s: null or misaligned qkv or q (16 B)", api);
+    void* kp = (char*)kv->pool + 2LL * layer * kv->plane_elems * 2;
+    void* vp = (char*)kp + kv->plane_elems * 2;
+    int kvh = kv->kv_heads, shift = log2i(kv->page), np = kv->n_pages, stride = kv->table_stride;
+    const int *table = kv->table, *lens = kv->lens;
+    double lt = theta > 0.f ? log2((double)theta) : -1.0;
+    int rotate = theta > 0.f;
+    void* args[] = {&qkv, &q, &kp, &vp, &table, &lens, &n_new, &q_heads, &kvh, &shift, &np, &stride, &rotate, &lt};
+    return launch_named(ctx, kv->head_dim == 64 ? "cima_rope_append_paged_d64" : "cima_rope_append_paged_d128",
+                        (unsigned)(seqs * n_new), 256, args, api);
+}
+
+int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* q, void* out, int seqs,
+                        int n_new, int q_heads, float scale, int prefix_pages, int prefix_slot, int window, void* slab,
+                        unsigned long long slab_bytes) {
+    const char* api = "cima_hip_attn_paged";
+    if (int rc = kv_check(ctx, kv, api)) return rc;
+    if (int rc = kv_layer(kv, layer, api)) return rc;
+    if (seqs < 0 || seqs > kv->max_seqs || n_new < 0 || q_heads <= 0 || q_heads % kv->kv_heads || q_heads > 0xffff ||
+        !(scale > 0.f && scale < INFINITY) || prefix_pages < 0 || prefix_pages > kv->table_stride || prefix_slot < 0 ||
+        prefix_slot >= kv->max_seqs || window < 0 || (long long)seqs * n_new * q_heads > 0x1000000LL)
+        return fail(CIMA_E_INVALID,
+                    "%s: seqs=%d (of %d) n_new=%d q_heads=%d kv_heads=%d scale=%g prefix_pages=%d (of %d) "
+                    "prefix_slot=%d window=%d (at most 2^24 rows x heads)",
+                    api, seqs, kv->max_seqs, n_new, q_heads, kv->kv_heads, scale, prefix_pages, kv->table_stride,
+                    prefix_slot, window);
+    if (seqs == 0 || n_new == 0) return 0;
+    if (!q || !out || !aligned(q, 16) || !aligned(out, 16))
+        return fail(CIMA_E_INVALID, "%s: null or misaligned q or out (16 B)", api);
+    if (slab_bytes && (!slab || !aligned(slab, 256))) return fail(CIMA_E_INVALID, "%s: null or misaligned slab (256 B)", api);
+    const int dim = kv->head_dim, g = q_heads / kv->kv_heads;
+    const long long rows = (long long)seqs * n_new * q_heads;  // rows of all heads
+    const int head_rows = seqs * n_new * g;                    // of one kv head
+    // parts that the slab holds
+    const long long part_bytes = rows * (dim + 2) * 4;
+    const int fit = (int)std::min<unsigned long long>(slab_bytes / (unsigned long long)part_bytes, 1024);
+    const int least = prefix_pages ? 2 : 1;
+    if (least > 1 && fit < least)
+        return fail(CIMA_E_INVALID, "%s: a slab of %llu bytes does not hold %d parts of %lld", api, slab_bytes, least,
+                    part_bytes);
+    // own tasks: at least 128 positions a part, and enough of them for the chip
+    const int own_rows = n_new * g, own_tiles = (own_rows + 31) / 32;
+    const long long own_base = (long long)seqs * kv->kv_heads * own_tiles;
+    const long long own_room = (long long)(kv->table_stride - prefix_pages) * kv->page;
+    long long own = std::min((4LL * ctx->num_cu + own_base - 1) / own_base, (own_room + 127) / 128);
+    own = std::max(1LL, std::min(own, 64LL));
+    // prefix tasks: rows to a workgroup by how many there are, its positions
+    // split until every CU has one
+    int wr = 0, wk = 0, tiles = 0;
+    long long pre = 0;
+    if (prefix_pages) {
+        wr = head_rows <= 32 ? 1 : head_rows <= 64 ? 2 : head_rows <= 128 ? 4 : 8;
+        wk = wr >= 4 ? 1 : 4 / wr;
+        tiles = (head_rows + 32 * wr - 1) / (32 * wr);
+        const long long base = (long long)kv->kv_heads * tiles;
+        pre = std::min((ctx->num_cu + base - 1) / base, ((long long)prefix_pages * kv->page + 127) / 128);
+        pre = std::max(1LL, std::min(pre, 256LL));
+    }
+    if (pre + own > 1 && pre + own > fit) {  // fewer parts, the prefix's half of them
+        if (fit < 2) pre = prefix_pages ? 1 : 0, own = 1;
+        else if (!prefix_pages) own = fit;
+        else {
+            pre = std::max(1LL, std::min(pre, (long long)fit - std::min(own, (long long)fit / 2)));
+            own = std::max(1LL, std::min(own, fit - pre));
+        }
+    }
+    const int all = (int)(pre + own);
+    PagedAttnArgs A{};
+    A.q = q;
+    A.kp = (const char*)kv->pool + 2LL * layer * kv->plane_elems * 2;
+    A.vp = (const char*)A.kp + kv->plane_elems * 2;
+    A.table = kv->table;
+    A.lens = kv->lens;
+    A.out = out;
+    A.acc = (float*)slab;
+    A.ml = (float*)slab + rows * all * dim;
+    A.seqs = seqs;
+    A.n_new = n_new;
+    A.q_heads = q_heads;
+    A.kv_heads = kv->kv_heads;
+    A.page_shift = log2i(kv->page);
+    A.n_pages = kv->n_pages;
+    A.table_stride = kv->table_stride;
+    A.prefix_pages = prefix_pages;
+    A.prefix_slot = prefix_slot;
+    A.window = window;
+    A.prefix_parts = (int)pre;
+    A.own_parts = (int)own;
+    A.row_tiles = tiles;
+    A.scale2 = scale * 1.44269504088896340736f;
+    void* args[] = {&A};
+    char name[64];
+    hipFunction_t f;
+    if (pre) {
+        snprintf(name, sizeof name, "cima_attn_paged_prefix_d%d_r%dk%d", dim, wr, wk);
+        if (int rc = get_fn(ctx, name, &f)) return rc;
+        const long long groups = (kv->kv_heads * pre + 7) / 8 * 8;
+        if (int rc = launch(ctx, f, (unsigned)(groups * tiles), 64 * wr * wk, args, api, paged_attn_lds(dim, wr, wk)))
+            return rc;
+    }
+    snprintf(name, sizeof name, "cima_attn_paged_own_d%d_k4", dim);
+    if (int rc = get_fn(ctx, name, &f)) return rc;
+    if (int rc = launch(ctx, f, (unsigned)(own_base * own), 256, args, api, paged_attn_lds(dim, 1, 4))) return rc;
+    if (all == 1) return 0;
+    int n_rows = (int)rows, parts = all;
+    const void *acc = A.acc, *ml = A.ml;
+    void* jargs[] = {&acc, &ml, &out, &n_rows, &parts};
+    const int per = 256 / (dim / 4);
+    return launch_named(ctx, dim == 64 ? "cima_attn_paged_join_d64" : "cima_attn_paged_join_d128",
+                        (unsigned)((rows + per - 1) / per), 256, jargs, api);
+}
+
+int cima_hip_kv_pages_copy(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int* src, const int* dst, int n) {
+    const char* api = "cima_hip_kv_pages_copy";
+    if (int rc = kv_check(ctx, kv, api)) return rc;
+    if (n < 0 || n > kMaxPages) return fail(CIMA_E_INVALID, "%s: n=%d", api, n);
+    if (n == 0) return 0;
+    if (!src || !dst || !aligned(src, 4) || !aligned(dst, 4))
+        return fail(CIMA_E_INVALID, "%s: null or misaligned lists", api);
+    void* pool = kv->pool;
+    long long plane = kv->plane_elems / 8, words = page_words(kv);
+    int pieces = page_pieces(kv), pages = kv->n_pages;
+    long long units = (long long)kv->n_planes * n * pieces;
+    void* args[] = {&pool, &plane, &words, &pieces, &n, &units, &src, &dst, &pages};
+    return launch_named(ctx, "cima_kv_pages_copy", copy_grid(ctx, units), 256, args, api);
+}
+
+int cima_hip_kv_pages_reserve(cima_hip_ctx* ctx, const cima_kv_pages* kv, int seqs, int n_new, int* status) {
+    const char* api = "cima_hip_kv_pages_reserve";
+    if (int rc = kv_check(ctx, kv, api)) return rc;
+    if (seqs < 0 || seqs > kv->max_seqs || n_new < 0 || n_new > 0x40000000)
+        return fail(CIMA_E_INVALID, "%s: seqs=%d (of %d) n_new=%d", api, seqs, kv->max_seqs, n_new);
+    if (!status || !aligned(status, 4)) return fail(CIMA_E_INVALID, "%s: null or misaligned status", api);
+    int *refs = kv->refs, *table = kv->table, *lens = kv->lens;
+    int np = kv->n_pages, stride = kv->table_stride, shift = log2i(kv->page);
+    void* args[] = {&refs, &np, &table, &lens, &seqs, &stride, &shift, &n_new, &status};
+    return launch_named(ctx, "cima_kv_pages_reserve", 1, 1024, args, api);
+}
+
+int cima_hip_kv_pages_fork(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int* parents, const int* children, int n,
+                           int* status) {
+    const char* api = "cima_hip_kv_pages_fork";
+    if (int rc = kv_check(ctx, kv, api)) return rc;
+    if (n < 0 || n > kv->max_seqs) return fail(CIMA_E_INVALID, "%s: n=%d of %d slots", api, n, kv->max_seqs);
+    if (!status || !aligned(status, 4)) return fail(CIMA_E_INVALID, "%s: null or misaligned status", api);
+    if (n && (!parents || !children || !aligned(parents, 4) || !aligned(children, 4)))
+        return fail(CIMA_E_INVALID, "%s: null or misaligned lists", api);
+    int *refs = kv->refs, *table = kv->table, *lens = kv->lens;
+    int np = kv->n_pages, seqs = kv->max_seqs, stride = kv->table_stride, shift = log2i(kv->page);
+    void* args[] = {&refs, &np, &table, &lens, &seqs, &stride, &shift, &parents, &children, &n, &status};
+    if (int rc = launch_named(ctx, "cima_kv_pages_fork", 1, 1024, args, api)) return rc;
+    if (n == 0) return 0;
+    void* pool = kv->pool;
+    long long plane = kv->plane_elems / 8;
+    int heads = kv->kv_heads, row = kv->head_dim / 8;
+    void* cargs[] = {&pool, &plane, &refs, &np, &table, &lens, &stride, &shift, &heads, &row, &parents, &children, &n,
+                     &status};
+    return launch_named(ctx, "cima_kv_pages_fork_copy", (unsigned)(n * (1 + kv->n_planes)), 256, cargs, api);
+}
+
+int cima_hip_kv_pages_free(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int* slots, int n) {
+    const char* api = "cima_hip_kv_pages_free";
+    if (int rc = kv_check(ctx, kv, api)) return rc;
+    if (n < 0 || n > kMaxSlots) return fail(CIMA_E_INVALID, "%s: n=%d", api, n);
+    if (n == 0) return 0;
+    if (!slots || !aligned(slots, 4)) return fail(CIMA_E_INVALID, "%s: null or misaligned list", api);
+    int *refs = kv->refs, *table = kv->table, *lens = kv->lens;
+    int np = kv->n_pages, seqs = kv->max_seqs, stride = kv->table_stride, parts = (stride + 1023) / 1024;
+    void* args[] = {&refs, &np, &table, &lens, &seqs, &stride, &slots, &parts};
+    return launch_named(ctx, "cima_kv_pages_free", (unsigned)n * parts, 256, args, api);
+}
+
+int cima_hip_kv_pages_compact(cima_hip_ctx* ctx, const cima_kv_pages* kv, int* refs_out, int* table_out, int* n_live,
+                              void* slab, unsigned long long slab_bytes) {
+    const char* api = "cima_hip_kv_pages_compact";
+    if (int rc = kv_check(ctx, kv, api)) return rc;
+    if (!refs_out || !table_out || !n_live || !aligned(refs_out, 4) || !aligned(table_out, 4) || !aligned(n_live, 4))
+        return fail(CIMA_E_INVALID, "%s: null or misaligned outputs", api);
+    if (!slab || !aligned(slab, 4) || slab_bytes < 12ULL * kv->n_pages + 64)
+        return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned", api, slab_bytes,
+                    12ULL * kv->n_pages + 64);
+    const int* refs = kv->refs;
+    const int* table = kv->table;
+    int np = kv->n_pages;
+    void* args[] = {&refs, &np, &refs_out, &n_live, &slab};
+    if (int rc = launch_named(ctx, "cima_kv_pages_compact", 1, 1024, args, api)) return rc;
+    void* pool = kv->pool;
+    long long plane = kv->plane_elems / 8, words = page_words(kv), entries = (long long)kv->max_seqs * kv->table_stride;
+    int pieces = page_pieces(kv), planes = kv->n_planes;
+    void* margs[] = {&pool, &plane, &words, &pieces, &planes, &np, &table, &table_out, &entries, &slab};
+    // at most half the pages move
+    const long long units = (long long)planes * ((np + 1) / 2) * pieces;
+    return launch_named(ctx, "cima_kv_pages_compact_move", copy_grid(ctx, units), 256, margs, api);
+}
+
+// ------------------------------------------------------------------ sampling
+
+namespace {
+// logits of a workgroup (SM_PART) and entries of a part (VF_PART), sample_ops.hip
+const int kSoftmaxPart = 8192, kVerifyPart = 2048;
+
+// kernel-argument mirror of VfArgs in sample_ops.hip (same member order)
+struct VerifyArgs {
+    const float *p, *q;
+    const int *drafts, *counts;
+    const float* u;
+    int *accepted, *tokens, *lens;
+    void* sums;
+    int n_draft, vocab, parts;
+};
+}  // namespace
+
+int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, int n, const float* temp,
+                          int rows_per_temp, float cap, int x_dtype, void* slab, unsigned long long slab_bytes) {
+    const char* api = "cima_hip_softmax_rows";
+    if (int rc = ready(ctx, api)) return rc;
+    if (rows < 0 || n <= 0 || n > 0x3fffffff || rows_per_temp <= 0 || !(cap >= 0.f && cap < INFINITY))
+        return fail(CIMA_E_INVALID, "%s: rows=%d n=%d rows_per_temp=%d cap=%g", api, rows, n, rows_per_temp, cap);
+    if (x_dtype != CIMA_DT_F32 && x_dtype != CIMA_DT_F16)
+        return fail(CIMA_E_INVALID, "%s: x_dtype %d is not f32 or f16", api, x_dtype);
+    if (rows == 0) return 0;
+    if (!x || !y || !aligned(x, x_dtype == CIMA_DT_F32 ? 4 : 2) || !aligned(y, 4) || !aligned(temp, 4))
+        return fail(CIMA_E_INVALID, "%s: null or misaligned x, y or temp", api);
+    int parts = (n + kSoftmaxPart - 1) / kSoftmaxPart;
+    const unsigned long long need = 16ULL * rows * parts;
+    if ((long long)rows * parts > 0x7fffffffLL || !slab || !aligned(slab, 8) || slab_bytes < need)
+        return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (8 B)", api,
+                    slab_bytes, need);
+    void* args[] = {&x, &slab, &n, &temp, &rows_per_temp, &cap, &parts};
+    const bool f32 = x_dtype == CIMA_DT_F32;
+    if (int rc = launch_named(ctx, f32 ? "cima_softmax_stats_f32" : "cima_softmax_stats_f16", (unsigned)(rows * parts),
+                              256, args, api))
+        return rc;
+    void* pargs[] = {&x, &y, &slab, &n, &temp, &rows_per_temp, &cap, &parts};
+    return launch_named(ctx, f32 ? "cima_softmax_probs_f32" : "cima_softmax_probs_f16", (unsigned)(rows * parts), 256,
+                        pargs, api);
+}
+
+int cima_hip_verify_drafts(cima_hip_ctx* ctx, const float* p, const float* q, const int* drafts, const int* counts,
+                           const float* u, int* accepted, int* tokens, int* lens, int seqs, int n_draft, int vocab,
+                           void* slab, unsigned long long slab_bytes) {
+    const char* api = "cima_hip_verify_drafts";
+    if (int rc = ready(ctx, api)) return rc;
+    if (seqs < 0 || n_draft < 0 || n_draft > 1 << 20 || vocab <= 0 || vocab > 0x3fffffff)
+        return fail(CIMA_E_INVALID, "%s: seqs=%d n_draft=%d vocab=%d", api, seqs, n_draft, vocab);
+    if (seqs == 0) return 0;
+    if (!p || !u || !accepted || !tokens || (n_draft && !drafts)) return fail(CIMA_E_INVALID, "%s: null pointer", api);
+    if (!aligned(p, 4) || !aligned(q, 4) || !aligned(drafts, 4) || !aligned(counts, 4) || !aligned(u, 4) ||
+        !aligned(accepted, 4) || !aligned(tokens, 4) || !aligned(lens, 4))
+        return fail(CIMA_E_INVALID, "%s: misaligned pointer (4 B)", api);
+    const long long parts = ((long long)vocab + kVerifyPart - 1) / kVerifyPart;
+    if (seqs * parts > 0x7fffffffLL || !slab || !aligned(slab, 8) || slab_bytes < 8ULL * seqs * parts)
+        return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (8 B)", api,
+                    slab_bytes, 8ULL * seqs * parts);
+    VerifyArgs A{p, q, drafts, counts, u, accepted, tokens, lens, slab, n_draft, vocab, (int)parts};
+    void* args[] = {&A};
+    if (int rc = launch_named(ctx, "cima_verify_sums", (unsigned)(seqs * parts), 256, args, api)) return rc;
+    return launch_named(ctx, "cima_verify_draw", (unsigned)seqs, 256, args, api);
+}
 
 struct cima_hip_graph {
     hipGraphExec_t exec = nullptr;

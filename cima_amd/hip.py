@@ -27,7 +27,8 @@ LIBHIP = os.path.join(LIB_DIR, "libcima_hip.so")
 # the gfx950 code objects cima_hip_init loads (names as cima_amd/build.py
 # writes them)
 CODE_OBJECTS = [os.path.join(LIB_DIR, f"cima_{n}.hsaco")
-                for n in ("gemv_a", "gemv_b", "gemv_c", "gemm", "dequant", "decode", "bnb4", "gemm_wide")]
+                for n in ("gemv_a", "gemv_b", "gemv_c", "gemm", "dequant", "decode", "bnb4", "gemm_wide", "paged",
+                          "paged_attn", "sample")]
 
 # declared in include/cima_hip.h, in order
 EXPORTS = (
@@ -41,6 +42,9 @@ EXPORTS = (
     "cima_hip_rmsnorm", "cima_hip_rope", "cima_hip_kv_append", "cima_hip_attn_decode_split", "cima_hip_attn_reduce",
     "cima_hip_attn_decode_noalloc", "cima_hip_attn_decode", "cima_hip_attn_gguf_gemv", "cima_hip_gguf_gemv_argmax", "cima_hip_argmax",
     "cima_hip_argmax_to_ids", "cima_hip_pos_bump", "cima_hip_decode_step",
+    "cima_hip_rope_append_paged", "cima_hip_attn_paged", "cima_hip_kv_pages_copy", "cima_hip_kv_pages_reserve",
+    "cima_hip_kv_pages_fork", "cima_hip_kv_pages_free", "cima_hip_kv_pages_compact", "cima_hip_softmax_rows",
+    "cima_hip_verify_drafts",
     "cima_hip_capture_begin", "cima_hip_capture_end", "cima_hip_graph_launch", "cima_hip_graph_destroy",
     "cima_hip_nf4_dequant", "cima_hip_nf4_gemv", "cima_hip_set_nf4_tuning", "cima_hip_nf4_gemm_slab",
     "cima_hip_stream_read", "cima_hip_stream_read_cfg",
@@ -66,6 +70,15 @@ class Decoder(ctypes.Structure):
         + [("layers", ctypes.POINTER(DecoderLayer))]
         + [(n, ctypes.c_void_p) for n in (
             "x", "qkv", "act", "logits", "part", "slot", "ids", "pos")])
+
+
+class KvPages(ctypes.Structure):
+    """``cima_kv_pages`` (include/cima_hip.h); ``cima_amd.paged.PagedKV`` fills it."""
+    _fields_ = ([("pool", ctypes.c_void_p), ("plane_elems", ctypes.c_longlong)]
+                + [(n, ctypes.c_void_p) for n in ("refs", "table", "lens")]
+                + [(n, ctypes.c_int) for n in ("n_planes", "n_pages", "kv_heads", "page", "head_dim", "max_seqs",
+                                               "table_stride")])
+
 
 E_INVALID, E_FORMAT, E_NO_KERNEL, E_NOT_INIT, E_LIBRARY = -1, -2, -3, -4, -5
 
@@ -126,6 +139,16 @@ def load_library(path: str = LIBHIP) -> ctypes.CDLL:
     L.cima_hip_argmax_to_ids.argtypes = [P, P, P, P]
     L.cima_hip_pos_bump.argtypes = [P, P]
     L.cima_hip_decode_step.argtypes = [P, ctypes.POINTER(Decoder)]
+    U = ctypes.c_ulonglong
+    L.cima_hip_rope_append_paged.argtypes = [P, P, I, P, P, I, I, I, F]
+    L.cima_hip_attn_paged.argtypes = [P, P, I, P, P, I, I, I, F, I, I, I, P, U]
+    L.cima_hip_kv_pages_copy.argtypes = [P, P, P, P, I]
+    L.cima_hip_kv_pages_reserve.argtypes = [P, P, I, I, P]
+    L.cima_hip_kv_pages_fork.argtypes = [P, P, P, P, I, P]
+    L.cima_hip_kv_pages_free.argtypes = [P, P, P, I]
+    L.cima_hip_kv_pages_compact.argtypes = [P, P, P, P, P, P, U]
+    L.cima_hip_softmax_rows.argtypes = [P, P, P, I, I, P, I, F, I, P, U]
+    L.cima_hip_verify_drafts.argtypes = [P] * 9 + [I, I, I, P, U]
     L.cima_hip_capture_begin.argtypes = [P]
     L.cima_hip_stream_read.argtypes = [P, P, LL, P]
     L.cima_hip_stream_read_cfg.argtypes = [P, P, LL, P, I, I, I, I]
@@ -180,6 +203,29 @@ def _ptr(a) -> Optional[int]:
     if not contiguous():
         raise EngineError("hip", E_INVALID, "tensor argument is not contiguous")
     return a.data_ptr()
+
+
+# Operands of the paged cache's calls and of sampling: a tensor must have the
+# element type and hold at least the elements that the call reads or writes
+# (torch's integers are 64-bit unless asked otherwise; read as 32-bit they would
+# name wrong pages).  A raw pointer is taken as it is.
+def _ptr_of(a, dtype: str, n: int, name: str) -> Optional[int]:
+    if a is None or isinstance(a, int):
+        return a or None
+    p = _ptr(a)
+    if str(a.dtype) != dtype:
+        raise EngineError("hip", E_INVALID, f"{name} is {a.dtype}, not {dtype}")
+    if a.numel() < n:
+        raise EngineError("hip", E_INVALID, f"{name} holds {a.numel()} elements, the call takes {n}")
+    return p
+
+
+_I32, _F32, _F16 = "torch.int32", "torch.float32", "torch.float16"
+
+
+def _slab(a) -> tuple:
+    """(pointer, bytes) of a scratch tensor."""
+    return (None, 0) if a is None else (_ptr(a), a.numel() * a.element_size())
 
 
 def _act_of(t) -> int:
@@ -475,6 +521,80 @@ class HipCtx:
     def decode_step(self, desc: "Decoder") -> None:
         """One greedy decode step of a whole decoder (cima_hip_decode_step)."""
         self._check(self.lib.cima_hip_decode_step(self.handle, ctypes.byref(desc)))
+
+    # -- a batch over a paged cache (kv: cima_amd.paged.PagedKV) ----------------
+    def rope_append_paged(self, kv, layer: int, qkv, q, seqs: int, n_new: int, q_heads: int, theta: float) -> None:
+        """RoPE of a step's queries (to ``q``) and keys, row ``s * n_new + j`` of
+        ``qkv`` at position ``lens[s] + j``, and the append of its keys and values
+        to the pages of ``layer`` (theta 0: no rotation)."""
+        rows = seqs * n_new
+        self._check(self.lib.cima_hip_rope_append_paged(
+            self.handle, kv.ref, layer, _ptr_of(qkv, _F16, rows * (q_heads + 2 * kv.kv_heads) * kv.head_dim, "qkv"),
+            _ptr_of(q, _F16, rows * q_heads * kv.head_dim, "q"), seqs, n_new, q_heads, theta))
+
+    def attn_paged(self, kv, layer: int, q, out, seqs: int, n_new: int, q_heads: int, scale: float, slab,
+                   prefix_pages: int = 0, prefix_slot: int = 0, window: int = 0) -> None:
+        """Attention of a step's queries over the pages of ``layer``; the first
+        ``prefix_pages`` entries, the same in every slot, are read once for all
+        from row ``prefix_slot`` of the table."""
+        n = seqs * n_new * q_heads * kv.head_dim
+        self._check(self.lib.cima_hip_attn_paged(self.handle, kv.ref, layer, _ptr_of(q, _F16, n, "q"),
+                                                 _ptr_of(out, _F16, n, "out"), seqs, n_new, q_heads, scale,
+                                                 prefix_pages, prefix_slot, window, *_slab(slab)))
+
+    def kv_pages_copy(self, kv, src, dst, n: int) -> None:
+        """Page ``dst[i]`` of every plane = page ``src[i]``."""
+        self._check(self.lib.cima_hip_kv_pages_copy(self.handle, kv.ref, _ptr_of(src, _I32, n, "src"),
+                                                    _ptr_of(dst, _I32, n, "dst"), n))
+
+    def kv_pages_reserve(self, kv, seqs: int, n_new: int, status) -> None:
+        """Pages for ``n_new`` more tokens in each of slots [0, seqs) in use;
+        ``status[0]`` = pages missing (then nothing is changed)."""
+        self._check(self.lib.cima_hip_kv_pages_reserve(self.handle, kv.ref, seqs, n_new,
+                                                       _ptr_of(status, _I32, 1, "status")))
+
+    def kv_pages_fork(self, kv, parents, children, n: int, status) -> None:
+        """Slots ``children[i]`` become copies of ``parents[i]``: whole pages
+        shared, a page begun copied; ``status[0]``: 0, pages missing, or -1."""
+        self._check(self.lib.cima_hip_kv_pages_fork(self.handle, kv.ref, _ptr_of(parents, _I32, n, "parents"),
+                                                    _ptr_of(children, _I32, n, "children"), n,
+                                                    _ptr_of(status, _I32, 1, "status")))
+
+    def kv_pages_free(self, kv, slots, n: int) -> None:
+        """The slots give their pages back and are free."""
+        self._check(self.lib.cima_hip_kv_pages_free(self.handle, kv.ref, _ptr_of(slots, _I32, n, "slots"), n))
+
+    def kv_pages_compact(self, kv, refs_out, table_out, n_live, slab) -> None:
+        """The pages in use move together to the front of the pool; the new counts
+        and table go to ``refs_out`` and ``table_out`` (or are the cache's own)."""
+        self._check(self.lib.cima_hip_kv_pages_compact(
+            self.handle, kv.ref, _ptr_of(refs_out, _I32, kv.n_pages, "refs_out"),
+            _ptr_of(table_out, _I32, kv.table.numel(), "table_out"), _ptr_of(n_live, _I32, 1, "n_live"), *_slab(slab)))
+
+    # -- sampling ---------------------------------------------------------------
+    def softmax_rows(self, x, y, rows: int, n: int, temp=None, rows_per_temp: int = 1, cap: float = 0.0,
+                     slab=None) -> None:
+        """``y[r] = softmax(x[r] / temp[r // rows_per_temp])`` in fp32 (temp <= 0:
+        the largest logit alone; cap > 0: logits through ``cap * tanh(x / cap)``)."""
+        if rows_per_temp <= 0:
+            raise EngineError("hip", E_INVALID, f"rows_per_temp is {rows_per_temp}")
+        act = _act_of(x)
+        self._check(self.lib.cima_hip_softmax_rows(
+            self.handle, _ptr_of(x, _F16 if act else _F32, rows * n, "x"), _ptr_of(y, _F32, rows * n, "y"), rows, n,
+            _ptr_of(temp, _F32, -(-rows // rows_per_temp), "temp"), rows_per_temp, cap, act, *_slab(slab)))
+
+    def verify_drafts(self, p, q, drafts, counts, u, accepted, tokens, lens, seqs: int, n_draft: int, vocab: int,
+                      slab) -> None:
+        """Drafted tokens kept while ``u * q[d] < p[d]`` and the token drawn after
+        them; ``q`` None: certain drafts, ``counts`` None: n_draft each, ``lens``
+        None: no lengths to advance."""
+        k = n_draft + 1
+        self._check(self.lib.cima_hip_verify_drafts(
+            self.handle, _ptr_of(p, _F32, seqs * k * vocab, "p"), _ptr_of(q, _F32, seqs * n_draft * vocab, "q"),
+            _ptr_of(drafts, _I32, seqs * n_draft, "drafts"), _ptr_of(counts, _I32, seqs, "counts"),
+            _ptr_of(u, _F32, seqs * k, "u"), _ptr_of(accepted, _I32, seqs, "accepted"),
+            _ptr_of(tokens, _I32, seqs * k, "tokens"), _ptr_of(lens, _I32, seqs, "lens"), seqs, n_draft, vocab,
+            *_slab(slab)))
 
     def stream_read_cfg(self, src, nbytes: int, sink, dest: int, depth: int, width: int = 16,
                         wgs_per_cu: int = 2) -> None:

@@ -55,9 +55,10 @@ typedef struct cima_hip_ctx cima_hip_ctx;
 /* Context creation: replaces CudaCtx::init (src/cuda.rs:691-908) -- device
  * selection, one non-blocking stream, then loading the prebuilt gfx950 code
  * objects (cima_gemv_a/b/c.hsaco, cima_gemm.hsaco, cima_gemm_wide.hsaco,
- * cima_dequant.hsaco, cima_decode.hsaco, cima_bnb4.hsaco) with hipModuleLoad
- * and resolving every kernel (the reference JIT-compiles with NVRTC and
- * resolves its KernelSet, src/cuda.rs:808-877).
+ * cima_dequant.hsaco, cima_decode.hsaco, cima_bnb4.hsaco, cima_paged.hsaco,
+ * cima_paged_attn.hsaco, cima_sample.hsaco) with hipModuleLoad and resolving
+ * every kernel (the reference JIT-compiles with NVRTC and resolves its
+ * KernelSet, src/cuda.rs:808-877).
  * code_dir: directory holding the code objects, or NULL for the directory
  * of this library. */
 int cima_hip_init(int device, const char* code_dir, cima_hip_ctx** out);
@@ -406,6 +407,122 @@ typedef struct cima_decoder {
  * (head_dim + 2) floats, pass 128 KB, the merge is a launch of its own: 6
  * per layer (8 with separate matrices). */
 int cima_hip_decode_step(cima_hip_ctx* ctx, const cima_decoder* d);
+
+/* ---------------------------------------------------------------------
+ * A batch of sequences over a paged KV cache (no counterpart in the
+ * reference, which decodes one sequence from a contiguous cache): several
+ * continuations of one prompt, or drafted tokens, share the prompt's pages.
+ * All integers of the cache live in device memory, so that a captured step
+ * replays as the batch grows; no call allocates or synchronises.  The
+ * caller's slab is scratch: calls that may run at the same time (other
+ * streams, other graphs in flight) need a slab each.
+ * --------------------------------------------------------------------- */
+
+/* The cache.  A page is [kv_heads, page, head_dim] f16 in every plane, two
+ * planes a layer: keys in plane 2 l, values in plane 2 l + 1.  Slot s holds
+ * position t of its sequence in row t % page of page table[s * table_stride +
+ * t / page]; unused entries are -1.  lens[s] is its number of cached tokens,
+ * -1 where the slot is not in use.  refs[i] counts the slots that hold page
+ * i: 0 = free.  page is a power of two from 16 to 256; pool is 16-byte
+ * aligned and plane_elems a multiple of 8. */
+typedef struct cima_kv_pages {
+    void* pool;             /* f16 planes of [n_pages, kv_heads, page, head_dim] */
+    long long plane_elems;  /* elements from one plane to the next */
+    int* refs;              /* [n_pages] */
+    int* table;             /* [max_seqs, table_stride] */
+    int* lens;              /* [max_seqs] */
+    int n_planes, n_pages, kv_heads, page, head_dim, max_seqs, table_stride;
+} cima_kv_pages;
+
+/* RoPE of a step's queries and keys, and the append of its keys and values:
+ * qkv f16 [seqs * n_new, (q_heads + 2 kv_heads) * head_dim] as the fused q|k|v
+ * GEMM writes it, row s * n_new + j at position lens[s] + j of slot s.  The
+ * rotated queries go to q [seqs * n_new, q_heads * head_dim], the rotated keys
+ * and the values to layer `layer`'s planes.  NeoX pairs as cima_hip_rope, the
+ * angle formed in fp64 (at position 100000 an fp32 angle is off by up to
+ * 0.008); theta 0 = no rotation.  lens is not changed: every layer of the step
+ * appends at the same positions.  Slots not in use write nothing, neither q;
+ * positions without a page (entry -1 or behind the row) write no key.
+ * head_dim 64 or 128; qkv and q 16-byte aligned. */
+int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* qkv, void* q,
+                               int seqs, int n_new, int q_heads, float theta);
+
+/* Attention of a step's queries q f16 [seqs * n_new, q_heads, head_dim] over
+ * the pages of `layer`, after the step's own keys and values were appended:
+ * row s * n_new + j sees positions [max(0, p - window + 1), p], p = lens[s] + j
+ * (window 0: all up to p), out f16 of q's shape.  The first prefix_pages
+ * entries of every slot in use are the same pages; they are read from row
+ * prefix_slot of the table, once for all rows.  Rows of slots not in use are
+ * written as zeros.  Pages that no row sees may be absent (-1) and hold
+ * anything; what some row sees must be finite.  Scores and sums are fp32; the
+ * probabilities are rounded to f16 for the product with the values.
+ *
+ * The work is split over the positions where there are few rows, as long as
+ * the slab (256-byte aligned) holds the partial sums: rows * q_heads *
+ * (head_dim + 2) * 4 bytes per part, rows = seqs * n_new.  Two parts are
+ * needed where prefix_pages > 0, else none.  head_dim 64 or 128; q_heads a
+ * multiple of kv_heads; scale positive; q and out 16-byte aligned. */
+int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* q, void* out, int seqs,
+                        int n_new, int q_heads, float scale, int prefix_pages, int prefix_slot, int window, void* slab,
+                        unsigned long long slab_bytes);
+
+/* Page dst[i] of every plane = page src[i], i < n; counts and tables stay.
+ * Pairs with an id outside [0, n_pages) are skipped.  No page may be written
+ * twice or be read and written by one call. */
+int cima_hip_kv_pages_copy(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int* src, const int* dst, int n);
+/* Room for n_new more tokens in each slot s < seqs in use: its entries
+ * [lens / page, (lens + n_new - 1) / page] that are -1 take the lowest free
+ * pages, slot by slot, with count 1.  All or nothing: *status = 0, or the
+ * number of pages that are missing, and nothing is changed.  Entries behind
+ * table_stride count as missing.  n_pages at most 1048576. */
+int cima_hip_kv_pages_reserve(cima_hip_ctx* ctx, const cima_kv_pages* kv, int seqs, int n_new, int* status);
+/* Slot children[i] becomes a copy of slot parents[i], i < n: the pages that
+ * the parent has filled are shared (counts + 1), the rows of a page begun are
+ * copied to the lowest free page; the child's other entries are -1.  The
+ * children must be free (lens -1), distinct and none of the parents in use as
+ * one; a parent may be named several times.  All or nothing: *status = 0, the
+ * number of missing pages (> 0), or -1 where a slot is not as it must be. */
+int cima_hip_kv_pages_fork(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int* parents, const int* children, int n,
+                           int* status);
+/* The slots' pages lose a holder each, their entries and lens become -1.
+ * Slots not in use or named twice, and ids outside [0, max_seqs), do no harm. */
+int cima_hip_kv_pages_free(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int* slots, int n);
+/* The L pages in use move together into pages [0, L): the k-th page in use
+ * from L on takes the k-th free page below L, in every plane.  The new counts
+ * and table go to refs_out and table_out (of refs' and table's sizes; they may
+ * be refs and table themselves), L to *n_live.  slab: 12 n_pages + 64 bytes,
+ * 4-byte aligned.  n_pages at most 1048576. */
+int cima_hip_kv_pages_compact(cima_hip_ctx* ctx, const cima_kv_pages* kv, int* refs_out, int* table_out, int* n_live,
+                              void* slab, unsigned long long slab_bytes);
+
+/* Probabilities of rows of logits: y[r] = softmax(f(x[r]) / temp[r /
+ * rows_per_temp]) fp32, x f32 or f16 [rows, n], f(v) = cap * tanh(v / cap)
+ * where cap > 0 (as cima_hip_argmax), else v.  temp NULL = 1; where it is <= 0
+ * the row is 1 at its largest logit (the lowest index of equals) and 0
+ * elsewhere.  A row of -inf alone becomes zeros; NaN or +inf make a row NaN
+ * (temp <= 0: they rank as the largest do, NaN as the lowest).  slab (8-byte
+ * aligned): 16 bytes for each 8192 logits of a row (rounded up) and row. */
+int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, int n, const float* temp,
+                          int rows_per_temp, float cap, int x_dtype, void* slab, unsigned long long slab_bytes);
+
+/* Speculative sampling: which drafted tokens the target keeps, and the token
+ * that follows, by given uniform numbers.  p f32 [seqs, n_draft + 1, vocab]
+ * are the target's probabilities, q f32 [seqs, n_draft, vocab] the draft's
+ * (NULL: the drafts were certain), drafts [seqs, n_draft], counts[s] <= n_draft
+ * the drafts of slot s (NULL: n_draft), u f32 [seqs, n_draft + 1] in [0, 1).
+ * Draft i is kept while u[i] * q[i][d] < p[i][d] (exact products; an id
+ * outside [0, vocab) is refused).  After a first refusal at row a the next token is
+ * drawn from max(p[a] - q[a], 0), after all were kept from p[count]: the lowest
+ * t whose running sum passes u[n_draft] times the whole (sums in fp64; NaN and
+ * negative values count 0; where nothing is left, from p[a]; where that holds
+ * nothing, -1).  tokens [seqs, n_draft + 1] = the kept drafts, the drawn token,
+ * then -1; accepted[s] = drafts kept.  lens (may be NULL): lens[s] += accepted
+ * + 1 where lens[s] >= 0; slots with lens[s] < 0 get accepted 0 and tokens -1.
+ * n_draft 0 draws one token a row.  slab (8-byte aligned): 8 bytes for each
+ * 2048 entries of vocab (rounded up) and slot. */
+int cima_hip_verify_drafts(cima_hip_ctx* ctx, const float* p, const float* q, const int* drafts, const int* counts,
+                           const float* u, int* accepted, int* tokens, int* lens, int seqs, int n_draft, int vocab,
+                           void* slab, unsigned long long slab_bytes);
 
 /* ---------------------------------------------------------------------
  * Graph capture of the context's stream (CudaCtx::capture_begin /
