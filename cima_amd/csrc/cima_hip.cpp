@@ -205,11 +205,6 @@ const char* const kPagedKernels[] = {
     "cima_rope_append_paged_d64", "cima_rope_append_paged_d128", "cima_kv_pages_copy", "cima_kv_pages_reserve",
     "cima_kv_pages_fork", "cima_kv_pages_fork_copy", "cima_kv_pages_free", "cima_kv_pages_compact",
     "cima_kv_pages_compact_move"};
-const char* const kPagedAttnKernels[] = {
-    "cima_attn_paged_prefix_d64_r1k4", "cima_attn_paged_prefix_d64_r2k2", "cima_attn_paged_prefix_d64_r4k1",
-    "cima_attn_paged_prefix_d64_r8k1", "cima_attn_paged_own_d64_k4", "cima_attn_paged_join_d64",
-    "cima_attn_paged_prefix_d128_r1k4", "cima_attn_paged_prefix_d128_r2k2", "cima_attn_paged_prefix_d128_r4k1",
-    "cima_attn_paged_prefix_d128_r8k1", "cima_attn_paged_own_d128_k4", "cima_attn_paged_join_d128"};
 const char* const kSampleKernels[] = {"cima_softmax_stats_f16", "cima_softmax_stats_f32", "cima_softmax_probs_f16",
                                       "cima_softmax_probs_f32", "cima_verify_sums", "cima_verify_draw"};
 
@@ -657,8 +652,15 @@ int cima_hip_init(int device, const char* code_dir, cima_hip_ctx** out) {
         if (!rc) rc = add(MOD_DECODE, kn);
     for (const char* kn : kPagedKernels)
         if (!rc) rc = add(MOD_PAGED, kn);
-    for (const char* kn : kPagedAttnKernels)
-        if (!rc) rc = add(MOD_PAGED_ATTN, kn);
+    for (int dim : {64, 128}) {
+        char name[64];
+        for (const char* kn : {"d%d_m0_n1", "d%d_m1_n1", "d%d_m2_n1", "d%d_m0_n2", "d%d_m1_n2", "d%d_m2_n2", "join_d%d"}) {
+            char fmt[64];
+            snprintf(fmt, sizeof fmt, "cima_attn_paged_%s", kn);
+            snprintf(name, sizeof name, fmt, dim);
+            if (!rc) rc = add(MOD_PAGED_ATTN, name);
+        }
+    }
     for (const char* kn : kSampleKernels)
         if (!rc) rc = add(MOD_SAMPLE, kn);
     if (rc) {
@@ -1651,14 +1653,16 @@ struct PagedAttnArgs {
     void* ml;
     int seqs, n_new, q_heads, kv_heads, page_shift, n_pages, table_stride;
     int prefix_pages, prefix_slot, window;
-    int prefix_parts, own_parts, row_tiles;
+    int prefix_parts, own_parts, row_tiles, prefix_tile, own_tile, prefix_wgs;
     float scale2;
 };
 
-// LDS of Tile<dim, wr, wk> in paged_attn.hip
-unsigned paged_attn_lds(int dim, int wr, int wk) {
-    const int kt = 32 * (wk == 1 ? 2 : 1) * wk, bytes = kt * dim * 2;
-    const int st = 2 * bytes * 3 <= 98304 ? 3 : 2;
+// LDS of Few<dim, nb> and of Tile<dim, wr, wk, st> in paged_attn.hip
+unsigned paged_few_lds(int dim, int nb) {
+    return (unsigned)(4 * std::max(2 * 32 * dim * 2, nb * (dim / 16) * 64 * 16) + 4 * nb * 16 * 8);
+}
+unsigned paged_attn_lds(int dim, int wr, int wk, int st) {
+    const int kt = 32 * (wk == 1 && wr > 1 ? 2 : 1) * wk, bytes = kt * dim * 2;
     return (unsigned)(st * 2 * bytes + 1024 * 4 + wr * wk * 32);
 }
 
@@ -1715,23 +1719,26 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     if (least > 1 && fit < least)
         return fail(CIMA_E_INVALID, "%s: a slab of %llu bytes does not hold %d parts of %lld", api, slab_bytes, least,
                     part_bytes);
-    // own tasks: at least 128 positions a part, and enough of them for the chip
-    const int own_rows = n_new * g, own_tiles = (own_rows + 31) / 32;
+    auto env = [](const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; };
+    const int own_rows = n_new * g;
+    const bool few = prefix_pages && head_rows <= 32;  // the prefix tasks run with the own tasks
+    const int nb = std::max(own_rows, few ? head_rows : 0) > 16 ? 2 : 1;
+    const int own_tiles = (own_rows + 16 * nb - 1) / (16 * nb);
     const long long own_base = (long long)seqs * kv->kv_heads * own_tiles;
     const long long own_room = (long long)(kv->table_stride - prefix_pages) * kv->page;
-    long long own = std::min((4LL * ctx->num_cu + own_base - 1) / own_base, (own_room + 127) / 128);
+    long long own = std::min((env("OT", 4) * (long long)ctx->num_cu + own_base - 1) / own_base, (own_room + 127) / 128);
     own = std::max(1LL, std::min(own, 64LL));
-    // prefix tasks: rows to a workgroup by how many there are, its positions
-    // split until every CU has one
-    int wr = 0, wk = 0, tiles = 0;
+    int tiles = 0, mode = 0;
     long long pre = 0;
     if (prefix_pages) {
-        wr = head_rows <= 32 ? 1 : head_rows <= 64 ? 2 : head_rows <= 128 ? 4 : 8;
-        wk = wr >= 4 ? 1 : 4 / wr;
-        tiles = (head_rows + 32 * wr - 1) / (32 * wr);
+        mode = few ? 0 : head_rows <= 64 ? 1 : 2;
+        if (!few) mode = env("MODE", mode);
+        const int per = 64 * mode;  // rows of a tile
+        tiles = few ? 1 : (head_rows + per - 1) / per;
         const long long base = (long long)kv->kv_heads * tiles;
-        pre = std::min((ctx->num_cu + base - 1) / base, ((long long)prefix_pages * kv->page + 127) / 128);
-        pre = std::max(1LL, std::min(pre, 256LL));
+        pre = std::min((env("PT", few ? 2 : 1) * (long long)ctx->num_cu + base - 1) / base,
+                       ((long long)prefix_pages * kv->page + 127) / 128);
+        pre = std::max(1LL, std::min(pre, 128LL));
     }
     if (pre + own > 1 && pre + own > fit) {  // fewer parts, the prefix's half of them
         if (fit < 2) pre = prefix_pages ? 1 : 0, own = 1;
@@ -1765,26 +1772,20 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     A.own_parts = (int)own;
     A.row_tiles = tiles;
     A.scale2 = scale * 1.44269504088896340736f;
-    void* args[] = {&A};
+    A.prefix_tile = few ? 16 * nb : 32;
+    A.own_tile = 16 * nb;
     char name[64];
     hipFunction_t f;
-    if (pre) {
-        snprintf(name, sizeof name, "cima_attn_paged_prefix_d%d_r%dk%d", dim, wr, wk);
-        if (int rc = get_fn(ctx, name, &f)) return rc;
-        const long long groups = (kv->kv_heads * pre + 7) / 8 * 8;
-        if (int rc = launch(ctx, f, (unsigned)(groups * tiles), 64 * wr * wk, args, api, paged_attn_lds(dim, wr, wk)))
-            return rc;
-    }
-    snprintf(name, sizeof name, "cima_attn_paged_own_d%d_k4", dim);
+    A.prefix_wgs = pre ? (int)((kv->kv_heads * pre + 7) / 8 * 8 * tiles) : 0;
+    snprintf(name, sizeof name, "cima_attn_paged_d%d_m%d_n%d", dim, mode, nb);
     if (int rc = get_fn(ctx, name, &f)) return rc;
-    if (int rc = launch(ctx, f, (unsigned)(own_base * own), 256, args, api, paged_attn_lds(dim, 1, 4))) return rc;
+    void* args[] = {&A};
+    const unsigned lds = std::max(paged_few_lds(dim, nb), mode ? paged_attn_lds(dim, 2 * mode, 2 / mode, 2) : 0u);
+    if (int rc = launch(ctx, f, (unsigned)(A.prefix_wgs + own_base * own), 256, args, api, lds)) return rc;
     if (all == 1) return 0;
-    int n_rows = (int)rows, parts = all;
-    const void *acc = A.acc, *ml = A.ml;
-    void* jargs[] = {&acc, &ml, &out, &n_rows, &parts};
-    const int per = 256 / (dim / 4);
-    return launch_named(ctx, dim == 64 ? "cima_attn_paged_join_d64" : "cima_attn_paged_join_d128",
-                        (unsigned)((rows + per - 1) / per), 256, jargs, api);
+    const long long join = (long long)kv->kv_heads * ((head_rows + 15) / 16) * (dim / 16);
+    return launch_named(ctx, dim == 64 ? "cima_attn_paged_join_d64" : "cima_attn_paged_join_d128", (unsigned)join, 256,
+                        args, api);
 }
 
 int cima_hip_kv_pages_copy(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int* src, const int* dst, int n) {

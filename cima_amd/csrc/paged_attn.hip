@@ -21,9 +21,12 @@
 // of read meets bank conflicts.
 #include "gguf_formats.h"
 
+#include <type_traits>
+
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 typedef short s4 __attribute__((ext_vector_type(4)));
+typedef float f4 __attribute__((ext_vector_type(4)));
 typedef float f16v __attribute__((ext_vector_type(16)));
 typedef float f2 __attribute__((ext_vector_type(2)));
 
@@ -51,6 +54,35 @@ DEV f2 halves(float v) {
     return f2{__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)};
 }
 
+// maximum over the four lanes that hold a row of a 16-row block (lanes 16 apart)
+DEV float quarters_max(float v) {
+    const f2 h = halves(v);
+    const uint32_t x = __builtin_bit_cast(uint32_t, fmaxf(h[0], h[1]));
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const uint32_t a = r[0], b = r[1];
+    return fmaxf(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+DEV float quarters_sum(float v) {
+    const f2 h = halves(v);
+    const uint32_t x = __builtin_bit_cast(uint32_t, h[0] + h[1]);
+    const auto r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    const uint32_t a = r[0], b = r[1];
+    return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
+}
+
+// minimum over aligned groups of 16 lanes
+template <int CTRL>
+DEV int dpp_min(int v) {
+    return min(v, __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, false));
+}
+DEV int min16(int v) {
+    v = dpp_min<0xB1>(v);      // quad_perm [1,0,3,2]
+    v = dpp_min<0x4E>(v);      // quad_perm [2,3,0,1]
+    v = dpp_min<0x141>(v);     // row_half_mirror
+    return dpp_min<0x140>(v);  // row_mirror
+}
+DEV int max16(int v) { return -min16(-v); }
+
 struct AttnArgs {
     const uint16_t* q;
     const uint16_t* kp;  // planes of the layer
@@ -58,11 +90,18 @@ struct AttnArgs {
     const int* table;
     const int* lens;
     uint16_t* out;
-    float* acc;  // [rows * q_heads][parts][D]
-    f2* ml;      // [rows * q_heads][parts]
+    // partial sums, R = seqs * n_new * q_heads / kv_heads rows of a kv head: {m,
+    // l} of (part, kv head, row) at ml[(part * kv_heads + head) * R + row]; the
+    // sums of a tile of rows [r0, r0 + cols) from acc + ((part * kv_heads + head)
+    // * R + r0) * D on, four elements d of all its rows after the other ([D /
+    // 4][cols][4]), which is how the matrix cores leave them
+    float* acc;
+    f2* ml;
     int seqs, n_new, q_heads, kv_heads, page_shift, n_pages, table_stride;
     int prefix_pages, prefix_slot, window;
     int prefix_parts, own_parts, row_tiles;  // row tiles of the prefix tasks
+    int prefix_tile, own_tile;               // their rows, and those of the own tasks
+    int prefix_wgs;                          // workgroups of prefix tasks
     float scale2;                            // scale * log2(e)
 };
 
@@ -73,27 +112,27 @@ constexpr float LOWEST = -1e30f;  // below any score: the running maximum's star
 // the largest, clear of f16's subnormals, and most tiles skip the rescaling.
 constexpr float RAISE = 14.f, ABOVE = 6.f;
 
-template <int D, int WR, int WK>
+template <int D, int WR, int WK, int STAGES>
 struct Tile {
     static constexpr int NW = WR * WK;
-    static constexpr int KB = WK == 1 ? 2 : 1;      // 32-key blocks of a wave
+    static constexpr int KB = WK == 1 && WR > 1 ? 2 : 1;  // 32-key blocks of a wave
     static constexpr int KT = 32 * KB * WK;         // keys of a tile
     static constexpr int BYTES = KT * D * 2;        // of its keys (or values)
-    static constexpr int ST = 2 * BYTES * 3 <= 98304 ? 3 : 2;  // ring of tiles
+    static constexpr int ST = STAGES;               // ring of tiles
     static constexpr int UNITS = 2 * (KT / 16) / NW;  // 16-row copies of a wave
     static constexpr int DPW = UNITS * (D / 32);      // copy instructions of a wave and tile
     static constexpr int RING = ST * 2 * BYTES;
     // the merge of WK waves' sums reuses the ring
-    static_assert((WK - 1) * WR * 64 * (D / 32) * 16 * 4 <= RING, "merge space");
+    static_assert(WK == 1 || (WK - 1) * WR * 64 * (D / 32) * 16 * 4 <= RING, "merge space");
     static constexpr int LDS = RING + IDS * 4 + NW * 32;
 };
 
 // Rows [r0, r0 + 32 WR) of [ra, rb) (row r of a kv head: head r % g, token r /
 // g), positions [plo, phi), part `part` of `parts`, results to column `col`.
-template <int D, int WR, int WK>
+template <int D, int WR, int WK, int STAGES>
 DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int plo, int phi, const int* trow,
                    int part, int parts, int col) {
-    using T = Tile<D, WR, WK>;
+    using T = Tile<D, WR, WK, STAGES>;
     constexpr int ROWB = D * 2, STEPS = D / 16, MT = D / 32, CH = D / 8;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave % WR, wk = wave / WR;
@@ -125,13 +164,15 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     // [lo_all, hi_all)
     int lo_any = live ? lo : 0x7fffffff, hi_any = live ? hi : 0, lo_all = live ? lo : 0, hi_all = live ? hi : 0x7fffffff;
     if (!live) lo = 0, hi = 0x7fffffff;  // masked by its l at the end
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        lo_any = min(lo_any, __shfl_xor(lo_any, o));
-        hi_any = max(hi_any, __shfl_xor(hi_any, o));
-        lo_all = max(lo_all, __shfl_xor(lo_all, o));
-        hi_all = min(hi_all, __shfl_xor(hi_all, o));
-    }
+    lo_any = min16(lo_any), hi_any = max16(hi_any), lo_all = max16(lo_all), hi_all = min16(hi_all);
+    lo_any = min(lo_any, __builtin_amdgcn_readlane(lo_any, 16));
+    hi_any = max(hi_any, __builtin_amdgcn_readlane(hi_any, 16));
+    lo_all = max(lo_all, __builtin_amdgcn_readlane(lo_all, 16));
+    hi_all = min(hi_all, __builtin_amdgcn_readlane(hi_all, 16));
+    lo_any = __builtin_amdgcn_readfirstlane(lo_any);
+    hi_any = __builtin_amdgcn_readfirstlane(hi_any);
+    lo_all = __builtin_amdgcn_readfirstlane(lo_all);
+    hi_all = __builtin_amdgcn_readfirstlane(hi_all);
     if (WR > 1) {
         if (lane == 0) red[8 * wave] = lo_any, red[8 * wave + 1] = hi_any, red[8 * wave + 2] = lo_all, red[8 * wave + 3] = hi_all;
         __syncthreads();
@@ -163,16 +204,17 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     // holds them all; rows that no one sees are replaced by the nearest that
     // someone does, so that what they hold is never multiplied
     const int page = 1 << A.page_shift;
+    auto page_of = [&](int p) { return min(max(p, lo_any), hi_any - 1) >> A.page_shift; };
     int ids_from = -IDS;  // first page of the ids in LDS
     auto fill_ids = [&](int first) {
         // all waves are past their last use of the ids (barrier before)
-        for (int i = threadIdx.x; i < IDS; i += 64 * T::NW) {
-            const int e = min(first + i, A.table_stride - 1);
+        const int n = min(IDS, page_of(base + t1 * T::KT - 1) - first + 1);
+        for (int i = threadIdx.x; i < n; i += 64 * T::NW) {
+            const int e = first + i;
             ids[i] = (int)min((unsigned)max(trow[e], 0), (unsigned)A.n_pages - 1u);
         }
         ids_from = first;
     };
-    auto page_of = [&](int p) { return min(max(p, lo_any), hi_any - 1) >> A.page_shift; };
     auto issue = [&](int t) {
         const uint32_t dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (uint32_t)(t % T::ST) * (2 * T::BYTES);
 #pragma unroll
@@ -205,8 +247,10 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         for (int i = 0; i < T::ST - 1; i++)
             if (t0 + i < t1) issue(t0 + i);
         for (int t = t0; t < t1; t++) {
-            if (t + T::ST - 2 < t1) wait_vm<(T::ST - 2) * T::DPW>();
-            else wait_vm<0>();
+            if (T::ST > 1) {
+                if (t + T::ST - 2 < t1) wait_vm<(T::ST > 1 ? T::ST - 2 : 0) * T::DPW>();
+                else wait_vm<0>();
+            }
             barrier();
             if (t + T::ST - 1 < t1) {
                 if (beyond(t + T::ST - 1)) {
@@ -214,6 +258,10 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
                     __syncthreads();
                 }
                 issue(t + T::ST - 1);
+            }
+            if (T::ST == 1) {
+                wait_vm<0>();
+                barrier();
             }
             const uint8_t* K = lds + (t % T::ST) * (2 * T::BYTES);
             const uint8_t* V = K + T::BYTES;
@@ -360,101 +408,416 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
             }
         return;
     }
-    if (half == 0) A.ml[qrow * all + col] = f2{some ? m : LOWEST, some ? l : 0.f};
+    const int R = A.seqs * A.n_new * g;
+    const size_t at = (size_t)(col * A.kv_heads + kvh) * R;
+    if (half == 0) A.ml[at + r] = f2{some ? m : LOWEST, some ? l : 0.f};
     if (!some) return;
-    float* to = A.acc + (qrow * all + col) * D + 4 * half;
+    const int c0 = r0 + 32 * wr, cols = min(32, rb - c0);
+    float4* to = reinterpret_cast<float4*>(A.acc + (at + c0) * D) + half * cols + (lane & 31);
 #pragma unroll
     for (int x = 0; x < MT; x++)
 #pragma unroll
         for (int i = 0; i < 16; i += 4)
-            *reinterpret_cast<float4*>(to + 32 * x + 2 * i) = make_float4(o[x][i], o[x][i + 1], o[x][i + 2], o[x][i + 3]);
+            to[(8 * x + i / 2) * cols] = make_float4(o[x][i], o[x][i + 1], o[x][i + 2], o[x][i + 3]);
 }
 
-// Prefix tasks.  Workgroups go to the XCDs in turn; the row tiles of one range
-// of one kv head follow each other on the same XCD, so that all but the first
-// find its pages in that XCD's L2.
-template <int D, int WR, int WK>
-DEV void attn_prefix_body(const AttnArgs& A, uint8_t* lds) {
-    const int slot = blockIdx.x >> 3, xcd = blockIdx.x & 7;
-    const int grp = slot / A.row_tiles * 8 + xcd, tile = slot % A.row_tiles;
-    if (grp >= A.kv_heads * A.prefix_parts) return;
-    const int kvh = grp / A.prefix_parts, part = grp % A.prefix_parts;
-    const int rows = A.seqs * A.n_new * (A.q_heads / A.kv_heads);
-    attn_task<D, WR, WK>(A, lds, kvh, tile * 32 * WR, rows, 0, A.prefix_pages << A.page_shift,
-                         A.table + (size_t)A.prefix_slot * A.table_stride, part, A.prefix_parts, part);
+// ------------------------------------------------------------- few rows
+//
+// Tasks of up to 16 NB rows (own tasks; prefix tasks where there are few
+// rows): bound by reading the keys and values, and short ones by the latency
+// of their chain of loads.  The four waves of a workgroup take 32-position
+// tiles in turn and do not wait for each other: keys go straight from memory
+// to the registers of the A operand (16 x 16 x 32 MFMA: a lane holds 16 bytes
+// of a key), values by direct copies to the wave's own LDS, one tile ahead.
+// The waves' sums are added at the end, in wave order.
+template <int D, int NB>
+struct Few {
+    static constexpr int VT = 32 * D * 2;                  // bytes of a tile's values
+    static constexpr int OB = NB * (D / 16) * 64 * 16;     // of a wave's sums
+    static constexpr int WAVE = 2 * VT > OB ? 2 * VT : OB;  // LDS of a wave
+    static constexpr int LDS = 4 * WAVE + 4 * NB * 16 * 8;
+};
+template <int D, int NB>
+DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int plo, int phi, const int* trow, int part,
+                  int parts, int col, int guess) {
+    using F = Few<D, NB>;
+    constexpr int STEPS = D / 32, XT = D / 16, CH = D / 8;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int li = lane & 15, q4 = lane >> 4;
+    const int g = A.q_heads / A.kv_heads;
+    // the ids of the 64 pages that the part most likely begins with, fetched
+    // before the lengths are known; lane i: id of page ids_from + i
+    auto fetch_ids = [&](int first) {
+        const int id = trow[min(first + lane, A.table_stride - 1)];
+        return (int)min((unsigned)max(id, 0), (unsigned)A.n_pages - 1u);
+    };
+    int ids_from = guess, ids = fetch_ids(guess);
+    // ---- this lane's rows
+    bool valid[NB], live[NB];
+    int lo[NB], hi[NB], len[NB], tok[NB];
+    size_t qrow[NB];
+    h8 qf[NB][STEPS];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const int r = r0 + 16 * b + li;
+        valid[b] = r < rb;
+        const int rr = valid[b] ? r : r0, sj = rr / g, s = sj / A.n_new;
+        len[b] = A.lens[s];
+        tok[b] = sj - s * A.n_new;
+        qrow[b] = (size_t)sj * A.q_heads + kvh * g + (rr - sj * g);
+#pragma unroll
+        for (int i = 0; i < STEPS; i++)
+            qf[b][i] = *reinterpret_cast<const h8*>(A.q + qrow[b] * D + 32 * i + 8 * q4);
+    }
+    int lo_any = 0x7fffffff, hi_any = 0, lo_all = 0, hi_all = 0x7fffffff;
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        const int pos = len[b] + tok[b];
+        hi[b] = min(min(pos + 1, phi), A.table_stride << A.page_shift);
+        lo[b] = max(plo, A.window ? pos + 1 - A.window : 0);
+        live[b] = valid[b] && len[b] >= 0 && lo[b] < hi[b];
+        if (live[b]) {
+            lo_any = min(lo_any, lo[b]);
+            hi_any = max(hi_any, hi[b]);
+            lo_all = max(lo_all, lo[b]);
+            hi_all = min(hi_all, hi[b]);
+        } else {
+            lo[b] = 0, hi[b] = 0x7fffffff;  // masked by its l at the end
+        }
+    }
+    lo_any = __builtin_amdgcn_readfirstlane(min16(lo_any));
+    hi_any = __builtin_amdgcn_readfirstlane(max16(hi_any));
+    lo_all = __builtin_amdgcn_readfirstlane(max16(lo_all));
+    hi_all = __builtin_amdgcn_readfirstlane(min16(hi_all));
+    const int base = lo_any & ~15;
+    const int tiles = hi_any > lo_any ? (hi_any - base + 31) / 32 : 0;
+    const int each = (tiles + parts - 1) / parts;
+    const int t0 = min(part * each, tiles), t1 = min(t0 + each, tiles);
+
+    f4 o[NB][XT];
+    float m[NB], l[NB];
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        m[b] = LOWEST, l[b] = 0.f;
+#pragma unroll
+        for (int x = 0; x < XT; x++) o[b][x] = f4{0.f, 0.f, 0.f, 0.f};
+    }
+    // ---- loads of a tile: two groups of 16 positions, each within a page; rows
+    // that no one sees are replaced by the nearest that someone does
+    const int page = 1 << A.page_shift;
+    const uint32_t vbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * F::WAVE;
+    h8 kf[2][2][STEPS];
+    auto issue = [&](int t, auto buf) {
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int p0 = base + 32 * t + 16 * u;
+            const int pg = min(max(p0, lo_any), hi_any - 1) >> A.page_shift;
+            if ((unsigned)(pg - ids_from) >= 64u) {
+                ids = fetch_ids(pg);
+                ids_from = pg;
+            }
+            const int id = __builtin_amdgcn_readlane(ids, pg - ids_from);
+            const size_t off = ((size_t)id * A.kv_heads + kvh) * page * D;
+            const int pk = min(max(p0 + li, lo_any), hi_any - 1) & (page - 1);
+#pragma unroll
+            for (int i = 0; i < STEPS; i++)
+                kf[buf][u][i] = *reinterpret_cast<const h8*>(A.kp + off + (size_t)pk * D + 32 * i + 8 * q4);
+#pragma unroll
+            for (int c = 0; c < D / 32; c++) {
+                const int row = c * (64 / CH) + lane / CH, w = lane % CH;
+                const int p = min(max(p0 + row, lo_any), hi_any - 1) & (page - 1);
+                const int f = D == 128 ? (row & 7) << 1 : (row >> 1 & 3) << 1;
+                dma16(A.vp + off + (size_t)p * D + 8 * (w ^ f), vbase + buf * F::VT + u * 16 * D * 2 + c * 1024);
+            }
+        }
+    };
+    auto step = [&](int t, auto buf) {
+        wait_vm<0>();
+        if (t + 4 < t1) issue(t + 4, std::integral_constant<int, 1 - buf>{});
+        const int p0 = base + 32 * t;
+        h8 pf[NB];
+#pragma unroll
+        for (int b = 0; b < NB; b++) {
+            f4 sc[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                sc[u] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < STEPS; i++)
+                    sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[buf][u][i], qf[b][i], sc[u], 0, 0, 0);
+            }
+            if (p0 < lo_all || p0 + 32 > hi_all) {
+#pragma unroll
+                for (int u = 0; u < 2; u++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int p = p0 + 16 * u + 4 * q4 + i;
+                        sc[u][i] = p >= lo[b] && p < hi[b] ? sc[u][i] : -INFINITY;
+                    }
+            }
+            float mx = sc[0][0];
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) mx = fmaxf(mx, sc[u][i]);
+            mx = quarters_max(mx) * A.scale2;
+            if (__any(mx > m[b] + RAISE)) {
+                const float mn = mx > m[b] + RAISE ? mx - ABOVE : m[b];
+                const float a = __builtin_amdgcn_exp2f(m[b] - mn);
+                l[b] *= a;
+#pragma unroll
+                for (int x = 0; x < XT; x++) o[b][x] *= a;
+                m[b] = mn;
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i += 2) {
+                    const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[u][i], A.scale2, -m[b]));
+                    const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[u][i + 1], A.scale2, -m[b]));
+                    l[b] += e0 + e1;
+                    const h2 v = __builtin_convertvector((f2{e0, e1}), h2);
+                    pf[b][4 * u + i] = v[0];
+                    pf[b][4 * u + i + 1] = v[1];
+                }
+        }
+        typedef __attribute__((address_space(3))) s4* lp;
+        typedef short s8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+        for (int x = 0; x < XT; x++) {
+            s4 vv[2];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int row = 16 * u + 4 * q4 + (li >> 2), w = 2 * x + ((li & 3) >> 1);
+                const int f = D == 128 ? (row & 7) << 1 : (row >> 1 & 3) << 1;
+                vv[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                    (lp)(uintptr_t)(vbase + buf * F::VT + row * D * 2 + (w ^ f) * 16 + (li & 1) * 8));
+            }
+            const s8 vf = __builtin_shufflevector(vv[0], vv[1], 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int b = 0; b < NB; b++)
+                o[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vf), pf[b], o[b][x], 0, 0, 0);
+        }
+        // the next copies into this buffer follow the reads
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    };
+    using B0 = std::integral_constant<int, 0>;
+    using B1 = std::integral_constant<int, 1>;
+    int t = t0 + wave;
+    if (t < t1) {
+        issue(t, B0{});
+        while (true) {
+            step(t, B0{});
+            if ((t += 4) >= t1) break;
+            step(t, B1{});
+            if ((t += 4) >= t1) break;
+        }
+    }
+    // ---- the waves' sums, brought to the largest maximum
+    f2* rm = reinterpret_cast<f2*>(lds + 4 * F::WAVE);
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        l[b] = quarters_sum(l[b]);
+        if (q4 == 0) rm[(wave * NB + b) * 16 + li] = f2{m[b], l[b]};
+    }
+    __syncthreads();
+    float M[NB], L[NB];
+    float4* mine = reinterpret_cast<float4*>(lds + wave * F::WAVE);
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        M[b] = LOWEST, L[b] = 0.f;
+#pragma unroll
+        for (int w = 0; w < 4; w++) M[b] = fmaxf(M[b], rm[(w * NB + b) * 16 + li][0]);
+#pragma unroll
+        for (int w = 0; w < 4; w++) {
+            const f2 v = rm[(w * NB + b) * 16 + li];
+            L[b] += v[1] * __builtin_amdgcn_exp2f(v[0] - M[b]);
+        }
+        const float a = __builtin_amdgcn_exp2f(m[b] - M[b]);
+#pragma unroll
+        for (int x = 0; x < XT; x++) {
+            const f4 v = o[b][x] * a;
+            mine[(b * XT + x) * 64 + lane] = make_float4(v[0], v[1], v[2], v[3]);
+        }
+    }
+    __syncthreads();
+    const int R = A.seqs * A.n_new * g, all = A.prefix_parts + A.own_parts, cols = min(16 * NB, rb - r0);
+    const size_t at = (size_t)(col * A.kv_heads + kvh) * R;
+#pragma unroll
+    for (int b = 0; b < NB; b++) {
+        if (!valid[b]) continue;
+        const bool some = live[b] && t0 < t1;
+        if (all > 1 && wave == 0 && q4 == 0) A.ml[at + r0 + 16 * b + li] = f2{some ? M[b] : LOWEST, some ? L[b] : 0.f};
+        if (all > 1 && !some) continue;
+        const float inv = some && L[b] != 0.f ? 1.f / L[b] : 0.f;
+#pragma unroll
+        for (int y = 0; y < XT / 4; y++) {
+            const int x = wave * (XT / 4) + y;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < 4; w++) {
+                const float4 z = reinterpret_cast<const float4*>(lds + w * F::WAVE)[(b * XT + x) * 64 + lane];
+                v.x += z.x, v.y += z.y, v.z += z.z, v.w += z.w;
+            }
+            if (all > 1) {
+                reinterpret_cast<float4*>(A.acc + (at + r0) * D)[(4 * x + q4) * cols + 16 * b + li] = v;
+            } else {  // nothing to join: the result, rounded once
+                uint2 z = make_uint2(0, 0);
+                if (some) z = make_uint2(f2h2(v.x * inv, v.y * inv), f2h2(v.z * inv, v.w * inv));
+                *reinterpret_cast<uint2*>(A.out + qrow[b] * D + 16 * x + 4 * q4) = z;
+            }
+        }
+    }
 }
-// Own tasks: one slot's rows, 32 at a time.
-template <int D, int WK>
-DEV void attn_own_body(const AttnArgs& A, uint8_t* lds) {
-    const int rows = A.n_new * (A.q_heads / A.kv_heads), tiles = (rows + 31) / 32;
+// One launch: first the prefix tasks (MODE 0: as few-row tasks, where all rows
+// fit one tile; 1 and 2: tiles of 64 and 128 rows), then the own tasks, one
+// slot's rows 16 NB at a time.  Workgroups go to the XCDs in turn; the row tiles
+// of one range of one kv head follow each other on the same XCD, so that all but
+// the first find its pages in that XCD's L2.
+template <int D, int MODE, int NB>
+DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
+    const int rows = A.n_new * (A.q_heads / A.kv_heads);
     int b = blockIdx.x;
+    if (b < A.prefix_wgs) {
+        const int slot = b >> 3, grp = slot / A.row_tiles * 8 + (b & 7), tile = slot % A.row_tiles;
+        if (grp >= A.kv_heads * A.prefix_parts) return;
+        const int kvh = grp / A.prefix_parts, part = grp % A.prefix_parts, phi = A.prefix_pages << A.page_shift;
+        const int* trow = A.table + (size_t)A.prefix_slot * A.table_stride;
+        if (MODE == 0)
+            few_task<D, NB>(A, lds, kvh, 0, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
+                            ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift);
+        else if (MODE == 1) attn_task<D, 2, 2, 2>(A, lds, kvh, tile * 64, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
+        else attn_task<D, 4, 1, 2>(A, lds, kvh, tile * 128, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
+        return;
+    }
+    b -= A.prefix_wgs;
+    const int tiles = (rows + 16 * NB - 1) / (16 * NB);
     const int part = b % A.own_parts;
     b /= A.own_parts;
     const int tile = b % tiles;
     b /= tiles;
     const int kvh = b % A.kv_heads, s = b / A.kv_heads;
-    attn_task<D, 1, WK>(A, lds, kvh, s * rows + tile * 32, (s + 1) * rows, A.prefix_pages << A.page_shift, 0x7fffffff,
-                        A.table + (size_t)s * A.table_stride, part, A.own_parts, A.prefix_parts + part);
+    few_task<D, NB>(A, lds, kvh, s * rows + tile * 16 * NB, (s + 1) * rows, A.prefix_pages << A.page_shift, 0x7fffffff,
+                    A.table + (size_t)s * A.table_stride, part, A.own_parts, A.prefix_parts + part, A.prefix_pages);
 }
-#define ATTN_PREFIX(D, WR, WK)                                                                                       \
-    extern "C" __global__ __launch_bounds__(64 * WR * WK) void cima_attn_paged_prefix_d##D##_r##WR##k##WK(           \
-        const AttnArgs A) {                                                                                          \
+#define ATTN(D, MODE, NB)                                                                                            \
+    extern "C" __global__ __launch_bounds__(256, 2) void cima_attn_paged_d##D##_m##MODE##_n##NB(const AttnArgs A) {  \
         extern __shared__ __align__(1024) uint8_t lds[];                                                             \
-        attn_prefix_body<D, WR, WK>(A, lds);                                                                         \
+        attn_body<D, MODE, NB>(A, lds);                                                                              \
     }
-#define ATTN_OWN(D, WK)                                                                                              \
-    extern "C" __global__ __launch_bounds__(64 * WK) void cima_attn_paged_own_d##D##_k##WK(const AttnArgs A) {       \
-        extern __shared__ __align__(1024) uint8_t lds[];                                                             \
-        attn_own_body<D, WK>(A, lds);                                                                                \
-    }
-#define ATTN_ALL(D)         \
-    ATTN_PREFIX(D, 1, 4)    \
-    ATTN_PREFIX(D, 2, 2)    \
-    ATTN_PREFIX(D, 4, 1)    \
-    ATTN_PREFIX(D, 8, 1)    \
-    ATTN_OWN(D, 4)
+#define ATTN_ALL(D) \
+    ATTN(D, 0, 1)   \
+    ATTN(D, 1, 1)   \
+    ATTN(D, 2, 1)   \
+    ATTN(D, 0, 2)   \
+    ATTN(D, 1, 2)   \
+    ATTN(D, 2, 2)
 ATTN_ALL(64)
 ATTN_ALL(128)
 
 // The parts of a row joined: out = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M)
-// l_c.  D / 4 threads a row, four elements each.  A row without any part (a
-// slot not in use) becomes zeros.
+// l_c.  A workgroup takes 16 rows and 16 elements.  First all parts' {m, l} of
+// the rows are read together and become weights in LDS, and the parts that any
+// of the rows has are listed; then each wave sums every fourth of them, a lane
+// four elements of a row, and the waves' sums are added in wave order.  A row
+// without any part (a slot not in use) becomes zeros.
+constexpr int MAX_PARTS = 192;
 template <int D>
-DEV void attn_join_body(const float* __restrict__ acc, const f2* __restrict__ ml, uint16_t* __restrict__ out, int rows,
-                        int parts) {
-    constexpr int TR = D / 4;
-    const int r = blockIdx.x * (256 / TR) + threadIdx.x / TR, e = threadIdx.x % TR * 4;
-    if (r >= rows) return;
-    const f2* p = ml + (size_t)r * parts;
-    const float* a = acc + (size_t)r * parts * D + e;
+DEV void attn_join_body(const AttnArgs& A) {
+    __shared__ float wt[MAX_PARTS][16], red[16][16];
+    __shared__ int list[MAX_PARTS], count;
+    __shared__ float4 ro[4][64];
+    const int g = A.q_heads / A.kv_heads, rows = A.n_new * g, R = A.seqs * rows, all = A.prefix_parts + A.own_parts;
+    const int t = threadIdx.x, lane = t & 63, wave = t >> 6, li = lane & 15, q4 = lane >> 4;
+    int b = blockIdx.x;
+    const int x = b % (D / 16);
+    b /= D / 16;
+    const int rts = (R + 15) / 16, r = min(b % rts * 16 + li, R - 1), kvh = b / rts;
+    const bool valid = b % rts * 16 + li < R;
+    const size_t step = (size_t)A.kv_heads * R, head = (size_t)kvh * R;
+    // ---- weights: thread (t / 16, row t % 16) takes parts t / 16 + 16 k
+    const f2* ml = A.ml + head + r;
+    f2 v[MAX_PARTS / 16];
     float M = LOWEST;
-    for (int c = 0; c < parts; c++) M = fmaxf(M, p[c][0]);
+#pragma unroll
+    for (int k = 0; k < MAX_PARTS / 16; k++) {
+        v[k] = f2{LOWEST, 0.f};
+        if (t / 16 + 16 * k < all) v[k] = ml[(t / 16 + 16 * k) * step];
+    }
+#pragma unroll
+    for (int k = 0; k < MAX_PARTS / 16; k++) M = fmaxf(M, v[k][0]);
+    red[t / 16][li] = M;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 16; i++) M = fmaxf(M, red[i][li]);
+    __syncthreads();
     float L = 0.f;
+#pragma unroll
+    for (int k = 0; k < MAX_PARTS / 16; k++) {
+        const int c = t / 16 + 16 * k;
+        if (c >= all) break;
+        // a part that saw nothing has not written its sums
+        const float w = v[k][1] == 0.f ? 0.f : __builtin_amdgcn_exp2f(v[k][0] - M);
+        L += v[k][1] * w;
+        wt[c][li] = w;
+    }
+    red[t / 16][li] = L;
+    __syncthreads();
+    if (wave == 0) {
+        int n = 0;
+        for (int c0 = 0; c0 < all; c0 += 64) {
+            bool any = false;
+            if (c0 + lane < all)
+#pragma unroll
+                for (int i = 0; i < 16; i++) any |= wt[c0 + lane][i] != 0.f;
+            const unsigned long long m = __ballot(any);
+            if (any) list[n + __popcll(m & ((1ull << lane) - 1))] = c0 + lane;
+            n += __popcll(m);
+        }
+        if (lane == 0) count = n;
+    }
+    __syncthreads();
+    const int n = count;
+    // where the row's elements 16 x + 4 q4 are in a prefix part and in an own part
+    const int pr0 = r / A.prefix_tile * A.prefix_tile, pc = min(A.prefix_tile, R - pr0);
+    const int s0 = r / rows * rows, or0 = s0 + (r - s0) / A.own_tile * A.own_tile, oc = min(A.own_tile, s0 + rows - or0);
+    const float4* ap = reinterpret_cast<const float4*>(A.acc + (head + pr0) * D) + (4 * x + q4) * pc + (r - pr0);
+    const float4* ao = reinterpret_cast<const float4*>(A.acc + (head + or0) * D) + (4 * x + q4) * oc + (r - or0);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int c = 0; c < parts; c++) {
-        const f2 v = p[c];
-        if (v[1] == 0.f) continue;  // nothing seen there, acc is not written
-        const float w = __builtin_amdgcn_exp2f(v[0] - M);
-        const float4 x = *reinterpret_cast<const float4*>(a + (size_t)c * D);
-        L += v[1] * w;
-        o.x += x.x * w;
-        o.y += x.y * w;
-        o.z += x.z * w;
-        o.w += x.w * w;
+    constexpr int U = 8;
+    for (int k0 = wave; k0 < n; k0 += 4 * U) {
+        float4 z[U];
+        float w[U];
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            const int k = k0 + 4 * u, c = list[min(k, n - 1)];
+            w[u] = k < n ? wt[c][li] : 0.f;
+            z[u] = (c < A.prefix_parts ? ap : ao)[c * step * (D / 4)];
+        }
+#pragma unroll
+        for (int u = 0; u < U; u++) {
+            // what a weight of 0 stands for may hold anything
+            o.x += w[u] != 0.f ? z[u].x * w[u] : 0.f;
+            o.y += w[u] != 0.f ? z[u].y * w[u] : 0.f;
+            o.z += w[u] != 0.f ? z[u].z * w[u] : 0.f;
+            o.w += w[u] != 0.f ? z[u].w * w[u] : 0.f;
+        }
+    }
+    ro[wave][lane] = o;
+    __syncthreads();
+    if (wave || !valid) return;
+    L = 0.f;
+#pragma unroll
+    for (int i = 0; i < 16; i++) L += red[i][li];
+#pragma unroll
+    for (int w = 1; w < 4; w++) {
+        const float4 z = ro[w][lane];
+        o.x += z.x, o.y += z.y, o.z += z.z, o.w += z.w;
     }
     const float inv = L != 0.f ? 1.f / L : 0.f;
-    *reinterpret_cast<uint2*>(out + (size_t)r * D + e) = make_uint2(f2h2(o.x * inv, o.y * inv), f2h2(o.z * inv, o.w * inv));
+    const int sj = r / g;
+    const size_t qrow = (size_t)sj * A.q_heads + kvh * g + (r - sj * g);
+    *reinterpret_cast<uint2*>(A.out + qrow * D + 16 * x + 4 * q4) = make_uint2(f2h2(o.x * inv, o.y * inv), f2h2(o.z * inv, o.w * inv));
 }
-extern "C" __global__ __launch_bounds__(256) void cima_attn_paged_join_d64(const float* __restrict__ acc,
-                                                                           const f2* __restrict__ ml,
-                                                                           uint16_t* __restrict__ out, int rows,
-                                                                           int parts) {
-    attn_join_body<64>(acc, ml, out, rows, parts);
-}
-extern "C" __global__ __launch_bounds__(256) void cima_attn_paged_join_d128(const float* __restrict__ acc,
-                                                                            const f2* __restrict__ ml,
-                                                                            uint16_t* __restrict__ out, int rows,
-                                                                            int parts) {
-    attn_join_body<128>(acc, ml, out, rows, parts);
-}
+extern "C" __global__ __launch_bounds__(256) void cima_attn_paged_join_d64(const AttnArgs A) { attn_join_body<64>(A); }
+extern "C" __global__ __launch_bounds__(256) void cima_attn_paged_join_d128(const AttnArgs A) { attn_join_body<128>(A); }
