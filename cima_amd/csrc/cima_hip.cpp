@@ -1719,25 +1719,24 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     if (least > 1 && fit < least)
         return fail(CIMA_E_INVALID, "%s: a slab of %llu bytes does not hold %d parts of %lld", api, slab_bytes, least,
                     part_bytes);
-    auto env = [](const char* n, int d) { const char* e = getenv(n); return e ? atoi(e) : d; };
     const int own_rows = n_new * g;
     const bool few = prefix_pages && head_rows <= 32;  // the prefix tasks run with the own tasks
     const int nb = std::max(own_rows, few ? head_rows : 0) > 16 ? 2 : 1;
     const int own_tiles = (own_rows + 16 * nb - 1) / (16 * nb);
     const long long own_base = (long long)seqs * kv->kv_heads * own_tiles;
     const long long own_room = (long long)(kv->table_stride - prefix_pages) * kv->page;
-    long long own = std::min((env("OT", 4) * (long long)ctx->num_cu + own_base - 1) / own_base, (own_room + 127) / 128);
+    long long own = std::min((ctx->num_cu + own_base - 1) / own_base, (own_room + 127) / 128);
     own = std::max(1LL, std::min(own, 64LL));
     int tiles = 0, mode = 0;
     long long pre = 0;
     if (prefix_pages) {
         mode = few ? 0 : head_rows <= 64 ? 1 : 2;
-        if (!few) mode = env("MODE", mode);
         const int per = 64 * mode;  // rows of a tile
         tiles = few ? 1 : (head_rows + per - 1) / per;
-        const long long base = (long long)kv->kv_heads * tiles;
-        pre = std::min((env("PT", few ? 2 : 1) * (long long)ctx->num_cu + base - 1) / base,
-                       ((long long)prefix_pages * kv->page + 127) / 128);
+        const long long base = (long long)kv->kv_heads * tiles, len = (long long)prefix_pages * kv->page;
+        pre = std::min((ctx->num_cu + base - 1) / base, (len + 127) / 128);
+        const long long twice = (2LL * ctx->num_cu + base - 1) / base;
+        if (len >= 512 * twice) pre = twice;
         pre = std::max(1LL, std::min(pre, 128LL));
     }
     if (pre + own > 1 && pre + own > fit) {  // fewer parts, the prefix's half of them

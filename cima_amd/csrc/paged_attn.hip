@@ -36,6 +36,11 @@ typedef float f2 __attribute__((ext_vector_type(2)));
 DEV void dma16(const void* g, uint32_t lds) {
     asm volatile("global_load_lds_dwordx4 %0, off" ::"v"(g), "{m0}"(__builtin_amdgcn_readfirstlane(lds)) : "memory");
 }
+// the same with a wave-uniform address and a byte offset per lane
+DEV void dma16(const void* base, uint32_t off, uint32_t lds) {
+    asm volatile("global_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "{m0}"(__builtin_amdgcn_readfirstlane(lds))
+                 : "memory");
+}
 template <int N>
 DEV void wait_vm() {
     asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
@@ -112,16 +117,14 @@ constexpr float LOWEST = -1e30f;  // below any score: the running maximum's star
 // the largest, clear of f16's subnormals, and most tiles skip the rescaling.
 constexpr float RAISE = 14.f, ABOVE = 6.f;
 
-template <int D, int WR, int WK, int STAGES>
+template <int D, int WR, int WK>
 struct Tile {
     static constexpr int NW = WR * WK;
     static constexpr int KB = WK == 1 && WR > 1 ? 2 : 1;  // 32-key blocks of a wave
     static constexpr int KT = 32 * KB * WK;         // keys of a tile
     static constexpr int BYTES = KT * D * 2;        // of its keys (or values)
-    static constexpr int ST = STAGES;               // ring of tiles
-    static constexpr int UNITS = 2 * (KT / 16) / NW;  // 16-row copies of a wave
-    static constexpr int DPW = UNITS * (D / 32);      // copy instructions of a wave and tile
-    static constexpr int RING = ST * 2 * BYTES;
+    static_assert(KT == 16 * NW, "a wave copies 16 rows of keys and of values");
+    static constexpr int RING = 2 * 2 * BYTES;        // two tiles: one being read, one on its way
     // the merge of WK waves' sums reuses the ring
     static_assert(WK == 1 || (WK - 1) * WR * 64 * (D / 32) * 16 * 4 <= RING, "merge space");
     static constexpr int LDS = RING + IDS * 4 + NW * 32;
@@ -129,10 +132,10 @@ struct Tile {
 
 // Rows [r0, r0 + 32 WR) of [ra, rb) (row r of a kv head: head r % g, token r /
 // g), positions [plo, phi), part `part` of `parts`, results to column `col`.
-template <int D, int WR, int WK, int STAGES>
+template <int D, int WR, int WK>
 DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int plo, int phi, const int* trow,
                    int part, int parts, int col) {
-    using T = Tile<D, WR, WK, STAGES>;
+    using T = Tile<D, WR, WK>;
     constexpr int ROWB = D * 2, STEPS = D / 16, MT = D / 32, CH = D / 8;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wr = wave % WR, wk = wave / WR;
@@ -200,8 +203,8 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         for (int i = 0; i < 16; i++) o[m][i] = 0.f;
     float m = LOWEST, l = 0.f;
 
-    // ---- copies: unit u of this wave is 16 rows of keys or values, a page
-    // holds them all; rows that no one sees are replaced by the nearest that
+    // ---- copies: a wave brings 16 rows of a tile's keys and of its values, which
+    // a page holds all; rows that no one sees are replaced by the nearest that
     // someone does, so that what they hold is never multiplied
     const int page = 1 << A.page_shift;
     auto page_of = [&](int p) { return min(max(p, lo_any), hi_any - 1) >> A.page_shift; };
@@ -209,137 +212,204 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     auto fill_ids = [&](int first) {
         // all waves are past their last use of the ids (barrier before)
         const int n = min(IDS, page_of(base + t1 * T::KT - 1) - first + 1);
-        for (int i = threadIdx.x; i < n; i += 64 * T::NW) {
-            const int e = first + i;
-            ids[i] = (int)min((unsigned)max(trow[e], 0), (unsigned)A.n_pages - 1u);
-        }
+        for (int i = threadIdx.x; i < n; i += 64 * T::NW)
+            ids[i] = (int)min((unsigned)max(trow[first + i], 0), (unsigned)A.n_pages - 1u);
         ids_from = first;
     };
-    auto issue = [&](int t) {
-        const uint32_t dst = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + (uint32_t)(t % T::ST) * (2 * T::BYTES);
+    // A copy instruction c takes 1024 bytes of the 16 rows: this lane's row and
+    // 16-byte word of the stored order.  Word w of row r holds the row's word w ^
+    // f(r) -- keys: f = r (D = 64: r / 2), so that 16 rows' reads of one word
+    // spread over the banks; values: f = r % 4 * 4 + r / 4 (D = 64: r / 2 % 2 * 4 +
+    // r / 4), so that four rows' transposing reads of four words do.  c enters by
+    // an exclusive or of constants.
+    const int lrow = lane / CH, lword = lane % CH;
+    const uint32_t kword = (uint32_t)(lword ^ (D == 128 ? lrow : lrow >> 1)) * 16;
+    const uint32_t vword = (uint32_t)(lword ^ (D == 128 ? lrow << 2 : ((lrow >> 1 & 1) << 2 | lrow >> 2))) * 16;
+    constexpr uint32_t KX = 64, VX = D == 128 ? 16 : 32;
+    const size_t page_elems = (size_t)A.kv_heads * page * D;
+    const uint16_t* kplane = A.kp + (size_t)kvh * page * D;
+    const uint16_t* vplane = A.vp + (size_t)kvh * page * D;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * 16 * ROWB;
+    auto id_at = [&](int t) { return ids[page_of(base + t * T::KT + 16 * wave) - ids_from]; };
+    auto issue = [&](int t, int id, const uint16_t* plane, uint32_t word, uint32_t flip, uint32_t ring) {
+        const int p0 = base + t * T::KT + 16 * wave;
+        const uint16_t* src = plane + (size_t)__builtin_amdgcn_readfirstlane(id) * page_elems;
+        const uint32_t dst = lds0 + ring + (uint32_t)(t & 1) * T::BYTES;
+        if (p0 >= lo_any && p0 + 16 <= hi_any) {
+            src += (size_t)(p0 & (page - 1)) * D;
 #pragma unroll
-        for (int u = 0; u < T::UNITS; u++) {
-            const int unit = wave * T::UNITS + u;
-            const bool isv = unit >= T::KT / 16;
-            const int grp = isv ? unit - T::KT / 16 : unit;
-            const int p0 = base + t * T::KT + 16 * grp;
-            const int id = __builtin_amdgcn_readfirstlane(ids[page_of(p0) - ids_from]);
-            const uint16_t* src = (isv ? A.vp : A.kp) + ((size_t)id * A.kv_heads + kvh) * page * D;
+            for (int c = 0; c < D / 32; c++)
+                dma16(src, (((uint32_t)lrow * ROWB + word) ^ c * flip) + c * 1024, dst + c * 1024);
+        } else {
 #pragma unroll
             for (int c = 0; c < D / 32; c++) {
-                const int row = c * (64 / CH) + lane / CH, w = lane % CH;  // row of 16, stored word
-                const int p = min(max(p0 + row, lo_any), hi_any - 1) & (page - 1);
-                int f;
-                if (D == 128) f = isv ? ((row & 3) << 2 | row >> 2) : row;
-                else f = isv ? ((row >> 1 & 1) << 2 | row >> 2) : row >> 1;
-                dma16(src + (size_t)p * D + 8 * (w ^ f), dst + (isv ? T::BYTES : 0) + (uint32_t)(grp * 16 * ROWB + c * 1024));
+                const int p = min(max(p0 + c * (64 / CH) + lrow, lo_any), hi_any - 1) & (page - 1);
+                dma16(src, (uint32_t)p * ROWB + (word ^ c * flip), dst + c * 1024);
             }
         }
     };
+    const int kw = wk * 32 * T::KB;  // this wave's keys of a tile
+    f16v sc[T::KB];
+    f16v zero16;
+#pragma unroll
+    for (int i = 0; i < 16; i++) zero16[i] = 0.f;
+    // fragments of keys and of transposed values: one address a lane each, the
+    // rest enters by an exclusive or and an offset
+    const int gi = lane >> 4, li = lane & 15, krow = lane & 31;
+    const uint32_t lbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds;
+    const uint32_t kread = lbase + (kw + krow) * ROWB + (half ^ (D == 128 ? krow & 15 : krow >> 1 & 7)) * 16;
+    const uint32_t vread = lbase + 2 * T::BYTES + (kw + 4 * half + (li >> 2)) * ROWB + (li & 1) * 8 +
+                           ((2 * (gi & 1) + ((li & 3) >> 1)) ^ ((D == 128 ? li >> 2 : li >> 3) << 2 | half)) * 16;
+    typedef short s8 __attribute__((ext_vector_type(8)));
+    typedef __attribute__((address_space(3))) s4* s4p;
+    typedef const __attribute__((address_space(3))) h8* h8p;
+    auto kfrag = [&](uint32_t at, int i) {
+        return *(h8p)(uintptr_t)((at ^ i / T::KB * 32) + (i % T::KB) * 32 * ROWB);
+    };
+    auto vfrag = [&](uint32_t at, int n) {
+        const int b = n / MT, x = n % MT;
+        const s4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(uintptr_t)((at ^ x * 64) + 16 * b * ROWB));
+        const s4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((s4p)(uintptr_t)((at ^ x * 64 ^ 32) + (16 * b + 8) * ROWB));
+        const s8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+        return __builtin_bit_cast(h8, v);
+    };
+    // the scores of tile t that a row does not see become -inf; the largest left
+    auto mask = [&](int t) {
+        const int p0 = base + t * T::KT;
+        float mx = -INFINITY;
+#pragma unroll
+        for (int b = 0; b < T::KB; b++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int p = p0 + kw + 32 * b + (i & 3) + 8 * (i >> 2) + 4 * half;
+                sc[b][i] = p >= lo && p < hi ? sc[b][i] : -INFINITY;
+                mx = fmaxf(mx, sc[b][i]);
+            }
+        return mx;
+    };
+    auto raise = [&](float mx) {
+        const f2 h = halves(mx);
+        mx = fmaxf(h[0], h[1]) * A.scale2;
+        if (!__any(mx > m + RAISE)) return;
+        const float mn = mx > m + RAISE ? mx - ABOVE : m;
+        const float a = __builtin_amdgcn_exp2f(m - mn);
+        l *= a;
+#pragma unroll
+        for (int x = 0; x < MT; x++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[x][i] *= a;
+        m = mn;
+    };
 
+    // The loop is two tiles deep, so that the exponentials of one tile run beside
+    // the next one's products: the scores of tile t are there when its turn
+    // begins, its values and the keys of tile t + 1 have arrived.
     if (t0 < t1) {
         __syncthreads();
         fill_ids(page_of(base + t0 * T::KT));
         __syncthreads();
-        // first tile whose pages are not in LDS
-        auto beyond = [&](int t) { return page_of(base + (t + 1) * T::KT - 1) - ids_from >= IDS; };
+        int id = id_at(t0);
+        issue(t0, id, kplane, kword, KX, 0);
+        issue(t0, id, vplane, vword, VX, 2 * T::BYTES);
+        if (t0 + 1 < t1) id = id_at(t0 + 1);
+        wait_vm<0>();
+        barrier();
+        if (t0 + 1 < t1) issue(t0 + 1, id, kplane, kword, KX, 0);
+        {
+            const uint32_t kr = kread + (uint32_t)(t0 & 1) * T::BYTES;
 #pragma unroll
-        for (int i = 0; i < T::ST - 1; i++)
-            if (t0 + i < t1) issue(t0 + i);
+            for (int b = 0; b < T::KB; b++) sc[b] = zero16;
+#pragma unroll
+            for (int i = 0; i < T::KB * STEPS; i++) {
+                const int b = i % T::KB;
+                sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kfrag(kr, i), qf[i / T::KB], sc[b], 0, 0, 0);
+            }
+        }
+        raise(mask(t0));
         for (int t = t0; t < t1; t++) {
-            if (T::ST > 1) {
-                if (t + T::ST - 2 < t1) wait_vm<(T::ST > 1 ? T::ST - 2 : 0) * T::DPW>();
-                else wait_vm<0>();
-            }
-            barrier();
-            if (t + T::ST - 1 < t1) {
-                if (beyond(t + T::ST - 1)) {
-                    fill_ids(page_of(base + (t + T::ST - 1) * T::KT));
-                    __syncthreads();
-                }
-                issue(t + T::ST - 1);
-            }
-            if (T::ST == 1) {
+            const bool more = t + 1 < t1;
+            if (t > t0 || more) {
                 wait_vm<0>();
                 barrier();
             }
-            const uint8_t* K = lds + (t % T::ST) * (2 * T::BYTES);
-            const uint8_t* V = K + T::BYTES;
-            const int kw = wk * 32 * T::KB;  // this wave's keys of the tile
-            f16v sc[T::KB];
-#pragma unroll
-            for (int b = 0; b < T::KB; b++) {
-#pragma unroll
-                for (int i = 0; i < 16; i++) sc[b][i] = 0.f;
-                const int row = lane & 31, fk = D == 128 ? row & 15 : row >> 1 & 7;
-                const uint8_t* kr = K + (kw + 32 * b + row) * ROWB;
-#pragma unroll
-                for (int i = 0; i < STEPS; i++) {
-                    const h8 kf = *reinterpret_cast<const h8*>(kr + ((2 * i + half) ^ fk) * 16);
-                    sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf, qf[i], sc[b], 0, 0, 0);
+            if (more) {
+                issue(t + 1, id, vplane, vword, VX, 2 * T::BYTES);
+                if (t + 2 < t1) {
+                    if (page_of(base + (t + 3) * T::KT - 1) - ids_from >= IDS) {
+                        fill_ids(page_of(base + (t + 2) * T::KT));
+                        __syncthreads();
+                    }
+                    id = id_at(t + 2);
+                    issue(t + 2, id, kplane, kword, KX, 0);
                 }
             }
-            const int p0 = base + t * T::KT;
-            if (p0 < lo_all || p0 + T::KT > hi_all) {
-#pragma unroll
-                for (int b = 0; b < T::KB; b++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) {
-                        const int p = p0 + kw + 32 * b + (i & 3) + 8 * (i >> 2) + 4 * half;
-                        sc[b][i] = p >= lo && p < hi ? sc[b][i] : -INFINITY;
-                    }
-            }
-            // ---- running maximum and sum
-            float mx = sc[0][0];
-#pragma unroll
-            for (int b = 0; b < T::KB; b++)
-#pragma unroll
-                for (int i = 0; i < 16; i++) mx = fmaxf(mx, sc[b][i]);
-            const f2 hm = halves(mx);
-            mx = fmaxf(hm[0], hm[1]) * A.scale2;
-            if (__any(mx > m + RAISE)) {
-                const float mn = mx > m + RAISE ? mx - ABOVE : m;
-                const float a = __builtin_amdgcn_exp2f(m - mn);
-                l *= a;
-#pragma unroll
-                for (int x = 0; x < MT; x++)
-#pragma unroll
-                    for (int i = 0; i < 16; i++) o[x][i] *= a;
-                m = mn;
-            }
+            f16v sn[T::KB];
             h8 pf[T::KB * 2];
+            // two weights: elements i, i + 1 of block j / 8
+            auto pair = [&](int j) {
+                const int b = j / 8, i = j % 8 * 2;
+                const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[b][i], A.scale2, -m));
+                const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[b][i + 1], A.scale2, -m));
+                l += e0 + e1;
+                const h2 v = __builtin_convertvector((f2{e0, e1}), h2);
+                pf[2 * b + (i >> 3)][i & 7] = v[0];
+                pf[2 * b + (i >> 3)][(i & 7) + 1] = v[1];
+            };
+            // ---- the next tile's scores beside the first half of the weights
+            // (behind the last tile LDS holds older keys: not used)
+            {
+                constexpr int N = T::KB * STEPS, AHEAD = 4, PAIRS = 4 * T::KB;
+                const uint32_t kr = kread + (uint32_t)((t + 1) & 1) * T::BYTES;
+                h8 kf[AHEAD];
+                auto frag = [&](int i) { return kfrag(kr, i); };
 #pragma unroll
-            for (int b = 0; b < T::KB; b++)
+                for (int i = 0; i < AHEAD; i++) kf[i] = frag(i);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int i = 0; i < 16; i += 2) {
-                    const float e0 = __builtin_amdgcn_exp2f(fmaf(sc[b][i], A.scale2, -m));
-                    const float e1 = __builtin_amdgcn_exp2f(fmaf(sc[b][i + 1], A.scale2, -m));
-                    l += e0 + e1;
-                    const h2 v = __builtin_convertvector((f2{e0, e1}), h2);
-                    pf[2 * b + (i >> 3)][i & 7] = v[0];
-                    pf[2 * b + (i >> 3)][(i & 7) + 1] = v[1];
+                for (int i = 0; i < N; i++) {
+                    const int b = i % T::KB;
+                    if (i < T::KB)
+                        sn[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % AHEAD], qf[i / T::KB], zero16, 0, 0, 0);
+                    else
+                        sn[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kf[i % AHEAD], qf[i / T::KB], sn[b], 0, 0, 0);
+                    if (i + AHEAD < N) kf[i % AHEAD] = frag(i + AHEAD);
+#pragma unroll
+                    for (int j = i * PAIRS / N; j < (i + 1) * PAIRS / N; j++) pair(j);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
-            // ---- O^T += V^T P^T
-            const int gi = lane >> 4, li = lane & 15;
-            typedef __attribute__((address_space(3))) s4* lp;
-            __attribute__((address_space(3))) uint8_t* V3 = (__attribute__((address_space(3))) uint8_t*)V;
+            }
+            // ---- O^T += V^T P^T, beside the other weights and the next tile's
+            // largest score
+            const uint32_t vr = vread + (uint32_t)(t & 1) * T::BYTES;
+            float mx = -INFINITY;
+            {
+                constexpr int N = 2 * T::KB * MT, AHEAD = 2;
+                h8 vf[AHEAD];
 #pragma unroll
-            for (int b = 0; b < 2 * T::KB; b++)
+                for (int i = 0; i < AHEAD; i++) vf[i] = vfrag(vr, i);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int x = 0; x < MT; x++) {
-                    s4 vv[2];
+                for (int i = 0; i < N; i++) {
+                    o[i % MT] = __builtin_amdgcn_mfma_f32_32x32x16_f16(vf[i % AHEAD], pf[i / MT], o[i % MT], 0, 0, 0);
+                    if (i + AHEAD < N) vf[i % AHEAD] = vfrag(vr, i + AHEAD);
+                    if (i < N / 2) {
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const int row = 16 * b + 8 * u + 4 * half + (li >> 2);  // key of the wave's
-                        const int word = 4 * x + 2 * (gi & 1) + ((li & 3) >> 1);
-                        const int f = D == 128 ? ((li >> 2) << 2 | 2 * u + half) : ((li >> 3) << 2 | 2 * u + half);
-                        vv[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lp)(V3 + (kw + row) * ROWB + ((word ^ f) * 16 + (li & 1) * 8)));
+                        for (int j = 0; j < 4 / MT + (4 % MT != 0); j++) pair(4 * T::KB + i * 4 / MT + j);
+                    } else {
+                        constexpr int E = 16 / MT;  // scores looked at beside a product
+#pragma unroll
+                        for (int j = (i - N / 2) * E; j < (i - N / 2 + 1) * E; j++) mx = fmaxf(mx, sn[j / 16][j % 16]);
                     }
-                    typedef short s8 __attribute__((ext_vector_type(8)));
-                    const s8 vf = __builtin_shufflevector(vv[0], vv[1], 0, 1, 2, 3, 4, 5, 6, 7);
-                    o[x] = __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(h8, vf), pf[b], o[x], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+            }
+            if (more) {
+#pragma unroll
+                for (int b = 0; b < T::KB; b++) sc[b] = sn[b];
+                const int p0 = base + (t + 1) * T::KT;
+                if (p0 < lo_all || p0 + T::KT > hi_all) mx = mask(t + 1);
+                raise(mx);
+            }
         }
     }
     const f2 hl = halves(l);
@@ -686,8 +756,8 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
         if (MODE == 0)
             few_task<D, NB>(A, lds, kvh, 0, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
                             ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift);
-        else if (MODE == 1) attn_task<D, 2, 2, 2>(A, lds, kvh, tile * 64, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
-        else attn_task<D, 4, 1, 2>(A, lds, kvh, tile * 128, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
+        else if (MODE == 1) attn_task<D, 2, 2>(A, lds, kvh, tile * 64, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
+        else attn_task<D, 4, 1>(A, lds, kvh, tile * 128, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
         return;
     }
     b -= A.prefix_wgs;
