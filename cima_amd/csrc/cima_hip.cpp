@@ -205,8 +205,12 @@ const char* const kPagedKernels[] = {
     "cima_rope_append_paged_d64", "cima_rope_append_paged_d128", "cima_kv_pages_copy", "cima_kv_pages_reserve",
     "cima_kv_pages_fork", "cima_kv_pages_fork_copy", "cima_kv_pages_free", "cima_kv_pages_compact",
     "cima_kv_pages_compact_move"};
-const char* const kSampleKernels[] = {"cima_softmax_stats_f16", "cima_softmax_stats_f32", "cima_softmax_probs_f16",
-                                      "cima_softmax_probs_f32", "cima_verify_sums", "cima_verify_draw"};
+const char* const kSampleKernels[] = {
+    "cima_softmax_stats_f16", "cima_softmax_stats_f32", "cima_softmax_stats_cap_f16", "cima_softmax_stats_cap_f32",
+    "cima_softmax_probs_f16", "cima_softmax_probs_f32", "cima_softmax_probs_cap_f16", "cima_softmax_probs_cap_f32",
+    "cima_softmax_t256_w2_f16", "cima_softmax_t256_w8_f16", "cima_softmax_t1024_w8_f16", "cima_softmax_t1024_w16_f16",
+    "cima_softmax_t256_w2_f32", "cima_softmax_t256_w8_f32", "cima_softmax_t1024_w8_f32", "cima_softmax_t1024_w16_f32",
+    "cima_verify_sums", "cima_verify_draw"};
 
 std::string default_code_dir() {
     Dl_info info;
@@ -1873,8 +1877,10 @@ int cima_hip_kv_pages_compact(cima_hip_ctx* ctx, const cima_kv_pages* kv, int* r
 // ------------------------------------------------------------------ sampling
 
 namespace {
-// logits of a workgroup (SM_PART) and entries of a part (VF_PART), sample_ops.hip
-const int kSoftmaxPart = 8192, kVerifyPart = 2048;
+// logits of a part (SM_PART), rows from which on the longest that fit a workgroup
+// go to one each, entries that a part is a multiple of (VF_STEP) and most parts
+// of a row: sample_ops.hip
+const int kSoftmaxPart = 8192, kSoftmaxLongRows = 128, kVerifyStep = 2048, kVerifyParts = 64;
 
 // kernel-argument mirror of VfArgs in sample_ops.hip (same member order)
 struct VerifyArgs {
@@ -1882,8 +1888,8 @@ struct VerifyArgs {
     const int *drafts, *counts;
     const float* u;
     int *accepted, *tokens, *lens;
-    void* sums;
-    int n_draft, vocab, parts;
+    void *sums, *state;
+    int n_draft, vocab, parts, part_len;
 };
 }  // namespace
 
@@ -1903,14 +1909,26 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
     if ((long long)rows * parts > 0x7fffffffLL || !slab || !aligned(slab, 8) || slab_bytes < need)
         return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (8 B)", api,
                     slab_bytes, need);
-    void* args[] = {&x, &slab, &n, &temp, &rows_per_temp, &cap, &parts};
     const bool f32 = x_dtype == CIMA_DT_F32;
-    if (int rc = launch_named(ctx, f32 ? "cima_softmax_stats_f32" : "cima_softmax_stats_f16", (unsigned)(rows * parts),
-                              256, args, api))
-        return rc;
+    // whole rows (sample_ops.hip): threads and four-logit words a thread of the
+    // kernels built, shortest first; rows of the longest kind only where there
+    // are enough of them for half the chip
+    static const int shapes[][2] = {{256, 2}, {256, 8}, {1024, 8}, {1024, 16}};
+    for (const auto& sh : shapes)
+        if (cap == 0.f && n <= sh[0] * sh[1] * 4 && (sh[1] < 16 || rows >= kSoftmaxLongRows)) {
+            char name[64];
+            snprintf(name, sizeof name, "cima_softmax_t%d_w%d_%s", sh[0], sh[1], f32 ? "f32" : "f16");
+            void* args[] = {&x, &y, &n, &temp, &rows_per_temp};
+            return launch_named(ctx, name, (unsigned)rows, (unsigned)sh[0], args, api);
+        }
+    char name[64];
+    const char* sfx = cap > 0.f ? (f32 ? "cap_f32" : "cap_f16") : (f32 ? "f32" : "f16");
+    snprintf(name, sizeof name, "cima_softmax_stats_%s", sfx);
+    void* args[] = {&x, &slab, &n, &temp, &rows_per_temp, &cap, &parts};
+    if (int rc = launch_named(ctx, name, (unsigned)(rows * parts), 256, args, api)) return rc;
+    snprintf(name, sizeof name, "cima_softmax_probs_%s", sfx);
     void* pargs[] = {&x, &y, &slab, &n, &temp, &rows_per_temp, &cap, &parts};
-    return launch_named(ctx, f32 ? "cima_softmax_probs_f32" : "cima_softmax_probs_f16", (unsigned)(rows * parts), 256,
-                        pargs, api);
+    return launch_named(ctx, name, (unsigned)(rows * parts), 256, pargs, api);
 }
 
 int cima_hip_verify_drafts(cima_hip_ctx* ctx, const float* p, const float* q, const int* drafts, const int* counts,
@@ -1925,11 +1943,14 @@ int cima_hip_verify_drafts(cima_hip_ctx* ctx, const float* p, const float* q, co
     if (!aligned(p, 4) || !aligned(q, 4) || !aligned(drafts, 4) || !aligned(counts, 4) || !aligned(u, 4) ||
         !aligned(accepted, 4) || !aligned(tokens, 4) || !aligned(lens, 4))
         return fail(CIMA_E_INVALID, "%s: misaligned pointer (4 B)", api);
-    const long long parts = ((long long)vocab + kVerifyPart - 1) / kVerifyPart;
-    if (seqs * parts > 0x7fffffffLL || !slab || !aligned(slab, 8) || slab_bytes < 8ULL * seqs * parts)
+    const unsigned long long need = 8ULL * seqs * (((long long)vocab + kVerifyStep - 1) / kVerifyStep + 1);
+    const long long len = ((vocab + kVerifyParts - 1LL) / kVerifyParts + kVerifyStep - 1) / kVerifyStep * kVerifyStep;
+    const long long parts = (vocab + len - 1) / len;
+    if (seqs * parts > 0x7fffffffLL || !slab || !aligned(slab, 8) || slab_bytes < need)
         return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (8 B)", api,
-                    slab_bytes, 8ULL * seqs * parts);
-    VerifyArgs A{p, q, drafts, counts, u, accepted, tokens, lens, slab, n_draft, vocab, (int)parts};
+                    slab_bytes, need);
+    VerifyArgs A{p, q, drafts, counts, u, accepted, tokens, lens, slab, (double*)slab + seqs * parts, n_draft, vocab,
+                 (int)parts, (int)len};
     void* args[] = {&A};
     if (int rc = launch_named(ctx, "cima_verify_sums", (unsigned)(seqs * parts), 256, args, api)) return rc;
     return launch_named(ctx, "cima_verify_draw", (unsigned)seqs, 256, args, api);

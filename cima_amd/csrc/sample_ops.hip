@@ -5,156 +5,258 @@
 
 // ------------------------------------------------------------------ softmax
 //
-// A row is taken by `parts` workgroups, PART logits each.  The first launch
-// leaves each part's maximum, its place and the sum of e^((f(x) - m) / T); the
-// second joins a row's parts, reads its own logits once more (from the caches)
-// and writes the probabilities.
+// A row's logits are read into registers: the maximum first, then the sum of
+// e^((f(x) - m) / T) = 2^((f(x) - m) log2(e) / T), then the same again times 1 /
+// sum.  Rows up to 65536 logits go to a workgroup each, in one launch.  Longer
+// ones, and few long ones, are split over `parts` workgroups of 8192: the first
+// launch leaves each part's maximum, its place and its sum, the second joins a
+// row's parts, reads its own logits once more and writes the probabilities.
+// Bound by memory: the probabilities go past the caches, which keep the logits
+// for the second reading.  Measured on MI355X, us: 384 rows of 128256 f16 63
+// (393 MB moved, 6.2 TB/s; through the caches 83, a row per workgroup in 32
+// words a thread 73); 256 rows of 60000 in one launch 21, in two 22.5; 64 of
+// 30000 7.3 and 8.6; one row of 151936 3.3 + 4.8.
 
-constexpr int SM_T = 256, SM_V = 8, SM_R = 4;     // threads, logits a word, words a thread
-constexpr int SM_PART = SM_T * SM_V * SM_R;       // logits of a part
 struct SmPart {
     float m, l;
     int at, pad;
 };
 
-// eight logits from element i on (i < n), those behind n as -inf
+// four logits from element i on, those behind n as -inf: a lane's word, so that
+// loads and stores of a wave are contiguous
 template <bool F32>
-DEV void sm_load(const void* __restrict__ x, size_t row, int i, int n, float (&v)[8]) {
-    if (i + 8 <= n) {
-        if (F32) {
-            const float* p = (const float*)x + row + i;
-            uint4 a, b;
-            __builtin_memcpy(&a, __builtin_assume_aligned(p, 4), 16);
-            __builtin_memcpy(&b, __builtin_assume_aligned(p + 4, 4), 16);
-            const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+DEV void sm_load(const void* __restrict__ x, size_t row, int i, int n, uint32_t (&v)[F32 ? 4 : 2]) {
+    if (i + 4 <= n) {
+        if constexpr (F32) __builtin_memcpy(v, __builtin_assume_aligned((const float*)x + row + i, 4), 16);
+        else __builtin_memcpy(v, __builtin_assume_aligned((const uint16_t*)x + row + i, 2), 8);
+    } else if constexpr (F32) {
 #pragma unroll
-            for (int j = 0; j < 8; j++) v[j] = __builtin_bit_cast(float, u[j]);
-        } else {
-            const uint4 a = ld16u((const uint8_t*)((const uint16_t*)x + row + i));
-            const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+        for (int j = 0; j < 4; j++) v[j] = i + j < n ? ((const uint32_t*)x)[row + i + j] : 0xff800000u;
+    } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) v[2 * j] = h2f(u[j] & 0xffffu), v[2 * j + 1] = h2f(u[j] >> 16);
+        for (int j = 0; j < 4; j += 2) {
+            const uint32_t a = i + j < n ? ((const uint16_t*)x)[row + i + j] : 0xfc00u;
+            const uint32_t b = i + j + 1 < n ? ((const uint16_t*)x)[row + i + j + 1] : 0xfc00u;
+            v[j / 2] = a | b << 16;
         }
-        return;
     }
-#pragma unroll
-    for (int j = 0; j < 8; j++)
-        v[j] = i + j >= n ? -INFINITY : F32 ? ((const float*)x)[row + i + j] : h2f(((const uint16_t*)x)[row + i + j]);
 }
-// f(x) of the same eight; those behind n stay -inf
-DEV void sm_cap(float (&v)[8], int i, int n, float cap) {
-    if (cap > 0.f) {
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = i + j < n ? cap * tanhf(v[j] / cap) : v[j];
+template <bool F32>
+DEV float sm_get(const uint32_t (&v)[F32 ? 4 : 2], int j) {
+    if constexpr (F32) {
+        const uint32_t a = v[j];
+        return __builtin_bit_cast(float, a);
+    } else {
+        return h2f(j & 1 ? v[j / 2] >> 16 : v[j / 2] & 0xffffu);
     }
+}
+DEV float uniform(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
 }
 // whether (a, i) ranks before (b, j): larger, or equal and at a lower place
 DEV bool sm_before(float a, int i, float b, int j) { return a > b || (a == b && i < j); }
 
-template <bool F32>
-DEV void sm_stats(const void* __restrict__ x, SmPart* __restrict__ part, int n, const float* __restrict__ temp,
-                  int rows_per_temp, float cap, int parts) {
-    __shared__ float rm[4], rl[4];
-    __shared__ int ra[4];
-    const int row = blockIdx.x / parts, pt = blockIdx.x % parts, t = threadIdx.x;
-    const float T = temp ? temp[row / rows_per_temp] : 1.f;
-    float v[SM_R][8];
+// f of a logit; those behind n stay -inf
+DEV float sm_f(float x, int i, int n, float cap) { return i < n ? cap * tanhf(x / cap) : x; }
+
+// R words a thread of a row by NT threads: the maximum, the first place of it
+// (T <= 0) or the sum (T > 0).  CAP: f is applied when the logits are loaded,
+// which are fp32 from there on.
+template <bool F32, bool CAP, int NT, int R>
+struct SmRow {
+    static constexpr bool W32 = F32 || CAP;
+    uint32_t v[R][W32 ? 4 : 2];
+    int base;
+    float m, l;
+    int at;
+
+    DEV float get(int r, int j) const { return sm_get<W32>(v[r], j); }
+    // keeps the compiler from holding all logits as fp32 from one pass to the next
+    DEV void fresh() {
 #pragma unroll
-    for (int r = 0; r < SM_R; r++) sm_load<F32>(x, (size_t)row * n, pt * SM_PART + (r * SM_T + t) * SM_V, n, v[r]);
-    float m = -INFINITY;
-    int at = 0x7fffffff;
+        for (int r = 0; r < R; r++)
 #pragma unroll
-    for (int r = 0; r < SM_R; r++) {
-        sm_cap(v[r], pt * SM_PART + (r * SM_T + t) * SM_V, n, cap);
+            for (int k = 0; k < (W32 ? 4 : 2); k++) __asm__ volatile("" : "+v"(v[r][k]));
+    }
+    DEV void load(const void* __restrict__ x, size_t row, int first, int n, float cap) {
+        base = first + threadIdx.x * 4;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const int i = pt * SM_PART + (r * SM_T + t) * SM_V + j;
-            if (v[r][j] > m) m = v[r][j], at = i;
+        for (int r = 0; r < R; r++) {
+            if constexpr (CAP) {
+                uint32_t w[F32 ? 4 : 2];
+                const int i = base + r * NT * 4;
+                sm_load<F32>(x, row, i, n, w);
+#pragma unroll
+                for (int j = 0; j < 4; j++) v[r][j] = __builtin_bit_cast(uint32_t, sm_f(sm_get<F32>(w, j), i + j, n, cap));
+            } else {
+                sm_load<F32>(x, row, base + r * NT * 4, n, v[r]);
+            }
         }
     }
-    // a thread's first largest is its lowest place; across threads the place decides
+    DEV void stats(float T) {
+        __shared__ float red[2][NT / 64];
+        __shared__ int place[NT / 64];
+        const int w = threadIdx.x >> 6;
+        m = -INFINITY;
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < 4; j++) m = fmaxf(m, get(r, j));
+        m = wave_max_u(m);
+        if ((threadIdx.x & 63) == 0) red[0][w] = m;
+        __syncthreads();
+#pragma unroll
+        for (int k = 0; k < NT / 64; k++) m = fmaxf(m, red[0][k]);
+        fresh();
+        l = 0.f;
+        at = 0x7fffffff;
+        if (T > 0.f) {
+            const float c = m == -INFINITY ? 0.f : m, s = 1.44269504088896340736f / T;
+#pragma unroll
+            for (int r = 0; r < R; r++) {
+                float p = 0.f;
+#pragma unroll
+                for (int j = 0; j < 4; j++) p += __builtin_amdgcn_exp2f((get(r, j) - c) * s);
+                l += p;
+            }
+            l = wave_sum_u(l);
+            if ((threadIdx.x & 63) == 0) red[1][w] = l;
+        } else {
+            // behind a row or part of -inf alone there is no place to find
+#pragma unroll
+            for (int r = R - 1; r >= 0; r--)
+#pragma unroll
+                for (int j = 3; j >= 0; j--)
+                    if (get(r, j) == m && m != -INFINITY) at = base + r * NT * 4 + j;
+#pragma unroll
+            for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
+            if ((threadIdx.x & 63) == 0) place[w] = at;
+        }
+        __syncthreads();
+        if (T > 0.f) {
+            l = 0.f;
+#pragma unroll
+            for (int k = 0; k < NT / 64; k++) l += red[1][k];
+        } else {
+#pragma unroll
+            for (int k = 0; k < NT / 64; k++) at = min(at, place[k]);
+        }
+        // the same in every lane: out of the vector registers, which the row fills
+        m = uniform(m), l = uniform(l);
+        at = __builtin_amdgcn_readfirstlane(at);
+        fresh();
+    }
+    // the probabilities of a row of maximum M at place A and sum L, by the square
+    // of the half exponent's power: the exponential itself would flush results
+    // below 2^-126
+    DEV void write(float* __restrict__ y, size_t row, int n, float T, float M, int A, float L) const {
+        const bool none = M == -INFINITY && L == 0.f;  // -inf alone
+        const float c = M == -INFINITY ? 0.f : M, inv = none ? 0.f : 1.f / L;
+        const float s = 0.72134752044448170368f / T;
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            const int i = base + r * NT * 4;
+            float p[4];
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float h = __builtin_amdgcn_exp2f((get(r, j) - c) * s);
+                p[j] = T > 0.f ? h * (h * inv) : (i + j == A ? 1.f : 0.f);
+            }
+            float* o = y + row + i;
+            if (i + 4 <= n) {
+                typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+                __builtin_nontemporal_store((f4u){p[0], p[1], p[2], p[3]}, (f4u*)o);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    if (i + j < n) o[j] = p[j];
+            }
+            __builtin_amdgcn_sched_barrier(0);  // a word at a time: the row fills the registers
+        }
+    }
+};
+
+constexpr int SM_T = 256, SM_R = 8;        // threads and words a thread of a part
+constexpr int SM_PART = SM_T * SM_R * 4;   // its logits
+
+// a row's parts joined by every wave: lane i takes parts i, i + 64, ...
+DEV float sm_join(const SmPart* __restrict__ p, int parts, float T, int* at, float* L) {
+    const int lane = threadIdx.x & 63;
+    float m = -INFINITY;
+    int a = 0x7fffffff;
+    for (int i = lane; i < parts; i += 64)
+        if (sm_before(p[i].m, p[i].at, m, a)) m = p[i].m, a = p[i].at;
 #pragma unroll
     for (int o = 32; o; o >>= 1) {
         const float om = __shfl_xor(m, o);
-        const int oa = __shfl_xor(at, o);
-        if (sm_before(om, oa, m, at)) m = om, at = oa;
+        const int oa = __shfl_xor(a, o);
+        if (sm_before(om, oa, m, a)) m = om, a = oa;
     }
-    if ((t & 63) == 0) rm[t >> 6] = m, ra[t >> 6] = at;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 4; w++)
-        if (sm_before(rm[w], ra[w], m, at)) m = rm[w], at = ra[w];
     float l = 0.f;
     if (T > 0.f) {
-        // a part of -inf alone adds nothing
-        const float c = m == -INFINITY ? 0.f : m;
-#pragma unroll
-        for (int r = 0; r < SM_R; r++)
-#pragma unroll
-            for (int j = 0; j < 8; j++) l += expf((v[r][j] - c) / T);
+        const float c = m == -INFINITY ? 0.f : m, s = 1.44269504088896340736f / T;
+        for (int i = lane; i < parts; i += 64)
+            l += p[i].l * (p[i].m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((p[i].m - c) * s));
     }
-    l = wave_sum_u(l);
-    if ((t & 63) == 0) rl[t >> 6] = l;
-    __syncthreads();
-    if (t == 0) part[blockIdx.x] = SmPart{m, (rl[0] + rl[1]) + (rl[2] + rl[3]), at, 0};
+    *L = wave_sum_u(l);
+    *at = a;
+    return m;
 }
-
-template <bool F32>
-DEV void sm_probs(const void* __restrict__ x, float* __restrict__ y, const SmPart* __restrict__ part, int n,
-                  const float* __restrict__ temp, int rows_per_temp, float cap, int parts) {
-    const int row = blockIdx.x / parts, pt = blockIdx.x % parts, t = threadIdx.x;
-    const float T = temp ? temp[row / rows_per_temp] : 1.f;
-    float m = -INFINITY;
-    int at = 0x7fffffff;
-    const SmPart* p = part + (size_t)row * parts;
-    for (int i = 0; i < parts; i++)
-        if (sm_before(p[i].m, p[i].at, m, at)) m = p[i].m, at = p[i].at;
-    const float c = m == -INFINITY ? 0.f : m;
-    float L = 0.f;
-    if (T > 0.f)
-        for (int i = 0; i < parts; i++) L += p[i].l * (p[i].m == -INFINITY ? 1.f : expf((p[i].m - c) / T));
-    const bool none = m == -INFINITY && L == 0.f;
-    const float inv = none ? 0.f : 1.f / L;
-#pragma unroll
-    for (int r = 0; r < SM_R; r++) {
-        const int i = pt * SM_PART + (r * SM_T + t) * SM_V;
-        if (i >= n) break;
-        float v[8];
-        sm_load<F32>(x, (size_t)row * n, i, n, v);
-        sm_cap(v, i, n, cap);
-        float* o = y + (size_t)row * n + i;
-#pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = T > 0.f ? expf((v[j] - c) / T) * inv : (i + j == at ? 1.f : 0.f);
-        if (i + 8 <= n) {
-            __builtin_memcpy(__builtin_assume_aligned(o, 4), v, 32);
-        } else {
-            for (int j = 0; j < 8 && i + j < n; j++) o[j] = v[j];
-        }
-    }
-}
-#define SOFTMAX(NAME, F32)                                                                                             \
+#define SOFTMAX_PARTS(NAME, F32, CAP)                                                                                  \
     extern "C" __global__ __launch_bounds__(SM_T) void cima_softmax_stats_##NAME(                                      \
         const void* __restrict__ x, SmPart* __restrict__ part, int n, const float* __restrict__ temp,                  \
         int rows_per_temp, float cap, int parts) {                                                                     \
-        sm_stats<F32>(x, part, n, temp, rows_per_temp, cap, parts);                                                    \
+        const int row = blockIdx.x / parts, pt = blockIdx.x % parts;                                                   \
+        SmRow<F32, CAP, SM_T, SM_R> R;                                                                                 \
+        R.load(x, (size_t)row * n, pt * SM_PART, n, cap);                                                              \
+        R.stats(temp ? temp[row / rows_per_temp] : 1.f);                                                               \
+        if (threadIdx.x == 0) part[blockIdx.x] = SmPart{R.m, R.l, R.at, 0};                                            \
     }                                                                                                                  \
     extern "C" __global__ __launch_bounds__(SM_T) void cima_softmax_probs_##NAME(                                      \
         const void* __restrict__ x, float* __restrict__ y, const SmPart* __restrict__ part, int n,                     \
         const float* __restrict__ temp, int rows_per_temp, float cap, int parts) {                                     \
-        sm_probs<F32>(x, y, part, n, temp, rows_per_temp, cap, parts);                                                 \
+        const int row = blockIdx.x / parts, pt = blockIdx.x % parts;                                                   \
+        const float T = temp ? temp[row / rows_per_temp] : 1.f;                                                        \
+        SmRow<F32, CAP, SM_T, SM_R> R;                                                                                 \
+        R.load(x, (size_t)row * n, pt * SM_PART, n, cap);                                                              \
+        float L;                                                                                                       \
+        int at;                                                                                                        \
+        const float m = sm_join(part + (size_t)row * parts, parts, T, &at, &L);                                        \
+        R.write(y, (size_t)row * n, n, T, m, at, L);                                                                   \
     }
-SOFTMAX(f16, false)
-SOFTMAX(f32, true)
+#define SOFTMAX_WHOLE(NAME, F32, NT, WORDS)                                                                            \
+    extern "C" __global__ __launch_bounds__(NT) void cima_softmax_t##NT##_w##WORDS##_##NAME(                           \
+        const void* __restrict__ x, float* __restrict__ y, int n, const float* __restrict__ temp, int rows_per_temp) { \
+        const int row = blockIdx.x;                                                                                    \
+        const float T = temp ? temp[row / rows_per_temp] : 1.f;                                                        \
+        SmRow<F32, false, NT, WORDS> R;                                                                                \
+        R.load(x, (size_t)row * n, 0, n, 0.f);                                                                         \
+        R.stats(T);                                                                                                    \
+        R.write(y, (size_t)row * n, n, T, R.m, R.at, R.l);                                                             \
+    }
+SOFTMAX_PARTS(f16, false, false)
+SOFTMAX_PARTS(f32, true, false)
+SOFTMAX_PARTS(cap_f16, false, true)
+SOFTMAX_PARTS(cap_f32, true, true)
+SOFTMAX_WHOLE(f16, false, 256, 2)
+SOFTMAX_WHOLE(f16, false, 256, 8)
+SOFTMAX_WHOLE(f16, false, 1024, 8)
+SOFTMAX_WHOLE(f16, false, 1024, 16)
+SOFTMAX_WHOLE(f32, true, 256, 2)
+SOFTMAX_WHOLE(f32, true, 256, 8)
+SOFTMAX_WHOLE(f32, true, 1024, 8)
+SOFTMAX_WHOLE(f32, true, 1024, 16)
 
 // ------------------------------------------------------------- verification
 //
 // Which drafts are kept needs one probability of p and q a draft; the token
 // that follows needs one row of each.  The first launch sums that row's
-// max(p - q, 0) in parts of VF_PART entries (fp64), the second finds the part
-// that holds u times the whole and looks through it.  Every workgroup works
-// out the kept drafts itself: one round of loads.
+// max(p - q, 0) in at most 64 parts (fp64), the second finds the part that holds
+// u times the whole, a wave's running sum, and looks through it.  Every
+// workgroup of the first works out the kept drafts itself, one round of loads.
+// Bound by reading the two rows, short batches by the chain of loads.
 
-constexpr int VF_T = 256, VF_V = 8, VF_PART = VF_T * VF_V;
+constexpr int VF_T = 256, VF_V = 8, VF_STEP = VF_T * VF_V;
 
 struct VfArgs {
     const float* p;
@@ -166,8 +268,10 @@ struct VfArgs {
     int* tokens;
     int* lens;
     double* sums;  // [seqs][parts]
-    int n_draft, vocab, parts;
+    int* state;    // [seqs]: kept drafts, + KEPT_REFUSED where the next was refused; -1: not in use
+    int n_draft, vocab, parts, part_len;  // at most 64 parts, part_len a multiple of VF_STEP
 };
+constexpr int KEPT_REFUSED = 1 << 30;
 
 // Drafts kept of slot s (-1: the slot is not in use), by the whole wave; the
 // row whose residual is drawn from is p[kept] less q[kept] where `*refused`.
@@ -232,107 +336,120 @@ DEV void vf_load(const VfRow& r, int i, int n, float (&v)[8]) {
         v[j] = v[j] > 0.f && i + j != r.one ? v[j] : 0.f;
     }
 }
-DEV double wave_sum_d(double v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+// v of the lane that a DPP pattern names, 0 where there is none
+template <int CTRL, int ROWS>
+DEV double dpp_d(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)u, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// inclusive running sum over the wave: within rows of 16, then from row to row
+DEV double wave_scan_d(double v) {
+    v += dpp_d<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v += dpp_d<0x112, 0xf>(v);
+    v += dpp_d<0x114, 0xf>(v);
+    v += dpp_d<0x118, 0xf>(v);
+    v += dpp_d<0x142, 0xa>(v);  // row_bcast:15 into rows 1, 3
+    v += dpp_d<0x143, 0xc>(v);  // row_bcast:31 into rows 2, 3
     return v;
 }
+DEV double lane_d(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, lane), hi = __builtin_amdgcn_readlane((uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
 // sum of one part by the workgroup
-DEV double vf_part(const VfRow& r, int part, int n) {
+DEV double vf_part(const VfArgs& A, const VfRow& r, int part) {
     __shared__ double red[4];
-    float v[8];
-    vf_load(r, part * VF_PART + threadIdx.x * VF_V, n, v);
     double s = 0;
+    for (int i = part * A.part_len; i < min((part + 1) * A.part_len, A.vocab); i += VF_STEP) {
+        float v[8];
+        vf_load(r, i + threadIdx.x * VF_V, A.vocab, v);
 #pragma unroll
-    for (int j = 0; j < 8; j++) s += v[j];
-    s = wave_sum_d(s);
+        for (int j = 0; j < 8; j++) s += v[j];
+    }
+    s = wave_scan_d(s);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
+    if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = s;
     __syncthreads();
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
 
 extern "C" __global__ __launch_bounds__(VF_T) void cima_verify_sums(const VfArgs A) {
     const int s = blockIdx.x / A.parts, part = blockIdx.x % A.parts;
-    bool refused;
+    bool refused = false;
     const int kept = vf_kept(A, s, &refused);
+    if (part == 0 && threadIdx.x == 0) A.state[s] = kept < 0 ? -1 : kept + (refused ? KEPT_REFUSED : 0);
     if (kept < 0) return;
-    const double v = vf_part(vf_row(A, s, kept, refused), part, A.vocab);
+    const double v = vf_part(A, vf_row(A, s, kept, refused), part);
     if (threadIdx.x == 0) A.sums[blockIdx.x] = v;
 }
 
 extern "C" __global__ __launch_bounds__(VF_T) void cima_verify_draw(const VfArgs A) {
-    const int s = blockIdx.x, t = threadIdx.x, n = A.vocab;
-    bool refused = false;
-    const int kept = vf_kept(A, s, &refused);
+    const int s = blockIdx.x, t = threadIdx.x, lane = t & 63, w = t >> 6;
+    double* sums = A.sums + (size_t)s * A.parts;
+    const int state = A.state[s];
+    double v = lane < A.parts ? sums[lane] : 0.0;  // a slot not in use has none: not used below
+    const float u = A.u[(size_t)s * (A.n_draft + 1) + A.n_draft];
+    const bool refused = state >= 0 && state & KEPT_REFUSED;
+    const int kept = state < 0 ? -1 : state & (KEPT_REFUSED - 1);
     int* out = A.tokens + (size_t)s * (A.n_draft + 1);
     for (int i = t; i <= A.n_draft; i += VF_T)
         if (i != kept) out[i] = i < kept ? A.drafts[(size_t)s * A.n_draft + i] : -1;
     if (t == 0) A.accepted[s] = max(kept, 0);
     if (kept < 0) return;
     VfRow r = vf_row(A, s, kept, refused);
-    double* sums = A.sums + (size_t)s * A.parts;
-    double whole = 0;
-    for (int i = 0; i < A.parts; i++) whole += sums[i];
+    double x = wave_scan_d(v), whole = lane_d(x, 63);
     if (!(whole > 0) && refused) {  // nothing left of p: from p itself
         r.q = nullptr;
         r.one = -1;
-        whole = 0;
         for (int i = 0; i < A.parts; i++) {
-            const double v = vf_part(r, i, n);
-            if (t == 0) sums[i] = v;
-            whole += v;
+            const double z = vf_part(A, r, i);
+            if (lane == i) v = z;
         }
-        __syncthreads();
+        x = wave_scan_d(v), whole = lane_d(x, 63);
     }
     __shared__ double wsum[4];
     __shared__ int found, last;
     int token = -1;
     if (whole > 0) {
-        const double goal = (double)A.u[(size_t)s * (A.n_draft + 1) + A.n_draft] * whole;
+        const double goal = (double)u * whole;
         // the part that passes the goal, else the last that holds anything
-        double before = 0, run = 0;
-        int part = 0;
-        for (int i = 0; i < A.parts; i++) {
-            const double v = sums[i];
-            if (v > 0) {
-                part = i;
-                before = run;
-            }
-            run += v;
-            if (run > goal) break;
-        }
-        float v[8];
-        vf_load(r, part * VF_PART + t * VF_V, n, v);
-        double mine = 0;
-#pragma unroll
-        for (int j = 0; j < 8; j++) mine += v[j];
-        double x = mine;
-        const int lane = t & 63, w = t >> 6;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double y = __shfl_up(x, o);
-            if (lane >= o) x += y;
-        }
+        const unsigned long long some = __ballot(v > 0), past = __ballot(v > 0 && x > goal);
+        const int part = past ? __ffsll(past) - 1 : 63 - __clzll(some);
+        double before = lane_d(x, part) - lane_d(v, part);
         if (t == 0) found = 0x7fffffff, last = -1;
-        if (lane == 63) wsum[w] = x;
-        __syncthreads();
-        double run2 = before;
-        for (int i = 0; i < w; i++) run2 += wsum[i];
-        run2 += x - mine;
-        int hit = 0x7fffffff, end = -1;
+        for (int i0 = part * A.part_len; i0 < min((part + 1) * A.part_len, A.vocab); i0 += VF_STEP) {
+            float p[8];
+            vf_load(r, i0 + t * VF_V, A.vocab, p);
+            double mine = 0;
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-            run2 += v[j];
-            const int i = part * VF_PART + t * VF_V + j;
-            if (v[j] > 0.f) {
-                end = i;
-                if (run2 > goal && hit == 0x7fffffff) hit = i;
+            for (int j = 0; j < 8; j++) mine += p[j];
+            const double y = wave_scan_d(mine);
+            __syncthreads();
+            if (lane == 63) wsum[w] = y;
+            __syncthreads();
+            double run = before;
+            for (int i = 0; i < w; i++) run += wsum[i];
+            run += y - mine;
+            int hit = 0x7fffffff, end = -1;
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                run += p[j];
+                if (p[j] > 0.f) {
+                    end = i0 + t * VF_V + j;
+                    if (run > goal && hit == 0x7fffffff) hit = end;
+                }
             }
+            // a wave's entries follow its lanes
+            const unsigned long long hits = __ballot(hit != 0x7fffffff), ends = __ballot(end >= 0);
+            if (hits && lane == __ffsll(hits) - 1) atomicMin(&found, hit);
+            if (ends && lane == 63 - __clzll(ends)) atomicMax(&last, end);
+            __syncthreads();
+            if (found != 0x7fffffff) break;
+            before += (wsum[0] + wsum[1]) + (wsum[2] + wsum[3]);
         }
-        if (hit != 0x7fffffff) atomicMin(&found, hit);
-        if (end >= 0) atomicMax(&last, end);
-        __syncthreads();
         token = found != 0x7fffffff ? found : last;
     }
     if (t == 0) {

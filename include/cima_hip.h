@@ -518,8 +518,8 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
  * nothing, -1).  tokens [seqs, n_draft + 1] = the kept drafts, the drawn token,
  * then -1; accepted[s] = drafts kept.  lens (may be NULL): lens[s] += accepted
  * + 1 where lens[s] >= 0; slots with lens[s] < 0 get accepted 0 and tokens -1.
- * n_draft 0 draws one token a row.  slab (8-byte aligned): 8 bytes for each
- * 2048 entries of vocab (rounded up) and slot. */
+ * n_draft 0 draws one token a row.  slab (8-byte aligned): for each slot 8
+ * bytes, and 8 for each 2048 entries of vocab (rounded up). */
 int cima_hip_verify_drafts(cima_hip_ctx* ctx, const float* p, const float* q, const int* drafts, const int* counts,
                            const float* u, int* accepted, int* tokens, int* lens, int seqs, int n_draft, int vocab,
                            void* slab, unsigned long long slab_bytes);
