@@ -1618,11 +1618,12 @@ int kv_check(cima_hip_ctx* ctx, const cima_kv_pages* kv, const char* api) {
     if (kv->n_planes <= 0 || kv->n_planes % 2 || kv->n_pages <= 0 || kv->n_pages > kMaxPages || kv->kv_heads <= 0 ||
         !pow2 || kv->page < 16 || kv->page > 256 || !attn_dim_ok(kv->head_dim) || kv->max_seqs <= 0 ||
         kv->max_seqs > kMaxSlots || kv->table_stride <= 0 || (long long)kv->table_stride * kv->page > 0x40000000LL ||
-        (long long)kv->kv_heads * kv->page * kv->head_dim > 0x10000000LL)
+        (long long)kv->kv_heads * kv->page * kv->head_dim > 0x10000000LL ||
+        (long long)kv->max_seqs * kv->table_stride > 0x7fffffffLL)
         return fail(CIMA_E_INVALID,
                     "%s: n_planes=%d n_pages=%d kv_heads=%d page=%d head_dim=%d max_seqs=%d table_stride=%d (planes in "
                     "pairs, at most %d pages and %d slots, page a power of two from 16 to 256, head_dim 64 or 128, at "
-                    "most 2^30 positions a slot)",
+                    "most 2^30 positions a slot and 2^31 - 1 table entries)",
                     api, kv->n_planes, kv->n_pages, kv->kv_heads, kv->page, kv->head_dim, kv->max_seqs,
                     kv->table_stride, kMaxPages, kMaxSlots);
     if (kv->plane_elems % 8 ||
@@ -1643,9 +1644,9 @@ int kv_layer(const cima_kv_pages* kv, int layer, const char* api) {
 // (paged_ops.hip)
 long long page_words(const cima_kv_pages* kv) { return (long long)kv->kv_heads * kv->page * kv->head_dim / 8; }
 int page_pieces(const cima_kv_pages* kv) { return (int)((page_words(kv) + 1023) / 1024); }
-// workgroups of the page copies: a piece each, at most eight to a CU
+// workgroups of the page copies: a piece each, up to 128 to a CU
 unsigned copy_grid(const cima_hip_ctx* ctx, long long units) {
-    return (unsigned)std::max(1LL, std::min(units, 8LL * ctx->num_cu));
+    return (unsigned)std::max(1LL, std::min(units, 128LL * ctx->num_cu));
 }
 
 // kernel-argument mirror of AttnArgs in paged_attn.hip (same member order)

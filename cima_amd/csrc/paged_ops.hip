@@ -82,35 +82,37 @@ ROPE_APPEND(128)
 
 // -------------------------------------------------------------- page copies
 
-// The copies go in pieces of 16 KB (256 threads, four 16-byte words each): a
-// piece is enough loads in flight for a CU and small enough that a few pages
-// spread over the chip.
+// The copies go in pieces of 16 KB (256 threads, four 16-byte words each), a
+// workgroup a piece as far as the grid goes, past the caches both ways: what is
+// moved once is not read soon.  Measured on MI355X, 52 pages in 32 planes (220
+// MB): 92 us, 4.8 TB/s read and written, as fast as a large copy; through the
+// caches 107, eight words a thread 93, eight workgroups to a CU 99.
 constexpr int PIECE = 1024;  // 16-byte words of a piece
+typedef uint32_t word4 __attribute__((ext_vector_type(4)));
 
-DEV void copy_piece(const uint4* __restrict__ src, uint4* __restrict__ dst, long long words, long long first) {
-    uint4 v[4];
+DEV void copy_piece(const word4* __restrict__ src, word4* __restrict__ dst, long long words, long long first) {
+    word4 v[4];
     const long long i = first + threadIdx.x;
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-        v[j] = src[min(i + 256 * j, words - 1)];
+    for (int j = 0; j < 4; j++) v[j] = __builtin_nontemporal_load(&src[min(i + 256 * j, words - 1)]);
 #pragma unroll
     for (int j = 0; j < 4; j++)
-        if (i + 256 * j < words) dst[i + 256 * j] = v[j];
+        if (i + 256 * j < words) __builtin_nontemporal_store(v[j], &dst[i + 256 * j]);
 }
 
 // Unit u of `pages` pages in n_planes planes: (plane, page pair, piece).
-DEV void copy_unit(uint4* pool, long long plane_words, long long page_words, int pieces, int pages, long long u,
+DEV void copy_unit(word4* pool, long long plane_words, long long page_words, int pieces, int pages, long long u,
                    const int* __restrict__ src, const int* __restrict__ dst, int n_pages) {
     const int piece = (int)(u % pieces);
     const long long v = u / pieces;
     const int k = (int)(v % pages);
     const int a = src[k], b = dst[k];
     if ((unsigned)a >= (unsigned)n_pages || (unsigned)b >= (unsigned)n_pages || a == b) return;
-    uint4* plane = pool + (v / pages) * plane_words;
+    word4* plane = pool + (v / pages) * plane_words;
     copy_piece(plane + a * page_words, plane + b * page_words, page_words, (long long)piece * PIECE);
 }
 
-extern "C" __global__ __launch_bounds__(256) void cima_kv_pages_copy(uint4* pool, long long plane_words,
+extern "C" __global__ __launch_bounds__(256) void cima_kv_pages_copy(word4* pool, long long plane_words,
                                                                      long long page_words, int pieces, int n,
                                                                      long long units, const int* __restrict__ src,
                                                                      const int* __restrict__ dst, int n_pages) {
@@ -128,63 +130,64 @@ constexpr int CH = 1024;         // pages of a chunk
 constexpr int MAX_CHUNKS = 1024;  // n_pages <= 1048576
 constexpr int MAX_SLOTS = 4096;
 
+template <int CTRL, int ROWS>
+DEV int dpp_i(int v) {
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+// inclusive running sum within rows of 16 lanes, and over the wave
+DEV int row_scan(int v) {
+    v += dpp_i<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v += dpp_i<0x112, 0xf>(v);
+    v += dpp_i<0x114, 0xf>(v);
+    return v + dpp_i<0x118, 0xf>(v);
+}
+DEV int wave_scan(int v) {
+    v = row_scan(v);
+    v += dpp_i<0x142, 0xa>(v);         // row_bcast:15 into rows 1, 3
+    return v + dpp_i<0x143, 0xc>(v);   // row_bcast:31 into rows 2, 3
+}
 // Exclusive prefix sum of v over the 1024 threads of the workgroup, the whole
 // in *total.
 DEV int block_scan(int v, int* total) {
-    __shared__ int part[17];
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
+    __shared__ int part[16];
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int x = wave_scan(v);
     __syncthreads();
     if (lane == 63) part[w] = x;
     __syncthreads();
-    if (threadIdx.x == 0) {
-        int s = 0;
-        for (int i = 0; i < 16; i++) {
-            const int c = part[i];
-            part[i] = s;
-            s += c;
-        }
-        part[16] = s;
-    }
-    __syncthreads();
-    *total = part[16];
-    return part[w] + x - v;
+    const int p = row_scan(part[lane & 15]);
+    *total = __builtin_amdgcn_readlane(p, 15);
+    return (w ? __builtin_amdgcn_readlane(p, w - 1) : 0) + x - v;
 }
 
-// bit i of the result: page first + i (i < 16, first = 16-page run of this
-// lane) exists and is free (FREE) or held
+// bit i of the result: page first + 64 i + lane of a chunk exists and is free
+// (FREE) or held
 template <bool FREE>
-DEV uint32_t run_bits(const int* refs, int n_pages, int first) {
+DEV uint32_t chunk_bits(const int* refs, int n_pages, int first) {
+    const int lane = threadIdx.x & 63;
+    int r[16];
+#pragma unroll
+    for (int i = 0; i < 16; i++) r[i] = refs[min(first + 64 * i + lane, n_pages - 1)];
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 16; i++)
-        if (first + i < n_pages && (refs[first + i] == 0) == FREE) m |= 1u << i;
+        if (first + 64 * i + lane < n_pages && (r[i] == 0) == FREE) m |= 1u << i;
     return m;
 }
-DEV int lane_scan(int v, int* total) {
-    const int lane = threadIdx.x & 63;
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const int y = __shfl_up(x, o);
-        if (lane >= o) x += y;
-    }
-    *total = __shfl(x, 63);
-    return x - v;
-}
-// sum[c] = pages of the kind in chunks before c; returns how many there are
+DEV int below_lane(unsigned long long m) { return __popcll(m & ((1ull << (threadIdx.x & 63)) - 1)); }
+// sum[c] = pages of the kind in chunks before c; returns how many there are.
+// *bits: those of this wave's first chunk, for each_lowest
 template <bool FREE>
-DEV int count_chunks(const int* refs, int n_pages, int* sum) {
-    const int chunks = (n_pages + CH - 1) / CH, lane = threadIdx.x & 63;
-    for (int c = threadIdx.x >> 6; c < chunks; c += 16) {
-        int n;
-        lane_scan(__popc(run_bits<FREE>(refs, n_pages, c * CH + 16 * lane)), &n);
-        if (lane == 0) sum[c] = n;
+DEV int count_chunks(const int* refs, int n_pages, int* sum, uint32_t* bits) {
+    const int chunks = (n_pages + CH - 1) / CH, w = threadIdx.x >> 6;
+    *bits = 0;
+    for (int c = w; c < chunks; c += 16) {
+        const uint32_t b = chunk_bits<FREE>(refs, n_pages, c * CH);
+        if (c == w) *bits = b;
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < 16; i++) n += __popcll(__ballot(b >> i & 1));
+        if ((threadIdx.x & 63) == 0) sum[c] = n;
     }
     __syncthreads();
     const int mine = (int)threadIdx.x < chunks ? sum[threadIdx.x] : 0;
@@ -196,65 +199,76 @@ DEV int count_chunks(const int* refs, int n_pages, int* sum) {
 }
 // emit(rank, page) for the `need` lowest pages of the kind
 template <bool FREE, typename F>
-DEV void each_lowest(const int* refs, int n_pages, const int* sum, int need, F emit) {
-    const int chunks = (n_pages + CH - 1) / CH, lane = threadIdx.x & 63;
-    for (int c = threadIdx.x >> 6; c < chunks && sum[c] < need; c += 16) {
-        const int first = c * CH + 16 * lane;
-        uint32_t m = run_bits<FREE>(refs, n_pages, first);
-        int n, rank = lane_scan(__popc(m), &n) + sum[c];
-        for (; m && rank < need; rank++) {
-            const int i = __ffs(m) - 1;
-            m &= m - 1;
-            emit(rank, first + i);
+DEV void each_lowest(const int* refs, int n_pages, const int* sum, uint32_t bits, int need, F emit) {
+    const int chunks = (n_pages + CH - 1) / CH, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    for (int c = w; c < chunks && sum[c] < need; c += 16) {
+        const uint32_t m = c == w ? bits : chunk_bits<FREE>(refs, n_pages, c * CH);
+        int rank = sum[c];
+        for (int i = 0; i < 16 && rank < need; i++) {
+            const unsigned long long b = __ballot(m >> i & 1);
+            const int mine = rank + below_lane(b);
+            if ((m >> i & 1) && mine < need) emit(mine, c * CH + 64 * i + lane);
+            rank += __popcll(b);
         }
     }
 }
 
 // Room for n_new tokens in slots [0, seqs): slot s lacks the entries from its
-// first -1 in [lens / page, end) on, found by bisection (entries are filled
-// from the left).  The page of rank r goes to the slot whose running sum holds
-// r.
+// first -1 in [lens / page, end) on (entries are filled from the left).  The
+// page of rank r goes to the slot whose running sum holds r.  Bound by the
+// latency of its loads: the counts are read beside the lengths.
 extern "C" __global__ __launch_bounds__(1024) void cima_kv_pages_reserve(int* refs, int n_pages, int* table,
                                                                          const int* lens, int seqs, int table_stride,
                                                                          int page_shift, int n_new, int* status) {
-    __shared__ int sum[MAX_CHUNKS], base[MAX_SLOTS + 1], from[MAX_SLOTS];
-    const int t = threadIdx.x;
-    int need = 0, behind = 0;  // pages wanted by the slots so far; entries behind the rows
+    __shared__ int sum[MAX_CHUNKS], base[MAX_SLOTS + 1], from[MAX_SLOTS], behind;
+    const int t = threadIdx.x, page = 1 << page_shift;
+    if (t == 0) behind = 0;
+    int len = t < seqs ? lens[t] : -1;
+    uint32_t bits;
+    const int have = count_chunks<true>(refs, n_pages, sum, &bits);
+    int need = 0;  // pages wanted by the slots so far
     for (int s0 = 0; s0 < seqs; s0 += 1024) {
         const int s = s0 + t;
-        int lack = 0, first = 0, off = 0;
-        if (s < seqs && lens[s] >= 0) {
-            const int page = 1 << page_shift, len = lens[s];
+        if (s0) len = s < seqs ? lens[s] : -1;
+        int lack = 0, lo = 0;
+        if (len >= 0) {
             const int* row = table + (size_t)s * table_stride;
-            int lo = len >> page_shift, end = (int)(((long long)len + n_new + page - 1) >> page_shift);
-            off = max(0, end - max(lo, table_stride));
+            lo = len >> page_shift;
+            int end = (int)(((long long)len + n_new + page - 1) >> page_shift);
+            const int off = end - max(lo, table_stride);  // entries behind the row
+            if (off > 0) atomicAdd(&behind, off);
             end = min(end, table_stride);
             int hi = max(end, lo);
-            while (lo < hi) {
-                const int mid = (lo + hi) >> 1;
-                if (row[mid] < 0) hi = mid;
-                else lo = mid + 1;
+            if (hi - lo <= 4) {  // a few entries: looked at together
+                int e[4];
+#pragma unroll
+                for (int i = 0; i < 4; i++) e[i] = lo + i < hi ? row[lo + i] : -1;
+#pragma unroll
+                for (int i = 3; i >= 0; i--)
+                    if (e[i] < 0) hi = min(hi, lo + i);
+                lo = hi;
+            } else {
+                while (lo < hi) {
+                    const int mid = (lo + hi) >> 1;
+                    if (row[mid] < 0) hi = mid;
+                    else lo = mid + 1;
+                }
             }
-            first = lo;
             lack = max(0, end - lo);
         }
-        int n, m;
+        int n;
         const int before = block_scan(lack, &n);
-        block_scan(off, &m);
         if (s < seqs) {
             base[s] = need + before;
-            from[s] = first;
+            from[s] = lo;
         }
         need += n;
-        behind += m;
-        __syncthreads();
     }
-    if (t == 0) base[seqs] = need;
-    const int have = count_chunks<true>(refs, n_pages, sum);
+    __syncthreads();
     const int missing = max(0, need - have) + behind;
     if (t == 0) *status = missing;
-    if (missing) return;
-    each_lowest<true>(refs, n_pages, sum, need, [&](int rank, int id) {
+    if (missing || need == 0) return;
+    each_lowest<true>(refs, n_pages, sum, bits, need, [&](int rank, int id) {
         int lo = 0, hi = seqs - 1;  // the last slot whose base is at most rank
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
@@ -274,44 +288,51 @@ extern "C" __global__ __launch_bounds__(1024) void cima_kv_pages_fork(int* refs,
                                                                       const int* __restrict__ parents,
                                                                       const int* __restrict__ children, int n,
                                                                       int* status) {
-    __shared__ int sum[MAX_CHUNKS], who[MAX_SLOTS];
+    __shared__ int sum[MAX_CHUNKS], entry[MAX_SLOTS], wrong;
+    constexpr int K = MAX_SLOTS / 1024;
     const int t = threadIdx.x, page = 1 << page_shift;
-    int need = 0, bad = 0;
-    for (int i0 = 0; i0 < n; i0 += 1024) {
-        const int i = i0 + t;
-        int part = 0, wrong = 0;
+    int p[K], c[K], len[K];
+    bool mine[K];
+    if (t == 0) wrong = 0;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        const int i = t + 1024 * k;
+        p[k] = i < n ? parents[i] : 0;
+        c[k] = i < n ? children[i] : -1;
+    }
+    uint32_t bits;
+    const int have = count_chunks<true>(refs, n_pages, sum, &bits);
+    int need = 0;
+#pragma unroll
+    for (int k = 0; k < K; k++) {
+        mine[k] = false;
+        if (1024 * k >= n) continue;
+        const int i = t + 1024 * k;
         if (i < n) {
-            const int p = parents[i], c = children[i];
-            wrong = (unsigned)p >= (unsigned)max_seqs || (unsigned)c >= (unsigned)max_seqs;
-            if (!wrong) {
-                const int len = lens[p];
-                wrong = len < 0 || (len + page - 1) >> page_shift > table_stride ||
-                        atomicCAS(&lens[c], -1, -2 - i) != -1;
-                part = !wrong && (len & (page - 1));
+            bool ok = (unsigned)p[k] < (unsigned)max_seqs && (unsigned)c[k] < (unsigned)max_seqs;
+            if (ok) {
+                len[k] = lens[p[k]];
+                ok = len[k] >= 0 && (len[k] + page - 1) >> page_shift <= table_stride;
+                if (ok) ok = mine[k] = atomicCAS(&lens[c[k]], -1, -2 - i) == -1;
             }
+            if (!ok) wrong = 1;
         }
-        int m, w;
+        int m;
+        const int part = mine[k] && len[k] & (page - 1);
         const int before = block_scan(part, &m);
-        block_scan(wrong, &w);
-        if (part) who[need + before] = i;
+        if (part) entry[need + before] = c[k] * table_stride + (len[k] >> page_shift);
         need += m;
-        bad += w;
     }
-    const int have = count_chunks<true>(refs, n_pages, sum);
+    __syncthreads();
     const int missing = max(0, need - have);
-    if (t == 0) *status = bad ? -1 : missing;
-    const bool fine = !bad && !missing;
-    for (int i = t; i < n; i += 1024) {
-        const int p = parents[i], c = children[i];
-        if ((unsigned)p >= (unsigned)max_seqs || (unsigned)c >= (unsigned)max_seqs) continue;
-        // the claims were made in L2, past what this CU's cache may hold
-        if (__hip_atomic_load(&lens[c], __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT) == -2 - i)
-            lens[c] = fine ? lens[p] : -1;
-    }
-    if (!fine) return;
-    each_lowest<true>(refs, n_pages, sum, need, [&](int rank, int id) {
-        const int i = who[rank];
-        table[(size_t)children[i] * table_stride + (lens[parents[i]] >> page_shift)] = id;
+    const bool fine = !wrong && !missing;
+    if (t == 0) *status = wrong ? -1 : missing;
+#pragma unroll
+    for (int k = 0; k < K; k++)
+        if (mine[k]) lens[c[k]] = fine ? len[k] : -1;
+    if (!fine || need == 0) return;
+    each_lowest<true>(refs, n_pages, sum, bits, need, [&](int rank, int id) {
+        table[entry[rank]] = id;
         refs[id] = 1;
     });
 }
@@ -379,18 +400,20 @@ extern "C" __global__ __launch_bounds__(1024) void cima_kv_pages_compact(const i
     int* src = work + 16;
     int* dst = src + n_pages;
     int* remap = dst + n_pages;
-    const int live = count_chunks<false>(refs, n_pages, held), lane = threadIdx.x & 63;
+    uint32_t bits;
+    const int live = count_chunks<false>(refs, n_pages, held, &bits), lane = threadIdx.x & 63;
     const int chunks = (n_pages + CH - 1) / CH;
     // ranks: of a held page among the held, of a free one among the free
     auto each = [&](auto f) {
         for (int c = threadIdx.x >> 6; c < chunks; c += 16) {
-            const int first = c * CH + 16 * lane;
-            const uint32_t m = run_bits<false>(refs, n_pages, first);
-            int n, rank = lane_scan(__popc(m), &n) + held[c];
-            for (int i = 0; i < 16 && first + i < n_pages; i++) {
+            const uint32_t m = chunk_bits<false>(refs, n_pages, c * CH);
+            int rank = held[c];
+            for (int i = 0; i < 16; i++) {
+                const unsigned long long b = __ballot(m >> i & 1);
+                const int p = c * CH + 64 * i + lane, r = rank + below_lane(b);
                 const bool h = m >> i & 1;
-                f(first + i, h, h ? rank : first + i - rank);
-                rank += h;
+                if (p < n_pages) f(p, h, h ? r : p - r);
+                rank += __popcll(b);
             }
         }
     };
@@ -428,7 +451,7 @@ extern "C" __global__ __launch_bounds__(1024) void cima_kv_pages_compact(const i
 // Compaction, second launch: the pages are moved and the table's entries
 // renamed; entries of pages that are not held stay.
 extern "C" __global__ __launch_bounds__(256) void cima_kv_pages_compact_move(
-    uint4* pool, long long plane_words, long long page_words, int pieces, int n_planes, int n_pages,
+    word4* pool, long long plane_words, long long page_words, int pieces, int n_planes, int n_pages,
     const int* table, int* table_out, long long entries, const int* __restrict__ work) {
     const int moves = work[0];
     const int* src = work + 16;

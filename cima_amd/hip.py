@@ -209,23 +209,32 @@ def _ptr(a) -> Optional[int]:
 # element type and hold at least the elements that the call reads or writes
 # (torch's integers are 64-bit unless asked otherwise; read as 32-bit they would
 # name wrong pages).  A raw pointer is taken as it is.
-def _ptr_of(a, dtype: str, n: int, name: str) -> Optional[int]:
-    if a is None or isinstance(a, int):
-        return a or None
+def _ptr_of(a, kind: int, n: int, name: str) -> Optional[int]:
+    try:  # the usual tensor, one look at each property
+        if a.dtype is _DTYPES[kind] and a.numel() >= n and a.is_cuda and a.is_contiguous():
+            return a.data_ptr()
+    except AttributeError:
+        if a is None or isinstance(a, int):
+            return a or None
     p = _ptr(a)
-    if str(a.dtype) != dtype:
-        raise EngineError("hip", E_INVALID, f"{name} is {a.dtype}, not {dtype}")
+    if _DTYPES[kind] is None:
+        import torch
+
+        _DTYPES[:] = torch.int32, torch.float32, torch.float16
+    if a.dtype is not _DTYPES[kind]:
+        raise EngineError("hip", E_INVALID, f"{name} is {a.dtype}, not {_DTYPES[kind]}")
     if a.numel() < n:
         raise EngineError("hip", E_INVALID, f"{name} holds {a.numel()} elements, the call takes {n}")
     return p
 
 
-_I32, _F32, _F16 = "torch.int32", "torch.float32", "torch.float16"
+_DTYPES: list = [None] * 3
+_I32, _F32, _F16 = range(3)
 
 
 def _slab(a) -> tuple:
     """(pointer, bytes) of a scratch tensor."""
-    return (None, 0) if a is None else (_ptr(a), a.numel() * a.element_size())
+    return (None, 0) if a is None else (_ptr(a), a.nbytes)
 
 
 def _act_of(t) -> int:

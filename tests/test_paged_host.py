@@ -29,7 +29,8 @@ def test_kv_pages_layout_matches_header(tmp_path):
 def test_code_objects_hold_every_kernel():
     want = {"paged": ["cima_rope_append_paged_d64", "cima_rope_append_paged_d128", "cima_kv_pages_copy",
                       "cima_kv_pages_reserve", "cima_kv_pages_fork", "cima_kv_pages_free", "cima_kv_pages_compact"],
-            "paged_attn": [f"cima_attn_paged_{k}_d{d}" for k in ("prefix", "own", "join") for d in (64, 128)],
+            "paged_attn": [f"cima_attn_paged_{k}" for d in (64, 128)
+                           for k in (f"join_d{d}", *(f"d{d}_m{m}_n{n}" for m in (0, 1, 2) for n in (1, 2)))],
             "sample": ["cima_softmax", "cima_verify"]}
     for name, kernels in want.items():
         blob = open(cbuild.HSACOS[name], "rb").read()
