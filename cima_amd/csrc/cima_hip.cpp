@@ -1658,18 +1658,17 @@ struct PagedAttnArgs {
     void* ml;
     int seqs, n_new, q_heads, kv_heads, page_shift, n_pages, table_stride;
     int prefix_pages, prefix_slot, window;
-    int prefix_parts, own_parts, row_tiles, prefix_tile, own_tile, prefix_wgs;
+    int prefix_parts, own_parts, row_tiles, prefix_tile, own_tile, prefix_wgs, least_tiles;
     float scale2;
 };
 
-// LDS of Few<dim, nb> and of Tile<dim, wr, wk, st> in paged_attn.hip
-unsigned paged_few_lds(int dim, int nb) {
-    return (unsigned)(4 * std::max(2 * 32 * dim * 2, nb * (dim / 16) * 64 * 16) + 4 * nb * 16 * 8);
+// few_wgs in paged_attn.hip: workgroups to a CU
+int paged_few_wgs(int dim, int mode, int nb) { return mode == 0 && !(dim == 128 && nb == 2) ? 4 : 2; }
+// LDS of Few<dim, nb, bufs> and of Tile<dim, 2 or 4, 2 or 1> in paged_attn.hip
+unsigned paged_few_lds(int dim, int nb, int bufs) {
+    return (unsigned)(4 * std::max(bufs * 32 * dim * 2, nb * (dim / 16) * 64 * 16) + 4 * nb * 16 * 8);
 }
-unsigned paged_attn_lds(int dim, int wr, int wk, int st) {
-    const int kt = 32 * (wk == 1 && wr > 1 ? 2 : 1) * wk, bytes = kt * dim * 2;
-    return (unsigned)(st * 2 * bytes + 1024 * 4 + wr * wk * 32);
-}
+unsigned paged_attn_lds(int dim) { return (unsigned)(4 * 64 * dim * 2 + 1024 * 4 + 4 * 32); }
 
 }  // namespace
 
@@ -1730,18 +1729,29 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     const int own_tiles = (own_rows + 16 * nb - 1) / (16 * nb);
     const long long own_base = (long long)seqs * kv->kv_heads * own_tiles;
     const long long own_room = (long long)(kv->table_stride - prefix_pages) * kv->page;
-    long long own = std::min((ctx->num_cu + own_base - 1) / own_base, (own_room + 127) / 128);
-    own = std::max(1LL, std::min(own, 64LL));
-    int tiles = 0, mode = 0;
+    const int mode = !prefix_pages || few ? 0 : head_rows <= 64 ? 1 : 2;
+    const int wgs = paged_few_wgs(dim, mode, nb);
+    // own tasks take 128 positions at least, twice that as often as it needs for
+    // the tasks of full tables not to pass four rounds of the chip (half of it
+    // where the prefix tasks take the other half)
+    const long long most = (mode ? 2LL : 4LL) * wgs * ctx->num_cu;
+    int least_tiles = 4;
+    auto parts_of = [&](int tiles) { return std::max(1LL, (own_room + 32LL * tiles - 1) / (32LL * tiles)); };
+    while (own_base * parts_of(least_tiles) > most && parts_of(least_tiles) > 1) least_tiles *= 2;
+    long long own = std::min(parts_of(least_tiles), 64LL);
+    int tiles = 0;
     long long pre = 0;
     if (prefix_pages) {
-        mode = few ? 0 : head_rows <= 64 ? 1 : 2;
         const int per = 64 * mode;  // rows of a tile
         tiles = few ? 1 : (head_rows + per - 1) / per;
         const long long base = (long long)kv->kv_heads * tiles, len = (long long)prefix_pages * kv->page;
-        pre = std::min((ctx->num_cu + base - 1) / base, (len + 127) / 128);
-        const long long twice = (2LL * ctx->num_cu + base - 1) / base;
-        if (len >= 512 * twice) pre = twice;
+        // a workgroup to a CU; two where each still has 512 positions, half of one
+        // where the own tasks have much to read (256 KB a CU in full tables)
+        const long long own_bytes = 4LL * seqs * kv->kv_heads * own_room * dim;
+        long long want = ctx->num_cu;
+        if (few || len * base >= 1024LL * ctx->num_cu) want *= 2;
+        else if (own_bytes >= (256LL << 10) * ctx->num_cu) want /= 2;
+        pre = std::min((want + base - 1) / base, (len + 127) / 128);
         pre = std::max(1LL, std::min(pre, 128LL));
     }
     if (pre + own > 1 && pre + own > fit) {  // fewer parts, the prefix's half of them
@@ -1776,6 +1786,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     A.own_parts = (int)own;
     A.row_tiles = tiles;
     A.scale2 = scale * 1.44269504088896340736f;
+    A.least_tiles = least_tiles;
     A.prefix_tile = few ? 16 * nb : 32;
     A.own_tile = 16 * nb;
     char name[64];
@@ -1784,7 +1795,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     snprintf(name, sizeof name, "cima_attn_paged_d%d_m%d_n%d", dim, mode, nb);
     if (int rc = get_fn(ctx, name, &f)) return rc;
     void* args[] = {&A};
-    const unsigned lds = std::max(paged_few_lds(dim, nb), mode ? paged_attn_lds(dim, 2 * mode, 2 / mode, 2) : 0u);
+    const unsigned lds = std::max(paged_few_lds(dim, nb, wgs == 4 ? 1 : 2), mode ? paged_attn_lds(dim) : 0u);
     if (int rc = launch(ctx, f, (unsigned)(A.prefix_wgs + own_base * own), 256, args, api, lds)) return rc;
     if (all == 1) return 0;
     const long long join = (long long)kv->kv_heads * ((head_rows + 15) / 16) * (dim / 16);

@@ -107,6 +107,7 @@ struct AttnArgs {
     int prefix_parts, own_parts, row_tiles;  // row tiles of the prefix tasks
     int prefix_tile, own_tile;               // their rows, and those of the own tasks
     int prefix_wgs;                          // workgroups of prefix tasks
+    int least_tiles;                         // of 32 positions, that an own task takes
     float scale2;                            // scale * log2(e)
 };
 
@@ -500,17 +501,26 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 // to the registers of the A operand (16 x 16 x 32 MFMA: a lane holds 16 bytes
 // of a key), values by direct copies to the wave's own LDS, one tile ahead.
 // The waves' sums are added at the end, in wave order.
-template <int D, int NB>
+//
+// BUFS 2: a tile is on its way while the one before it is computed, 64 KB of LDS
+// a workgroup, two of them to a CU.  BUFS 1: the loads of a tile are waited for,
+// but the registers and LDS suffice for four workgroups to a CU, whose waves
+// cover each other; it is taken where the launch holds nothing larger.
+// Measured on MI355X, 8 kv heads of 128, one / two in flight: 64 slots of up
+// to 4000 positions (524 MB) 107 / 146 us (4.9 TB/s), 128 of up to 500 27 / 33.
+constexpr int few_bufs(int D, int mode, int nb) { return mode == 0 && !(D == 128 && nb == 2) ? 1 : 2; }
+constexpr int few_wgs(int D, int mode, int nb) { return few_bufs(D, mode, nb) == 1 ? 4 : 2; }
+template <int D, int NB, int BUFS>
 struct Few {
     static constexpr int VT = 32 * D * 2;                  // bytes of a tile's values
     static constexpr int OB = NB * (D / 16) * 64 * 16;     // of a wave's sums
-    static constexpr int WAVE = 2 * VT > OB ? 2 * VT : OB;  // LDS of a wave
+    static constexpr int WAVE = BUFS * VT > OB ? BUFS * VT : OB;  // LDS of a wave
     static constexpr int LDS = 4 * WAVE + 4 * NB * 16 * 8;
 };
-template <int D, int NB>
+template <int D, int NB, int BUFS>
 DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int plo, int phi, const int* trow, int part,
-                  int parts, int col, int guess) {
-    using F = Few<D, NB>;
+                  int parts, int col, int guess, int least) {
+    using F = Few<D, NB, BUFS>;
     constexpr int STEPS = D / 32, XT = D / 16, CH = D / 8;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, q4 = lane >> 4;
@@ -561,7 +571,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
     hi_all = __builtin_amdgcn_readfirstlane(min16(hi_all));
     const int base = lo_any & ~15;
     const int tiles = hi_any > lo_any ? (hi_any - base + 31) / 32 : 0;
-    const int each = (tiles + parts - 1) / parts;
+    const int each = max((tiles + parts - 1) / parts, least);
     const int t0 = min(part * each, tiles), t1 = min(t0 + each, tiles);
 
     f4 o[NB][XT];
@@ -576,7 +586,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
     // that no one sees are replaced by the nearest that someone does
     const int page = 1 << A.page_shift;
     const uint32_t vbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * F::WAVE;
-    h8 kf[2][2][STEPS];
+    h8 kf[BUFS][2][STEPS];
     auto issue = [&](int t, auto buf) {
 #pragma unroll
         for (int u = 0; u < 2; u++) {
@@ -602,8 +612,10 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
         }
     };
     auto step = [&](int t, auto buf) {
+        if constexpr (BUFS == 1) issue(t, buf);
         wait_vm<0>();
-        if (t + 4 < t1) issue(t + 4, std::integral_constant<int, 1 - buf>{});
+        if constexpr (BUFS == 2)
+            if (t + 4 < t1) issue(t + 4, std::integral_constant<int, 1 - buf>{});
         const int p0 = base + 32 * t;
         h8 pf[NB];
 #pragma unroll
@@ -674,7 +686,9 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
     using B0 = std::integral_constant<int, 0>;
     using B1 = std::integral_constant<int, 1>;
     int t = t0 + wave;
-    if (t < t1) {
+    if constexpr (BUFS == 1) {
+        for (; t < t1; t += 4) step(t, B0{});
+    } else if (t < t1) {
         issue(t, B0{});
         while (true) {
             step(t, B0{});
@@ -746,6 +760,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
 // the first find its pages in that XCD's L2.
 template <int D, int MODE, int NB>
 DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
+    constexpr int BUFS = few_bufs(D, MODE, NB);
     const int rows = A.n_new * (A.q_heads / A.kv_heads);
     int b = blockIdx.x;
     if (b < A.prefix_wgs) {
@@ -754,8 +769,8 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
         const int kvh = grp / A.prefix_parts, part = grp % A.prefix_parts, phi = A.prefix_pages << A.page_shift;
         const int* trow = A.table + (size_t)A.prefix_slot * A.table_stride;
         if (MODE == 0)
-            few_task<D, NB>(A, lds, kvh, 0, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
-                            ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift);
+            few_task<D, NB, BUFS>(A, lds, kvh, 0, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
+                            ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1);
         else if (MODE == 1) attn_task<D, 2, 2>(A, lds, kvh, tile * 64, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
         else attn_task<D, 4, 1>(A, lds, kvh, tile * 128, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
         return;
@@ -767,11 +782,11 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
     const int tile = b % tiles;
     b /= tiles;
     const int kvh = b % A.kv_heads, s = b / A.kv_heads;
-    few_task<D, NB>(A, lds, kvh, s * rows + tile * 16 * NB, (s + 1) * rows, A.prefix_pages << A.page_shift, 0x7fffffff,
-                    A.table + (size_t)s * A.table_stride, part, A.own_parts, A.prefix_parts + part, A.prefix_pages);
+    few_task<D, NB, BUFS>(A, lds, kvh, s * rows + tile * 16 * NB, (s + 1) * rows, A.prefix_pages << A.page_shift, 0x7fffffff,
+                    A.table + (size_t)s * A.table_stride, part, A.own_parts, A.prefix_parts + part, A.prefix_pages, A.least_tiles);
 }
 #define ATTN(D, MODE, NB)                                                                                            \
-    extern "C" __global__ __launch_bounds__(256, 2) void cima_attn_paged_d##D##_m##MODE##_n##NB(const AttnArgs A) {  \
+    extern "C" __global__ __launch_bounds__(256, few_wgs(D, MODE, NB)) void cima_attn_paged_d##D##_m##MODE##_n##NB(const AttnArgs A) {  \
         extern __shared__ __align__(1024) uint8_t lds[];                                                             \
         attn_body<D, MODE, NB>(A, lds);                                                                              \
     }
