@@ -1743,7 +1743,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     long long pre = 0;
     if (prefix_pages) {
         const int per = 64 * mode;  // rows of a tile
-        tiles = few ? 1 : (head_rows + per - 1) / per;
+        tiles = few ? (head_rows + 16 * nb - 1) / (16 * nb) : (head_rows + per - 1) / per;
         const long long base = (long long)kv->kv_heads * tiles, len = (long long)prefix_pages * kv->page;
         // a workgroup to a CU; two where each still has 512 positions, half of one
         // where the own tasks have much to read (256 KB a CU in full tables)

@@ -419,8 +419,6 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     // ---- waves that shared rows: sums brought to the largest maximum and
     // added in wave order
     if (WK > 1) {
-        float* mm = reinterpret_cast<float*>(red);  // [NW][8]: not enough for 32 rows, so in the ring
-        (void)mm;
         __syncthreads();
         float* ro = reinterpret_cast<float*>(lds);
         constexpr int N = MT * 16;
@@ -464,21 +462,6 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     }
     if (!valid) return;
     const bool some = live && t0 < t1;
-    const int all = A.prefix_parts + A.own_parts;
-    if (all == 1) {
-        // nothing to join: the result, rounded once
-        const float inv = some && l != 0.f ? 1.f / l : 0.f;
-        uint16_t* to = A.out + qrow * D + 4 * half;
-#pragma unroll
-        for (int x = 0; x < MT; x++)
-#pragma unroll
-            for (int i = 0; i < 16; i += 4) {
-                uint2 w = make_uint2(0, 0);
-                if (some) w = make_uint2(f2h2(o[x][i] * inv, o[x][i + 1] * inv), f2h2(o[x][i + 2] * inv, o[x][i + 3] * inv));
-                *reinterpret_cast<uint2*>(to + 32 * x + 2 * i) = w;
-            }
-        return;
-    }
     const int R = A.seqs * A.n_new * g;
     const size_t at = (size_t)(col * A.kv_heads + kvh) * R;
     if (half == 0) A.ml[at + r] = f2{some ? m : LOWEST, some ? l : 0.f};
@@ -769,7 +752,7 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
         const int kvh = grp / A.prefix_parts, part = grp % A.prefix_parts, phi = A.prefix_pages << A.page_shift;
         const int* trow = A.table + (size_t)A.prefix_slot * A.table_stride;
         if (MODE == 0)
-            few_task<D, NB, BUFS>(A, lds, kvh, 0, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
+            few_task<D, NB, BUFS>(A, lds, kvh, tile * 16 * NB, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
                             ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1);
         else if (MODE == 1) attn_task<D, 2, 2>(A, lds, kvh, tile * 64, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
         else attn_task<D, 4, 1>(A, lds, kvh, tile * 128, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
