@@ -205,12 +205,9 @@ const char* const kPagedKernels[] = {
     "cima_rope_append_paged_d64", "cima_rope_append_paged_d128", "cima_kv_pages_copy", "cima_kv_pages_reserve",
     "cima_kv_pages_fork", "cima_kv_pages_fork_copy", "cima_kv_pages_free", "cima_kv_pages_compact",
     "cima_kv_pages_compact_move"};
-const char* const kSampleKernels[] = {
-    "cima_softmax_stats_f16", "cima_softmax_stats_f32", "cima_softmax_stats_cap_f16", "cima_softmax_stats_cap_f32",
-    "cima_softmax_probs_f16", "cima_softmax_probs_f32", "cima_softmax_probs_cap_f16", "cima_softmax_probs_cap_f32",
-    "cima_softmax_t256_w2_f16", "cima_softmax_t256_w8_f16", "cima_softmax_t1024_w8_f16", "cima_softmax_t1024_w16_f16",
-    "cima_softmax_t256_w2_f32", "cima_softmax_t256_w8_f32", "cima_softmax_t1024_w8_f32", "cima_softmax_t1024_w16_f32",
-    "cima_verify_sums", "cima_verify_draw"};
+const char* const kSampleTypes[] = {"f16", "f32", "cap_f16", "cap_f32"};
+const char* const kSampleKernels[] = {"cima_softmax_t1024_w16_f16", "cima_softmax_t1024_w16_f32", "cima_verify_sums",
+                                      "cima_verify_draw"};
 
 std::string default_code_dir() {
     Dl_info info;
@@ -667,6 +664,9 @@ int cima_hip_init(int device, const char* code_dir, cima_hip_ctx** out) {
     }
     for (const char* kn : kSampleKernels)
         if (!rc) rc = add(MOD_SAMPLE, kn);
+    for (const char* t : kSampleTypes)
+        for (const char* kn : {"stats", "probs", "t256_w2", "t256_w8", "t1024_w8"})
+            if (!rc) rc = add(MOD_SAMPLE, std::string("cima_softmax_") + kn + "_" + t);
     if (rc) {
         unload(ctx);
         delete ctx;
@@ -1922,19 +1922,18 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
         return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (8 B)", api,
                     slab_bytes, need);
     const bool f32 = x_dtype == CIMA_DT_F32;
+    char name[64];
+    const char* sfx = kSampleTypes[(cap > 0.f ? 2 : 0) + (f32 ? 1 : 0)];
     // whole rows (sample_ops.hip): threads and four-logit words a thread of the
-    // kernels built, shortest first; rows of the longest kind only where there
-    // are enough of them for half the chip
+    // kernels built, shortest first; rows of the longest kind, which keeps logits
+    // as they come, only where there are enough of them for half the chip
     static const int shapes[][2] = {{256, 2}, {256, 8}, {1024, 8}, {1024, 16}};
     for (const auto& sh : shapes)
-        if (cap == 0.f && n <= sh[0] * sh[1] * 4 && (sh[1] < 16 || rows >= kSoftmaxLongRows)) {
-            char name[64];
-            snprintf(name, sizeof name, "cima_softmax_t%d_w%d_%s", sh[0], sh[1], f32 ? "f32" : "f16");
-            void* args[] = {&x, &y, &n, &temp, &rows_per_temp};
+        if (n <= sh[0] * sh[1] * 4 && (sh[1] < 16 || (cap == 0.f && rows >= kSoftmaxLongRows))) {
+            snprintf(name, sizeof name, "cima_softmax_t%d_w%d_%s", sh[0], sh[1], sfx);
+            void* args[] = {&x, &y, &n, &temp, &rows_per_temp, &cap};
             return launch_named(ctx, name, (unsigned)rows, (unsigned)sh[0], args, api);
         }
-    char name[64];
-    const char* sfx = cap > 0.f ? (f32 ? "cap_f32" : "cap_f16") : (f32 ? "f32" : "f16");
     snprintf(name, sizeof name, "cima_softmax_stats_%s", sfx);
     void* args[] = {&x, &slab, &n, &temp, &rows_per_temp, &cap, &parts};
     if (int rc = launch_named(ctx, name, (unsigned)(rows * parts), 256, args, api)) return rc;

@@ -803,6 +803,19 @@ DEV void attn_join_body(const AttnArgs& A) {
     const int rts = (R + 15) / 16, r = min(b % rts * 16 + li, R - 1), kvh = b / rts;
     const bool valid = b % rts * 16 + li < R;
     const size_t step = (size_t)A.kv_heads * R, head = (size_t)kvh * R;
+    // where the row's elements 16 x + 4 q4 are in a prefix part and in an own part
+    const int pr0 = r / A.prefix_tile * A.prefix_tile, pc = min(A.prefix_tile, R - pr0);
+    const int s0 = r / rows * rows, or0 = s0 + (r - s0) / A.own_tile * A.own_tile, oc = min(A.own_tile, s0 + rows - or0);
+    const float4* ap = reinterpret_cast<const float4*>(A.acc + (head + pr0) * D) + (4 * x + q4) * pc + (r - pr0);
+    const float4* ao = reinterpret_cast<const float4*>(A.acc + (head + or0) * D) + (4 * x + q4) * oc + (r - or0);
+    auto part = [&](int c) { return (c < A.prefix_parts ? ap : ao)[c * step * (D / 4)]; };
+    // few parts: their sums are fetched beside the weights, needed or not
+    const bool few = all <= 8;
+    float4 e0 = make_float4(0.f, 0.f, 0.f, 0.f), e1 = e0;
+    if (few) {
+        e0 = part(min(wave, all - 1));
+        e1 = part(min(wave + 4, all - 1));
+    }
     // ---- weights: thread (t / 16, row t % 16) takes parts t / 16 + 16 k
     const f2* ml = A.ml + head + r;
     f2 v[MAX_PARTS / 16];
@@ -831,44 +844,45 @@ DEV void attn_join_body(const AttnArgs& A) {
     }
     red[t / 16][li] = L;
     __syncthreads();
-    if (wave == 0) {
-        int n = 0;
-        for (int c0 = 0; c0 < all; c0 += 64) {
-            bool any = false;
-            if (c0 + lane < all)
-#pragma unroll
-                for (int i = 0; i < 16; i++) any |= wt[c0 + lane][i] != 0.f;
-            const unsigned long long m = __ballot(any);
-            if (any) list[n + __popcll(m & ((1ull << lane) - 1))] = c0 + lane;
-            n += __popcll(m);
-        }
-        if (lane == 0) count = n;
-    }
-    __syncthreads();
-    const int n = count;
-    // where the row's elements 16 x + 4 q4 are in a prefix part and in an own part
-    const int pr0 = r / A.prefix_tile * A.prefix_tile, pc = min(A.prefix_tile, R - pr0);
-    const int s0 = r / rows * rows, or0 = s0 + (r - s0) / A.own_tile * A.own_tile, oc = min(A.own_tile, s0 + rows - or0);
-    const float4* ap = reinterpret_cast<const float4*>(A.acc + (head + pr0) * D) + (4 * x + q4) * pc + (r - pr0);
-    const float4* ao = reinterpret_cast<const float4*>(A.acc + (head + or0) * D) + (4 * x + q4) * oc + (r - or0);
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    constexpr int U = 8;
-    for (int k0 = wave; k0 < n; k0 += 4 * U) {
-        float4 z[U];
-        float w[U];
+    // what a weight of 0 stands for may hold anything
+    auto add = [&](const float4& z, float w) {
+        o.x += w != 0.f ? z.x * w : 0.f;
+        o.y += w != 0.f ? z.y * w : 0.f;
+        o.z += w != 0.f ? z.z * w : 0.f;
+        o.w += w != 0.f ? z.w * w : 0.f;
+    };
+    if (few) {
+        add(e0, wave < all ? wt[wave][li] : 0.f);
+        add(e1, wave + 4 < all ? wt[wave + 4][li] : 0.f);
+    } else {
+        if (wave == 0) {
+            int n = 0;
+            for (int c0 = 0; c0 < all; c0 += 64) {
+                bool any = false;
+                if (c0 + lane < all)
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            const int k = k0 + 4 * u, c = list[min(k, n - 1)];
-            w[u] = k < n ? wt[c][li] : 0.f;
-            z[u] = (c < A.prefix_parts ? ap : ao)[c * step * (D / 4)];
+                    for (int i = 0; i < 16; i++) any |= wt[c0 + lane][i] != 0.f;
+                const unsigned long long m = __ballot(any);
+                if (any) list[n + __popcll(m & ((1ull << lane) - 1))] = c0 + lane;
+                n += __popcll(m);
+            }
+            if (lane == 0) count = n;
         }
+        __syncthreads();
+        const int n = count;
+        constexpr int U = 8;
+        for (int k0 = wave; k0 < n; k0 += 4 * U) {
+            float4 z[U];
+            float w[U];
 #pragma unroll
-        for (int u = 0; u < U; u++) {
-            // what a weight of 0 stands for may hold anything
-            o.x += w[u] != 0.f ? z[u].x * w[u] : 0.f;
-            o.y += w[u] != 0.f ? z[u].y * w[u] : 0.f;
-            o.z += w[u] != 0.f ? z[u].z * w[u] : 0.f;
-            o.w += w[u] != 0.f ? z[u].w * w[u] : 0.f;
+            for (int u = 0; u < U; u++) {
+                const int k = k0 + 4 * u, c = list[min(k, n - 1)];
+                w[u] = k < n ? wt[c][li] : 0.f;
+                z[u] = part(c);
+            }
+#pragma unroll
+            for (int u = 0; u < U; u++) add(z[u], w[u]);
         }
     }
     ro[wave][lane] = o;

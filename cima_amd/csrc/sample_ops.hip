@@ -224,28 +224,28 @@ DEV float sm_join(const SmPart* __restrict__ p, int parts, float T, int* at, flo
         const float m = sm_join(part + (size_t)row * parts, parts, T, &at, &L);                                        \
         R.write(y, (size_t)row * n, n, T, m, at, L);                                                                   \
     }
-#define SOFTMAX_WHOLE(NAME, F32, NT, WORDS)                                                                            \
+#define SOFTMAX_WHOLE(NAME, F32, CAP, NT, WORDS)                                                                       \
     extern "C" __global__ __launch_bounds__(NT) void cima_softmax_t##NT##_w##WORDS##_##NAME(                           \
-        const void* __restrict__ x, float* __restrict__ y, int n, const float* __restrict__ temp, int rows_per_temp) { \
+        const void* __restrict__ x, float* __restrict__ y, int n, const float* __restrict__ temp, int rows_per_temp,   \
+        float cap) {                                                                                                   \
         const int row = blockIdx.x;                                                                                    \
         const float T = temp ? temp[row / rows_per_temp] : 1.f;                                                        \
-        SmRow<F32, false, NT, WORDS> R;                                                                                \
-        R.load(x, (size_t)row * n, 0, n, 0.f);                                                                         \
+        SmRow<F32, CAP, NT, WORDS> R;                                                                                  \
+        R.load(x, (size_t)row * n, 0, n, cap);                                                                         \
         R.stats(T);                                                                                                    \
         R.write(y, (size_t)row * n, n, T, R.m, R.at, R.l);                                                             \
     }
-SOFTMAX_PARTS(f16, false, false)
-SOFTMAX_PARTS(f32, true, false)
-SOFTMAX_PARTS(cap_f16, false, true)
-SOFTMAX_PARTS(cap_f32, true, true)
-SOFTMAX_WHOLE(f16, false, 256, 2)
-SOFTMAX_WHOLE(f16, false, 256, 8)
-SOFTMAX_WHOLE(f16, false, 1024, 8)
-SOFTMAX_WHOLE(f16, false, 1024, 16)
-SOFTMAX_WHOLE(f32, true, 256, 2)
-SOFTMAX_WHOLE(f32, true, 256, 8)
-SOFTMAX_WHOLE(f32, true, 1024, 8)
-SOFTMAX_WHOLE(f32, true, 1024, 16)
+#define SOFTMAX(NAME, F32, CAP)            \
+    SOFTMAX_PARTS(NAME, F32, CAP)          \
+    SOFTMAX_WHOLE(NAME, F32, CAP, 256, 2)  \
+    SOFTMAX_WHOLE(NAME, F32, CAP, 256, 8)  \
+    SOFTMAX_WHOLE(NAME, F32, CAP, 1024, 8)
+SOFTMAX(f16, false, false)
+SOFTMAX(f32, true, false)
+SOFTMAX(cap_f16, false, true)
+SOFTMAX(cap_f32, true, true)
+SOFTMAX_WHOLE(f16, false, false, 1024, 16)
+SOFTMAX_WHOLE(f32, true, false, 1024, 16)
 
 // ------------------------------------------------------------- verification
 //
