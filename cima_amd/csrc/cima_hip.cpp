@@ -1917,10 +1917,6 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
     if (!x || !y || !aligned(x, x_dtype == CIMA_DT_F32 ? 4 : 2) || !aligned(y, 4) || !aligned(temp, 4))
         return fail(CIMA_E_INVALID, "%s: null or misaligned x, y or temp", api);
     int parts = (n + kSoftmaxPart - 1) / kSoftmaxPart;
-    const unsigned long long need = 16ULL * rows * parts;
-    if ((long long)rows * parts > 0x7fffffffLL || !slab || !aligned(slab, 8) || slab_bytes < need)
-        return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (8 B)", api,
-                    slab_bytes, need);
     const bool f32 = x_dtype == CIMA_DT_F32;
     char name[64];
     const char* sfx = kSampleTypes[(cap > 0.f ? 2 : 0) + (f32 ? 1 : 0)];
@@ -1934,6 +1930,10 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
             void* args[] = {&x, &y, &n, &temp, &rows_per_temp, &cap};
             return launch_named(ctx, name, (unsigned)rows, (unsigned)sh[0], args, api);
         }
+    const unsigned long long need = 16ULL * rows * parts;
+    if ((long long)rows * parts > 0x7fffffffLL || !slab || !aligned(slab, 8) || slab_bytes < need)
+        return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (8 B)", api,
+                    slab_bytes, need);
     snprintf(name, sizeof name, "cima_softmax_stats_%s", sfx);
     void* args[] = {&x, &slab, &n, &temp, &rows_per_temp, &cap, &parts};
     if (int rc = launch_named(ctx, name, (unsigned)(rows * parts), 256, args, api)) return rc;

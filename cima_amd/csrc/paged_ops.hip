@@ -24,7 +24,7 @@ DEV void rope_append_body(const uint16_t* __restrict__ qkv, uint16_t* __restrict
     const int pos = len + (row - s * n_new);
     const int at = pos >> page_shift;
     int id = -1;
-    if (at < table_stride) id = table[(size_t)s * table_stride + at];
+    if ((unsigned)at < (unsigned)table_stride) id = table[(size_t)s * table_stride + at];
     if (t < D / 2) {
         float sv = 0.f, cv = 1.f;
         if (rotate) {
@@ -236,7 +236,7 @@ extern "C" __global__ __launch_bounds__(1024) void cima_kv_pages_reserve(int* re
             lo = len >> page_shift;
             int end = (int)(((long long)len + n_new + page - 1) >> page_shift);
             const int off = end - max(lo, table_stride);  // entries behind the row
-            if (off > 0) atomicAdd(&behind, off);
+            if (off > 0) atomicAdd(&behind, min(off, 1 << 18));
             end = min(end, table_stride);
             int hi = max(end, lo);
             if (hi - lo <= 4) {  // a few entries: looked at together
@@ -312,7 +312,7 @@ extern "C" __global__ __launch_bounds__(1024) void cima_kv_pages_fork(int* refs,
             bool ok = (unsigned)p[k] < (unsigned)max_seqs && (unsigned)c[k] < (unsigned)max_seqs;
             if (ok) {
                 len[k] = lens[p[k]];
-                ok = len[k] >= 0 && (len[k] + page - 1) >> page_shift <= table_stride;
+                ok = len[k] >= 0 && len[k] <= table_stride << page_shift;
                 if (ok) ok = mine[k] = atomicCAS(&lens[c[k]], -1, -2 - i) == -1;
             }
             if (!ok) wrong = 1;

@@ -209,9 +209,9 @@ def _ptr(a) -> Optional[int]:
 # element type and hold at least the elements that the call reads or writes
 # (torch's integers are 64-bit unless asked otherwise; read as 32-bit they would
 # name wrong pages).  A raw pointer is taken as it is.
-def _ptr_of(a, kind: int, n: int, name: str) -> Optional[int]:
+def _ptr_of(a, kind: int, n: int, name: str, device: int = 0) -> Optional[int]:
     try:  # the usual tensor, one look at each property
-        if a.dtype is _DTYPES[kind] and a.numel() >= n and a.is_cuda and a.is_contiguous():
+        if a.dtype is _DTYPES[kind] and a.numel() >= n and a.get_device() == device and a.is_contiguous():
             return a.data_ptr()
     except AttributeError:
         if a is None or isinstance(a, int):
@@ -225,6 +225,8 @@ def _ptr_of(a, kind: int, n: int, name: str) -> Optional[int]:
         raise EngineError("hip", E_INVALID, f"{name} is {a.dtype}, not {_DTYPES[kind]}")
     if a.numel() < n:
         raise EngineError("hip", E_INVALID, f"{name} holds {a.numel()} elements, the call takes {n}")
+    if a.get_device() != device:
+        raise EngineError("hip", E_INVALID, f"{name} is on device {a.get_device()}, the context on {device}")
     return p
 
 
@@ -234,7 +236,7 @@ _I32, _F32, _F16 = range(3)
 
 def _slab(a) -> tuple:
     """(pointer, bytes) of a scratch tensor."""
-    return (None, 0) if a is None else (_ptr(a), a.nbytes)
+    return (None, 0) if a is None else (_ptr(a), a.numel() * a.element_size())
 
 
 def _act_of(t) -> int:
@@ -532,14 +534,22 @@ class HipCtx:
         self._check(self.lib.cima_hip_decode_step(self.handle, ctypes.byref(desc)))
 
     # -- a batch over a paged cache (kv: cima_amd.paged.PagedKV) ----------------
+    def _kv(self, kv):
+        if kv.device != self.device:
+            raise EngineError("hip", E_INVALID, f"the cache is on device {kv.device}, the context on {self.device}")
+        return kv.ref
+
+    def _op(self, a, kind: int, n: int, name: str) -> Optional[int]:
+        return _ptr_of(a, kind, n, name, self.device)
+
     def rope_append_paged(self, kv, layer: int, qkv, q, seqs: int, n_new: int, q_heads: int, theta: float) -> None:
         """RoPE of a step's queries (to ``q``) and keys, row ``s * n_new + j`` of
         ``qkv`` at position ``lens[s] + j``, and the append of its keys and values
         to the pages of ``layer`` (theta 0: no rotation)."""
         rows = seqs * n_new
         self._check(self.lib.cima_hip_rope_append_paged(
-            self.handle, kv.ref, layer, _ptr_of(qkv, _F16, rows * (q_heads + 2 * kv.kv_heads) * kv.head_dim, "qkv"),
-            _ptr_of(q, _F16, rows * q_heads * kv.head_dim, "q"), seqs, n_new, q_heads, theta))
+            self.handle, self._kv(kv), layer, self._op(qkv, _F16, rows * (q_heads + 2 * kv.kv_heads) * kv.head_dim, "qkv"),
+            self._op(q, _F16, rows * q_heads * kv.head_dim, "q"), seqs, n_new, q_heads, theta))
 
     def attn_paged(self, kv, layer: int, q, out, seqs: int, n_new: int, q_heads: int, scale: float, slab,
                    prefix_pages: int = 0, prefix_slot: int = 0, window: int = 0) -> None:
@@ -547,38 +557,38 @@ class HipCtx:
         ``prefix_pages`` entries, the same in every slot, are read once for all
         from row ``prefix_slot`` of the table."""
         n = seqs * n_new * q_heads * kv.head_dim
-        self._check(self.lib.cima_hip_attn_paged(self.handle, kv.ref, layer, _ptr_of(q, _F16, n, "q"),
-                                                 _ptr_of(out, _F16, n, "out"), seqs, n_new, q_heads, scale,
+        self._check(self.lib.cima_hip_attn_paged(self.handle, self._kv(kv), layer, self._op(q, _F16, n, "q"),
+                                                 self._op(out, _F16, n, "out"), seqs, n_new, q_heads, scale,
                                                  prefix_pages, prefix_slot, window, *_slab(slab)))
 
     def kv_pages_copy(self, kv, src, dst, n: int) -> None:
         """Page ``dst[i]`` of every plane = page ``src[i]``."""
-        self._check(self.lib.cima_hip_kv_pages_copy(self.handle, kv.ref, _ptr_of(src, _I32, n, "src"),
-                                                    _ptr_of(dst, _I32, n, "dst"), n))
+        self._check(self.lib.cima_hip_kv_pages_copy(self.handle, self._kv(kv), self._op(src, _I32, n, "src"),
+                                                    self._op(dst, _I32, n, "dst"), n))
 
     def kv_pages_reserve(self, kv, seqs: int, n_new: int, status) -> None:
         """Pages for ``n_new`` more tokens in each of slots [0, seqs) in use;
         ``status[0]`` = pages missing (then nothing is changed)."""
-        self._check(self.lib.cima_hip_kv_pages_reserve(self.handle, kv.ref, seqs, n_new,
-                                                       _ptr_of(status, _I32, 1, "status")))
+        self._check(self.lib.cima_hip_kv_pages_reserve(self.handle, self._kv(kv), seqs, n_new,
+                                                       self._op(status, _I32, 1, "status")))
 
     def kv_pages_fork(self, kv, parents, children, n: int, status) -> None:
         """Slots ``children[i]`` become copies of ``parents[i]``: whole pages
         shared, a page begun copied; ``status[0]``: 0, pages missing, or -1."""
-        self._check(self.lib.cima_hip_kv_pages_fork(self.handle, kv.ref, _ptr_of(parents, _I32, n, "parents"),
-                                                    _ptr_of(children, _I32, n, "children"), n,
-                                                    _ptr_of(status, _I32, 1, "status")))
+        self._check(self.lib.cima_hip_kv_pages_fork(self.handle, self._kv(kv), self._op(parents, _I32, n, "parents"),
+                                                    self._op(children, _I32, n, "children"), n,
+                                                    self._op(status, _I32, 1, "status")))
 
     def kv_pages_free(self, kv, slots, n: int) -> None:
         """The slots give their pages back and are free."""
-        self._check(self.lib.cima_hip_kv_pages_free(self.handle, kv.ref, _ptr_of(slots, _I32, n, "slots"), n))
+        self._check(self.lib.cima_hip_kv_pages_free(self.handle, self._kv(kv), self._op(slots, _I32, n, "slots"), n))
 
     def kv_pages_compact(self, kv, refs_out, table_out, n_live, slab) -> None:
         """The pages in use move together to the front of the pool; the new counts
         and table go to ``refs_out`` and ``table_out`` (or are the cache's own)."""
         self._check(self.lib.cima_hip_kv_pages_compact(
-            self.handle, kv.ref, _ptr_of(refs_out, _I32, kv.n_pages, "refs_out"),
-            _ptr_of(table_out, _I32, kv.table.numel(), "table_out"), _ptr_of(n_live, _I32, 1, "n_live"), *_slab(slab)))
+            self.handle, self._kv(kv), self._op(refs_out, _I32, kv.n_pages, "refs_out"),
+            self._op(table_out, _I32, kv.table.numel(), "table_out"), self._op(n_live, _I32, 1, "n_live"), *_slab(slab)))
 
     # -- sampling ---------------------------------------------------------------
     def softmax_rows(self, x, y, rows: int, n: int, temp=None, rows_per_temp: int = 1, cap: float = 0.0,
@@ -589,8 +599,8 @@ class HipCtx:
             raise EngineError("hip", E_INVALID, f"rows_per_temp is {rows_per_temp}")
         act = _act_of(x)
         self._check(self.lib.cima_hip_softmax_rows(
-            self.handle, _ptr_of(x, _F16 if act else _F32, rows * n, "x"), _ptr_of(y, _F32, rows * n, "y"), rows, n,
-            _ptr_of(temp, _F32, -(-rows // rows_per_temp), "temp"), rows_per_temp, cap, act, *_slab(slab)))
+            self.handle, self._op(x, _F16 if act else _F32, rows * n, "x"), self._op(y, _F32, rows * n, "y"), rows, n,
+            self._op(temp, _F32, -(-rows // rows_per_temp), "temp"), rows_per_temp, cap, act, *_slab(slab)))
 
     def verify_drafts(self, p, q, drafts, counts, u, accepted, tokens, lens, seqs: int, n_draft: int, vocab: int,
                       slab) -> None:
@@ -599,10 +609,10 @@ class HipCtx:
         None: no lengths to advance."""
         k = n_draft + 1
         self._check(self.lib.cima_hip_verify_drafts(
-            self.handle, _ptr_of(p, _F32, seqs * k * vocab, "p"), _ptr_of(q, _F32, seqs * n_draft * vocab, "q"),
-            _ptr_of(drafts, _I32, seqs * n_draft, "drafts"), _ptr_of(counts, _I32, seqs, "counts"),
-            _ptr_of(u, _F32, seqs * k, "u"), _ptr_of(accepted, _I32, seqs, "accepted"),
-            _ptr_of(tokens, _I32, seqs * k, "tokens"), _ptr_of(lens, _I32, seqs, "lens"), seqs, n_draft, vocab,
+            self.handle, self._op(p, _F32, seqs * k * vocab, "p"), self._op(q, _F32, seqs * n_draft * vocab, "q"),
+            self._op(drafts, _I32, seqs * n_draft, "drafts"), self._op(counts, _I32, seqs, "counts"),
+            self._op(u, _F32, seqs * k, "u"), self._op(accepted, _I32, seqs, "accepted"),
+            self._op(tokens, _I32, seqs * k, "tokens"), self._op(lens, _I32, seqs, "lens"), seqs, n_draft, vocab,
             *_slab(slab)))
 
     def stream_read_cfg(self, src, nbytes: int, sink, dest: int, depth: int, width: int = 16,

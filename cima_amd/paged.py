@@ -46,7 +46,7 @@ class PagedKV:
             _bad("the pool is not on a HIP device")
         self.pool, self.refs, self.table, self.lens = pool, refs, table, lens
         self.layers, self.n_pages, self.kv_heads, self.page, self.head_dim = planes // 2, n_pages, heads, page, dim
-        self.max_seqs = lens.shape[0]
+        self.max_seqs, self.device = lens.shape[0], pool.get_device()
         self.desc = KvPages(pool.data_ptr(), pool.stride(0), refs.data_ptr(), table.data_ptr(), lens.data_ptr(), planes,
                             n_pages, heads, page, dim, self.max_seqs, table.shape[1])
         self.ref = ctypes.byref(self.desc)

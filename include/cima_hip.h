@@ -423,8 +423,11 @@ int cima_hip_decode_step(cima_hip_ctx* ctx, const cima_decoder* d);
  * position t of its sequence in row t % page of page table[s * table_stride +
  * t / page]; unused entries are -1.  lens[s] is its number of cached tokens,
  * -1 where the slot is not in use.  refs[i] counts the slots that hold page
- * i: 0 = free.  page is a power of two from 16 to 256; pool is 16-byte
- * aligned and plane_elems a multiple of 8. */
+ * i: 0 = free.  page is a power of two from 16 to 256, head_dim 64 or 128, at
+ * most 1048576 pages, 4096 slots and 2^30 positions a slot; pool is 16-byte
+ * aligned and plane_elems a multiple of 8.  A page that several slots hold is
+ * full: cima_hip_kv_pages_fork copies one that is begun, so that no two slots
+ * append to the same. */
 typedef struct cima_kv_pages {
     void* pool;             /* f16 planes of [n_pages, kv_heads, page, head_dim] */
     long long plane_elems;  /* elements from one plane to the next */
@@ -443,7 +446,7 @@ typedef struct cima_kv_pages {
  * 0.008); theta 0 = no rotation.  lens is not changed: every layer of the step
  * appends at the same positions.  Slots not in use write nothing, neither q;
  * positions without a page (entry -1 or behind the row) write no key.
- * head_dim 64 or 128; qkv and q 16-byte aligned. */
+ * qkv and q 16-byte aligned, not overlapping. */
 int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* qkv, void* q,
                                int seqs, int n_new, int q_heads, float theta);
 
@@ -460,8 +463,9 @@ int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int l
  * The work is split over the positions where there are few rows, as long as
  * the slab (256-byte aligned) holds the partial sums: rows * q_heads *
  * (head_dim + 2) * 4 bytes per part, rows = seqs * n_new.  Two parts are
- * needed where prefix_pages > 0, else none.  head_dim 64 or 128; q_heads a
- * multiple of kv_heads; scale positive; q and out 16-byte aligned. */
+ * needed where prefix_pages > 0, else none; 192 are the most that are used.
+ * q_heads a multiple of kv_heads, rows * q_heads at most 2^24; scale positive;
+ * q and out 16-byte aligned, not overlapping. */
 int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* q, void* out, int seqs,
                         int n_new, int q_heads, float scale, int prefix_pages, int prefix_slot, int window, void* slab,
                         unsigned long long slab_bytes);
@@ -474,7 +478,8 @@ int cima_hip_kv_pages_copy(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int
  * [lens / page, (lens + n_new - 1) / page] that are -1 take the lowest free
  * pages, slot by slot, with count 1.  All or nothing: *status = 0, or the
  * number of pages that are missing, and nothing is changed.  Entries behind
- * table_stride count as missing.  n_pages at most 1048576. */
+ * table_stride count as missing (at most 262144 a slot).  Behind a slot's first
+ * -1 there is no page. */
 int cima_hip_kv_pages_reserve(cima_hip_ctx* ctx, const cima_kv_pages* kv, int seqs, int n_new, int* status);
 /* Slot children[i] becomes a copy of slot parents[i], i < n: the pages that
  * the parent has filled are shared (counts + 1), the rows of a page begun are
@@ -491,7 +496,7 @@ int cima_hip_kv_pages_free(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int
  * from L on takes the k-th free page below L, in every plane.  The new counts
  * and table go to refs_out and table_out (of refs' and table's sizes; they may
  * be refs and table themselves), L to *n_live.  slab: 12 n_pages + 64 bytes,
- * 4-byte aligned.  n_pages at most 1048576. */
+ * 4-byte aligned. */
 int cima_hip_kv_pages_compact(cima_hip_ctx* ctx, const cima_kv_pages* kv, int* refs_out, int* table_out, int* n_live,
                               void* slab, unsigned long long slab_bytes);
 
@@ -500,8 +505,9 @@ int cima_hip_kv_pages_compact(cima_hip_ctx* ctx, const cima_kv_pages* kv, int* r
  * where cap > 0 (as cima_hip_argmax), else v.  temp NULL = 1; where it is <= 0
  * the row is 1 at its largest logit (the lowest index of equals) and 0
  * elsewhere.  A row of -inf alone becomes zeros; NaN or +inf make a row NaN
- * (temp <= 0: they rank as the largest do, NaN as the lowest).  slab (8-byte
- * aligned): 16 bytes for each 8192 logits of a row (rounded up) and row. */
+ * (temp <= 0: +inf ranks as the largest, NaN as the lowest).  x and y do not
+ * overlap.  slab (8-byte aligned): 16 bytes for each 8192 logits of a row
+ * (rounded up) and row; none is needed up to 32768 logits. */
 int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, int n, const float* temp,
                           int rows_per_temp, float cap, int x_dtype, void* slab, unsigned long long slab_bytes);
 
@@ -514,8 +520,8 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
  * outside [0, vocab) is refused).  After a first refusal at row a the next token is
  * drawn from max(p[a] - q[a], 0), after all were kept from p[count]: the lowest
  * t whose running sum passes u[n_draft] times the whole (sums in fp64; NaN and
- * negative values count 0; where nothing is left, from p[a]; where that holds
- * nothing, -1).  tokens [seqs, n_draft + 1] = the kept drafts, the drawn token,
+ * negative values count 0, infinite ones are not allowed; where nothing is
+ * left, from p[a]; where that holds nothing, -1).  tokens [seqs, n_draft + 1] = the kept drafts, the drawn token,
  * then -1; accepted[s] = drafts kept.  lens (may be NULL): lens[s] += accepted
  * + 1 where lens[s] >= 0; slots with lens[s] < 0 get accepted 0 and tokens -1.
  * n_draft 0 draws one token a row.  slab (8-byte aligned): for each slot 8

@@ -183,6 +183,57 @@ def test_attention_second_layer_and_many_pages(hip):
     _check(hip, Batch([33000, 32768], 1, (2, 2, 64), 16, 32768, seed=13), slab_mb=0.01)
 
 
+@pytest.mark.parametrize("seqs", [40, 70])
+def test_attention_of_many_rows_over_more_pages_than_are_kept(hip, seqs):
+    """One part over 33000 positions in pages of 16, tiles of 64 and 128 rows."""
+    b = Batch([33008 + s % 5 for s in range(seqs)], 1, (1, 1, 64), 16, 33008, seed=16)
+    q = b.r.standard_normal((b.rows, 1, 64)).astype(np.float16)
+    got = _attend(hip, b, q, slab_mb=2.2 * seqs * 66 * 4 / (1 << 20))
+    pick = [0, 33, seqs - 1]
+    b.lens = [n if s in pick else -1 for s, n in enumerate(b.lens)]
+    want, tol = b.want(q, 1.0 / 8, 0)
+    # fp32 sums of 33000 positions: 2^-24 a term, in the worst case all one way
+    assert (np.abs(got - want)[pick] <= (tol + 33000 * 2.0 ** -24 * 4)[pick]).all()
+
+
+def test_attention_leaves_rows_behind_the_last_slot(hip):
+    b = Batch([100, 64, 90], 2, (8, 2, 128), 32, 64, seed=17)
+    q = torch.from_numpy(b.r.standard_normal((20, 8, 128)).astype(np.float16)).cuda()
+    out = torch.full((20, 8, 128), 5.0, dtype=torch.float16, device="cuda")
+    hip.attn_paged(b.kv, 0, q, out, 2, 2, 8, 0.1, torch.empty(1 << 20, dtype=torch.uint8, device="cuda"), prefix_pages=2)
+    torch.cuda.synchronize()
+    assert (out[4:] == 5.0).all() and not (out[:4] == 5.0).all()
+
+
+def test_lengths_and_entries_out_of_range_do_no_harm(hip):
+    """Lengths behind the table, entries that name no page: nothing is written
+    outside, and the other slots' results are what they are alone."""
+    big = 2 ** 31 - 2
+    b = Batch([70, 64, 90], 3, (8, 2, 64), 32, 64, seed=18)
+    q = b.r.standard_normal((b.rows, 8, 64)).astype(np.float16)
+    want = _attend(hip, b, q)
+    b.kv.lens[1] = big
+    b.kv.table[2, 2:] = torch.tensor([10 ** 6] * (b.table.shape[1] - 2), dtype=torch.int32, device="cuda")
+    got = _attend(hip, b, q)
+    assert np.array_equal(got[:3], want[:3])
+    pool = b.kv.pool.clone()
+    qkv = torch.zeros((9, 12 * 64), dtype=torch.float16, device="cuda")
+    hip.rope_append_paged(b.kv, 0, qkv, torch.empty((9, 8, 64), dtype=torch.float16, device="cuda"), 3, 3, 8, 1e4)
+    status = _i32([3])
+    hip.kv_pages_reserve(b.kv, 3, 5, status)
+    assert int(status.item()) > 0                       # behind the row
+    b.kv.lens[0] = -1
+    refs = b.kv.refs.clone()
+    hip.kv_pages_fork(b.kv, _i32([1]), _i32([0]), 1, status)
+    assert int(status.item()) == -1 and int(b.kv.lens[0].item()) == -1
+    torch.cuda.synchronize()
+    same = (b.kv.pool == pool).all(-1)                  # [planes, pages, heads, rows]
+    mine = torch.zeros_like(same)
+    for p in range(70, 73):
+        mine[:, int(b.table[0, p // 32]), :, p % 32] = True
+    assert (same | mine).all() and torch.equal(refs, b.kv.refs)
+
+
 def test_attention_scores_far_apart(hip):
     """Scores over hundreds of powers of two, rising and falling along the
     positions: the running maximum is raised often, old sums vanish."""

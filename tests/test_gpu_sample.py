@@ -77,6 +77,23 @@ def test_softmax_of_strided_starts_and_no_temp(hip):
             assert (got[off + 9 * 4099:] == -3.0).all() and (off == 0 or (got[:off] < 1.01).all())
 
 
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("rows,n", [(130, 33001), (128, 65536), (127, 40000), (130, 65537), (3, 32768), (3, 32769)])
+def test_softmax_on_both_sides_of_every_path(hip, dtype, rows, n):
+    """Rows to a workgroup or in parts, by their length and number."""
+    r = np.random.default_rng(rows + n)
+    x = (r.standard_normal((rows, n), np.float32) * 3).astype(dtype)
+    temp = np.where(np.arange(rows) % 5 == 1, 0, r.uniform(0.4, 1.4, rows)).astype(np.float32)
+    y = torch.empty((rows, n), device="cuda")
+    hip.softmax_rows(_cuda(x), y, rows, n, _cuda(temp), 1, 0.0, _slab())
+    torch.cuda.synchronize()
+    y = y.cpu().numpy()
+    for i in range(0, rows, 3):
+        want, tol = _softmax_want(x[i:i + 1], temp[i:i + 1], 1, 0.0)
+        assert (np.abs(y[i:i + 1] - want) <= tol).all(), i
+    assert np.allclose(y.sum(1, dtype=np.float64), 1, atol=1e-5)
+
+
 @pytest.mark.parametrize("n", [5, 9000, 40000])
 def test_softmax_edges(hip, n):
     """Rows of -inf become zeros, temperature 0 takes the first of equal
@@ -306,9 +323,12 @@ def test_refusals(hip):
     no(hip.softmax_rows, x, y, 2, 100, y[0, :1], 1, 0.0, slab)
     no(hip.softmax_rows, x, y.half(), 2, 100, None, 1, 0.0, slab)
     no(hip.softmax_rows, x.bfloat16(), y, 2, 100, None, 1, 0.0, slab)
-    no(hip.softmax_rows, x, y, 2, 100, None, 1, 0.0, slab[:16])
-    no(hip.softmax_rows, x, y, 2, 100, None, 1, 0.0, None)
-    no(hip.softmax_rows, x, y, 2, 100, None, 1, 0.0, slab[4:])
+    hip.softmax_rows(x, y, 2, 100)                      # short rows need no slab
+    long = torch.zeros(2 * 40000, device="cuda")
+    hip.softmax_rows(long, long.clone(), 2, 40000, None, 1, 0.0, slab[:160])
+    no(hip.softmax_rows, long, long.clone(), 2, 40000, None, 1, 0.0, slab[:152])
+    no(hip.softmax_rows, long, long.clone(), 2, 40000)
+    no(hip.softmax_rows, long, long.clone(), 2, 40000, None, 1, 0.0, slab[4:])
     hip.verify_drafts(x, y, i, None, y, i, i, None, 1, 1, 100, slab)
     hip.verify_drafts(x, y, i, None, y, i, i, None, 0, 1, 100, slab)
     no(hip.verify_drafts, x, y, i, None, y, i, i, None, 2, 1, 100, slab)

@@ -81,11 +81,11 @@ def test_paged_kv_refuses_wrong_tensors():
 def test_binding_checks_element_types_and_sizes(monkeypatch):
     monkeypatch.setattr(hipmod, "_ptr", lambda a: 4096)
     t = torch.zeros(6, dtype=torch.int32)
-    assert hipmod._ptr_of(t, hipmod._I32, 6, "x") == 4096
+    assert hipmod._ptr_of(t, hipmod._I32, 6, "x", -1) in (4096, t.data_ptr())
     assert hipmod._ptr_of(None, hipmod._I32, 6, "x") is None and hipmod._ptr_of(64, hipmod._I32, 6, "x") == 64
-    for a, n in ((t, 7), (t.long(), 6), (t.float(), 6)):
+    for a, n, device in ((t, 7, -1), (t.long(), 6, -1), (t.float(), 6, -1), (t, 6, 0), (t, 6, 1)):
         with pytest.raises(hipmod.EngineError):
-            hipmod._ptr_of(a, hipmod._I32, n, "x")
+            hipmod._ptr_of(a, hipmod._I32, n, "x", device)
 
 
 def test_kernels_do_not_spill():
