@@ -22,27 +22,28 @@ struct SmPart {
     int at, pad;
 };
 
-// four logits from element i on, those behind n as -inf: a lane's word, so that
-// loads and stores of a wave are contiguous
-template <bool F32>
-DEV void sm_load(const void* __restrict__ x, size_t row, int i, int n, uint32_t (&v)[F32 ? 4 : 2]) {
-    if (i + 4 <= n) {
-        if constexpr (F32) __builtin_memcpy(v, __builtin_assume_aligned((const float*)x + row + i, 4), 16);
-        else __builtin_memcpy(v, __builtin_assume_aligned((const uint16_t*)x + row + i, 2), 8);
+// V logits from element i on, those behind n as -inf: a lane's word.  Four, so
+// that the probabilities of a wave are written contiguously; eight of f16 where
+// nothing is written.
+template <bool F32, int V>
+DEV void sm_load(const void* __restrict__ x, size_t row, int i, int n, uint32_t (&v)[F32 ? V : V / 2]) {
+    if (i + V <= n) {
+        if constexpr (F32) __builtin_memcpy(v, __builtin_assume_aligned((const float*)x + row + i, 4), 4 * V);
+        else __builtin_memcpy(v, __builtin_assume_aligned((const uint16_t*)x + row + i, 2), 2 * V);
     } else if constexpr (F32) {
 #pragma unroll
-        for (int j = 0; j < 4; j++) v[j] = i + j < n ? ((const uint32_t*)x)[row + i + j] : 0xff800000u;
+        for (int j = 0; j < V; j++) v[j] = i + j < n ? ((const uint32_t*)x)[row + i + j] : 0xff800000u;
     } else {
 #pragma unroll
-        for (int j = 0; j < 4; j += 2) {
+        for (int j = 0; j < V; j += 2) {
             const uint32_t a = i + j < n ? ((const uint16_t*)x)[row + i + j] : 0xfc00u;
             const uint32_t b = i + j + 1 < n ? ((const uint16_t*)x)[row + i + j + 1] : 0xfc00u;
             v[j / 2] = a | b << 16;
         }
     }
 }
-template <bool F32>
-DEV float sm_get(const uint32_t (&v)[F32 ? 4 : 2], int j) {
+template <bool F32, int V>
+DEV float sm_get(const uint32_t (&v)[F32 ? V : V / 2], int j) {
     if constexpr (F32) {
         const uint32_t a = v[j];
         return __builtin_bit_cast(float, a);
@@ -53,43 +54,40 @@ DEV float sm_get(const uint32_t (&v)[F32 ? 4 : 2], int j) {
 DEV float uniform(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
 }
-// whether (a, i) ranks before (b, j): larger, or equal and at a lower place
-DEV bool sm_before(float a, int i, float b, int j) { return a > b || (a == b && i < j); }
-
 // f of a logit; those behind n stay -inf
 DEV float sm_f(float x, int i, int n, float cap) { return i < n ? cap * tanhf(x / cap) : x; }
 
-// R words a thread of a row by NT threads: the maximum, the first place of it
+// R words of V logits a thread of a row by NT threads: the maximum, the first place of it
 // (T <= 0) or the sum (T > 0).  CAP: f is applied when the logits are loaded,
 // which are fp32 from there on.
-template <bool F32, bool CAP, int NT, int R>
+template <bool F32, bool CAP, int NT, int R, int V = 4>
 struct SmRow {
     static constexpr bool W32 = F32 || CAP;
-    uint32_t v[R][W32 ? 4 : 2];
+    uint32_t v[R][W32 ? V : V / 2];
     int base;
     float m, l;
     int at;
 
-    DEV float get(int r, int j) const { return sm_get<W32>(v[r], j); }
+    DEV float get(int r, int j) const { return sm_get<W32, V>(v[r], j); }
     // keeps the compiler from holding all logits as fp32 from one pass to the next
     DEV void fresh() {
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int k = 0; k < (W32 ? 4 : 2); k++) __asm__ volatile("" : "+v"(v[r][k]));
+            for (int k = 0; k < (W32 ? V : V / 2); k++) __asm__ volatile("" : "+v"(v[r][k]));
     }
     DEV void load(const void* __restrict__ x, size_t row, int first, int n, float cap) {
-        base = first + threadIdx.x * 4;
+        base = first + threadIdx.x * V;
 #pragma unroll
         for (int r = 0; r < R; r++) {
             if constexpr (CAP) {
-                uint32_t w[F32 ? 4 : 2];
-                const int i = base + r * NT * 4;
-                sm_load<F32>(x, row, i, n, w);
+                uint32_t w[F32 ? V : V / 2];
+                const int i = base + r * NT * V;
+                sm_load<F32, V>(x, row, i, n, w);
 #pragma unroll
-                for (int j = 0; j < 4; j++) v[r][j] = __builtin_bit_cast(uint32_t, sm_f(sm_get<F32>(w, j), i + j, n, cap));
+                for (int j = 0; j < V; j++) v[r][j] = __builtin_bit_cast(uint32_t, sm_f(sm_get<F32, V>(w, j), i + j, n, cap));
             } else {
-                sm_load<F32>(x, row, base + r * NT * 4, n, v[r]);
+                sm_load<F32, V>(x, row, base + r * NT * V, n, v[r]);
             }
         }
     }
@@ -101,7 +99,7 @@ struct SmRow {
 #pragma unroll
         for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int j = 0; j < 4; j++) m = fmaxf(m, get(r, j));
+            for (int j = 0; j < V; j++) m = fmaxf(m, get(r, j));
         m = wave_max_u(m);
         if ((threadIdx.x & 63) == 0) red[0][w] = m;
         __syncthreads();
@@ -116,7 +114,7 @@ struct SmRow {
             for (int r = 0; r < R; r++) {
                 float p = 0.f;
 #pragma unroll
-                for (int j = 0; j < 4; j++) p += __builtin_amdgcn_exp2f((get(r, j) - c) * s);
+                for (int j = 0; j < V; j++) p += __builtin_amdgcn_exp2f((get(r, j) - c) * s);
                 l += p;
             }
             l = wave_sum_u(l);
@@ -126,8 +124,8 @@ struct SmRow {
 #pragma unroll
             for (int r = R - 1; r >= 0; r--)
 #pragma unroll
-                for (int j = 3; j >= 0; j--)
-                    if (get(r, j) == m && m != -INFINITY) at = base + r * NT * 4 + j;
+                for (int j = V - 1; j >= 0; j--)
+                    if (get(r, j) == m && m != -INFINITY) at = base + r * NT * V + j;
 #pragma unroll
             for (int o = 32; o; o >>= 1) at = min(at, __shfl_xor(at, o));
             if ((threadIdx.x & 63) == 0) place[w] = at;
@@ -150,15 +148,16 @@ struct SmRow {
     // of the half exponent's power: the exponential itself would flush results
     // below 2^-126
     DEV void write(float* __restrict__ y, size_t row, int n, float T, float M, int A, float L) const {
+        static_assert(V == 4, "a 16-byte store a word");
         const bool none = M == -INFINITY && L == 0.f;  // -inf alone
         const float c = M == -INFINITY ? 0.f : M, inv = none ? 0.f : 1.f / L;
         const float s = 0.72134752044448170368f / T;
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            const int i = base + r * NT * 4;
+            const int i = base + r * NT * V;
             float p[4];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
+            for (int j = 0; j < V; j++) {
                 const float h = __builtin_amdgcn_exp2f((get(r, j) - c) * s);
                 p[j] = T > 0.f ? h * (h * inv) : (i + j == A ? 1.f : 0.f);
             }
@@ -168,7 +167,7 @@ struct SmRow {
                 __builtin_nontemporal_store((f4u){p[0], p[1], p[2], p[3]}, (f4u*)o);
             } else {
 #pragma unroll
-                for (int j = 0; j < 4; j++)
+                for (int j = 0; j < V; j++)
                     if (i + j < n) o[j] = p[j];
             }
             __builtin_amdgcn_sched_barrier(0);  // a word at a time: the row fills the registers
@@ -182,21 +181,20 @@ constexpr int SM_PART = SM_T * SM_R * 4;   // its logits
 // a row's parts joined by every wave: lane i takes parts i, i + 64, ...
 DEV float sm_join(const SmPart* __restrict__ p, int parts, float T, int* at, float* L) {
     const int lane = threadIdx.x & 63;
-    float m = -INFINITY;
+    float m = -INFINITY, l = 0.f;
+    for (int i = lane; i < parts; i += 64) m = fmaxf(m, p[i].m);
+    m = wave_max_u(m);
     int a = 0x7fffffff;
-    for (int i = lane; i < parts; i += 64)
-        if (sm_before(p[i].m, p[i].at, m, a)) m = p[i].m, a = p[i].at;
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        const float om = __shfl_xor(m, o);
-        const int oa = __shfl_xor(a, o);
-        if (sm_before(om, oa, m, a)) m = om, a = oa;
-    }
-    float l = 0.f;
     if (T > 0.f) {
         const float c = m == -INFINITY ? 0.f : m, s = 1.44269504088896340736f / T;
         for (int i = lane; i < parts; i += 64)
             l += p[i].l * (p[i].m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((p[i].m - c) * s));
+    } else {
+        // the first of the parts that have the maximum has its first place
+        for (int i = lane; i < parts; i += 64)
+            if (p[i].m == m) a = min(a, p[i].at);
+#pragma unroll
+        for (int o = 32; o; o >>= 1) a = min(a, __shfl_xor(a, o));
     }
     *L = wave_sum_u(l);
     *at = a;
@@ -207,7 +205,7 @@ DEV float sm_join(const SmPart* __restrict__ p, int parts, float T, int* at, flo
         const void* __restrict__ x, SmPart* __restrict__ part, int n, const float* __restrict__ temp,                  \
         int rows_per_temp, float cap, int parts) {                                                                     \
         const int row = blockIdx.x / parts, pt = blockIdx.x % parts;                                                   \
-        SmRow<F32, CAP, SM_T, SM_R> R;                                                                                 \
+        SmRow<F32, CAP, SM_T, F32 ? SM_R : SM_R / 2, F32 ? 4 : 8> R;                                                   \
         R.load(x, (size_t)row * n, pt * SM_PART, n, cap);                                                              \
         R.stats(temp ? temp[row / rows_per_temp] : 1.f);                                                               \
         if (threadIdx.x == 0) part[blockIdx.x] = SmPart{R.m, R.l, R.at, 0};                                            \
@@ -276,29 +274,38 @@ constexpr int KEPT_REFUSED = 1 << 30;
 // Drafts kept of slot s (-1: the slot is not in use), by the whole wave; the
 // row whose residual is drawn from is p[kept] less q[kept] where `*refused`.
 DEV int vf_kept(const VfArgs& A, int s, bool* refused) {
-    if (A.lens && A.lens[s] < 0) return -1;
-    int count = A.counts ? A.counts[s] : A.n_draft;
-    count = max(0, min(count, A.n_draft));
     const int lane = threadIdx.x & 63;
+    // what the answer needs is fetched together, whether it is used or not
+    const int len = A.lens ? A.lens[s] : 0;
+    int count = A.counts ? A.counts[s] : A.n_draft;
+    int d = -1;
+    float u = 0.f;
+    auto fetch = [&](int i) {
+        d = i < A.n_draft ? A.drafts[(size_t)s * A.n_draft + i] : -1;
+        u = i < A.n_draft ? A.u[(size_t)s * (A.n_draft + 1) + i] : 0.f;
+    };
+    fetch(lane);
+    count = max(0, min(count, A.n_draft));
+    *refused = false;
+    if (len < 0) return -1;
     for (int i0 = 0; i0 < count; i0 += 64) {
         const int i = i0 + lane;
+        if (i0) fetch(i);
         bool no = false;
         if (i < count) {
-            const int d = A.drafts[(size_t)s * A.n_draft + i];
             no = true;
             if ((unsigned)d < (unsigned)A.vocab) {
                 const double pd = A.p[((size_t)s * (A.n_draft + 1) + i) * A.vocab + d];
                 const double qd = A.q ? A.q[((size_t)s * A.n_draft + i) * A.vocab + d] : 1.f;
-                no = !((double)A.u[(size_t)s * (A.n_draft + 1) + i] * qd < pd);
+                no = !((double)u * qd < pd);
             }
         }
         const unsigned long long b = __ballot(no);
         if (b) {
             *refused = true;
-            return i0 + __ffsll((unsigned long long)b) - 1;
+            return i0 + __ffsll(b) - 1;
         }
     }
-    *refused = false;
     return count;
 }
 // eight entries of the residual from i on, those behind the vocabulary 0
