@@ -1724,8 +1724,16 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
         return fail(CIMA_E_INVALID, "%s: a slab of %llu bytes does not hold %d parts of %lld", api, slab_bytes, least,
                     part_bytes);
     const int own_rows = n_new * g;
-    const bool few = prefix_pages && head_rows <= 32;  // the prefix tasks run with the own tasks
-    const int nb = std::max(own_rows, few ? head_rows : 0) > 16 ? 2 : 1;
+    // Up to 16 rows the prefix runs in the own tasks' kernel, whose waves fetch
+    // for themselves; above, in tiles of 64 rows, from 65 rows on of 128.  us,
+    // one side / the other: 16 rows of 128, 8000 positions 14.8 / 17.4, 8 rows, 512
+    // 9.0 / 10.0, 24 rows, 8000 20.9 / 16.6; 64 rows a tile / 128: 40 rows 17.8 /
+    // 19.0, 80 rows 20.3 / 20.4, 63 rows of 64 17.2 / 18.7.
+    const bool few = prefix_pages && head_rows <= 16;
+    // Own tasks of more than 16 rows take 32 at a time, the pages read half as
+    // often.  64 slots of up to 4000 positions, 32 rows: 103 us by 16, 77 by 32; of
+    // up to 600: 41 and 36 (128 a head), 27.6 and 29.6 (64).
+    const int nb = own_rows > 16 ? 2 : 1;
     const int own_tiles = (own_rows + 16 * nb - 1) / (16 * nb);
     const long long own_base = (long long)seqs * kv->kv_heads * own_tiles;
     const long long own_room = (long long)(kv->table_stride - prefix_pages) * kv->page;
@@ -1743,13 +1751,16 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     long long pre = 0;
     if (prefix_pages) {
         const int per = 64 * mode;  // rows of a tile
-        tiles = few ? (head_rows + 16 * nb - 1) / (16 * nb) : (head_rows + per - 1) / per;
+        tiles = few ? 1 : (head_rows + per - 1) / per;
         const long long base = (long long)kv->kv_heads * tiles, len = (long long)prefix_pages * kv->page;
         // a workgroup to a CU; two where each still has 512 positions, half of one
-        // where the own tasks have much to read (256 KB a CU in full tables)
+        // where the own tasks have much to read (256 KB a CU in full tables).  With
+        // the join, half of that / that / twice that: 128 slots of 8 heads of 128 over
+        // 65536 235 / 184 / 193 us, 32 slots over 30016 51.7 / 39.6 / 45.6, over 8000
+        // 27.0 / 25.4 / 33.4, over 8000 with up to 1023 own 34.8 / 28.8 / 34.5.
         const long long own_bytes = 4LL * seqs * kv->kv_heads * own_room * dim;
         long long want = ctx->num_cu;
-        if (few || len * base >= 1024LL * ctx->num_cu) want *= 2;
+        if (len * base >= 1024LL * ctx->num_cu) want *= 2;
         else if (own_bytes >= (256LL << 10) * ctx->num_cu) want /= 2;
         pre = std::min((want + base - 1) / base, (len + 127) / 128);
         pre = std::max(1LL, std::min(pre, 128LL));
@@ -1787,7 +1798,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     A.row_tiles = tiles;
     A.scale2 = scale * 1.44269504088896340736f;
     A.least_tiles = least_tiles;
-    A.prefix_tile = few ? 16 * nb : 32;
+    A.prefix_tile = few ? 16 : 32;
     A.own_tile = 16 * nb;
     char name[64];
     hipFunction_t f;

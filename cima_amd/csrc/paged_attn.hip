@@ -9,7 +9,12 @@
 // rows alone (own tasks).  Both kinds run the same code on a tile of rows and a
 // range of positions and leave {m, l, sum} per row; a second launch joins them.
 //
-// Both products run on the matrix cores with 32 x 32 x 16 f16 MFMA.  S^T = K
+// Rounding: q, keys and values are f16 as given; scores, maxima, sums of weights
+// and of values are fp32.  The weights are rounded to f16 for the second product,
+// by at most 2^-11 of each, their sum l is not: an error of at most 2^-11 of sum
+// w |v| / sum w, as the result's own rounding.  Partial sums stay fp32.
+//
+// Both products of a row tile run on the matrix cores with 32 x 32 x 16 f16 MFMA.  S^T = K
 // Q^T: a lane then holds the scores of ONE row (column lane % 32) for half of
 // the 32 keys, so that the row maximum and sum are per-lane operations and one
 // exchange between the halves of the wave, and the probabilities are in the
@@ -129,10 +134,20 @@ struct Tile {
     // the merge of WK waves' sums reuses the ring
     static_assert(WK == 1 || (WK - 1) * WR * 64 * (D / 32) * 16 * 4 <= RING, "merge space");
     static constexpr int LDS = RING + IDS * 4 + NW * 32;
+    static_assert(LDS <= 80 * 1024, "two workgroups to a CU");
 };
 
-// Rows [r0, r0 + 32 WR) of [ra, rb) (row r of a kv head: head r % g, token r /
+// Rows [r0, r0 + 32 WR) of [0, rb) (row r of a kv head: head r % g, token r /
 // g), positions [plo, phi), part `part` of `parts`, results to column `col`.
+//
+// Bound by issue: beside a tile's MFMA stand 32 exponentials a lane, the
+// conversions and the reads of its fragments.  64 positions a tile, two tiles in
+// LDS (64 KB), two workgroups of four waves to a CU: 250 registers hold 32 rows'
+// sums, two tiles' scores and q; the two workgroups cover each other's barriers.
+// Measured on MI355X, 128 slots of 4 x 8 heads of 128 over 65536 positions (137
+// GFLOP): 158 us, 870 TFLOP/s; without exponentials, copies and barriers
+// 108.  One workgroup of eight waves and 256 rows, which copies half as much:
+// 176; 64 rows a wave: 572, its registers spill.
 template <int D, int WR, int WK>
 DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int plo, int phi, const int* trow,
                    int part, int parts, int col) {
@@ -477,20 +492,23 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 
 // ------------------------------------------------------------- few rows
 //
-// Tasks of up to 16 NB rows (own tasks; prefix tasks where there are few
-// rows): bound by reading the keys and values, and short ones by the latency
-// of their chain of loads.  The four waves of a workgroup take 32-position
+// Tasks of up to 16 NB rows (own tasks; prefix tasks of up to 16 rows): bound by
+// reading the keys and values, and short ones by the latency of their chain of
+// loads (lengths, ids, pages).  The four waves of a workgroup take 32-position
 // tiles in turn and do not wait for each other: keys go straight from memory
 // to the registers of the A operand (16 x 16 x 32 MFMA: a lane holds 16 bytes
-// of a key), values by direct copies to the wave's own LDS, one tile ahead.
-// The waves' sums are added at the end, in wave order.
+// of a key), values by direct copies to the wave's own LDS.  The waves' sums are
+// added at the end, in wave order.  Rounding: the weights to f16, as in the row
+// tiles; sums, maxima and the waves' joining are fp32.
 //
 // BUFS 2: a tile is on its way while the one before it is computed, 64 KB of LDS
 // a workgroup, two of them to a CU.  BUFS 1: the loads of a tile are waited for,
 // but the registers and LDS suffice for four workgroups to a CU, whose waves
 // cover each other; it is taken where the launch holds nothing larger.
 // Measured on MI355X, 8 kv heads of 128, one / two in flight: 64 slots of up
-// to 4000 positions (524 MB) 107 / 146 us (4.9 TB/s), 128 of up to 500 27 / 33.
+// to 4000 positions (524 MB) 107 / 146 us (4.9 TB/s), 128 of up to 500 27 / 33;
+// 128 full slots of 8192 (4.3 GB) 765 us with the join, 5.6 TB/s.  Values by
+// loads to registers and LDS writes: 127 and 36 us.
 constexpr int few_bufs(int D, int mode, int nb) { return mode == 0 && !(D == 128 && nb == 2) ? 1 : 2; }
 constexpr int few_wgs(int D, int mode, int nb) { return few_bufs(D, mode, nb) == 1 ? 4 : 2; }
 template <int D, int NB, int BUFS>
@@ -499,6 +517,7 @@ struct Few {
     static constexpr int OB = NB * (D / 16) * 64 * 16;     // of a wave's sums
     static constexpr int WAVE = BUFS * VT > OB ? BUFS * VT : OB;  // LDS of a wave
     static constexpr int LDS = 4 * WAVE + 4 * NB * 16 * 8;
+    static_assert(LDS <= (BUFS == 1 ? 40 : 80) * 1024, "workgroups to a CU");
 };
 template <int D, int NB, int BUFS>
 DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int plo, int phi, const int* trow, int part,
@@ -736,9 +755,9 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
         }
     }
 }
-// One launch: first the prefix tasks (MODE 0: as few-row tasks, where all rows
-// fit one tile; 1 and 2: tiles of 64 and 128 rows), then the own tasks, one
-// slot's rows 16 NB at a time.  Workgroups go to the XCDs in turn; the row tiles
+// One launch: first the prefix tasks (MODE 0: as few-row tasks, up to 16 rows; 1
+// and 2: tiles of 64 and 128 rows), then the own tasks, one slot's rows 16 NB at
+// a time, so that they fill what the prefix tasks leave.  Workgroups go to the XCDs in turn; the row tiles
 // of one range of one kv head follow each other on the same XCD, so that all but
 // the first find its pages in that XCD's L2.
 template <int D, int MODE, int NB>
@@ -751,11 +770,13 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
         if (grp >= A.kv_heads * A.prefix_parts) return;
         const int kvh = grp / A.prefix_parts, part = grp % A.prefix_parts, phi = A.prefix_pages << A.page_shift;
         const int* trow = A.table + (size_t)A.prefix_slot * A.table_stride;
-        if (MODE == 0)
-            few_task<D, NB, BUFS>(A, lds, kvh, tile * 16 * NB, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
+        if constexpr (MODE == 0 && NB == 1)
+            few_task<D, NB, BUFS>(A, lds, kvh, 0, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
                             ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1);
-        else if (MODE == 1) attn_task<D, 2, 2>(A, lds, kvh, tile * 64, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
-        else attn_task<D, 4, 1>(A, lds, kvh, tile * 128, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
+        else if constexpr (MODE == 1)
+            attn_task<D, 2, 2>(A, lds, kvh, tile * 64, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
+        else if constexpr (MODE == 2)
+            attn_task<D, 4, 1>(A, lds, kvh, tile * 128, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
         return;
     }
     b -= A.prefix_wgs;
