@@ -665,7 +665,7 @@ int cima_hip_init(int device, const char* code_dir, cima_hip_ctx** out) {
     for (const char* kn : kSampleKernels)
         if (!rc) rc = add(MOD_SAMPLE, kn);
     for (const char* t : kSampleTypes)
-        for (const char* kn : {"stats", "probs", "t256_w2", "t256_w8", "t1024_w8"})
+        for (const char* kn : {"stats_w2", "probs_w2", "stats_w8", "probs_w8", "t256_w2", "t256_w8", "t1024_w8"})
             if (!rc) rc = add(MOD_SAMPLE, std::string("cima_softmax_") + kn + "_" + t);
     if (rc) {
         unload(ctx);
@@ -1658,7 +1658,7 @@ struct PagedAttnArgs {
     void* ml;
     int seqs, n_new, q_heads, kv_heads, page_shift, n_pages, table_stride;
     int prefix_pages, prefix_slot, window;
-    int prefix_parts, own_parts, row_tiles, prefix_tile, own_tile, prefix_wgs, least_tiles;
+    int prefix_parts, own_parts, row_tiles, prefix_tile, own_tile, prefix_wgs;
     float scale2;
 };
 
@@ -1739,14 +1739,15 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     const long long own_room = (long long)(kv->table_stride - prefix_pages) * kv->page;
     const int mode = !prefix_pages || few ? 0 : head_rows <= 64 ? 1 : 2;
     const int wgs = paged_few_wgs(dim, mode, nb);
-    // own tasks take 128 positions at least, twice that as often as it needs for
-    // the tasks of full tables not to pass four rounds of the chip (half of it
-    // where the prefix tasks take the other half)
-    const long long most = (mode ? 2LL : 4LL) * wgs * ctx->num_cu;
-    int least_tiles = 4;
-    auto parts_of = [&](int tiles) { return std::max(1LL, (own_room + 32LL * tiles - 1) / (32LL * tiles)); };
-    while (own_base * parts_of(least_tiles) > most && parts_of(least_tiles) > 1) least_tiles *= 2;
-    long long own = std::min(parts_of(least_tiles), 64LL);
+    // Parts of own tasks: as many as have 128 positions in a full table, in at most
+    // two rounds of the chip.  A slot's positions are shared by all of them (128 at
+    // least), so that slots of any length load the XCDs, which take workgroups in
+    // turn, alike.  8 kv heads of 128, one round / two / four: 64 slots of up to 4000
+    // 113 / 111 / 109 us, 128 of up to 6000 326 / 304 / 297, 64 of up to 2000 behind
+    // a prefix of 4096 72 / 65 / 63, but more for the join: 0 / 6 / 6 at 128 slots.
+    long long own = (own_room + 127) / 128;
+    while (own > 1 && own_base * own > 2LL * wgs * ctx->num_cu) own = (own + 1) / 2;
+    own = std::max(1LL, std::min(own, 64LL));
     int tiles = 0;
     long long pre = 0;
     if (prefix_pages) {
@@ -1797,7 +1798,6 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     A.own_parts = (int)own;
     A.row_tiles = tiles;
     A.scale2 = scale * 1.44269504088896340736f;
-    A.least_tiles = least_tiles;
     A.prefix_tile = few ? 16 : 32;
     A.own_tile = 16 * nb;
     char name[64];
@@ -1900,10 +1900,10 @@ int cima_hip_kv_pages_compact(cima_hip_ctx* ctx, const cima_kv_pages* kv, int* r
 // ------------------------------------------------------------------ sampling
 
 namespace {
-// logits of a part (SM_PART), rows from which on the longest that fit a workgroup
-// go to one each, entries that a part is a multiple of (VF_STEP) and most parts
-// of a row: sample_ops.hip
-const int kSoftmaxPart = 8192, kSoftmaxLongRows = 128, kVerifyStep = 2048, kVerifyParts = 64;
+// sample_ops.hip: logits of a word of each thread of a part, rows from which on
+// the longest that fit a workgroup go to one each, entries that a part is a
+// multiple of (VF_STEP) and most parts of a row
+const int kSoftmaxWord = 1024, kSoftmaxLongRows = 128, kVerifyStep = 2048, kVerifyParts = 64;
 
 // kernel-argument mirror of VfArgs in sample_ops.hip (same member order)
 struct VerifyArgs {
@@ -1927,7 +1927,6 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
     if (rows == 0) return 0;
     if (!x || !y || !aligned(x, x_dtype == CIMA_DT_F32 ? 4 : 2) || !aligned(y, 4) || !aligned(temp, 4))
         return fail(CIMA_E_INVALID, "%s: null or misaligned x, y or temp", api);
-    int parts = (n + kSoftmaxPart - 1) / kSoftmaxPart;
     const bool f32 = x_dtype == CIMA_DT_F32;
     char name[64];
     const char* sfx = kSampleTypes[(cap > 0.f ? 2 : 0) + (f32 ? 1 : 0)];
@@ -1941,14 +1940,20 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
             void* args[] = {&x, &y, &n, &temp, &rows_per_temp, &cap};
             return launch_named(ctx, name, (unsigned)rows, (unsigned)sh[0], args, api);
         }
+    // two words a thread where that makes at most four workgroups to a CU (and the
+    // slab holds their parts), else eight
+    const auto parts_of = [&](int words) { return (n - 1) / (kSoftmaxWord * words) + 1; };
+    int words = 8;
+    if ((long long)rows * parts_of(2) <= 4LL * ctx->num_cu && slab_bytes >= 16ULL * rows * parts_of(2)) words = 2;
+    int parts = parts_of(words);
     const unsigned long long need = 16ULL * rows * parts;
     if ((long long)rows * parts > 0x7fffffffLL || !slab || !aligned(slab, 8) || slab_bytes < need)
         return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (8 B)", api,
                     slab_bytes, need);
-    snprintf(name, sizeof name, "cima_softmax_stats_%s", sfx);
+    snprintf(name, sizeof name, "cima_softmax_stats_w%d_%s", words, sfx);
     void* args[] = {&x, &slab, &n, &temp, &rows_per_temp, &cap, &parts};
     if (int rc = launch_named(ctx, name, (unsigned)(rows * parts), 256, args, api)) return rc;
-    snprintf(name, sizeof name, "cima_softmax_probs_%s", sfx);
+    snprintf(name, sizeof name, "cima_softmax_probs_w%d_%s", words, sfx);
     void* pargs[] = {&x, &y, &slab, &n, &temp, &rows_per_temp, &cap, &parts};
     return launch_named(ctx, name, (unsigned)(rows * parts), 256, pargs, api);
 }

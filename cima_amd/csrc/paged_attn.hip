@@ -112,7 +112,6 @@ struct AttnArgs {
     int prefix_parts, own_parts, row_tiles;  // row tiles of the prefix tasks
     int prefix_tile, own_tile;               // their rows, and those of the own tasks
     int prefix_wgs;                          // workgroups of prefix tasks
-    int least_tiles;                         // of 32 positions, that an own task takes
     float scale2;                            // scale * log2(e)
 };
 
@@ -511,6 +510,7 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 // loads to registers and LDS writes: 127 and 36 us.
 constexpr int few_bufs(int D, int mode, int nb) { return mode == 0 && !(D == 128 && nb == 2) ? 1 : 2; }
 constexpr int few_wgs(int D, int mode, int nb) { return few_bufs(D, mode, nb) == 1 ? 4 : 2; }
+constexpr int OWN_LEAST = 4;  // tiles that a part of an own task has at least, where there are
 template <int D, int NB, int BUFS>
 struct Few {
     static constexpr int VT = 32 * D * 2;                  // bytes of a tile's values
@@ -787,7 +787,7 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
     b /= tiles;
     const int kvh = b % A.kv_heads, s = b / A.kv_heads;
     few_task<D, NB, BUFS>(A, lds, kvh, s * rows + tile * 16 * NB, (s + 1) * rows, A.prefix_pages << A.page_shift, 0x7fffffff,
-                    A.table + (size_t)s * A.table_stride, part, A.own_parts, A.prefix_parts + part, A.prefix_pages, A.least_tiles);
+                    A.table + (size_t)s * A.table_stride, part, A.own_parts, A.prefix_parts + part, A.prefix_pages, OWN_LEAST);
 }
 #define ATTN(D, MODE, NB)                                                                                            \
     extern "C" __global__ __launch_bounds__(256, few_wgs(D, MODE, NB)) void cima_attn_paged_d##D##_m##MODE##_n##NB(const AttnArgs A) {  \

@@ -8,14 +8,16 @@
 // A row's logits are read into registers: the maximum first, then the sum of
 // e^((f(x) - m) / T) = 2^((f(x) - m) log2(e) / T), then the same again times 1 /
 // sum.  Rows up to 65536 logits go to a workgroup each, in one launch.  Longer
-// ones, and few long ones, are split over `parts` workgroups of 8192: the first
-// launch leaves each part's maximum, its place and its sum, the second joins a
-// row's parts, reads its own logits once more and writes the probabilities.
+// ones, and few long ones, are split over `parts` workgroups of 8192 logits, or
+// of 2048 where those are at most four to a CU: the first launch leaves each
+// part's maximum, its place and its sum, the second joins a row's parts, reads
+// its own logits once more and writes the probabilities.
 // Bound by memory: the probabilities go past the caches, which keep the logits
 // for the second reading.  Measured on MI355X, us: 384 rows of 128256 f16 63
 // (393 MB moved, 6.2 TB/s; through the caches 83, a row per workgroup in 32
 // words a thread 73); 256 rows of 60000 in one launch 21, in two 22.5; 64 of
-// 30000 7.3 and 8.6; one row of 151936 3.3 + 4.8.
+// 30000 7.3 and 8.6.  Parts of 2048 / 8192: one row of 151936 6.2 / 7.5, capped 3
+// of 40000 8.0 / 14.8, eight of 151936 7.7 / 8.2; 384 of 128256 72 / 62.
 
 struct SmPart {
     float m, l;
@@ -175,8 +177,7 @@ struct SmRow {
     }
 };
 
-constexpr int SM_T = 256, SM_R = 8;        // threads and words a thread of a part
-constexpr int SM_PART = SM_T * SM_R * 4;   // its logits
+constexpr int SM_T = 256;  // threads of a part, of R words a thread
 
 // a row's parts joined by every wave: lane i takes parts i, i + 64, ...
 DEV float sm_join(const SmPart* __restrict__ p, int parts, float T, int* at, float* L) {
@@ -200,27 +201,27 @@ DEV float sm_join(const SmPart* __restrict__ p, int parts, float T, int* at, flo
     *at = a;
     return m;
 }
-#define SOFTMAX_PARTS(NAME, F32, CAP)                                                                                  \
-    extern "C" __global__ __launch_bounds__(SM_T) void cima_softmax_stats_##NAME(                                      \
+#define SOFTMAX_PARTS(NAME, F32, CAP, R)                                                                               \
+    extern "C" __global__ __launch_bounds__(SM_T) void cima_softmax_stats_w##R##_##NAME(                               \
         const void* __restrict__ x, SmPart* __restrict__ part, int n, const float* __restrict__ temp,                  \
         int rows_per_temp, float cap, int parts) {                                                                     \
         const int row = blockIdx.x / parts, pt = blockIdx.x % parts;                                                   \
-        SmRow<F32, CAP, SM_T, F32 ? SM_R : SM_R / 2, F32 ? 4 : 8> R;                                                   \
-        R.load(x, (size_t)row * n, pt * SM_PART, n, cap);                                                              \
-        R.stats(temp ? temp[row / rows_per_temp] : 1.f);                                                               \
-        if (threadIdx.x == 0) part[blockIdx.x] = SmPart{R.m, R.l, R.at, 0};                                            \
+        SmRow<F32, CAP, SM_T, F32 ? R : R / 2, F32 ? 4 : 8> S;                                                         \
+        S.load(x, (size_t)row * n, pt * SM_T * R * 4, n, cap);                                                         \
+        S.stats(temp ? temp[row / rows_per_temp] : 1.f);                                                               \
+        if (threadIdx.x == 0) part[blockIdx.x] = SmPart{S.m, S.l, S.at, 0};                                            \
     }                                                                                                                  \
-    extern "C" __global__ __launch_bounds__(SM_T) void cima_softmax_probs_##NAME(                                      \
+    extern "C" __global__ __launch_bounds__(SM_T) void cima_softmax_probs_w##R##_##NAME(                               \
         const void* __restrict__ x, float* __restrict__ y, const SmPart* __restrict__ part, int n,                     \
         const float* __restrict__ temp, int rows_per_temp, float cap, int parts) {                                     \
         const int row = blockIdx.x / parts, pt = blockIdx.x % parts;                                                   \
         const float T = temp ? temp[row / rows_per_temp] : 1.f;                                                        \
-        SmRow<F32, CAP, SM_T, SM_R> R;                                                                                 \
-        R.load(x, (size_t)row * n, pt * SM_PART, n, cap);                                                              \
+        SmRow<F32, CAP, SM_T, R> S;                                                                                    \
+        S.load(x, (size_t)row * n, pt * SM_T * R * 4, n, cap);                                                         \
         float L;                                                                                                       \
         int at;                                                                                                        \
         const float m = sm_join(part + (size_t)row * parts, parts, T, &at, &L);                                        \
-        R.write(y, (size_t)row * n, n, T, m, at, L);                                                                   \
+        S.write(y, (size_t)row * n, n, T, m, at, L);                                                                   \
     }
 #define SOFTMAX_WHOLE(NAME, F32, CAP, NT, WORDS)                                                                       \
     extern "C" __global__ __launch_bounds__(NT) void cima_softmax_t##NT##_w##WORDS##_##NAME(                           \
@@ -234,7 +235,8 @@ DEV float sm_join(const SmPart* __restrict__ p, int parts, float T, int* at, flo
         R.write(y, (size_t)row * n, n, T, R.m, R.at, R.l);                                                             \
     }
 #define SOFTMAX(NAME, F32, CAP)            \
-    SOFTMAX_PARTS(NAME, F32, CAP)          \
+    SOFTMAX_PARTS(NAME, F32, CAP, 2)       \
+    SOFTMAX_PARTS(NAME, F32, CAP, 8)       \
     SOFTMAX_WHOLE(NAME, F32, CAP, 256, 2)  \
     SOFTMAX_WHOLE(NAME, F32, CAP, 256, 8)  \
     SOFTMAX_WHOLE(NAME, F32, CAP, 1024, 8)

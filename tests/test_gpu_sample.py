@@ -94,6 +94,25 @@ def test_softmax_on_both_sides_of_every_path(hip, dtype, rows, n):
     assert np.allclose(y.sum(1, dtype=np.float64), 1, atol=1e-5)
 
 
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("cap", [0.0, 20.0])
+@pytest.mark.parametrize("n", [32769, 40960, 151936])
+def test_softmax_of_few_rows_by_the_slab(hip, dtype, cap, n):
+    """A slab of 16 bytes for each 8192 logits suffices, a larger one lets the
+    row be split further."""
+    r = np.random.default_rng(n)
+    x = (r.standard_normal((3, n), np.float32) * 4).astype(dtype)
+    temp = np.array([0.8, 0, 1.3], np.float32)
+    want, tol = _softmax_want(x, temp, 1, cap)
+    for size in (3 * 16 * -(-n // 8192), 3 * 16 * -(-n // 2048) - 8, 3 * 16 * -(-n // 2048), 1 << 16):
+        y = torch.full((3, n), 7.0, device="cuda")
+        slab = torch.full((size + 64,), 0x5a, dtype=torch.uint8, device="cuda")
+        hip.softmax_rows(_cuda(x), y, 3, n, _cuda(temp), 1, cap, slab[:size])
+        torch.cuda.synchronize()
+        assert (np.abs(y.cpu().numpy() - want) <= tol).all(), size
+        assert (slab[size:] == 0x5a).all()
+
+
 @pytest.mark.parametrize("n", [5, 9000, 40000])
 def test_softmax_edges(hip, n):
     """Rows of -inf become zeros, temperature 0 takes the first of equal
