@@ -139,14 +139,15 @@ struct Tile {
 // Rows [r0, r0 + 32 WR) of [0, rb) (row r of a kv head: head r % g, token r /
 // g), positions [plo, phi), part `part` of `parts`, results to column `col`.
 //
-// Bound by issue: beside a tile's MFMA stand 32 exponentials a lane, the
-// conversions and the reads of its fragments.  64 positions a tile, two tiles in
-// LDS (64 KB), two workgroups of four waves to a CU: 250 registers hold 32 rows'
-// sums, two tiles' scores and q; the two workgroups cover each other's barriers.
-// Measured on MI355X, 128 slots of 4 x 8 heads of 128 over 65536 positions (137
-// GFLOP): 158 us, 870 TFLOP/s; without exponentials, copies and barriers
-// 108.  One workgroup of eight waves and 256 rows, which copies half as much:
-// 176; 64 rows a wave: 572, its registers spill.
+// 64 positions a tile, two tiles in LDS (64 KB), two workgroups of four waves to
+// a CU: 250 registers hold 32 rows' sums, two tiles' scores and q, and the two
+// workgroups cover each other's barriers.  Measured on MI355X, 128 slots of 4 x 8
+// heads of 128 over 65536 positions (137 GFLOP): 155 us, 885 TFLOP/s, the matrix
+// cores 0.45 busy at the 1.9 GHz that the card holds under this load.  No one part
+// bounds it: without the copies 133 us, without reads from LDS 123, without the
+// weights 138, with the products alone 85; reading fragments 2 to 8 products ahead
+// changes nothing.  One workgroup of eight waves and 256 rows, which copies half
+// as much: 176; 64 rows a wave: 572, its registers spill.
 template <int D, int WR, int WK>
 DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int plo, int phi, const int* trow,
                    int part, int parts, int col) {
@@ -264,7 +265,6 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         }
     };
     const int kw = wk * 32 * T::KB;  // this wave's keys of a tile
-    f16v sc[T::KB];
     f16v zero16;
 #pragma unroll
     for (int i = 0; i < 16; i++) zero16[i] = 0.f;
@@ -289,7 +289,7 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         return __builtin_bit_cast(h8, v);
     };
     // the scores of tile t that a row does not see become -inf; the largest left
-    auto mask = [&](int t) {
+    auto mask = [&](int t, f16v (&sc)[T::KB]) {
         const int p0 = base + t * T::KT;
         float mx = -INFINITY;
 #pragma unroll
@@ -323,6 +323,7 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         __syncthreads();
         fill_ids(page_of(base + t0 * T::KT));
         __syncthreads();
+        f16v sa[T::KB], sb[T::KB];  // scores of even and of odd tiles from t0 on
         int id = id_at(t0);
         issue(t0, id, kplane, kword, KX, 0);
         issue(t0, id, vplane, vword, VX, 2 * T::BYTES);
@@ -333,15 +334,16 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         {
             const uint32_t kr = kread + (uint32_t)(t0 & 1) * T::BYTES;
 #pragma unroll
-            for (int b = 0; b < T::KB; b++) sc[b] = zero16;
+            for (int b = 0; b < T::KB; b++) sa[b] = zero16;
 #pragma unroll
             for (int i = 0; i < T::KB * STEPS; i++) {
                 const int b = i % T::KB;
-                sc[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kfrag(kr, i), qf[i / T::KB], sc[b], 0, 0, 0);
+                sa[b] = __builtin_amdgcn_mfma_f32_32x32x16_f16(kfrag(kr, i), qf[i / T::KB], sa[b], 0, 0, 0);
             }
         }
-        raise(mask(t0));
-        for (int t = t0; t < t1; t++) {
+        raise(mask(t0, sa));
+        // tile t, whose scores are in sc; those of the next go to sn
+        auto turn = [&](int t, f16v (&sc)[T::KB], f16v (&sn)[T::KB]) {
             const bool more = t + 1 < t1;
             if (t > t0 || more) {
                 wait_vm<0>();
@@ -358,7 +360,6 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
                     issue(t + 2, id, kplane, kword, KX, 0);
                 }
             }
-            f16v sn[T::KB];
             h8 pf[T::KB * 2];
             // two weights: elements i, i + 1 of block j / 8
             auto pair = [&](int j) {
@@ -418,13 +419,16 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
+            __asm__ volatile("" : "+v"(mx));  // found beside the products, not behind them
             if (more) {
-#pragma unroll
-                for (int b = 0; b < T::KB; b++) sc[b] = sn[b];
                 const int p0 = base + (t + 1) * T::KT;
-                if (p0 < lo_all || p0 + T::KT > hi_all) mx = mask(t + 1);
+                if (p0 < lo_all || p0 + T::KT > hi_all) mx = mask(t + 1, sn);
                 raise(mx);
             }
+        };
+        for (int t = t0; t < t1; t += 2) {
+            turn(t, sa, sb);
+            if (t + 1 < t1) turn(t + 1, sb, sa);
         }
     }
     const f2 hl = halves(l);
