@@ -1640,6 +1640,8 @@ int kv_layer(const cima_kv_pages* kv, int layer, const char* api) {
         return fail(CIMA_E_INVALID, "%s: layer %d of %d", api, layer, kv->n_planes / 2);
     return 0;
 }
+// workgroups of 256 threads that a launch takes (2^32 threads)
+const long long kMaxGrid = 0xffffff;
 // 16-byte words of a page, and pieces of PIECE words that it is copied in
 // (paged_ops.hip)
 long long page_words(const cima_kv_pages* kv) { return (long long)kv->kv_heads * kv->page * kv->head_dim / 8; }
@@ -1677,10 +1679,10 @@ int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int l
     const char* api = "cima_hip_rope_append_paged";
     if (int rc = kv_check(ctx, kv, api)) return rc;
     if (int rc = kv_layer(kv, layer, api)) return rc;
-    if (seqs < 0 || seqs > kv->max_seqs || n_new < 0 || q_heads <= 0 || (long long)seqs * n_new > 0x7fffffffLL ||
+    if (seqs < 0 || seqs > kv->max_seqs || n_new < 0 || q_heads <= 0 || (long long)seqs * n_new > kMaxGrid ||
         q_heads > 0xffff || !(theta == 0.f || (theta > 0.f && theta < INFINITY)))
-        return fail(CIMA_E_INVALID, "%s: seqs=%d (of %d) n_new=%d q_heads=%d theta=%g", api, seqs, kv->max_seqs, n_new,
-                    q_heads, theta);
+        return fail(CIMA_E_INVALID, "%s: seqs=%d (of %d) n_new=%d q_heads=%d theta=%g (less than 2^24 rows)", api, seqs,
+                    kv->max_seqs, n_new, q_heads, theta);
     if (seqs == 0 || n_new == 0) return 0;
     if (!qkv || !q || !aligned(qkv, 16) || !aligned(q, 16))
         return fail(CIMA_E_INVALID, "%s: null or misaligned qkv or q (16 B)", api);
@@ -1702,7 +1704,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     if (int rc = kv_check(ctx, kv, api)) return rc;
     if (int rc = kv_layer(kv, layer, api)) return rc;
     if (seqs < 0 || seqs > kv->max_seqs || n_new < 0 || q_heads <= 0 || q_heads % kv->kv_heads || q_heads > 0xffff ||
-        !(scale > 0.f && scale < INFINITY) || prefix_pages < 0 || prefix_pages > kv->table_stride || prefix_slot < 0 ||
+        !(scale > 0.f && scale <= 65536.f) || prefix_pages < 0 || prefix_pages > kv->table_stride || prefix_slot < 0 ||
         prefix_slot >= kv->max_seqs || window < 0 || (long long)seqs * n_new * q_heads > 0x1000000LL)
         return fail(CIMA_E_INVALID,
                     "%s: seqs=%d (of %d) n_new=%d q_heads=%d kv_heads=%d scale=%g prefix_pages=%d (of %d) "
@@ -1845,7 +1847,8 @@ int cima_hip_kv_pages_fork(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int
                            int* status) {
     const char* api = "cima_hip_kv_pages_fork";
     if (int rc = kv_check(ctx, kv, api)) return rc;
-    if (n < 0 || n > kv->max_seqs) return fail(CIMA_E_INVALID, "%s: n=%d of %d slots", api, n, kv->max_seqs);
+    if (n < 0 || n > kv->max_seqs || n * (1LL + kv->n_planes) > kMaxGrid)
+        return fail(CIMA_E_INVALID, "%s: n=%d of %d slots in %d planes", api, n, kv->max_seqs, kv->n_planes);
     if (!status || !aligned(status, 4)) return fail(CIMA_E_INVALID, "%s: null or misaligned status", api);
     if (n && (!parents || !children || !aligned(parents, 4) || !aligned(children, 4)))
         return fail(CIMA_E_INVALID, "%s: null or misaligned lists", api);
@@ -1865,7 +1868,8 @@ int cima_hip_kv_pages_fork(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int
 int cima_hip_kv_pages_free(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int* slots, int n) {
     const char* api = "cima_hip_kv_pages_free";
     if (int rc = kv_check(ctx, kv, api)) return rc;
-    if (n < 0 || n > kMaxSlots) return fail(CIMA_E_INVALID, "%s: n=%d", api, n);
+    if (n < 0 || n > kMaxSlots || n * ((kv->table_stride + 1023LL) / 1024) > kMaxGrid)
+        return fail(CIMA_E_INVALID, "%s: n=%d slots of %d entries", api, n, kv->table_stride);
     if (n == 0) return 0;
     if (!slots || !aligned(slots, 4)) return fail(CIMA_E_INVALID, "%s: null or misaligned list", api);
     int *refs = kv->refs, *table = kv->table, *lens = kv->lens;
@@ -1920,7 +1924,7 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
                           int rows_per_temp, float cap, int x_dtype, void* slab, unsigned long long slab_bytes) {
     const char* api = "cima_hip_softmax_rows";
     if (int rc = ready(ctx, api)) return rc;
-    if (rows < 0 || n <= 0 || n > 0x3fffffff || rows_per_temp <= 0 || !(cap >= 0.f && cap < INFINITY))
+    if (rows < 0 || rows > kMaxGrid / 4 || n <= 0 || n > 0x3fffffff || rows_per_temp <= 0 || !(cap >= 0.f && cap < INFINITY))
         return fail(CIMA_E_INVALID, "%s: rows=%d n=%d rows_per_temp=%d cap=%g", api, rows, n, rows_per_temp, cap);
     if (x_dtype != CIMA_DT_F32 && x_dtype != CIMA_DT_F16)
         return fail(CIMA_E_INVALID, "%s: x_dtype %d is not f32 or f16", api, x_dtype);
@@ -1947,7 +1951,7 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
     if ((long long)rows * parts_of(2) <= 4LL * ctx->num_cu && slab_bytes >= 16ULL * rows * parts_of(2)) words = 2;
     int parts = parts_of(words);
     const unsigned long long need = 16ULL * rows * parts;
-    if ((long long)rows * parts > 0x7fffffffLL || !slab || !aligned(slab, 8) || slab_bytes < need)
+    if ((long long)rows * parts > kMaxGrid || !slab || !aligned(slab, 8) || slab_bytes < need)
         return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (8 B)", api,
                     slab_bytes, need);
     snprintf(name, sizeof name, "cima_softmax_stats_w%d_%s", words, sfx);
@@ -1973,7 +1977,7 @@ int cima_hip_verify_drafts(cima_hip_ctx* ctx, const float* p, const float* q, co
     const unsigned long long need = 8ULL * seqs * (((long long)vocab + kVerifyStep - 1) / kVerifyStep + 1);
     const long long len = ((vocab + kVerifyParts - 1LL) / kVerifyParts + kVerifyStep - 1) / kVerifyStep * kVerifyStep;
     const long long parts = (vocab + len - 1) / len;
-    if (seqs * parts > 0x7fffffffLL || !slab || !aligned(slab, 8) || slab_bytes < need)
+    if (seqs * parts > kMaxGrid || !slab || !aligned(slab, 8) || slab_bytes < need)
         return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (8 B)", api,
                     slab_bytes, need);
     VerifyArgs A{p, q, drafts, counts, u, accepted, tokens, lens, slab, (double*)slab + seqs * parts, n_draft, vocab,

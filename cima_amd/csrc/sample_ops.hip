@@ -56,6 +56,9 @@ DEV float sm_get(const uint32_t (&v)[F32 ? V : V / 2], int j) {
 DEV float uniform(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, v)));
 }
+// c / T within fp32's range, so that no difference of logits becomes 0 * inf at a
+// temperature that is infinite or next to nothing
+DEV float sm_scale(float c, float T) { return fminf(fmaxf(c / T, 1e-37f), 1e38f); }
 // f of a logit; those behind n stay -inf
 DEV float sm_f(float x, int i, int n, float cap) { return i < n ? cap * tanhf(x / cap) : x; }
 
@@ -111,7 +114,7 @@ struct SmRow {
         l = 0.f;
         at = 0x7fffffff;
         if (T > 0.f) {
-            const float c = m == -INFINITY ? 0.f : m, s = 1.44269504088896340736f / T;
+            const float c = m == -INFINITY ? 0.f : m, s = sm_scale(1.44269504088896340736f, T);
 #pragma unroll
             for (int r = 0; r < R; r++) {
                 float p = 0.f;
@@ -153,7 +156,7 @@ struct SmRow {
         static_assert(V == 4, "a 16-byte store a word");
         const bool none = M == -INFINITY && L == 0.f;  // -inf alone
         const float c = M == -INFINITY ? 0.f : M, inv = none ? 0.f : 1.f / L;
-        const float s = 0.72134752044448170368f / T;
+        const float s = sm_scale(0.72134752044448170368f, T);
 #pragma unroll
         for (int r = 0; r < R; r++) {
             const int i = base + r * NT * V;
@@ -187,7 +190,7 @@ DEV float sm_join(const SmPart* __restrict__ p, int parts, float T, int* at, flo
     m = wave_max_u(m);
     int a = 0x7fffffff;
     if (T > 0.f) {
-        const float c = m == -INFINITY ? 0.f : m, s = 1.44269504088896340736f / T;
+        const float c = m == -INFINITY ? 0.f : m, s = sm_scale(1.44269504088896340736f, T);
         for (int i = lane; i < parts; i += 64)
             l += p[i].l * (p[i].m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((p[i].m - c) * s));
     } else {

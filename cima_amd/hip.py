@@ -234,11 +234,6 @@ _DTYPES: list = [None] * 3
 _I32, _F32, _F16 = range(3)
 
 
-def _slab(a) -> tuple:
-    """(pointer, bytes) of a scratch tensor."""
-    return (None, 0) if a is None else (_ptr(a), a.numel() * a.element_size())
-
-
 def _act_of(t) -> int:
     if not _act_types:
         _torch_names()
@@ -542,6 +537,17 @@ class HipCtx:
     def _op(self, a, kind: int, n: int, name: str) -> Optional[int]:
         return _ptr_of(a, kind, n, name, self.device)
 
+    def _slab(self, a) -> tuple:
+        """(pointer, bytes) of a scratch tensor."""
+        if a is None:
+            return None, 0
+        p = _ptr(a)
+        if isinstance(a, int):
+            raise EngineError("hip", E_INVALID, "the slab is a bare pointer, its size unknown")
+        if a.get_device() != self.device:
+            raise EngineError("hip", E_INVALID, f"the slab is on device {a.get_device()}, the context on {self.device}")
+        return p, a.numel() * a.element_size()
+
     def rope_append_paged(self, kv, layer: int, qkv, q, seqs: int, n_new: int, q_heads: int, theta: float) -> None:
         """RoPE of a step's queries (to ``q``) and keys, row ``s * n_new + j`` of
         ``qkv`` at position ``lens[s] + j``, and the append of its keys and values
@@ -559,7 +565,7 @@ class HipCtx:
         n = seqs * n_new * q_heads * kv.head_dim
         self._check(self.lib.cima_hip_attn_paged(self.handle, self._kv(kv), layer, self._op(q, _F16, n, "q"),
                                                  self._op(out, _F16, n, "out"), seqs, n_new, q_heads, scale,
-                                                 prefix_pages, prefix_slot, window, *_slab(slab)))
+                                                 prefix_pages, prefix_slot, window, *self._slab(slab)))
 
     def kv_pages_copy(self, kv, src, dst, n: int) -> None:
         """Page ``dst[i]`` of every plane = page ``src[i]``."""
@@ -588,7 +594,7 @@ class HipCtx:
         and table go to ``refs_out`` and ``table_out`` (or are the cache's own)."""
         self._check(self.lib.cima_hip_kv_pages_compact(
             self.handle, self._kv(kv), self._op(refs_out, _I32, kv.n_pages, "refs_out"),
-            self._op(table_out, _I32, kv.table.numel(), "table_out"), self._op(n_live, _I32, 1, "n_live"), *_slab(slab)))
+            self._op(table_out, _I32, kv.table.numel(), "table_out"), self._op(n_live, _I32, 1, "n_live"), *self._slab(slab)))
 
     # -- sampling ---------------------------------------------------------------
     def softmax_rows(self, x, y, rows: int, n: int, temp=None, rows_per_temp: int = 1, cap: float = 0.0,
@@ -600,7 +606,7 @@ class HipCtx:
         act = _act_of(x)
         self._check(self.lib.cima_hip_softmax_rows(
             self.handle, self._op(x, _F16 if act else _F32, rows * n, "x"), self._op(y, _F32, rows * n, "y"), rows, n,
-            self._op(temp, _F32, -(-rows // rows_per_temp), "temp"), rows_per_temp, cap, act, *_slab(slab)))
+            self._op(temp, _F32, -(-rows // rows_per_temp), "temp"), rows_per_temp, cap, act, *self._slab(slab)))
 
     def verify_drafts(self, p, q, drafts, counts, u, accepted, tokens, lens, seqs: int, n_draft: int, vocab: int,
                       slab) -> None:
@@ -613,7 +619,7 @@ class HipCtx:
             self._op(drafts, _I32, seqs * n_draft, "drafts"), self._op(counts, _I32, seqs, "counts"),
             self._op(u, _F32, seqs * k, "u"), self._op(accepted, _I32, seqs, "accepted"),
             self._op(tokens, _I32, seqs * k, "tokens"), self._op(lens, _I32, seqs, "lens"), seqs, n_draft, vocab,
-            *_slab(slab)))
+            *self._slab(slab)))
 
     def stream_read_cfg(self, src, nbytes: int, sink, dest: int, depth: int, width: int = 16,
                         wgs_per_cu: int = 2) -> None:

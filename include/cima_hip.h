@@ -445,7 +445,8 @@ typedef struct cima_kv_pages {
  * angle formed in fp64 (at position 100000 an fp32 angle is off by up to
  * 0.008); theta 0 = no rotation.  lens is not changed: every layer of the step
  * appends at the same positions.  Slots not in use write nothing, neither q;
- * positions without a page (entry -1 or behind the row) write no key.
+ * positions without a page (entry -1 or behind the row) write no key.  Less
+ * than 2^24 rows.
  * qkv and q 16-byte aligned, not overlapping. */
 int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* qkv, void* q,
                                int seqs, int n_new, int q_heads, float theta);
@@ -464,7 +465,7 @@ int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int l
  * the slab (256-byte aligned) holds the partial sums: rows * q_heads *
  * (head_dim + 2) * 4 bytes per part, rows = seqs * n_new.  Two parts are
  * needed where prefix_pages > 0, else none; 192 are the most that are used.
- * q_heads a multiple of kv_heads, rows * q_heads at most 2^24; scale positive;
+ * q_heads a multiple of kv_heads, rows * q_heads at most 2^24; scale in (0, 2^16];
  * q and out 16-byte aligned, not overlapping. */
 int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* q, void* out, int seqs,
                         int n_new, int q_heads, float scale, int prefix_pages, int prefix_slot, int window, void* slab,
@@ -506,7 +507,7 @@ int cima_hip_kv_pages_compact(cima_hip_ctx* ctx, const cima_kv_pages* kv, int* r
  * the row is 1 at its largest logit (the lowest index of equals) and 0
  * elsewhere.  A row of -inf alone becomes zeros; NaN or +inf make a row NaN
  * (temp <= 0: +inf ranks as the largest, NaN as the lowest).  x and y do not
- * overlap.  slab (8-byte aligned): 16 bytes for each 8192 logits of a row
+ * overlap; less than 2^22 rows.  slab (8-byte aligned): 16 bytes for each 8192 logits of a row
  * (rounded up) and row; none is needed up to 32768 logits.  One of 16 KB or
  * more makes few rows faster. */
 int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, int n, const float* temp,
@@ -525,7 +526,8 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
  * left, from p[a]; where that holds nothing, -1).  tokens [seqs, n_draft + 1] = the kept drafts, the drawn token,
  * then -1; accepted[s] = drafts kept.  lens (may be NULL): lens[s] += accepted
  * + 1 where lens[s] >= 0; slots with lens[s] < 0 get accepted 0 and tokens -1.
- * n_draft 0 draws one token a row.  slab (8-byte aligned): for each slot 8
+ * n_draft 0 draws one token a row.  No output overlaps an input but lens
+ * itself.  slab (8-byte aligned): for each slot 8
  * bytes, and 8 for each 2048 entries of vocab (rounded up). */
 int cima_hip_verify_drafts(cima_hip_ctx* ctx, const float* p, const float* q, const int* drafts, const int* counts,
                            const float* u, int* accepted, int* tokens, int* lens, int seqs, int n_draft, int vocab,

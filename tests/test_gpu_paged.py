@@ -253,6 +253,53 @@ def test_attention_scores_far_apart(hip):
         assert (np.abs(got - want) <= tol + 2.0 ** -21 * z * 5).all()
 
 
+@pytest.mark.parametrize("prefix", [0, 128])
+def test_attention_of_many_new_tokens(hip, prefix):
+    """A prompt's own tokens in one call: tiles of 32 rows behind each other."""
+    _check(hip, Batch([prefix, prefix + 3, -1], 150, (8, 2, 128), 32, prefix, seed=16))
+    _check(hip, Batch([prefix + 17], 201, (14, 2, 64), 64, prefix, seed=17), window=90)
+
+
+@pytest.mark.parametrize("heads", [(14, 2, 64), (8, 8, 128)], ids=str)
+def test_attention_of_a_ragged_batch(hip, heads):
+    """Short and long slots side by side: every part of a slot has its share."""
+    r = np.random.default_rng(18)
+    lens = list((700 ** r.random(70)).astype(int)) + [-1, 1500, 0]
+    _check(hip, Batch(lens, 1, heads, 16, 0, seed=19))
+
+
+def test_attention_ignores_a_prefix_before_every_window(hip):
+    lens, n_new, window = [300, 331, 280], 3, 50
+    b = Batch(lens, n_new, (14, 2, 64), 64, 256, seed=20, poison=[n + 1 - window for n in lens])
+    assert np.isnan(b.pool).any()
+    _check(hip, b, window)
+
+
+def test_attention_on_two_streams_at_once(hip):
+    """Two calls that may run together, a slab each."""
+    a, b = (Batch([512, 700, 513, 999], 2, (14, 2, 64), 64, 512, seed=s) for s in (21, 22))
+    qs = [x.r.standard_normal((x.rows, x.q_heads, x.D)).astype(np.float16) for x in (a, b)]
+    alone = [_attend(hip, x, q) for x, q in zip((a, b), qs)]
+    dev = [torch.from_numpy(q).cuda() for q in qs]
+    outs = [torch.zeros((x.rows, x.q_heads, x.D), dtype=torch.float16, device="cuda") for x in (a, b)]
+    slabs = [torch.empty(8 << 20, dtype=torch.uint8, device="cuda") for _ in (a, b)]
+    streams = [torch.cuda.Stream() for _ in (a, b)]
+    torch.cuda.synchronize()
+    try:
+        for _ in range(10):
+            for x, q, out, slab, st in zip((a, b), dev, outs, slabs, streams):
+                hip.set_stream(st)
+                hip.attn_paged(x.kv, 0, q, out, 4, 2, 14, 1.0 / np.sqrt(64), slab, prefix_pages=x.pp)
+    finally:
+        hip.use_torch_stream()
+    torch.cuda.synchronize()
+    # the slabs are smaller: fewer parts, another order of the same sums
+    for x, q, out, want in zip((a, b), qs, outs, alone):
+        same = _attend(hip, x, q, slab_mb=8)
+        assert np.array_equal(out.cpu().numpy().astype(np.float64), same)
+        assert np.abs(same - want).max() < 2.0 ** -9 * np.abs(x.pool[1]).max()
+
+
 def test_attention_is_deterministic_and_replays(hip):
     b = Batch([520, 700, 513, -1, 999], 2, (14, 2, 64), 64, 512, seed=15)
     q = b.r.standard_normal((b.rows, b.q_heads, b.D)).astype(np.float16)
@@ -615,7 +662,7 @@ def test_refusals(hip):
                       k.get("scale", 0.1), k.get("slab", slab))
     hip.attn_paged(*at(), prefix_pages=2)
     for bad in ({"layer": 1}, {"layer": -1}, {"seqs": 3}, {"heads": 7}, {"heads": 16}, {"scale": 0.0},
-                {"scale": float("inf")}, {"q": q.float()}, {"q": q[:1]}):
+                {"scale": float("inf")}, {"scale": 1e9}, {"q": q.float()}, {"q": q[:1]}, {"slab": 4096}):
         no(hip.attn_paged, *at(**bad), prefix_pages=2)
     no(hip.attn_paged, *at(), prefix_pages=99)
     no(hip.attn_paged, *at(), prefix_pages=2, prefix_slot=2)

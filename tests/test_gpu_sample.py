@@ -94,6 +94,27 @@ def test_softmax_on_both_sides_of_every_path(hip, dtype, rows, n):
     assert np.allclose(y.sum(1, dtype=np.float64), 1, atol=1e-5)
 
 
+@pytest.mark.parametrize("n", [100, 5000, 40000])
+def test_softmax_of_extreme_temperatures(hip, n):
+    """Next to nothing: the largest logits alone share the row; infinite: all
+    that are not -inf do.  In between nothing overflows."""
+    x = np.random.default_rng(n).standard_normal((4, n)).astype(np.float32)
+    x[:, 7] = x[:, 90] = 9.0
+    x[:, 11] = -np.inf
+    temp = np.array([1e-40, 1e-30, np.inf, 1e30], np.float32)
+    y = torch.empty((4, n), device="cuda")
+    hip.softmax_rows(_cuda(x), y, 4, n, _cuda(temp), 1, 0.0, _slab())
+    torch.cuda.synchronize()
+    y = y.cpu().numpy()
+    want = np.zeros(n)
+    want[[7, 90]] = 0.5
+    assert (y[0] == want).all() and (y[1] == want).all()
+    want = np.full(n, 1 / (n - 1))
+    want[11] = 0
+    # n terms in fp32, at most n / 1024 of them one after the other, then a division
+    assert np.abs(y[2:] / want.max() - want / want.max()).max() < 2.0 ** -23 * (n / 1024 + 20)
+
+
 @pytest.mark.parametrize("dtype", [np.float16, np.float32])
 @pytest.mark.parametrize("cap", [0.0, 20.0])
 @pytest.mark.parametrize("n", [32769, 40960, 151936])
