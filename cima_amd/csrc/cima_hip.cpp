@@ -1747,14 +1747,15 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     // turn, alike.  8 kv heads of 128, one round / two / four: 64 slots of up to 4000
     // 113 / 111 / 109 us, 128 of up to 6000 326 / 304 / 297, 64 of up to 2000 behind
     // a prefix of 4096 72 / 65 / 63, but more for the join: 0 / 6 / 6 at 128 slots.
-    // Without a prefix one part needs no join: taken up to 512 positions, and where
-    // the slots' tasks are one to a CU for each 1024 positions or two.  One part /
-    // several and the join, us: 16 slots of up to 300 8.0 / 10.9, 48 of up to 700
+    // One part up to 512 positions, and without a prefix, where it needs no join,
+    // where the slots' tasks are one to a CU for each 1024 positions or two.  One /
+    // several with the join, us: 16 slots of up to 300 8.0 / 10.9, 48 of up to 700
     // 17.5 / 21.4, 128 of up to 500 27.2 / 34.0, 64 of up to 4000 113 / 116, 64 of up
-    // to 600 with 8 tokens 20.5 / 40; but 8 of up to 1000 17 / 12.5.
+    // to 600 with 8 tokens 20.5 / 40; but 8 of up to 1000 17 / 12.5; 20 of up to 300
+    // behind 8000 21.0 / 23.9, 30 with 8 tokens behind 4096 47.6 / 52.3.
     long long own = (own_room + 127) / 128;
     while (own > 1 && own_base * own > 2LL * wgs * ctx->num_cu) own = (own + 1) / 2;
-    if (!prefix_pages && (own_room <= 512 || own_base * 1024 >= std::min(own_room, 2048LL) * ctx->num_cu)) own = 1;
+    if (own_room <= 512 || (!prefix_pages && own_base * 1024 >= std::min(own_room, 2048LL) * ctx->num_cu)) own = 1;
     own = std::max(1LL, std::min(own, 64LL));
     int tiles = 0;
     long long pre = 0;
