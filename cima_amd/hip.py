@@ -534,9 +534,6 @@ class HipCtx:
             raise EngineError("hip", E_INVALID, f"the cache is on device {kv.device}, the context on {self.device}")
         return kv.ref
 
-    def _op(self, a, kind: int, n: int, name: str) -> Optional[int]:
-        return _ptr_of(a, kind, n, name, self.device)
-
     def _slab(self, a) -> tuple:
         """(pointer, bytes) of a scratch tensor."""
         if a is None:
@@ -552,49 +549,54 @@ class HipCtx:
         """RoPE of a step's queries (to ``q``) and keys, row ``s * n_new + j`` of
         ``qkv`` at position ``lens[s] + j``, and the append of its keys and values
         to the pages of ``layer`` (theta 0: no rotation)."""
-        rows = seqs * n_new
+        n, d = seqs * n_new * kv.head_dim, self.device
         self._check(self.lib.cima_hip_rope_append_paged(
-            self.handle, self._kv(kv), layer, self._op(qkv, _F16, rows * (q_heads + 2 * kv.kv_heads) * kv.head_dim, "qkv"),
-            self._op(q, _F16, rows * q_heads * kv.head_dim, "q"), seqs, n_new, q_heads, theta))
+            self.handle, self._kv(kv), layer, _ptr_of(qkv, _F16, n * (q_heads + 2 * kv.kv_heads), "qkv", d),
+            _ptr_of(q, _F16, n * q_heads, "q", d), seqs, n_new, q_heads, theta))
 
     def attn_paged(self, kv, layer: int, q, out, seqs: int, n_new: int, q_heads: int, scale: float, slab,
                    prefix_pages: int = 0, prefix_slot: int = 0, window: int = 0) -> None:
         """Attention of a step's queries over the pages of ``layer``; the first
         ``prefix_pages`` entries, the same in every slot, are read once for all
         from row ``prefix_slot`` of the table."""
-        n = seqs * n_new * q_heads * kv.head_dim
-        self._check(self.lib.cima_hip_attn_paged(self.handle, self._kv(kv), layer, self._op(q, _F16, n, "q"),
-                                                 self._op(out, _F16, n, "out"), seqs, n_new, q_heads, scale,
-                                                 prefix_pages, prefix_slot, window, *self._slab(slab)))
+        n, d = seqs * n_new * q_heads * kv.head_dim, self.device
+        self._check(self.lib.cima_hip_attn_paged(
+            self.handle, self._kv(kv), layer, _ptr_of(q, _F16, n, "q", d), _ptr_of(out, _F16, n, "out", d), seqs, n_new,
+            q_heads, scale, prefix_pages, prefix_slot, window, *self._slab(slab)))
 
     def kv_pages_copy(self, kv, src, dst, n: int) -> None:
         """Page ``dst[i]`` of every plane = page ``src[i]``."""
-        self._check(self.lib.cima_hip_kv_pages_copy(self.handle, self._kv(kv), self._op(src, _I32, n, "src"),
-                                                    self._op(dst, _I32, n, "dst"), n))
+        d = self.device
+        self._check(self.lib.cima_hip_kv_pages_copy(self.handle, self._kv(kv), _ptr_of(src, _I32, n, "src", d),
+                                                    _ptr_of(dst, _I32, n, "dst", d), n))
 
     def kv_pages_reserve(self, kv, seqs: int, n_new: int, status) -> None:
         """Pages for ``n_new`` more tokens in each of slots [0, seqs) in use;
         ``status[0]`` = pages missing (then nothing is changed)."""
         self._check(self.lib.cima_hip_kv_pages_reserve(self.handle, self._kv(kv), seqs, n_new,
-                                                       self._op(status, _I32, 1, "status")))
+                                                       _ptr_of(status, _I32, 1, "status", self.device)))
 
     def kv_pages_fork(self, kv, parents, children, n: int, status) -> None:
         """Slots ``children[i]`` become copies of ``parents[i]``: whole pages
         shared, a page begun copied; ``status[0]``: 0, pages missing, or -1."""
-        self._check(self.lib.cima_hip_kv_pages_fork(self.handle, self._kv(kv), self._op(parents, _I32, n, "parents"),
-                                                    self._op(children, _I32, n, "children"), n,
-                                                    self._op(status, _I32, 1, "status")))
+        d = self.device
+        self._check(self.lib.cima_hip_kv_pages_fork(
+            self.handle, self._kv(kv), _ptr_of(parents, _I32, n, "parents", d), _ptr_of(children, _I32, n, "children", d),
+            n, _ptr_of(status, _I32, 1, "status", d)))
 
     def kv_pages_free(self, kv, slots, n: int) -> None:
         """The slots give their pages back and are free."""
-        self._check(self.lib.cima_hip_kv_pages_free(self.handle, self._kv(kv), self._op(slots, _I32, n, "slots"), n))
+        self._check(self.lib.cima_hip_kv_pages_free(self.handle, self._kv(kv),
+                                                    _ptr_of(slots, _I32, n, "slots", self.device), n))
 
     def kv_pages_compact(self, kv, refs_out, table_out, n_live, slab) -> None:
         """The pages in use move together to the front of the pool; the new counts
         and table go to ``refs_out`` and ``table_out`` (or are the cache's own)."""
+        d = self.device
         self._check(self.lib.cima_hip_kv_pages_compact(
-            self.handle, self._kv(kv), self._op(refs_out, _I32, kv.n_pages, "refs_out"),
-            self._op(table_out, _I32, kv.table.numel(), "table_out"), self._op(n_live, _I32, 1, "n_live"), *self._slab(slab)))
+            self.handle, self._kv(kv), _ptr_of(refs_out, _I32, kv.n_pages, "refs_out", d),
+            _ptr_of(table_out, _I32, kv.table.numel(), "table_out", d), _ptr_of(n_live, _I32, 1, "n_live", d),
+            *self._slab(slab)))
 
     # -- sampling ---------------------------------------------------------------
     def softmax_rows(self, x, y, rows: int, n: int, temp=None, rows_per_temp: int = 1, cap: float = 0.0,
@@ -603,22 +605,22 @@ class HipCtx:
         the largest logit alone; cap > 0: logits through ``cap * tanh(x / cap)``)."""
         if rows_per_temp <= 0:
             raise EngineError("hip", E_INVALID, f"rows_per_temp is {rows_per_temp}")
-        act = _act_of(x)
+        act, d = _act_of(x), self.device
         self._check(self.lib.cima_hip_softmax_rows(
-            self.handle, self._op(x, _F16 if act else _F32, rows * n, "x"), self._op(y, _F32, rows * n, "y"), rows, n,
-            self._op(temp, _F32, -(-rows // rows_per_temp), "temp"), rows_per_temp, cap, act, *self._slab(slab)))
+            self.handle, _ptr_of(x, _F16 if act else _F32, rows * n, "x", d), _ptr_of(y, _F32, rows * n, "y", d), rows, n,
+            _ptr_of(temp, _F32, -(-rows // rows_per_temp), "temp", d), rows_per_temp, cap, act, *self._slab(slab)))
 
     def verify_drafts(self, p, q, drafts, counts, u, accepted, tokens, lens, seqs: int, n_draft: int, vocab: int,
                       slab) -> None:
         """Drafted tokens kept while ``u * q[d] < p[d]`` and the token drawn after
         them; ``q`` None: certain drafts, ``counts`` None: n_draft each, ``lens``
         None: no lengths to advance."""
-        k = n_draft + 1
+        k, d = n_draft + 1, self.device
         self._check(self.lib.cima_hip_verify_drafts(
-            self.handle, self._op(p, _F32, seqs * k * vocab, "p"), self._op(q, _F32, seqs * n_draft * vocab, "q"),
-            self._op(drafts, _I32, seqs * n_draft, "drafts"), self._op(counts, _I32, seqs, "counts"),
-            self._op(u, _F32, seqs * k, "u"), self._op(accepted, _I32, seqs, "accepted"),
-            self._op(tokens, _I32, seqs * k, "tokens"), self._op(lens, _I32, seqs, "lens"), seqs, n_draft, vocab,
+            self.handle, _ptr_of(p, _F32, seqs * k * vocab, "p", d), _ptr_of(q, _F32, seqs * n_draft * vocab, "q", d),
+            _ptr_of(drafts, _I32, seqs * n_draft, "drafts", d), _ptr_of(counts, _I32, seqs, "counts", d),
+            _ptr_of(u, _F32, seqs * k, "u", d), _ptr_of(accepted, _I32, seqs, "accepted", d),
+            _ptr_of(tokens, _I32, seqs * k, "tokens", d), _ptr_of(lens, _I32, seqs, "lens", d), seqs, n_draft, vocab,
             *self._slab(slab)))
 
     def stream_read_cfg(self, src, nbytes: int, sink, dest: int, depth: int, width: int = 16,
