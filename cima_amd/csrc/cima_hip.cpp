@@ -1725,20 +1725,25 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     if (least > 1 && fit < least)
         return fail(CIMA_E_INVALID, "%s: a slab of %llu bytes does not hold %d parts of %lld", api, slab_bytes, least,
                     part_bytes);
-    const int own_rows = n_new * g;
+    // Own tasks of more than 16 rows take 32 at a time, the pages read half as
+    // often.  64 slots of up to 4000 positions, 32 rows: 103 us by 16, 77 by 32; of
+    // up to 600: 41 and 36 (128 a head), 27.6 and 29.6 (64).
+    const int own_rows = n_new * g, nb = own_rows > 16 ? 2 : 1;
+    const int own_tiles = (own_rows + 16 * nb - 1) / (16 * nb);
+    const long long own_base = (long long)seqs * kv->kv_heads * own_tiles;
+    // Tables of few positions and slots: each slot reads the prefix for itself, in
+    // one launch.  us, shared and joined / not: 4 slots of 14/2 heads of 64 over 256
+    // + 100 8.6 / 6.2, over 512 + 61 8.9 / 7.7, 8 of 32/8 of 128 over 256 + 100 10.4 /
+    // 8.3, 30 of those 11.5 / 8.8; 16 of them over 512 + 60 10.7 / 11.2.
+    const long long brief = dim == 64 ? 640 : 512, room = (long long)kv->table_stride * kv->page;
+    if (room <= brief && nb == 1 && own_base <= ctx->num_cu) prefix_pages = 0;
+    const long long own_room = room - (long long)prefix_pages * kv->page;
     // Up to 16 rows the prefix runs in the own tasks' kernel, whose waves fetch
     // for themselves; above, in tiles of 64 rows, from 65 rows on of 128.  us,
     // one side / the other: 16 rows of 128, 8000 positions 14.8 / 17.4, 8 rows, 512
     // 9.0 / 10.0, 24 rows, 8000 20.9 / 16.6; 64 rows a tile / 128: 40 rows 17.8 /
     // 19.0, 80 rows 20.3 / 20.4, 63 rows of 64 17.2 / 18.7.
     const bool few = prefix_pages && head_rows <= 16;
-    // Own tasks of more than 16 rows take 32 at a time, the pages read half as
-    // often.  64 slots of up to 4000 positions, 32 rows: 103 us by 16, 77 by 32; of
-    // up to 600: 41 and 36 (128 a head), 27.6 and 29.6 (64).
-    const int nb = own_rows > 16 ? 2 : 1;
-    const int own_tiles = (own_rows + 16 * nb - 1) / (16 * nb);
-    const long long own_base = (long long)seqs * kv->kv_heads * own_tiles;
-    const long long own_room = (long long)(kv->table_stride - prefix_pages) * kv->page;
     const int mode = !prefix_pages || few ? 0 : head_rows <= 64 ? 1 : 2;
     const int wgs = paged_few_wgs(dim, mode, nb);
     // Parts of own tasks: as many as have 128 positions in a full table, in at most
@@ -1747,7 +1752,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     // turn, alike.  8 kv heads of 128, one round / two / four: 64 slots of up to 4000
     // 113 / 111 / 109 us, 128 of up to 6000 326 / 304 / 297, 64 of up to 2000 behind
     // a prefix of 4096 72 / 65 / 63, but more for the join: 0 / 6 / 6 at 128 slots.
-    // One part up to 512 positions, and without a prefix, where it needs no join,
+    // One part up to `brief` positions, and without a prefix, where it needs no join,
     // where the slots' tasks are one to a CU for each 1024 positions or two.  One /
     // several with the join, us: 16 slots of up to 300 8.0 / 10.9, 48 of up to 700
     // 17.5 / 21.4, 128 of up to 500 27.2 / 34.0, 64 of up to 4000 113 / 116, 64 of up
@@ -1755,7 +1760,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     // behind 8000 21.0 / 23.9, 30 with 8 tokens behind 4096 47.6 / 52.3.
     long long own = (own_room + 127) / 128;
     while (own > 1 && own_base * own > 2LL * wgs * ctx->num_cu) own = (own + 1) / 2;
-    if (own_room <= 512 || (!prefix_pages && own_base * 1024 >= std::min(own_room, 2048LL) * ctx->num_cu)) own = 1;
+    if (own_room <= brief || (!prefix_pages && own_base * 1024 >= std::min(own_room, 2048LL) * ctx->num_cu)) own = 1;
     own = std::max(1LL, std::min(own, 64LL));
     int tiles = 0;
     long long pre = 0;

@@ -28,9 +28,10 @@ def _i32(v):
 
 class Batch:
     """A host-side cache of seqs slots with the given lengths, whose first
-    `prefix` positions are shared pages; `n_new` tokens are held on top."""
+    `prefix` positions are shared pages; `n_new` tokens are held on top.  Rows of
+    the table have `spare` entries more than the longest slot needs."""
 
-    def __init__(self, lens, n_new, heads, page, prefix=0, layers=1, seed=0, poison=None):
+    def __init__(self, lens, n_new, heads, page, prefix=0, layers=1, seed=0, poison=None, spare=1):
         from cima_amd.paged import PagedKV
 
         r = np.random.default_rng(seed)
@@ -38,7 +39,7 @@ class Batch:
         self.lens, self.n_new, self.page, self.pp = list(lens), n_new, page, prefix // page
         S = len(lens)
         held = [max(0, -(-(n + n_new) // page) - self.pp) if n >= 0 else 0 for n in lens]
-        stride = self.pp + max(held + [1]) + 1
+        stride = self.pp + max(held + [1]) + spare
         n_pages = self.pp + sum(held) + 3
         ids = r.permutation(n_pages)
         self.table = np.full((S, stride), -1, np.int32)
@@ -122,6 +123,17 @@ def test_attention_own_pages_only(hip, heads, page):
 @pytest.mark.parametrize("page,prefix", [(16, 16), (16, 48), (32, 320), (128, 1024), (256, 2048)])
 def test_attention_shared_prefix(hip, heads, page, prefix):
     _check(hip, Batch([prefix, prefix + 1, prefix + 40, prefix + 200, prefix + page], 1, heads, page, prefix, seed=2))
+
+
+@pytest.mark.parametrize("heads", HEADS, ids=str)
+@pytest.mark.parametrize("page,prefix", [(16, 16), (16, 48), (32, 320)])
+def test_attention_short_prefix_in_a_long_table(hip, heads, page, prefix):
+    """The same slots in tables of more than 640 positions: the prefix has tasks
+    of its own."""
+    for seqs in (1, 5):
+        lens = [prefix, prefix + 1, prefix + 40, prefix + 200, prefix + page][:seqs]
+        _check(hip, Batch(lens, 1, heads, page, prefix, seed=2, spare=700 // page))
+    _check(hip, Batch([prefix + 3, prefix + 90, -1], 4, heads, page, prefix, seed=23, spare=700 // page), window=60)
 
 
 @pytest.mark.parametrize("seqs", [1, 9, 20, 40, 80])
