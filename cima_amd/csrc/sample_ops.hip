@@ -13,10 +13,10 @@
 // part's maximum, its place and its sum, the second joins a row's parts, reads
 // its own logits once more and writes the probabilities.
 // Bound by memory: the probabilities go past the caches, which keep the logits
-// for the second reading.  Measured on MI355X, us: 384 rows of 128256 f16 63
-// (393 MB moved, 6.2 TB/s; through the caches 83, a row per workgroup in 32
-// words a thread 73); 256 rows of 60000 in one launch 21, in two 22.5; 64 of
-// 30000 7.3 and 8.6.  Parts of 2048 / 8192: one row of 151936 6.2 / 7.5, capped 3
+// for the second reading.  Measured on MI355X, us: 384 rows of 128256 f16 61
+// (393 MB moved, 6.5 TB/s; through the caches 83, a row per workgroup in 32
+// words a thread 73); 256 rows of 60000 in one launch 20.6, in two 22.5; 64 of
+// 30000 6.9 and 8.6.  Parts of 2048 / 8192: one row of 151936 6.2 / 7.5, capped 3
 // of 40000 8.0 / 14.8, eight of 151936 7.7 / 8.2; 384 of 128256 72 / 62.
 
 struct SmPart {
@@ -74,6 +74,17 @@ struct SmRow {
     int at;
 
     DEV float get(int r, int j) const { return sm_get<W32, V>(v[r], j); }
+    // a logit less c: of f16 logits as x * 1 - c, one instruction with the
+    // conversion, the same number
+    DEV float less(int r, int j, float c) const {
+        if constexpr (W32) return get(r, j) - c;
+        float d;
+        if (j & 1)
+            __asm__("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(v[r][j / 2]), "v"(c));
+        else
+            __asm__("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(v[r][j / 2]), "v"(c));
+        return d;
+    }
     // keeps the compiler from holding all logits as fp32 from one pass to the next
     DEV void fresh() {
 #pragma unroll
@@ -101,10 +112,20 @@ struct SmRow {
         __shared__ int place[NT / 64];
         const int w = threadIdx.x >> 6;
         m = -INFINITY;
+        if constexpr (W32) {
 #pragma unroll
-        for (int r = 0; r < R; r++)
+            for (int r = 0; r < R; r++)
 #pragma unroll
-            for (int j = 0; j < V; j++) m = fmaxf(m, get(r, j));
+                for (int j = 0; j < V; j++) m = fmaxf(m, get(r, j));
+        } else {  // two f16 at a time, exact
+            typedef _Float16 hp __attribute__((ext_vector_type(2)));
+            hp h = {(_Float16)-INFINITY, (_Float16)-INFINITY};
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int k = 0; k < V / 2; k++) h = __builtin_elementwise_max(h, __builtin_bit_cast(hp, v[r][k]));
+            m = fmaxf((float)h[0], (float)h[1]);
+        }
         m = wave_max_u(m);
         if ((threadIdx.x & 63) == 0) red[0][w] = m;
         __syncthreads();
@@ -119,7 +140,7 @@ struct SmRow {
             for (int r = 0; r < R; r++) {
                 float p = 0.f;
 #pragma unroll
-                for (int j = 0; j < V; j++) p += __builtin_amdgcn_exp2f((get(r, j) - c) * s);
+                for (int j = 0; j < V; j++) p += __builtin_amdgcn_exp2f(less(r, j, c) * s);
                 l += p;
             }
             l = wave_sum_u(l);
@@ -163,7 +184,7 @@ struct SmRow {
             float p[4];
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                const float h = __builtin_amdgcn_exp2f((get(r, j) - c) * s);
+                const float h = __builtin_amdgcn_exp2f(less(r, j, c) * s);
                 p[j] = T > 0.f ? h * (h * inv) : (i + j == A ? 1.f : 0.f);
             }
             float* o = y + row + i;
