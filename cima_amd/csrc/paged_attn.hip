@@ -6,8 +6,9 @@
 // step's tokens; those of all slots share the prefix's pages, so one workgroup
 // takes up to 256 of them through a range of the prefix and its keys and values
 // are read once for all (prefix tasks).  A slot's own pages are seen by its own
-// rows alone (own tasks).  Both kinds run the same code on a tile of rows and a
-// range of positions and leave {m, l, sum} per row; a second launch joins them.
+// rows alone (own tasks).  Both take a tile of rows through a range of positions
+// and leave {m, l, sum} per row, which a second launch joins; a row's only part
+// is its result.
 //
 // Rounding: q, keys and values are f16 as given; scores, maxima, sums of weights
 // and of values are fp32.  The weights are rounded to f16 for the second product,

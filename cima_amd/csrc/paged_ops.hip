@@ -10,7 +10,10 @@
 // once (pos * theta^(-2i/D) in fp64, reduced to a fraction of a turn there, so
 // that far positions keep their angle), then every thread rotates eight pairs
 // of a head, two 16-byte words.  Keys and values go to the row's place in its
-// page.
+// page.  Rotated in fp32 (the angle's sine and cosine are rounded to it) and
+// rounded to f16 once.  Bound by memory: 2048 rows of 48 heads of 128 (50 MB read
+// and written) 9.8 us on MI355X, 5.1 TB/s; four rows 3 us, the chain lens, table,
+// sine.
 template <int D>
 DEV void rope_append_body(const uint16_t* __restrict__ qkv, uint16_t* __restrict__ q, uint16_t* __restrict__ kp,
                           uint16_t* __restrict__ vp, const int* __restrict__ table, const int* __restrict__ lens,
@@ -216,7 +219,8 @@ DEV void each_lowest(const int* refs, int n_pages, const int* sum, uint32_t bits
 // Room for n_new tokens in slots [0, seqs): slot s lacks the entries from its
 // first -1 in [lens / page, end) on (entries are filled from the left).  The
 // page of rank r goes to the slot whose running sum holds r.  Bound by the
-// latency of its loads: the counts are read beside the lengths.
+// latency of its loads: the counts are read beside the lengths.  9 slots in 1024
+// pages 4.6 us on MI355X.
 extern "C" __global__ __launch_bounds__(1024) void cima_kv_pages_reserve(int* refs, int n_pages, int* table,
                                                                          const int* lens, int seqs, int table_stride,
                                                                          int page_shift, int n_new, int* status) {
@@ -282,7 +286,8 @@ extern "C" __global__ __launch_bounds__(1024) void cima_kv_pages_reserve(int* re
 
 // Fork, first launch: the slots are looked over and claimed (a child's lens
 // goes from -1 to -2 - i, so that one named twice shows), pages are found for
-// the children whose parent has begun a page, and entered.
+// the children whose parent has begun a page, and entered.  8 children in 1024
+// pages 4.5 us on MI355X, the second launch 3.5.
 extern "C" __global__ __launch_bounds__(1024) void cima_kv_pages_fork(int* refs, int n_pages, int* table, int* lens,
                                                                       int max_seqs, int table_stride, int page_shift,
                                                                       const int* __restrict__ parents,

@@ -538,12 +538,12 @@ class HipCtx:
         """(pointer, bytes) of a scratch tensor."""
         if a is None:
             return None, 0
-        p = _ptr(a)
         if isinstance(a, int):
             raise EngineError("hip", E_INVALID, "the slab is a bare pointer, its size unknown")
-        if a.get_device() != self.device:
-            raise EngineError("hip", E_INVALID, f"the slab is on device {a.get_device()}, the context on {self.device}")
-        return p, a.numel() * a.element_size()
+        if a.get_device() == self.device and a.is_contiguous():
+            return a.data_ptr(), a.nbytes
+        _ptr(a)
+        raise EngineError("hip", E_INVALID, f"the slab is on device {a.get_device()}, the context on {self.device}")
 
     def rope_append_paged(self, kv, layer: int, qkv, q, seqs: int, n_new: int, q_heads: int, theta: float) -> None:
         """RoPE of a step's queries (to ``q``) and keys, row ``s * n_new + j`` of
