@@ -160,6 +160,11 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     int* ids = reinterpret_cast<int*>(lds + T::RING);
     int* red = ids + IDS;  // per wave 8 ints
 
+    // the ids of pages about where the part begins if all of [plo, phi) is seen, a
+    // page a thread, fetched before the lengths are known
+    const int guess =
+        max(0, (plo + ((phi - plo + T::KT - 1) / T::KT + parts - 1) / parts * part * T::KT >> A.page_shift) - 64);
+    const int guess_id = trow[min(guess + (int)threadIdx.x, A.table_stride - 1)];
     // ---- this lane's row
     const int g = A.q_heads / A.kv_heads;
     const int r = r0 + 32 * wr + (lane & 31);
@@ -229,8 +234,13 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     auto fill_ids = [&](int first) {
         // all waves are past their last use of the ids (barrier before)
         const int n = min(IDS, page_of(base + t1 * T::KT - 1) - first + 1);
-        for (int i = threadIdx.x; i < n; i += 64 * T::NW)
-            ids[i] = (int)min((unsigned)max(trow[first + i], 0), (unsigned)A.n_pages - 1u);
+        auto put = [&](int i, int id) { ids[i] = (int)min((unsigned)max(id, 0), (unsigned)A.n_pages - 1u); };
+        if (first >= guess && first + n <= guess + 64 * T::NW) {
+            const int i = guess + (int)threadIdx.x - first;
+            if (i >= 0 && i < n) put(i, guess_id);
+        } else {
+            for (int i = threadIdx.x; i < n; i += 64 * T::NW) put(i, trow[first + i]);
+        }
         ids_from = first;
     };
     // A copy instruction c takes 1024 bytes of the 16 rows: this lane's row and
@@ -326,12 +336,17 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         __syncthreads();
         f16v sa[T::KB], sb[T::KB];  // scores of even and of odd tiles from t0 on
         int id = id_at(t0);
+        // the first keys, waited for alone, the first values and the second keys
         issue(t0, id, kplane, kword, KX, 0);
         issue(t0, id, vplane, vword, VX, 2 * T::BYTES);
-        if (t0 + 1 < t1) id = id_at(t0 + 1);
-        wait_vm<0>();
+        if (t0 + 1 < t1) {
+            id = id_at(t0 + 1);
+            issue(t0 + 1, id, kplane, kword, KX, 0);
+            wait_vm<2 * (D / 32)>();
+        } else {
+            wait_vm<D / 32>();
+        }
         barrier();
-        if (t0 + 1 < t1) issue(t0 + 1, id, kplane, kword, KX, 0);
         {
             const uint32_t kr = kread + (uint32_t)(t0 & 1) * T::BYTES;
 #pragma unroll
@@ -346,10 +361,8 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         // tile t, whose scores are in sc; those of the next go to sn
         auto turn = [&](int t, f16v (&sc)[T::KB], f16v (&sn)[T::KB]) {
             const bool more = t + 1 < t1;
-            if (t > t0 || more) {
-                wait_vm<0>();
-                barrier();
-            }
+            wait_vm<0>();
+            barrier();
             if (more) {
                 issue(t + 1, id, vplane, vword, VX, 2 * T::BYTES);
                 if (t + 2 < t1) {
