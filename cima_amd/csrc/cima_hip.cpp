@@ -1817,10 +1817,15 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     char name[64];
     hipFunction_t f;
     A.prefix_wgs = pre ? (int)((kv->kv_heads * pre + 7) / 8 * 8 * tiles) : 0;
-    snprintf(name, sizeof name, "cima_attn_paged_d%d_m%d_n%d", dim, mode, nb);
+    // Own tasks alone, no more than two to a CU, run in a kernel that has two of
+    // their tiles in flight.  us, one / two: 16 slots of 8 heads of 128 up to 300 7.9 /
+    // 7.5, 32 of them 9.2 / 8.7, 4 slots of 14/2 heads of 64 over 573 7.7 / 7.3.
+    const int kind = !pre && own_base * own <= 2LL * ctx->num_cu ? 1 : mode;
+    snprintf(name, sizeof name, "cima_attn_paged_d%d_m%d_n%d", dim, kind, nb);
     if (int rc = get_fn(ctx, name, &f)) return rc;
     void* args[] = {&A};
-    const unsigned lds = std::max(paged_few_lds(dim, nb, wgs == 4 ? 1 : 2), mode ? paged_attn_lds(dim) : 0u);
+    const int bufs = paged_few_wgs(dim, kind, nb) == 4 ? 1 : 2;
+    const unsigned lds = std::max(paged_few_lds(dim, nb, bufs), mode ? paged_attn_lds(dim) : 0u);
     if (int rc = launch(ctx, f, (unsigned)(A.prefix_wgs + own_base * own), 256, args, api, lds)) return rc;
     if (all == 1) return 0;
     const long long join = (long long)kv->kv_heads * ((head_rows + 15) / 16) * (dim / 16);

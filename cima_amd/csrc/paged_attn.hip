@@ -329,7 +329,10 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 
     // The loop is two tiles deep, so that the exponentials of one tile run beside
     // the next one's products: the scores of tile t are there when its turn
-    // begins, its values and the keys of tile t + 1 have arrived.
+    // begins, its values and the keys of tile t + 1 have arrived.  A short task (7
+    // tiles of 64) spends 0.7 us on the lengths, 0.2 on the ids, 0.4 to 0.8 on the
+    // first keys and 1 us a tile; around them stand the launch and, at its end, the
+    // write-back of the partial sums (2.7 us for 6 MB).
     if (t0 < t1) {
         __syncthreads();
         fill_ids(page_of(base + t0 * T::KT));
@@ -521,7 +524,8 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 // BUFS 2: a tile is on its way while the one before it is computed, 64 KB of LDS
 // a workgroup, two of them to a CU.  BUFS 1: the loads of a tile are waited for,
 // but the registers and LDS suffice for four workgroups to a CU, whose waves
-// cover each other; it is taken where the launch holds nothing larger.
+// cover each other; it is taken where the launch holds nothing larger and more
+// than two workgroups to a CU.
 // Measured on MI355X, 8 kv heads of 128, one / two in flight: 64 slots of up
 // to 4000 positions (524 MB) 107 / 146 us (4.9 TB/s), 128 of up to 500 27 / 33;
 // 128 full slots of 8192 (4.3 GB) 765 us with the join, 5.6 TB/s.  Values by
