@@ -660,6 +660,49 @@ def test_a_batch_of_continuations_step_by_step(hip):
 
 # --------------------------------------------------------------- refusals
 
+def test_pages_behind_4_gib(hip):
+    """The same slots in the first pages and in the last ones of planes of 6 GB:
+    every operator gives the same bits."""
+    from cima_amd.paged import PagedKV
+
+    heads, H, D, page, S = 8, 2, 128, 256, 3
+    lens, stride = [700, 512, 3], 5
+    r = np.random.default_rng(60)
+    rows = r.standard_normal((2, 12, H, page, D)).astype(np.float16)
+    qkv = torch.from_numpy(r.standard_normal((S, (heads + 2 * H) * D)).astype(np.float16)).cuda()
+    results = []
+    for n_pages, first in ((40, 0), (50000, 50000 - 40)):
+        pool = torch.empty((2, n_pages, H, page, D), dtype=torch.float16, device="cuda")
+        assert first == 0 or pool[0].numel() * 2 > 6 << 30
+        pool[:, first:first + 12] = torch.from_numpy(rows).cuda()
+        table = np.full((S + 1, stride), -1, np.int32)
+        table[0, :4], table[1, :4], table[2, :1] = [0, 1, 5, 9], [0, 1, 11, 7], [3]
+        table[table >= 0] += first
+        refs = torch.zeros(n_pages, dtype=torch.int32, device="cuda")
+        refs += 1                                       # free pages lie at the end alone
+        refs[first + 20:first + 30] = 0
+        kv = PagedKV(pool, refs, _i32(table), _i32(lens + [-1]))
+        q, out = (torch.zeros((S, heads, D), dtype=torch.float16, device="cuda") for _ in range(2))
+        slab = torch.empty(8 << 20, dtype=torch.uint8, device="cuda")
+        status = _i32([9])
+        hip.kv_pages_fork(kv, _i32([0]), _i32([3]), 1, status)   # the page begun: first + 20
+        torch.cuda.synchronize()
+        assert status.item() == 0 and kv.table[3].tolist() == [first, first + 1, first + 20, -1, -1]
+        hip.rope_append_paged(kv, 0, qkv, q, S, 1, heads, 1e6)
+        hip.attn_paged(kv, 0, q, out, S, 1, heads, 0.1, slab)
+        shared = torch.zeros_like(out)
+        hip.attn_paged(kv, 0, q[:2], shared[:2], 2, 1, heads, 0.1, slab, prefix_pages=2)
+        hip.kv_pages_copy(kv, _i32([first + 11]), _i32([first + 33]), 1)
+        torch.cuda.synchronize()
+        results.append([t.cpu() for t in (q, out, shared, pool[:, first:first + 12], pool[:, first + 33],
+                                          pool[:, first + 20, :, :700 - 512])])
+        del pool, kv
+        torch.cuda.empty_cache()
+    for a, b in zip(*results):
+        assert torch.equal(a.view(torch.int16), b.view(torch.int16))
+    assert torch.isfinite(results[0][1]).all() and results[0][1].abs().max() > 0
+
+
 def test_refusals(hip):
     b = Batch([64, 70], 1, (8, 2, 64), 32, 64, seed=50)
     q = torch.zeros((2, 8, 64), dtype=torch.float16, device="cuda")

@@ -345,6 +345,37 @@ def test_a_sampling_step_in_a_graph(hip):
         hip.use_torch_stream()
 
 
+def test_rows_behind_2_to_31_elements(hip):
+    """Offsets of rows and probabilities in 64 bits."""
+    rows, n = 17000, 128256
+    assert rows * n > 2 ** 31
+    x = torch.empty((rows, n), dtype=torch.float16, device="cuda")
+    x[:-5] = 0
+    x[-5:] = torch.randn((5, n), device="cuda", generator=torch.Generator("cuda").manual_seed(1)).half()
+    y = torch.empty((rows, n), device="cuda")
+    hip.softmax_rows(x, y, rows, n, None, 1, 0.0, torch.empty(rows * 16 * 16, dtype=torch.uint8, device="cuda"))
+    want, tol = _softmax_want(x[-5:].cpu().numpy(), np.ones(5, np.float32), 1, 0.0)
+    assert (np.abs(y[-5:].cpu().numpy() - want) <= tol).all()
+    assert (y[:-5:500] - 1 / n).abs().max().item() < 2.0 ** -20 / n
+    del x, y
+    S, K, V = 9000, 1, 128256
+    assert S * (K + 1) * V > 2 ** 31
+    p = torch.zeros((S, K + 1, V), device="cuda")
+    at = (torch.arange(S, device="cuda")[:, None] * 14 + torch.arange(2, device="cuda")) % V
+    p.scatter_(2, at[:, :, None], 1.0)
+    drafts = at[:, :1].clone()
+    drafts[1::2] += 1                                   # refused: all of p is at another token
+    f = dict(device="cuda", dtype=torch.int32)
+    acc, tokens = torch.empty(S, **f), torch.empty((S, 2), **f)
+    hip.verify_drafts(p, None, drafts.int(), None, torch.full((S, 2), 0.5, device="cuda"), acc, tokens, None, S, K, V,
+                      torch.empty(8 * S * 64, dtype=torch.uint8, device="cuda"))
+    torch.cuda.synchronize()
+    want = torch.where((torch.arange(S, device="cuda") % 2 == 0)[:, None], at, torch.stack([at[:, 0], at[:, 0] * 0 - 1], 1))
+    assert torch.equal(acc, 1 - torch.arange(S, **f) % 2) and torch.equal(tokens.long(), want)
+    del p
+    torch.cuda.empty_cache()
+
+
 def test_refusals(hip):
     x, y, slab = torch.zeros((2, 100), device="cuda"), torch.zeros((2, 100), device="cuda"), _slab()
     i = torch.zeros(200, dtype=torch.int32, device="cuda")
