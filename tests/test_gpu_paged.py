@@ -658,6 +658,82 @@ def test_a_batch_of_continuations_step_by_step(hip):
     assert not kv.refs.any() and (kv.table == -1).all() and (kv.lens == -1).all()
 
 
+def test_a_captured_step_replays_as_the_batch_grows(hip):
+    """Reserve, append, attention, softmax and verification of a step recorded
+    once and replayed while lengths, pages and slots change; an eager twin on
+    another cache gives the same bits after every step."""
+    Q, H, D, page, layers, S, n, V = 14, 2, 64, 16, 2, 4, 3, 5000
+    r = np.random.default_rng(70)
+    twins = [_some_cache(96, page, max_seqs=S, max_len=900, heads=H, dim=D, layers=layers, seed=71) for _ in range(2)]
+    f32, i32 = dict(device="cuda"), dict(device="cuda", dtype=torch.int32)
+    qkv = torch.zeros((layers, S * n, (Q + 2 * H) * D), dtype=torch.float16, device="cuda")
+    logits = torch.zeros((S * n, V), dtype=torch.float16, device="cuda")
+    drafts, u = torch.zeros((S, n - 1), **i32), torch.zeros((S, n), **f32)
+    temp = torch.tensor([0.7, 0.0, 1.2, 1.0], **f32)
+    bufs = [dict(q=torch.zeros((S * n, Q, D), dtype=torch.float16, device="cuda"),
+                 out=torch.zeros((layers, S * n, Q, D), dtype=torch.float16, device="cuda"),
+                 p=torch.zeros((S * n, V), **f32), acc=torch.zeros(S, **i32), tok=torch.zeros((S, n), **i32),
+                 status=torch.zeros(1, **i32), slab=torch.zeros(16 << 20, dtype=torch.uint8, device="cuda"))
+            for _ in twins]
+
+    def step(kv, b):
+        hip.kv_pages_reserve(kv, S, n, b["status"])
+        for layer in range(layers):
+            hip.rope_append_paged(kv, layer, qkv[layer], b["q"], S, n, Q, THETA)
+            hip.attn_paged(kv, layer, b["q"], b["out"][layer], S, n, Q, 0.125, b["slab"], prefix_pages=2, window=200)
+        hip.softmax_rows(logits, b["p"], S * n, V, temp, n, 0.0, b["slab"])
+        hip.verify_drafts(b["p"], None, drafts, None, u, b["acc"], b["tok"], kv.lens, S, n - 1, V, b["slab"])
+
+    for kv, b in zip(twins, bufs):                      # a prompt of 37 tokens in slot 0, forked into 1 and 2
+        kv.lens[0] = 0
+        hip.kv_pages_reserve(kv, 1, 37, b["status"])
+        for layer in range(layers):
+            x = torch.from_numpy(np.random.default_rng(layer).standard_normal((37, (Q + 2 * H) * D)).astype(np.float16))
+            hip.rope_append_paged(kv, layer, x.cuda(), torch.zeros((37, Q * D), dtype=torch.float16, device="cuda"), 1, 37,
+                                  Q, THETA)
+        kv.lens[0] = 37
+        hip.kv_pages_fork(kv, _i32([0, 0]), _i32([1, 2]), 2, b["status"])
+        torch.cuda.synchronize()
+        assert b["status"].item() == 0
+    st = torch.cuda.Stream()
+    hip.set_stream(st)
+    try:
+        hip.capture_begin()
+        try:
+            step(twins[0], bufs[0])
+        finally:
+            g = hip.capture_end()
+    finally:
+        hip.use_torch_stream()
+    for k in range(8):
+        qkv.copy_(torch.from_numpy(r.standard_normal(qkv.shape).astype(np.float16)))
+        logits.copy_(torch.from_numpy((r.standard_normal(logits.shape) * 3).astype(np.float16)))
+        drafts.copy_(logits.view(S, n, V)[:, :n - 1].argmax(-1))
+        u.copy_(torch.from_numpy(r.random((S, n)).astype(np.float32)))
+        torch.cuda.synchronize()
+        before = twins[1].lens.tolist()
+        g.launch()
+        torch.cuda.synchronize()
+        step(twins[1], bufs[1])
+        torch.cuda.synchronize()
+        for key in ("out", "p", "acc", "tok", "status"):
+            assert torch.equal(bufs[0][key], bufs[1][key]), (k, key)
+        for key in ("lens", "table", "refs", "pool"):
+            assert torch.equal(getattr(twins[0], key), getattr(twins[1], key)), (k, key)
+        assert bufs[0]["status"].item() == 0
+        assert twins[0].lens.tolist() == [m + a + 1 if m >= 0 else -1 for m, a in zip(before, bufs[0]["acc"].tolist())]
+        for kv, b in zip(twins, bufs):                  # the batch changes between the steps
+            if k == 2:
+                hip.kv_pages_fork(kv, _i32([2]), _i32([3]), 1, b["status"])
+            if k == 4:
+                hip.kv_pages_free(kv, _i32([1]), 1)
+            if k == 5:
+                hip.kv_pages_compact(kv, kv.refs, kv.table, b["status"], b["slab"])
+            if k == 6:
+                hip.kv_pages_fork(kv, _i32([3]), _i32([1]), 1, b["status"])
+        torch.cuda.synchronize()
+
+
 # --------------------------------------------------------------- refusals
 
 def test_pages_behind_4_gib(hip):
