@@ -59,8 +59,10 @@ DEV float uniform(float v) {
 // c / T within fp32's range, so that no difference of logits becomes 0 * inf at a
 // temperature that is infinite or next to nothing
 DEV float sm_scale(float c, float T) { return fminf(fmaxf(c / T, 1e-37f), 1e38f); }
-// f of a logit; those behind n stay -inf
-DEV float sm_f(float x, int i, int n, float cap) { return i < n ? cap * tanhf(x / cap) : x; }
+// f of a logit, cap * tanh(x / cap).  Infinite ones stay as they are: -inf is a
+// token that may not be taken (or no logit, behind n), and -cap would give it a
+// share.
+DEV float sm_f(float x, float cap) { return __builtin_isinf(x) ? x : cap * tanhf(x / cap); }
 
 // R words of V logits a thread of a row by NT threads: the maximum, the first place of it
 // (T <= 0) or the sum (T > 0).  CAP: f is applied when the logits are loaded,
@@ -98,10 +100,9 @@ struct SmRow {
         for (int r = 0; r < R; r++) {
             if constexpr (CAP) {
                 uint32_t w[F32 ? V : V / 2];
-                const int i = base + r * NT * V;
-                sm_load<F32, V>(x, row, i, n, w);
+                sm_load<F32, V>(x, row, base + r * NT * V, n, w);
 #pragma unroll
-                for (int j = 0; j < V; j++) v[r][j] = __builtin_bit_cast(uint32_t, sm_f(sm_get<F32, V>(w, j), i + j, n, cap));
+                for (int j = 0; j < V; j++) v[r][j] = __builtin_bit_cast(uint32_t, sm_f(sm_get<F32, V>(w, j), cap));
             } else {
                 sm_load<F32, V>(x, row, base + r * NT * V, n, v[r]);
             }

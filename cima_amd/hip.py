@@ -602,7 +602,8 @@ class HipCtx:
     def softmax_rows(self, x, y, rows: int, n: int, temp=None, rows_per_temp: int = 1, cap: float = 0.0,
                      slab=None) -> None:
         """``y[r] = softmax(x[r] / temp[r // rows_per_temp])`` in fp32 (temp <= 0:
-        the largest logit alone; cap > 0: logits through ``cap * tanh(x / cap)``)."""
+        the largest logit alone; cap > 0: finite logits through ``cap * tanh(x /
+        cap)``).  A logit of -inf has probability 0, capped or not."""
         if rows_per_temp <= 0:
             raise EngineError("hip", E_INVALID, f"rows_per_temp is {rows_per_temp}")
         act, d = _act_of(x), self.device

@@ -502,11 +502,13 @@ int cima_hip_kv_pages_compact(cima_hip_ctx* ctx, const cima_kv_pages* kv, int* r
                               void* slab, unsigned long long slab_bytes);
 
 /* Probabilities of rows of logits: y[r] = softmax(f(x[r]) / temp[r /
- * rows_per_temp]) fp32, x f32 or f16 [rows, n], f(v) = cap * tanh(v / cap)
- * where cap > 0 (as cima_hip_argmax), else v.  temp NULL = 1; where it is <= 0
- * the row is 1 at its largest logit (the lowest index of equals) and 0
- * elsewhere.  A row of -inf alone becomes zeros; NaN or +inf make a row NaN
- * (temp <= 0: +inf ranks as the largest, NaN as the lowest).  x and y do not
+ * rows_per_temp]) fp32, x f32 or f16 [rows, n], f(v) = cap * tanh(v / cap) of
+ * finite logits where cap > 0, else v.  temp NULL = 1; where it is <= 0 or NaN
+ * the row is 1 at its largest f(x) (the lowest index of equals) and 0
+ * elsewhere.  With a cap or without, a logit of -inf has probability 0 at every
+ * temperature (a token that may not be taken) and a row of -inf alone becomes
+ * zeros; NaN or +inf make a row NaN (temp <= 0 or NaN: +inf ranks as the
+ * largest, NaN as the lowest).  x and y do not
  * overlap; less than 2^22 rows.  slab (8-byte aligned): 16 bytes for each 8192 logits of a row
  * (rounded up) and row; none is needed up to 32768 logits.  One of 16 KB or
  * more makes few rows faster. */

@@ -23,6 +23,22 @@ def pytest_configure(config):
     config.addinivalue_line("markers", "slow: large shapes (minutes on CPU)")
 
 
+# tests whose expected value is wrong, kept as they were written: they run and
+# are expected to fail
+_WRONG_VALUES = {
+    "test_gpu_sample.py::test_softmax[30.0-":
+        "the host form sends a logit of -inf through the cap, to -cap: a token that may not be taken gets a "
+        "probability, a row of such tokens alone 1 / n; test_gpu_sample_cap.py holds the right values at these sizes",
+}
+
+
+def pytest_collection_modifyitems(items):
+    for item in items:
+        for start, reason in _WRONG_VALUES.items():
+            if item.nodeid.rsplit("/", 1)[-1].startswith(start):
+                item.add_marker(pytest.mark.xfail(strict=True, reason=reason))
+
+
 def _ensure_built():
     # load what is built; build only when nothing is
     import cima_amd.build as b
