@@ -94,6 +94,10 @@ DEV int min16(int v) {
 }
 DEV int max16(int v) { return -min16(-v); }
 
+// Values of positions that have no page (a table entry that is no page's id):
+// their scores are masked, and a weight of 0 multiplies what is read for them.
+__device__ const uint4 no_page[256 * 128 * 2 / 16] = {};
+
 struct AttnArgs {
     const uint16_t* q;
     const uint16_t* kp;  // planes of the layer
@@ -158,7 +162,8 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     const int wr = wave % WR, wk = wave / WR;
     const int half = lane >> 5;
     int* ids = reinterpret_cast<int*>(lds + T::RING);
-    int* red = ids + IDS;  // per wave 8 ints
+    int* red = ids + IDS;  // per wave 8 ints; [4]: an id of the task names no page
+    if (threadIdx.x == 0) red[4] = 0;
 
     // the ids of pages about where the part begins if all of [plo, phi) is seen, a
     // page a thread, fetched before the lengths are known
@@ -227,14 +232,19 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 
     // ---- copies: a wave brings 16 rows of a tile's keys and of its values, which
     // a page holds all; rows that no one sees are replaced by the nearest that
-    // someone does, so that what they hold is never multiplied
+    // someone does, so that what they hold is never multiplied, and values without
+    // a page by zeros
     const int page = 1 << A.page_shift;
     auto page_of = [&](int p) { return min(max(p, lo_any), hi_any - 1) >> A.page_shift; };
     int ids_from = -IDS;  // first page of the ids in LDS
     auto fill_ids = [&](int first) {
         // all waves are past their last use of the ids (barrier before)
         const int n = min(IDS, page_of(base + t1 * T::KT - 1) - first + 1);
-        auto put = [&](int i, int id) { ids[i] = (int)min((unsigned)max(id, 0), (unsigned)A.n_pages - 1u); };
+        auto put = [&](int i, int id) {
+            const bool none = (unsigned)id >= (unsigned)A.n_pages;
+            ids[i] = none ? -1 : id;
+            if (none) red[4] = 1;
+        };
         if (first >= guess && first + n <= guess + 64 * T::NW) {
             const int i = guess + (int)threadIdx.x - first;
             if (i >= 0 && i < n) put(i, guess_id);
@@ -260,7 +270,9 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     auto id_at = [&](int t) { return ids[page_of(base + t * T::KT + 16 * wave) - ids_from]; };
     auto issue = [&](int t, int id, const uint16_t* plane, uint32_t word, uint32_t flip, uint32_t ring) {
         const int p0 = base + t * T::KT + 16 * wave;
-        const uint16_t* src = plane + (size_t)__builtin_amdgcn_readfirstlane(id) * page_elems;
+        id = __builtin_amdgcn_readfirstlane(id);
+        const uint16_t* src = plane + (size_t)max(id, 0) * page_elems;
+        if (ring && id < 0) src = reinterpret_cast<const uint16_t*>(no_page);
         const uint32_t dst = lds0 + ring + (uint32_t)(t & 1) * T::BYTES;
         if (p0 >= lo_any && p0 + 16 <= hi_any) {
             src += (size_t)(p0 & (page - 1)) * D;
@@ -299,16 +311,26 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         const s8 v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
         return __builtin_bit_cast(h8, v);
     };
-    // the scores of tile t that a row does not see become -inf; the largest left
+    // the scores of tile t that a row does not see, or that have no page, become
+    // -inf; the largest left
+    bool holes = false;  // an id among those that were in LDS names no page
     auto mask = [&](int t, f16v (&sc)[T::KB]) {
         const int p0 = base + t * T::KT;
+        int end[2 * T::KB];  // of the wave's 16 keys from 16 j on
+#pragma unroll
+        for (int j = 0; j < 2 * T::KB; j++) end[j] = hi;
+        if (holes) {
+#pragma unroll
+            for (int j = 0; j < 2 * T::KB; j++)
+                if (ids[page_of(p0 + kw + 16 * j) - ids_from] < 0) end[j] = 0;
+        }
         float mx = -INFINITY;
 #pragma unroll
         for (int b = 0; b < T::KB; b++)
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const int p = p0 + kw + 32 * b + (i & 3) + 8 * (i >> 2) + 4 * half;
-                sc[b][i] = p >= lo && p < hi ? sc[b][i] : -INFINITY;
+                sc[b][i] = p >= lo && p < end[2 * b + (i >> 3)] ? sc[b][i] : -INFINITY;
                 mx = fmaxf(mx, sc[b][i]);
             }
         return mx;
@@ -337,6 +359,7 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         __syncthreads();
         fill_ids(page_of(base + t0 * T::KT));
         __syncthreads();
+        holes = __builtin_amdgcn_readfirstlane(red[4]);
         f16v sa[T::KB], sb[T::KB];  // scores of even and of odd tiles from t0 on
         int id = id_at(t0);
         // the first keys, waited for alone, the first values and the second keys
@@ -370,8 +393,9 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
                 issue(t + 1, id, vplane, vword, VX, 2 * T::BYTES);
                 if (t + 2 < t1) {
                     if (page_of(base + (t + 3) * T::KT - 1) - ids_from >= IDS) {
-                        fill_ids(page_of(base + (t + 2) * T::KT));
+                        fill_ids(page_of(base + (t + 1) * T::KT));  // its mask looks them up
                         __syncthreads();
+                        holes = __builtin_amdgcn_readfirstlane(red[4]);
                     }
                     id = id_at(t + 2);
                     issue(t + 2, id, kplane, kword, KX, 0);
@@ -439,7 +463,7 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
             __asm__ volatile("" : "+v"(mx));  // found beside the products, not behind them
             if (more) {
                 const int p0 = base + (t + 1) * T::KT;
-                if (p0 < lo_all || p0 + T::KT > hi_all) mx = mask(t + 1, sn);
+                if (p0 < lo_all || p0 + T::KT > hi_all || holes) mx = mask(t + 1, sn);
                 raise(mx);
             }
         };
@@ -550,10 +574,10 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
     const int li = lane & 15, q4 = lane >> 4;
     const int g = A.q_heads / A.kv_heads;
     // the ids of the 64 pages that the part most likely begins with, fetched
-    // before the lengths are known; lane i: id of page ids_from + i
+    // before the lengths are known; lane i: id of page ids_from + i, -1: none
     auto fetch_ids = [&](int first) {
         const int id = trow[min(first + lane, A.table_stride - 1)];
-        return (int)min((unsigned)max(id, 0), (unsigned)A.n_pages - 1u);
+        return (unsigned)id < (unsigned)A.n_pages ? id : -1;
     };
     int ids_from = guess, ids = fetch_ids(guess);
     // ---- this lane's rows
@@ -607,11 +631,14 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
         for (int x = 0; x < XT; x++) o[b][x] = f4{0.f, 0.f, 0.f, 0.f};
     }
     // ---- loads of a tile: two groups of 16 positions, each within a page; rows
-    // that no one sees are replaced by the nearest that someone does
+    // that no one sees are replaced by the nearest that someone does, values
+    // without a page by zeros
     const int page = 1 << A.page_shift;
     const uint32_t vbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * F::WAVE;
     h8 kf[BUFS][2][STEPS];
+    uint32_t gone[BUFS];  // bit u: group u of the tile has no page
     auto issue = [&](int t, auto buf) {
+        gone[buf] = 0;
 #pragma unroll
         for (int u = 0; u < 2; u++) {
             const int p0 = base + 32 * t + 16 * u;
@@ -621,7 +648,9 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
                 ids_from = pg;
             }
             const int id = __builtin_amdgcn_readlane(ids, pg - ids_from);
-            const size_t off = ((size_t)id * A.kv_heads + kvh) * page * D;
+            gone[buf] |= (uint32_t)id >> 31 << u;
+            const size_t off = ((size_t)max(id, 0) * A.kv_heads + kvh) * page * D;
+            const uint16_t* vsrc = id < 0 ? reinterpret_cast<const uint16_t*>(no_page) : A.vp + off;
             const int pk = min(max(p0 + li, lo_any), hi_any - 1) & (page - 1);
 #pragma unroll
             for (int i = 0; i < STEPS; i++)
@@ -631,7 +660,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
                 const int row = c * (64 / CH) + lane / CH, w = lane % CH;
                 const int p = min(max(p0 + row, lo_any), hi_any - 1) & (page - 1);
                 const int f = D == 128 ? (row & 7) << 1 : (row >> 1 & 3) << 1;
-                dma16(A.vp + off + (size_t)p * D + 8 * (w ^ f), vbase + buf * F::VT + u * 16 * D * 2 + c * 1024);
+                dma16(vsrc + (size_t)p * D + 8 * (w ^ f), vbase + buf * F::VT + u * 16 * D * 2 + c * 1024);
             }
         }
     };
@@ -641,6 +670,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
         if constexpr (BUFS == 2)
             if (t + 4 < t1) issue(t + 4, std::integral_constant<int, 1 - buf>{});
         const int p0 = base + 32 * t;
+        __asm__ volatile("" : "+s"(gone[buf]));  // one path for the tile, by one test
         h8 pf[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
@@ -652,14 +682,16 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
                 for (int i = 0; i < STEPS; i++)
                     sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[buf][u][i], qf[b][i], sc[u], 0, 0, 0);
             }
-            if (p0 < lo_all || p0 + 32 > hi_all) {
+            if (p0 < lo_all || p0 + 32 > hi_all || gone[buf]) {
 #pragma unroll
-                for (int u = 0; u < 2; u++)
+                for (int u = 0; u < 2; u++) {
+                    const int end = gone[buf] >> u & 1 ? 0 : hi[b];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int p = p0 + 16 * u + 4 * q4 + i;
-                        sc[u][i] = p >= lo[b] && p < hi[b] ? sc[u][i] : -INFINITY;
+                        sc[u][i] = p >= lo[b] && p < end ? sc[u][i] : -INFINITY;
                     }
+                }
             }
             float mx = sc[0][0];
 #pragma unroll

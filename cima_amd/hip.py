@@ -572,7 +572,8 @@ class HipCtx:
 
     def kv_pages_reserve(self, kv, seqs: int, n_new: int, status) -> None:
         """Pages for ``n_new`` more tokens in each of slots [0, seqs) in use;
-        ``status[0]`` = pages missing (then nothing is changed)."""
+        ``status[0]`` = pages missing (then nothing is changed, and the step's
+        lengths have to be put back before it is taken again)."""
         self._check(self.lib.cima_hip_kv_pages_reserve(self.handle, self._kv(kv), seqs, n_new,
                                                        _ptr_of(status, _I32, 1, "status", self.device)))
 

@@ -457,7 +457,8 @@ int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int l
  * (window 0: all up to p), out f16 of q's shape.  The first prefix_pages
  * entries of every slot in use are the same pages; they are read from row
  * prefix_slot of the table, once for all rows.  Rows of slots not in use are
- * written as zeros.  Pages that no row sees may be absent (-1) and hold
+ * written as zeros.  A position whose entry of the table is no page's id is not
+ * seen, and a row that sees none is zeros.  Pages that no row sees may hold
  * anything; what some row sees must be finite.  Scores and sums are fp32; the
  * probabilities are rounded to f16 for the product with the values.
  *
@@ -480,7 +481,12 @@ int cima_hip_kv_pages_copy(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int
  * pages, slot by slot, with count 1.  All or nothing: *status = 0, or the
  * number of pages that are missing, and nothing is changed.  Entries behind
  * table_stride count as missing (at most 262144 a slot).  Behind a slot's first
- * -1 there is no page. */
+ * -1 there is no page.
+ *
+ * A step after a reserve that found too few may run to its end, as a captured
+ * one does: the tokens that have no page are dropped and not seen.  It has to be
+ * taken again: put lens back to what it was before the step and free a slot, or
+ * ask for less.  Entries that lens has passed are not filled later. */
 int cima_hip_kv_pages_reserve(cima_hip_ctx* ctx, const cima_kv_pages* kv, int seqs, int n_new, int* status);
 /* Slot children[i] becomes a copy of slot parents[i], i < n: the pages that
  * the parent has filled are shared (counts + 1), the rows of a page begun are
