@@ -1670,7 +1670,7 @@ int paged_few_wgs(int dim, int mode, int nb) { return mode == 0 && !(dim == 128 
 unsigned paged_few_lds(int dim, int nb, int bufs) {
     return (unsigned)(4 * std::max(bufs * 32 * dim * 2, nb * (dim / 16) * 64 * 16) + 4 * nb * 16 * 8);
 }
-unsigned paged_attn_lds(int dim) { return (unsigned)(4 * 64 * dim * 2 + 1024 * 4 + 4 * 32); }
+unsigned paged_attn_lds(int dim) { return (unsigned)(4 * 64 * dim * 2 + 1024 * 4 + 4 * 32 + 128 * 8); }
 
 }  // namespace
 

@@ -81,6 +81,14 @@ DEV float quarters_sum(float v) {
     return __builtin_bit_cast(float, a) + __builtin_bit_cast(float, b);
 }
 
+// this lane, anew: where it is needed rarely, nothing made of it is kept in a
+// register until then
+DEV int lane_now() {
+    int lane = __builtin_amdgcn_mbcnt_hi(-1, __builtin_amdgcn_mbcnt_lo(-1, 0));
+    __asm__ volatile("" : "+v"(lane));
+    return lane;
+}
+
 // minimum over aligned groups of 16 lanes
 template <int CTRL>
 DEV int dpp_min(int v) {
@@ -94,8 +102,9 @@ DEV int min16(int v) {
 }
 DEV int max16(int v) { return -min16(-v); }
 
-// Values of positions that have no page (a table entry that is no page's id):
-// their scores are masked, and a weight of 0 multiplies what is read for them.
+// Values of positions that have no page (a table entry that is no page's id) or
+// lie between the windows of a task's rows: their scores are masked, and a weight
+// of 0 multiplies what is read for them.
 __device__ const uint4 no_page[256 * 128 * 2 / 16] = {};
 
 struct AttnArgs {
@@ -137,7 +146,7 @@ struct Tile {
     static constexpr int RING = 2 * 2 * BYTES;        // two tiles: one being read, one on its way
     // the merge of WK waves' sums reuses the ring
     static_assert(WK == 1 || (WK - 1) * WR * 64 * (D / 32) * 16 * 4 <= RING, "merge space");
-    static constexpr int LDS = RING + IDS * 4 + NW * 32;
+    static constexpr int LDS = RING + IDS * 4 + NW * 32 + WR * 32 * 8;
     static_assert(LDS <= 80 * 1024, "two workgroups to a CU");
 };
 
@@ -163,6 +172,7 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     const int half = lane >> 5;
     int* ids = reinterpret_cast<int*>(lds + T::RING);
     int* red = ids + IDS;  // per wave 8 ints; [4]: an id of the task names no page
+    int2* span = reinterpret_cast<int2*>(red + 8 * T::NW);  // the positions that each row sees
     if (threadIdx.x == 0) red[4] = 0;
 
     // the ids of pages about where the part begins if all of [plo, phi) is seen, a
@@ -193,6 +203,7 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     // ---- the positions that rows of the workgroup see: any of [lo, hi), all of
     // [lo_all, hi_all)
     int lo_any = live ? lo : 0x7fffffff, hi_any = live ? hi : 0, lo_all = live ? lo : 0, hi_all = live ? hi : 0x7fffffff;
+    if (wk == 0 && half == 0) span[32 * wr + lane] = live ? make_int2(lo, hi) : make_int2(0, 0);
     if (!live) lo = 0, hi = 0x7fffffff;  // masked by its l at the end
     lo_any = min16(lo_any), hi_any = max16(hi_any), lo_all = max16(lo_all), hi_all = min16(hi_all);
     lo_any = min(lo_any, __builtin_amdgcn_readlane(lo_any, 16));
@@ -233,11 +244,12 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     // ---- copies: a wave brings 16 rows of a tile's keys and of its values, which
     // a page holds all; rows that no one sees are replaced by the nearest that
     // someone does, so that what they hold is never multiplied, and values without
-    // a page by zeros
+    // a page by zeros.  Where the rows have no position in common their windows may
+    // lie apart (slots that end within the prefix): values that none sees are zeros
     const int page = 1 << A.page_shift;
     auto page_of = [&](int p) { return min(max(p, lo_any), hi_any - 1) >> A.page_shift; };
     int ids_from = -IDS;  // first page of the ids in LDS
-    auto fill_ids = [&](int first) {
+    auto fill_ids = [&](int first, auto begin) {
         // all waves are past their last use of the ids (barrier before)
         const int n = min(IDS, page_of(base + t1 * T::KT - 1) - first + 1);
         auto put = [&](int i, int id) {
@@ -245,11 +257,11 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
             ids[i] = none ? -1 : id;
             if (none) red[4] = 1;
         };
-        if (first >= guess && first + n <= guess + 64 * T::NW) {
+        if (begin && first >= guess && first + n <= guess + 64 * T::NW) {
             const int i = guess + (int)threadIdx.x - first;
             if (i >= 0 && i < n) put(i, guess_id);
         } else {
-            for (int i = threadIdx.x; i < n; i += 64 * T::NW) put(i, trow[first + i]);
+            for (int i = 64 * wave + lane_now(); i < n; i += 64 * T::NW) put(i, trow[first + i]);
         }
         ids_from = first;
     };
@@ -286,6 +298,19 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
                 dma16(src, (uint32_t)p * ROWB + (word ^ c * flip), dst + c * 1024);
             }
         }
+    };
+    // the wave's 16 rows of tile t's values, which have arrived: zeros where none of
+    // the workgroup's rows sees the position
+    auto clear = [&](int t) {
+        const int ln = lane_now();
+        const int2 a = span[ln & (32 * WR - 1)], b = span[(64 + ln) & (32 * WR - 1)];
+        uint32_t seen = 0;  // bit i: position p0 + i
+        for (int i = 0, p = base + t * T::KT + 16 * wave; i < 16; i++, p++)
+            if (__ballot((a.x <= p && p < a.y) || (b.x <= p && p < b.y))) seen |= 1u << i;
+        uint4* v = reinterpret_cast<uint4*>(lds + 2 * T::BYTES + (t & 1) * T::BYTES + wave * 16 * ROWB) + ln;
+#pragma unroll
+        for (int c = 0; c < D / 32; c++)
+            if (!(seen >> (c * (64 / CH) + ln / CH) & 1)) v[64 * c] = make_uint4(0, 0, 0, 0);
     };
     const int kw = wk * 32 * T::KB;  // this wave's keys of a tile
     f16v zero16;
@@ -357,7 +382,7 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     // write-back of the partial sums (2.7 us for 6 MB).
     if (t0 < t1) {
         __syncthreads();
-        fill_ids(page_of(base + t0 * T::KT));
+        fill_ids(page_of(base + t0 * T::KT), std::true_type{});
         __syncthreads();
         holes = __builtin_amdgcn_readfirstlane(red[4]);
         f16v sa[T::KB], sb[T::KB];  // scores of even and of odd tiles from t0 on
@@ -388,12 +413,13 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         auto turn = [&](int t, f16v (&sc)[T::KB], f16v (&sn)[T::KB]) {
             const bool more = t + 1 < t1;
             wait_vm<0>();
+            if (lo_all > hi_all) clear(t);
             barrier();
             if (more) {
                 issue(t + 1, id, vplane, vword, VX, 2 * T::BYTES);
                 if (t + 2 < t1) {
                     if (page_of(base + (t + 3) * T::KT - 1) - ids_from >= IDS) {
-                        fill_ids(page_of(base + (t + 1) * T::KT));  // its mask looks them up
+                        fill_ids(page_of(base + (t + 1) * T::KT), std::false_type{});  // its mask looks them up
                         __syncthreads();
                         holes = __builtin_amdgcn_readfirstlane(red[4]);
                     }
@@ -523,10 +549,10 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     const bool some = live && t0 < t1;
     const int R = A.seqs * A.n_new * g;
     const size_t at = (size_t)(col * A.kv_heads + kvh) * R;
-    if (half == 0) A.ml[at + r] = f2{some ? m : LOWEST, some ? l : 0.f};
+    const int c0 = r0 + 32 * wr, cols = min(32, rb - c0), ln = lane_now();
+    if (ln < 32) A.ml[at + c0 + ln] = f2{some ? m : LOWEST, some ? l : 0.f};
     if (!some) return;
-    const int c0 = r0 + 32 * wr, cols = min(32, rb - c0);
-    float4* to = reinterpret_cast<float4*>(A.acc + (at + c0) * D) + half * cols + (lane & 31);
+    float4* to = reinterpret_cast<float4*>(A.acc + (at + c0) * D) + (ln >> 5) * cols + (ln & 31);
 #pragma unroll
     for (int x = 0; x < MT; x++)
 #pragma unroll
@@ -567,7 +593,7 @@ struct Few {
 };
 template <int D, int NB, int BUFS>
 DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int plo, int phi, const int* trow, int part,
-                  int parts, int col, int guess, int least) {
+                  int parts, int col, int guess, int least, bool slots) {
     using F = Few<D, NB, BUFS>;
     constexpr int STEPS = D / 32, XT = D / 16, CH = D / 8;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -632,7 +658,8 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
     }
     // ---- loads of a tile: two groups of 16 positions, each within a page; rows
     // that no one sees are replaced by the nearest that someone does, values
-    // without a page by zeros
+    // without a page by zeros, and where the windows of several slots' rows lie
+    // apart what is between them too
     const int page = 1 << A.page_shift;
     const uint32_t vbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * F::WAVE;
     h8 kf[BUFS][2][STEPS];
@@ -650,6 +677,12 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
             const int id = __builtin_amdgcn_readlane(ids, pg - ids_from);
             gone[buf] |= (uint32_t)id >> 31 << u;
             const size_t off = ((size_t)max(id, 0) * A.kv_heads + kvh) * page * D;
+            uint32_t seen = 0xffff;  // bit i: position p0 + i
+            if (slots && lo_all > hi_all) {
+                seen = 0;
+                for (int i = 0, p = p0; i < 16; i++, p++)
+                    if (__ballot(live[0] && lo[0] <= p && p < hi[0])) seen |= 1u << i;
+            }
             const uint16_t* vsrc = id < 0 ? reinterpret_cast<const uint16_t*>(no_page) : A.vp + off;
             const int pk = min(max(p0 + li, lo_any), hi_any - 1) & (page - 1);
 #pragma unroll
@@ -660,7 +693,9 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
                 const int row = c * (64 / CH) + lane / CH, w = lane % CH;
                 const int p = min(max(p0 + row, lo_any), hi_any - 1) & (page - 1);
                 const int f = D == 128 ? (row & 7) << 1 : (row >> 1 & 3) << 1;
-                dma16(vsrc + (size_t)p * D + 8 * (w ^ f), vbase + buf * F::VT + u * 16 * D * 2 + c * 1024);
+                const uint16_t* at = vsrc + (size_t)p * D;
+                if (slots && !(seen >> row & 1)) at = reinterpret_cast<const uint16_t*>(no_page);
+                dma16(at + 8 * (w ^ f), vbase + buf * F::VT + u * 16 * D * 2 + c * 1024);
             }
         }
     };
@@ -826,7 +861,7 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
         const int* trow = A.table + (size_t)A.prefix_slot * A.table_stride;
         if constexpr (MODE == 0 && NB == 1)
             few_task<D, NB, BUFS>(A, lds, kvh, 0, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
-                            ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1);
+                            ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1, true);
         else if constexpr (MODE == 1)
             attn_task<D, 2, 2>(A, lds, kvh, tile * 64, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
         else if constexpr (MODE == 2)
@@ -841,7 +876,7 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
     b /= tiles;
     const int kvh = b % A.kv_heads, s = b / A.kv_heads;
     few_task<D, NB, BUFS>(A, lds, kvh, s * rows + tile * 16 * NB, (s + 1) * rows, A.prefix_pages << A.page_shift, 0x7fffffff,
-                    A.table + (size_t)s * A.table_stride, part, A.own_parts, A.prefix_parts + part, A.prefix_pages, OWN_LEAST);
+                    A.table + (size_t)s * A.table_stride, part, A.own_parts, A.prefix_parts + part, A.prefix_pages, OWN_LEAST, false);
 }
 #define ATTN(D, MODE, NB)                                                                                            \
     extern "C" __global__ __launch_bounds__(256, few_wgs(D, MODE, NB)) void cima_attn_paged_d##D##_m##MODE##_n##NB(const AttnArgs A) {  \
