@@ -318,7 +318,13 @@ extern "C" __global__ __launch_bounds__(1024) void cima_kv_pages_fork(int* refs,
             if (ok) {
                 len[k] = lens[p[k]];
                 ok = len[k] >= 0 && len[k] <= table_stride << page_shift;
-                if (ok) ok = mine[k] = atomicCAS(&lens[c[k]], -1, -2 - i) == -1;
+                if (ok) {
+                    // the page that the parent has begun is copied: it has to be one
+                    const bool begun = len[k] & (page - 1);
+                    const int id = begun ? table[(size_t)p[k] * table_stride + (len[k] >> page_shift)] : 0;
+                    mine[k] = atomicCAS(&lens[c[k]], -1, -2 - i) == -1;
+                    ok = mine[k] && (unsigned)id < (unsigned)n_pages;
+                }
             }
             if (!ok) wrong = 1;
         }

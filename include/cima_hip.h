@@ -493,7 +493,8 @@ int cima_hip_kv_pages_reserve(cima_hip_ctx* ctx, const cima_kv_pages* kv, int se
  * copied to the lowest free page; the child's other entries are -1.  The
  * children must be free (lens -1), distinct and none of the parents in use as
  * one; a parent may be named several times.  All or nothing: *status = 0, the
- * number of missing pages (> 0), or -1 where a slot is not as it must be. */
+ * number of missing pages (> 0), or -1 where a slot is not as it must be (a
+ * parent that has begun a page it does not hold among them). */
 int cima_hip_kv_pages_fork(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int* parents, const int* children, int n,
                            int* status);
 /* The slots' pages lose a holder each, their entries and lens become -1.
