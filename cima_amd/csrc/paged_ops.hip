@@ -269,7 +269,7 @@ extern "C" __global__ __launch_bounds__(1024) void cima_kv_pages_reserve(int* re
         need += n;
     }
     __syncthreads();
-    const int missing = max(0, need - have) + behind;
+    const int missing = (int)min((long long)max(0, need - have) + behind, 0x7fffffffLL);
     if (t == 0) *status = missing;
     if (missing || need == 0) return;
     each_lowest<true>(refs, n_pages, sum, bits, need, [&](int rank, int id) {

@@ -480,8 +480,8 @@ int cima_hip_kv_pages_copy(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int
  * [lens / page, (lens + n_new - 1) / page] that are -1 take the lowest free
  * pages, slot by slot, with count 1.  All or nothing: *status = 0, or the
  * number of pages that are missing, and nothing is changed.  Entries behind
- * table_stride count as missing (at most 262144 a slot).  Behind a slot's first
- * -1 there is no page.
+ * table_stride count as missing (at most 262144 a slot); *status stops at 2^31 -
+ * 1.  Behind a slot's first -1 there is no page.
  *
  * A step after a reserve that found too few may run to its end, as a captured
  * one does: the tokens that have no page are dropped and not seen.  It has to be
