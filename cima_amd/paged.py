@@ -26,7 +26,8 @@ def _bad(msg: str):
 class PagedKV:
     """The tensors of a paged cache: ``pool`` f16 [2 * layers, n_pages, kv_heads,
     page, head_dim] (planes may lie apart), ``refs`` [n_pages], ``table``
-    [max_seqs, entries] and ``lens`` [max_seqs] int32."""
+    [max_seqs, entries] and ``lens`` [max_seqs] int32.  They are written in place:
+    the descriptor holds their addresses, so none is exchanged for another."""
 
     def __init__(self, pool, refs, table, lens):
         import torch
@@ -50,6 +51,11 @@ class PagedKV:
         self.desc = KvPages(pool.data_ptr(), pool.stride(0), refs.data_ptr(), table.data_ptr(), lens.data_ptr(), planes,
                             n_pages, heads, page, dim, self.max_seqs, table.shape[1])
         self.ref = ctypes.byref(self.desc)
+
+    def __setattr__(self, name, value):
+        if name in ("pool", "refs", "table", "lens") and self.__dict__.get(name, value) is not value:
+            _bad(f"{name} stays the tensor that the descriptor points to: write into it, or make another PagedKV")
+        super().__setattr__(name, value)
 
     @classmethod
     def empty(cls, layers: int, n_pages: int, kv_heads: int, page: int, head_dim: int, max_seqs: int, max_len: int,
