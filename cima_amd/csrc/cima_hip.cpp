@@ -1817,6 +1817,10 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     char name[64];
     hipFunction_t f;
     A.prefix_wgs = pre ? (int)((kv->kv_heads * pre + 7) / 8 * 8 * tiles) : 0;
+    const long long grid = A.prefix_wgs + own_base * own;
+    if (grid > kMaxGrid)
+        return fail(CIMA_E_INVALID, "%s: %lld workgroups (less than 2^24: %d slots of %d rows, %d kv heads)", api, grid,
+                    seqs, own_rows, kv->kv_heads);
     // Own tasks alone, no more than two to a CU, run in a kernel that has two of
     // their tiles in flight.  us, one / two: 16 slots of 8 heads of 128 up to 300 7.9 /
     // 7.5, 32 of them 9.2 / 8.7, 4 slots of 14/2 heads of 64 over 573 7.7 / 7.3.
@@ -1826,7 +1830,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     void* args[] = {&A};
     const int bufs = paged_few_wgs(dim, kind, nb) == 4 ? 1 : 2;
     const unsigned lds = std::max(paged_few_lds(dim, nb, bufs), mode ? paged_attn_lds(dim) : 0u);
-    if (int rc = launch(ctx, f, (unsigned)(A.prefix_wgs + own_base * own), 256, args, api, lds)) return rc;
+    if (int rc = launch(ctx, f, (unsigned)grid, 256, args, api, lds)) return rc;
     if (all == 1) return 0;
     const long long join = (long long)kv->kv_heads * ((head_rows + 15) / 16) * (dim / 16);
     return launch_named(ctx, dim == 64 ? "cima_attn_paged_join_d64" : "cima_attn_paged_join_d128", (unsigned)join, 256,

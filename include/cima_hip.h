@@ -466,7 +466,9 @@ int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int l
  * the slab (256-byte aligned) holds the partial sums: rows * q_heads *
  * (head_dim + 2) * 4 bytes per part, rows = seqs * n_new.  Two parts are
  * needed where prefix_pages > 0, else none; 192 are the most that are used.
- * q_heads a multiple of kv_heads, rows * q_heads at most 2^24; scale in (0, 2^16];
+ * q_heads a multiple of kv_heads, rows * q_heads at most 2^24 and less than 2^24
+ * tasks (seqs * kv_heads for each 16 rows of a slot, and the prefix's); scale in
+ * (0, 2^16];
  * q and out 16-byte aligned, not overlapping. */
 int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* q, void* out, int seqs,
                         int n_new, int q_heads, float scale, int prefix_pages, int prefix_slot, int window, void* slab,
