@@ -1732,10 +1732,17 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     const int own_tiles = (own_rows + 16 * nb - 1) / (16 * nb);
     const long long own_base = (long long)seqs * kv->kv_heads * own_tiles;
     // Tables of few positions and slots: each slot reads the prefix for itself, in
-    // one launch.  us, shared and joined / not: 4 slots of 14/2 heads of 64 over 256
-    // + 100 8.6 / 6.2, over 512 + 61 8.9 / 7.7, 8 of 32/8 of 128 over 256 + 100 10.4 /
-    // 8.3, 30 of those 11.5 / 8.8; 16 of them over 512 + 60 10.7 / 11.2.
-    const long long brief = dim == 64 ? 640 : 512, room = (long long)kv->table_stride * kv->page;
+    // one launch without a join.  Its time grows with the positions, the other's
+    // hardly; us, shared and joined / not, in tables of 384, 512, 640, 768, 1024
+    // positions: 4 slots of 14/2 heads of 64 8.2 / 5.5, 8.4 / 6.2, 8.3 / 7.0, 8.4 /
+    // 7.8, 9.3 / 9.2, one slot 7.9 / 5.5, 7.7 / 6.1, 7.8 / 6.7, 7.7 / 7.6, 8.0 / 9.0;
+    // 8 slots of 32/8 heads of 128 9.4 / 7.4, 9.5 / 8.9, 9.6 / 10.1, 9.7 / 11.5, 10.7 /
+    // 14.3, one slot 8.2 / 7.5, 8.2 / 8.8, 30 slots 10.9 / 7.5, 11.1 / 9.0, 11.6 / 10.2,
+    // 11.9 / 11.7, 13.0 / 14.6.  More than 16 rows, split / not, without a prefix: 4
+    // slots of 35 rows of 64 8.9 / 6.8, 8.7 / 7.5, 8.6 / 8.4, 8.7 / 9.2; of 20 of 128
+    // 9.8 / 9.2, 9.9 / 10.8.
+    const long long brief = dim == 64 ? (nb == 1 ? 768 : 640) : (nb == 1 ? 512 : 384);
+    const long long room = (long long)kv->table_stride * kv->page;
     if (room <= brief && nb == 1 && own_base <= ctx->num_cu) prefix_pages = 0;
     const long long own_room = room - (long long)prefix_pages * kv->page;
     // Up to 16 rows the prefix runs in the own tasks' kernel, whose waves fetch
@@ -1752,15 +1759,25 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     // turn, alike.  8 kv heads of 128, one round / two / four: 64 slots of up to 4000
     // 113 / 111 / 109 us, 128 of up to 6000 326 / 304 / 297, 64 of up to 2000 behind
     // a prefix of 4096 72 / 65 / 63, but more for the join: 0 / 6 / 6 at 128 slots.
-    // One part up to `brief` positions, and without a prefix, where it needs no join,
-    // where the slots' tasks are one to a CU for each 1024 positions or two.  One /
+    // One part without a prefix, where it needs no join, up to `brief` positions and
+    // where the slots' tasks are one to a CU for each 1024 positions or two; one /
     // several with the join, us: 16 slots of up to 300 8.0 / 10.9, 48 of up to 700
     // 17.5 / 21.4, 128 of up to 500 27.2 / 34.0, 64 of up to 4000 113 / 116, 64 of up
-    // to 600 with 8 tokens 20.5 / 40; but 8 of up to 1000 17 / 12.5; 20 of up to 300
-    // behind 8000 21.0 / 23.9, 30 with 8 tokens behind 4096 47.6 / 52.3.
+    // to 600 with 8 tokens 20.5 / 40; but 8 of up to 1000 17 / 12.5.  One behind a
+    // prefix where the own tasks fill a third of the CUs and their tables are short:
+    // behind 4096, tables of 368 / 624 / 1008 positions, 24 slots of 64/8 heads of 64
+    // 14.0, 15.1, 17.7 / 15.9, 17.4, 18.3, 64 of 14/2 of 64 14.6, 15.4, 18.0 / 15.6,
+    // 16.0, 18.3, 24 of 32/8 of 128 18.4, 21.1, 22.6 / 20.0, 22.8, 21.5, 64 of those
+    // 23.5, 29.8, 45.9 / 24.4, 28.4, 43.1; but 8 slots of 64/8 heads 12.9, 14.5, 17.2 /
+    // 12.2, 12.2, 13.0, 2 of 32/8 of 128 15.1, 18.5, 23.5 / 12.3, 12.6, 12.9.  Fewer
+    // slots only up to 256 positions, beside row tiles: 5 of 16/1 of 128 behind 8000
+    // 12.9 / 13.5, 12 of 24/8 of 64 12.8 / 13.2, 8 of 28/4 of 128 behind 576 9.2 /
+    // 9.6; beside few-row tasks 2 of 32/8 of 128 13.5 / 12.1.
     long long own = (own_room + 127) / 128;
     while (own > 1 && own_base * own > 2LL * wgs * ctx->num_cu) own = (own + 1) / 2;
-    if (own_room <= brief || (!prefix_pages && own_base * 1024 >= std::min(own_room, 2048LL) * ctx->num_cu)) own = 1;
+    if (prefix_pages ? (own_room <= (dim == 64 ? 640 : 512) && 3 * own_base >= ctx->num_cu) || (mode && own_room <= 256)
+                     : own_room <= brief || own_base * 1024 >= std::min(own_room, 2048LL) * ctx->num_cu)
+        own = 1;
     own = std::max(1LL, std::min(own, 64LL));
     int tiles = 0;
     long long pre = 0;
