@@ -1601,8 +1601,6 @@ int cima_hip_decode_step(cima_hip_ctx* ctx, const cima_decoder* d) {
     return cima_hip_argmax_to_ids(ctx, d->slot, d->ids, d->pos);
 }
 
-// ---------------------------------------------------------------- graphs
-
 // -------------------------------------------------------------- paged cache
 
 namespace {
@@ -2024,6 +2022,8 @@ int cima_hip_verify_drafts(cima_hip_ctx* ctx, const float* p, const float* q, co
     if (int rc = launch_named(ctx, "cima_verify_sums", (unsigned)(seqs * parts), 256, args, api)) return rc;
     return launch_named(ctx, "cima_verify_draw", (unsigned)seqs, 256, args, api);
 }
+
+// ---------------------------------------------------------------- graphs
 
 struct cima_hip_graph {
     hipGraphExec_t exec = nullptr;

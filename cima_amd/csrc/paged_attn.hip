@@ -4,7 +4,7 @@
 // out = sum_t w_t v_t / sum_t w_t, w_t = e^(scale q.k_t - m), over the positions
 // t that a row sees.  The rows of a kv head are its query heads times the
 // step's tokens; those of all slots share the prefix's pages, so one workgroup
-// takes up to 256 of them through a range of the prefix and its keys and values
+// takes up to 128 of them through a range of the prefix and its keys and values
 // are read once for all (prefix tasks).  A slot's own pages are seen by its own
 // rows alone (own tasks).  Both take a tile of rows through a range of positions
 // and leave {m, l, sum} per row, which a second launch joins; a row's only part
@@ -156,11 +156,11 @@ struct Tile {
 // 64 positions a tile, two tiles in LDS (64 KB), two workgroups of four waves to
 // a CU: 250 registers hold 32 rows' sums, two tiles' scores and q, and the two
 // workgroups cover each other's barriers.  Measured on MI355X, 128 slots of 4 x 8
-// heads of 128 over 65536 positions (137 GFLOP): 155 us, 885 TFLOP/s, the matrix
-// cores 0.45 busy at the 1.9 GHz that the card holds under this load.  No one part
-// bounds it: without the copies 133 us, without reads from LDS 123, without the
-// weights 138, with the products alone 85; reading fragments 2 to 8 products ahead
-// changes nothing.  One workgroup of eight waves and 256 rows, which copies half
+// heads of 128 over 65536 positions (137 GFLOP): 153 us, 899 TFLOP/s, the matrix
+// cores 0.47 busy at the 1.9 GHz that the card holds under this load.  No one part
+// bounds it: of 155 us, without the copies 133, without reads from LDS 123, without
+// the weights 138, with the products alone 85; reading fragments 2 to 8 products
+// ahead changes nothing.  One workgroup of eight waves and 256 rows, which copies half
 // as much: 176; 64 rows a wave: 572, its registers spill.
 template <int D, int WR, int WK>
 DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int plo, int phi, const int* trow,

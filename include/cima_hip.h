@@ -441,9 +441,9 @@ typedef struct cima_kv_pages {
  * qkv f16 [seqs * n_new, (q_heads + 2 kv_heads) * head_dim] as the fused q|k|v
  * GEMM writes it, row s * n_new + j at position lens[s] + j of slot s.  The
  * rotated queries go to q [seqs * n_new, q_heads * head_dim], the rotated keys
- * and the values to layer `layer`'s planes.  NeoX pairs as cima_hip_rope, the
- * angle formed in fp64 (at position 100000 an fp32 angle is off by up to
- * 0.008); theta 0 = no rotation.  lens is not changed: every layer of the step
+ * and the values to layer `layer`'s planes.  NeoX pairs as cima_hip_rope, all of
+ * them (as its nfreqs = head_dim / 2), the angle formed in fp64 (at position
+ * 100000 an fp32 angle is off by up to 0.008); theta 0 = no rotation.  lens is not changed: every layer of the step
  * appends at the same positions.  Slots not in use write nothing, neither q;
  * positions without a page (entry -1 or behind the row) write no key.  Less
  * than 2^24 rows.
@@ -465,7 +465,9 @@ int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int l
  * The work is split over the positions where there are few rows, as long as
  * the slab (256-byte aligned) holds the partial sums: rows * q_heads *
  * (head_dim + 2) * 4 bytes per part, rows = seqs * n_new.  Two parts are
- * needed where prefix_pages > 0, else none; 192 are the most that are used.
+ * needed where prefix_pages > 0, else none; 192 are the most that are used.  The
+ * split goes by seqs and the table's capacity, table_stride * page: a table and a
+ * batch cut to what is in use are the faster.
  * q_heads a multiple of kv_heads, rows * q_heads at most 2^24 and less than 2^24
  * tasks (seqs * kv_heads for each 16 rows of a slot, and the prefix's); scale in
  * (0, 2^16];
