@@ -99,3 +99,18 @@ def test_masked_tokens_are_not_drawn(hip):
     torch.cuda.synchronize()
     got = tokens.cpu().numpy()
     assert left[got].all() and len(np.unique(got)) == left.sum()
+
+
+@pytest.mark.parametrize("cap", [0.0, 30.0])
+@pytest.mark.parametrize("n", [5, 9000, 40000])
+def test_a_temperature_that_is_no_number_takes_the_largest(hip, n, cap):
+    x = np.random.default_rng(n).standard_normal((3, n)).astype(np.float16)
+    x[:, :2] = -np.inf
+    temp = np.array([np.nan, -0.0, -np.inf], np.float32)
+    y = torch.empty((3, n), device="cuda")
+    hip.softmax_rows(torch.from_numpy(x).cuda(), y, 3, n, torch.from_numpy(temp).cuda(), 1, cap,
+                     torch.empty(1 << 16, dtype=torch.uint8, device="cuda"))
+    torch.cuda.synchronize()
+    want = np.zeros((3, n))
+    want[np.arange(3), x.argmax(1)] = 1
+    assert np.array_equal(y.cpu().numpy(), want)
