@@ -340,6 +340,13 @@ def _up(q):
     return torch.where(t.double() < q, (t.view(torch.int16) + 1).view(torch.float16), t)
 
 
+def _half(x):
+    """float64 to float16, rounded once: an inexact float32 on the way is made odd, which no tie is."""
+    f = x.float()
+    b = f.view(torch.int32) - (f.double().abs() > x.abs()).int()
+    return (b | (f.double() != x).int()).view(torch.float32).half()
+
+
 def _quantised(x, bits):
     """Rows of f16 values [.., D] as a head's page keeps them: codes and scales.  In 64 bits:
     a quotient next to a border of two codes has to fall on the right side."""
@@ -365,7 +372,7 @@ def _plain_append(s):
     x = s["qkv"].view(S * n, -1, D)
     r = x[:, :c["q_heads"] + H].double()
     a, b = r[..., :D // 2], r[..., D // 2:]
-    r = torch.cat([a * cos - b * sin, a * sin + b * cos], -1).half()
+    r = _half(torch.cat([a * cos - b * sin, a * sin + b * cos], -1))
     s["q"].copy_(r[:, :c["q_heads"]])
     ids = s["table"].gather(1, (at // page).long()).view(-1).long()
     row = (at % page).view(-1).long()
