@@ -3,8 +3,8 @@
 Native parts (built by ``cima_amd.build`` into ``cima_amd/lib``):
   * ``cima_gemv_{a,b,c}.hsaco``, ``cima_gemm.hsaco``, ``cima_gemm_wide.hsaco``,
     ``cima_dequant.hsaco``, ``cima_decode.hsaco``, ``cima_bnb4.hsaco``,
-    ``cima_paged.hsaco``, ``cima_paged_attn.hsaco``, ``cima_sample.hsaco`` --
-    hand-written HIP kernels for gfx950
+    ``cima_paged.hsaco``, ``cima_paged_attn{,_q4,_q8}.hsaco``,
+    ``cima_sample.hsaco`` -- hand-written HIP kernels for gfx950
   * ``libcima_hip.so``  -- the C ABI of ``include/cima_hip.h``
   * ``libcima_synth.so`` -- seeded synthetic weights (``include/cima_synth.h``)
 

@@ -7,9 +7,10 @@ Produces, in ``cima_amd/lib/``:
   cima_dequant.hsaco    dequant-to-f16 and packed gather,
   cima_decode.hsaco     decode-step support (norm, RoPE, attention, argmax)
   cima_bnb4.hsaco       bitsandbytes NF4/FP4 dequant and decode GEMV
-  cima_paged.hsaco      paged KV cache: RoPE with append, page operations
-  cima_paged_attn.hsaco  attention of a batch over the paged cache
-  cima_sample.hsaco     row softmax, verification of drafted tokens
+  cima_paged.hsaco      paged KV cache: RoPE with append, read back, page operations
+  cima_paged_attn.hsaco  attention of a batch over the paged cache, and
+  cima_paged_attn_q4/q8.hsaco  over one of 4- or 8-bit elements
+  cima_sample.hsaco     row softmax, token log probabilities, verification of drafted tokens
   libcima_hip.so      host C ABI (include/cima_hip.h), links libamdhip64
   libcima_synth.so    seeded synthetic weights + quantisers (include/cima_synth.h)
 
@@ -37,7 +38,9 @@ SOURCES = {"gemv_a": ("gguf_gemv.hip", ["-DCIMA_GEMV_SET=0"]), "gemv_b": ("gguf_
            "gemv_c": ("gguf_gemv.hip", ["-DCIMA_GEMV_SET=2"]), "gemm": ("gguf_gemm.hip", []),
            "dequant": ("gguf_dequant.hip", []), "decode": ("decode_ops.hip", []),
            "bnb4": ("bnb4.hip", []), "gemm_wide": ("gguf_gemm_wide.hip", []),
-           "paged": ("paged_ops.hip", []), "paged_attn": ("paged_attn.hip", []), "sample": ("sample_ops.hip", [])}
+           "paged": ("paged_ops.hip", []), "paged_attn": ("paged_attn.hip", []),
+           "paged_attn_q4": ("paged_attn.hip", ["-DCIMA_KV_BITS=4"]),
+           "paged_attn_q8": ("paged_attn.hip", ["-DCIMA_KV_BITS=8"]), "sample": ("sample_ops.hip", [])}
 HSACOS = {name: os.path.join(LIB, f"cima_{name}.hsaco") for name in SOURCES}
 GEMV_OBJECTS = ("gemv_a", "gemv_b", "gemv_c")
 LIBHIP = os.path.join(LIB, "libcima_hip.so")

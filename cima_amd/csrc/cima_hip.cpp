@@ -111,7 +111,7 @@ struct cima_hip_ctx {
     int device = 0;
     int num_cu = 0;
     int max_lds = 0;  // bytes of LDS one workgroup may use
-    hipModule_t modules[11] = {};  // kModuleFiles
+    hipModule_t modules[13] = {};  // kModuleFiles
     bool loaded = false;
     hipStream_t own_stream = nullptr;
     hipStream_t stream = nullptr;
@@ -158,13 +158,14 @@ int launch(cima_hip_ctx* ctx, hipFunction_t f, unsigned grid, unsigned block, vo
 // code objects: the GEMVs in three (format sets compiled in parallel),
 // the prefill GEMMs, dequant / gather, the decode-step kernels, the
 // 256 x 256 prefill tiles (compiled beside the other GEMMs), the paged cache's
-// operations, its attention, and sampling
+// operations, its attention (of f16, 4-bit and 8-bit elements), and sampling
 enum { MOD_GEMM = 3, MOD_DEQUANT = 4, MOD_DECODE = 5, MOD_BNB4 = 6, MOD_GEMM_WIDE = 7, MOD_PAGED = 8,
-       MOD_PAGED_ATTN = 9, MOD_SAMPLE = 10, NUM_MODULES = 11 };
+       MOD_PAGED_ATTN = 9, MOD_SAMPLE = 10, MOD_PAGED_ATTN_Q4 = 11, MOD_PAGED_ATTN_Q8 = 12, NUM_MODULES = 13 };
 const char* const kModuleFiles[NUM_MODULES] = {"cima_gemv_a.hsaco", "cima_gemv_b.hsaco", "cima_gemv_c.hsaco",
                                                "cima_gemm.hsaco",   "cima_dequant.hsaco", "cima_decode.hsaco",
                                                "cima_bnb4.hsaco",   "cima_gemm_wide.hsaco",
-                                               "cima_paged.hsaco",  "cima_paged_attn.hsaco", "cima_sample.hsaco"};
+                                               "cima_paged.hsaco",  "cima_paged_attn.hsaco", "cima_sample.hsaco",
+                                               "cima_paged_attn_q4.hsaco", "cima_paged_attn_q8.hsaco"};
 
 // weights and X types whose 32 x 16 prefill tiles are built twice: _b16_ decodes
 // in one go, _b16l_ in parts (sk16_serial in gguf_gemm.hip)
@@ -204,7 +205,10 @@ const char* const kDecodeKernels[] = {
 const char* const kPagedKernels[] = {
     "cima_rope_append_paged_d64", "cima_rope_append_paged_d128", "cima_kv_pages_copy", "cima_kv_pages_reserve",
     "cima_kv_pages_fork", "cima_kv_pages_fork_copy", "cima_kv_pages_free", "cima_kv_pages_compact",
-    "cima_kv_pages_compact_move"};
+    "cima_kv_pages_compact_move", "cima_rope_append_paged_q4_d64", "cima_rope_append_paged_q4_d128",
+    "cima_rope_append_paged_q8_d64", "cima_rope_append_paged_q8_d128", "cima_kv_pages_read_b4_d64",
+    "cima_kv_pages_read_b4_d128", "cima_kv_pages_read_b8_d64", "cima_kv_pages_read_b8_d128",
+    "cima_kv_pages_read_b16_d64", "cima_kv_pages_read_b16_d128"};
 const char* const kSampleTypes[] = {"f16", "f32", "cap_f16", "cap_f32"};
 const char* const kSampleKernels[] = {"cima_softmax_t1024_w16_f16", "cima_softmax_t1024_w16_f32", "cima_verify_sums",
                                       "cima_verify_draw"};
@@ -661,6 +665,12 @@ int cima_hip_init(int device, const char* code_dir, cima_hip_ctx** out) {
             snprintf(name, sizeof name, fmt, dim);
             if (!rc) rc = add(MOD_PAGED_ATTN, name);
         }
+        for (int bits : {4, 8})
+            for (int mode : {0, 1, 2})
+                for (int nb : {1, 2}) {
+                    snprintf(name, sizeof name, "cima_attn_paged_q%d_d%d_m%d_n%d", bits, dim, mode, nb);
+                    if (!rc) rc = add(bits == 4 ? MOD_PAGED_ATTN_Q4 : MOD_PAGED_ATTN_Q8, name);
+                }
     }
     for (const char* kn : kSampleKernels)
         if (!rc) rc = add(MOD_SAMPLE, kn);
@@ -1609,6 +1619,19 @@ namespace {
 // CH and MAX_SLOTS in paged_ops.hip)
 const int kMaxPages = 1 << 20, kMaxSlots = 4096;
 
+// bits of an element of the cache (0: no such type), bytes of a head's page and
+// of a plane (KvQ in kv_quant.h)
+int kv_bits(const cima_kv_pages* kv) {
+    return kv->ggml_type == 0 ? 16 : kv->ggml_type == CIMA_GGML_Q8_0 ? 8 : kv->ggml_type == CIMA_GGML_Q4_1 ? 4 : 0;
+}
+int kv_scale_bytes(const cima_kv_pages* kv) {  // of a row
+    return kv->head_dim / 32 * (kv_bits(kv) == 4 ? 4 : kv_bits(kv) == 8 ? 2 : 0);
+}
+long long kv_head_bytes(const cima_kv_pages* kv) {
+    return (long long)kv->page * (kv->head_dim * kv_bits(kv) / 8 + kv_scale_bytes(kv));
+}
+long long kv_plane_bytes(const cima_kv_pages* kv) { return kv->plane_elems * (kv->ggml_type ? 1 : 2); }
+
 int kv_check(cima_hip_ctx* ctx, const cima_kv_pages* kv, const char* api) {
     if (int rc = ready(ctx, api)) return rc;
     if (!kv) return fail(CIMA_E_INVALID, "%s: null cache", api);
@@ -1624,10 +1647,12 @@ int kv_check(cima_hip_ctx* ctx, const cima_kv_pages* kv, const char* api) {
                     "most 2^30 positions a slot and 2^31 - 1 table entries)",
                     api, kv->n_planes, kv->n_pages, kv->kv_heads, kv->page, kv->head_dim, kv->max_seqs,
                     kv->table_stride, kMaxPages, kMaxSlots);
-    if (kv->plane_elems % 8 ||
-        kv->plane_elems < (long long)kv->n_pages * kv->kv_heads * kv->page * kv->head_dim)
-        return fail(CIMA_E_INVALID, "%s: plane_elems=%lld is less than a plane or no multiple of 8", api,
-                    kv->plane_elems);
+    if (!kv_bits(kv))
+        return fail(CIMA_E_FORMAT, "%s: a cache of ggml type %d (0 for f16, Q4_1 or Q8_0)", api, kv->ggml_type);
+    if (kv->plane_elems % (kv->ggml_type ? 16 : 8) ||
+        kv_plane_bytes(kv) < kv->n_pages * (kv->kv_heads * kv_head_bytes(kv)))
+        return fail(CIMA_E_INVALID, "%s: plane_elems=%lld is less than a plane or no multiple of %d", api,
+                    kv->plane_elems, kv->ggml_type ? 16 : 8);
     if (!kv->pool || !kv->refs || !kv->table || !kv->lens) return fail(CIMA_E_INVALID, "%s: null tensor in the cache", api);
     if (!aligned(kv->pool, 16) || !aligned(kv->refs, 4) || !aligned(kv->table, 4) || !aligned(kv->lens, 4))
         return fail(CIMA_E_INVALID, "%s: misaligned pool (16 B) or bookkeeping (4 B)", api);
@@ -1642,7 +1667,7 @@ int kv_layer(const cima_kv_pages* kv, int layer, const char* api) {
 const long long kMaxGrid = 0xffffff;
 // 16-byte words of a page, and pieces of PIECE words that it is copied in
 // (paged_ops.hip)
-long long page_words(const cima_kv_pages* kv) { return (long long)kv->kv_heads * kv->page * kv->head_dim / 8; }
+long long page_words(const cima_kv_pages* kv) { return kv->kv_heads * kv_head_bytes(kv) / 16; }
 int page_pieces(const cima_kv_pages* kv) { return (int)((page_words(kv) + 1023) / 1024); }
 // workgroups of the page copies: a piece each, up to 128 to a CU
 unsigned copy_grid(const cima_hip_ctx* ctx, long long units) {
@@ -1684,15 +1709,43 @@ int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int l
     if (seqs == 0 || n_new == 0) return 0;
     if (!qkv || !q || !aligned(qkv, 16) || !aligned(q, 16))
         return fail(CIMA_E_INVALID, "%s: null or misaligned qkv or q (16 B)", api);
-    void* kp = (char*)kv->pool + 2LL * layer * kv->plane_elems * 2;
-    void* vp = (char*)kp + kv->plane_elems * 2;
+    void* kp = (char*)kv->pool + 2LL * layer * kv_plane_bytes(kv);
+    void* vp = (char*)kp + kv_plane_bytes(kv);
     int kvh = kv->kv_heads, shift = log2i(kv->page), np = kv->n_pages, stride = kv->table_stride;
     const int *table = kv->table, *lens = kv->lens;
     double lt = theta > 0.f ? log2((double)theta) : -1.0;
     int rotate = theta > 0.f;
     void* args[] = {&qkv, &q, &kp, &vp, &table, &lens, &n_new, &q_heads, &kvh, &shift, &np, &stride, &rotate, &lt};
-    return launch_named(ctx, kv->head_dim == 64 ? "cima_rope_append_paged_d64" : "cima_rope_append_paged_d128",
-                        (unsigned)(seqs * n_new), 256, args, api);
+    char name[64];
+    if (kv->ggml_type) snprintf(name, sizeof name, "cima_rope_append_paged_q%d_d%d", kv_bits(kv), kv->head_dim);
+    else snprintf(name, sizeof name, "cima_rope_append_paged_d%d", kv->head_dim);
+    return launch_named(ctx, name, (unsigned)(seqs * n_new), 256, args, api);
+}
+
+int cima_hip_kv_pages_read(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const int* slots, const int* first,
+                           void* k, void* v, int n_slots, int n, int max_seq) {
+    const char* api = "cima_hip_kv_pages_read";
+    if (int rc = kv_check(ctx, kv, api)) return rc;
+    if (int rc = kv_layer(kv, layer, api)) return rc;
+    // rows of a workgroup (READ_ROWS passes of 256 threads, paged_ops.hip)
+    const int rows = 4 * 256 / (kv->head_dim / 8);
+    long long mine = max_seq;
+    int blocks = n > 0 ? (n - 1) / rows + 1 : 0;
+    if (n_slots < 0 || n < 0 || n > max_seq || n > 0x40000000 || (long long)n_slots * kv->kv_heads > kMaxGrid ||
+        (long long)n_slots * kv->kv_heads * blocks > kMaxGrid)
+        return fail(CIMA_E_INVALID, "%s: n_slots=%d n=%d max_seq=%d (at most 2^30 positions, less than 2^24 workgroups of "
+                                    "%d rows of a head)", api, n_slots, n, max_seq, rows);
+    if (n_slots == 0 || n == 0) return 0;
+    if (!k || !v || !aligned(k, 16) || !aligned(v, 16) || !aligned(slots, 4) || !aligned(first, 4))
+        return fail(CIMA_E_INVALID, "%s: null or misaligned k or v (16 B), or misaligned lists (4 B)", api);
+    const void* kp = (const char*)kv->pool + 2LL * layer * kv_plane_bytes(kv);
+    const void* vp = (const char*)kp + kv_plane_bytes(kv);
+    const int* table = kv->table;
+    int kvh = kv->kv_heads, shift = log2i(kv->page), np = kv->n_pages, stride = kv->table_stride, seqs = kv->max_seqs;
+    void* args[] = {&kp, &vp, &table, &slots, &first, &k, &v, &kvh, &shift, &np, &stride, &seqs, &n, &blocks, &mine};
+    char name[64];
+    snprintf(name, sizeof name, "cima_kv_pages_read_b%d_d%d", kv_bits(kv), kv->head_dim);
+    return launch_named(ctx, name, (unsigned)(n_slots * kvh * blocks), 256, args, api);
 }
 
 int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* q, void* out, int seqs,
@@ -1788,7 +1841,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
         // the join, half of that / that / twice that: 128 slots of 8 heads of 128 over
         // 65536 235 / 184 / 193 us, 32 slots over 30016 51.7 / 39.6 / 45.6, over 8000
         // 27.0 / 25.4 / 33.4, over 8000 with up to 1023 own 34.8 / 28.8 / 34.5.
-        const long long own_bytes = 4LL * seqs * kv->kv_heads * own_room * dim;
+        const long long own_bytes = 2 * own_room / kv->page * seqs * kv->kv_heads * kv_head_bytes(kv);
         long long want = ctx->num_cu;
         if (len * base >= 1024LL * ctx->num_cu) want *= 2;
         else if (own_bytes >= (256LL << 10) * ctx->num_cu) want /= 2;
@@ -1806,8 +1859,8 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     const int all = (int)(pre + own);
     PagedAttnArgs A{};
     A.q = q;
-    A.kp = (const char*)kv->pool + 2LL * layer * kv->plane_elems * 2;
-    A.vp = (const char*)A.kp + kv->plane_elems * 2;
+    A.kp = (const char*)kv->pool + 2LL * layer * kv_plane_bytes(kv);
+    A.vp = (const char*)A.kp + kv_plane_bytes(kv);
     A.table = kv->table;
     A.lens = kv->lens;
     A.out = out;
@@ -1836,14 +1889,15 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     if (grid > kMaxGrid)
         return fail(CIMA_E_INVALID, "%s: %lld workgroups (less than 2^24: %d slots of %d rows, %d kv heads)", api, grid,
                     seqs, own_rows, kv->kv_heads);
-    // Own tasks alone, no more than two to a CU, run in a kernel that has two of
+    // Own tasks of f16 alone, no more than two to a CU, run in a kernel that has two of
     // their tiles in flight.  us, one / two: 16 slots of 8 heads of 128 up to 300 7.9 /
     // 7.5, 32 of them 9.2 / 8.7, 4 slots of 14/2 heads of 64 over 573 7.7 / 7.3.
-    const int kind = !pre && own_base * own <= 2LL * ctx->num_cu ? 1 : mode;
-    snprintf(name, sizeof name, "cima_attn_paged_d%d_m%d_n%d", dim, kind, nb);
+    const int kind = !pre && !kv->ggml_type && own_base * own <= 2LL * ctx->num_cu ? 1 : mode;
+    if (kv->ggml_type) snprintf(name, sizeof name, "cima_attn_paged_q%d_d%d_m%d_n%d", kv_bits(kv), dim, kind, nb);
+    else snprintf(name, sizeof name, "cima_attn_paged_d%d_m%d_n%d", dim, kind, nb);
     if (int rc = get_fn(ctx, name, &f)) return rc;
     void* args[] = {&A};
-    const int bufs = paged_few_wgs(dim, kind, nb) == 4 ? 1 : 2;
+    const int bufs = kv->ggml_type || paged_few_wgs(dim, kind, nb) == 4 ? 1 : 2;
     const unsigned lds = std::max(paged_few_lds(dim, nb, bufs), mode ? paged_attn_lds(dim) : 0u);
     if (int rc = launch(ctx, f, (unsigned)grid, 256, args, api, lds)) return rc;
     if (all == 1) return 0;
@@ -1860,7 +1914,7 @@ int cima_hip_kv_pages_copy(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int
     if (!src || !dst || !aligned(src, 4) || !aligned(dst, 4))
         return fail(CIMA_E_INVALID, "%s: null or misaligned lists", api);
     void* pool = kv->pool;
-    long long plane = kv->plane_elems / 8, words = page_words(kv);
+    long long plane = kv_plane_bytes(kv) / 16, words = page_words(kv);
     int pieces = page_pieces(kv), pages = kv->n_pages;
     long long units = (long long)kv->n_planes * n * pieces;
     void* args[] = {&pool, &plane, &words, &pieces, &n, &units, &src, &dst, &pages};
@@ -1894,10 +1948,10 @@ int cima_hip_kv_pages_fork(cima_hip_ctx* ctx, const cima_kv_pages* kv, const int
     if (int rc = launch_named(ctx, "cima_kv_pages_fork", 1, 1024, args, api)) return rc;
     if (n == 0) return 0;
     void* pool = kv->pool;
-    long long plane = kv->plane_elems / 8;
-    int heads = kv->kv_heads, row = kv->head_dim / 8;
-    void* cargs[] = {&pool, &plane, &refs, &np, &table, &lens, &stride, &shift, &heads, &row, &parents, &children, &n,
-                     &status};
+    long long plane = kv_plane_bytes(kv) / 16;
+    int heads = kv->kv_heads, row = kv->head_dim * kv_bits(kv) / 128, scale = kv_scale_bytes(kv) / 4;
+    void* cargs[] = {&pool, &plane, &refs, &np, &table, &lens, &stride, &shift, &heads, &row, &scale, &parents, &children,
+                     &n, &status};
     return launch_named(ctx, "cima_kv_pages_fork_copy", (unsigned)(n * (1 + kv->n_planes)), 256, cargs, api);
 }
 
@@ -1929,7 +1983,7 @@ int cima_hip_kv_pages_compact(cima_hip_ctx* ctx, const cima_kv_pages* kv, int* r
     void* args[] = {&refs, &np, &refs_out, &n_live, &slab};
     if (int rc = launch_named(ctx, "cima_kv_pages_compact", 1, 1024, args, api)) return rc;
     void* pool = kv->pool;
-    long long plane = kv->plane_elems / 8, words = page_words(kv), entries = (long long)kv->max_seqs * kv->table_stride;
+    long long plane = kv_plane_bytes(kv) / 16, words = page_words(kv), entries = (long long)kv->max_seqs * kv->table_stride;
     int pieces = page_pieces(kv), planes = kv->n_planes;
     void* margs[] = {&pool, &plane, &words, &pieces, &planes, &np, &table, &table_out, &entries, &slab};
     // at most half the pages move

@@ -1,5 +1,6 @@
 // Attention of a batch over a paged KV cache for gfx950 (CDNA4): the code
-// object cima_paged_attn.hsaco.
+// object cima_paged_attn.hsaco, and with CIMA_KV_BITS 4 and 8 those of quantised
+// caches (kv_quant.h), cima_paged_attn_q4.hsaco and cima_paged_attn_q8.hsaco.
 //
 // out = sum_t w_t v_t / sum_t w_t, w_t = e^(scale q.k_t - m), over the positions
 // t that a row sees.  The rows of a kv head are its query heads times the
@@ -25,9 +26,22 @@
 // values reach LDS by direct copies (global_load_lds_dwordx4) a ring of tiles
 // ahead; the 16-byte words of a row are stored permuted so that neither kind
 // of read meets bank conflicts.
+//
+// Of a quantised cache a lane reads a quarter of a row's codes, 16 bytes of 128
+// Q4_1 elements, into registers a tile ahead, and makes f16 elements of them: keys
+// and values of a row tile into the ring of LDS, once for all of its rows; keys of a
+// few-row task in place, as the A operand (the queries' elements in the same
+// order), its values into the wave's LDS.
 #include "gguf_formats.h"
+#include "kv_quant.h"
 
 #include <type_traits>
+
+#ifndef CIMA_KV_BITS
+#define CIMA_KV_BITS 16
+#endif
+constexpr int BITS = CIMA_KV_BITS;  // of the cache's elements: 16 (f16), 4 or 8
+using Q = KvQ<BITS>;
 
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h2 __attribute__((ext_vector_type(2)));
@@ -109,7 +123,7 @@ __device__ const uint4 no_page[256 * 128 * 2 / 16] = {};
 
 struct AttnArgs {
     const uint16_t* q;
-    const uint16_t* kp;  // planes of the layer
+    const uint16_t* kp;  // planes of the layer (of bytes where the cache is quantised)
     const uint16_t* vp;
     const int* table;
     const int* lens;
@@ -135,6 +149,34 @@ constexpr float LOWEST = -1e30f;  // below any score: the running maximum's star
 // to 2^6 above the score's: probabilities stay between 2^-14 * 2^6 and 2^14 of
 // the largest, clear of f16's subnormals, and most tiles skip the rescaling.
 constexpr float RAISE = 14.f, ABOVE = 6.f;
+
+// A lane's quarter of a row of a quantised cache (row lane % 16, quarter lane / 16),
+// D / 4 elements of one group
+template <int D>
+struct Raw {
+    static constexpr int STEPS = D / 32, W = Q::WORDS;
+    uint32_t w[STEPS * W], s;
+    // row r of the head's page at `head`
+    DEV void load(const uint8_t* head, int page, int r, int q4) {
+        const uint32_t at = (uint32_t)(r * Q::codes(D) + q4 * (Q::codes(D) / 4));
+        __builtin_memcpy(w, __builtin_assume_aligned(head + at, STEPS * W * 4 < 16 ? STEPS * W * 4 : 16), STEPS * W * 4);
+        s = Q::load_scale(head, page, D, r, q4 * (D / 4) / 32);
+    }
+    // elements 8 i, ... of the quarter
+    DEV h8 get(int i) const {
+        uint32_t u[W], o[4];
+#pragma unroll
+        for (int k = 0; k < W; k++) u[k] = w[i * W + k];
+        Q::decode(u, s, o);
+        return __builtin_bit_cast(h8, make_uint4(o[0], o[1], o[2], o[3]));
+    }
+};
+// the head's page that id names (page 0 where it names none)
+template <int D>
+DEV const uint8_t* head_page(const AttnArgs& A, const uint16_t* plane, int id, int kvh) {
+    return reinterpret_cast<const uint8_t*>(plane) +
+           ((size_t)max(id, 0) * A.kv_heads + kvh) * ((size_t)Q::row(D) << A.page_shift);
+}
 
 template <int D, int WR, int WK>
 struct Tile {
@@ -280,6 +322,24 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
     const uint16_t* vplane = A.vp + (size_t)kvh * page * D;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * 16 * ROWB;
     auto id_at = [&](int t) { return ids[page_of(base + t * T::KT + 16 * wave) - ids_from]; };
+    // a quantised cache: the wave's 16 rows of tile t to registers, and from there
+    // as f16 to their place, words in the order above
+    Raw<D> kraw, vraw;
+    auto fetch = [&](int t, int id, const uint16_t* plane, Raw<D>& raw, bool values) {
+        id = __builtin_amdgcn_readfirstlane(id);
+        const int ln = lane_now();
+        const int p = min(max(base + t * T::KT + 16 * wave + (ln & 15), lo_any), hi_any - 1) & (page - 1);
+        raw.load(head_page<D>(A, plane, id, kvh), page, p, ln >> 4);
+        if (values && id < 0) raw.s = 0;
+    };
+    auto spread = [&](int t, const Raw<D>& raw, bool values) {
+        const int ln = lane_now(), r = ln & 15;
+        const int f = !values ? (D == 128 ? r : r >> 1) : D == 128 ? (r & 3) << 2 | r >> 2 : (r >> 1 & 1) << 2 | r >> 2;
+        uint8_t* to = lds + (values ? 2 * T::BYTES : 0) + (t & 1) * T::BYTES + (16 * wave + r) * ROWB;
+#pragma unroll
+        for (int i = 0; i < Raw<D>::STEPS; i++)
+            *reinterpret_cast<h8*>(to + (((ln >> 4) * Raw<D>::STEPS + i) ^ f) * 16) = raw.get(i);
+    };
     auto issue = [&](int t, int id, const uint16_t* plane, uint32_t word, uint32_t flip, uint32_t ring) {
         const int p0 = base + t * T::KT + 16 * wave;
         id = __builtin_amdgcn_readfirstlane(id);
@@ -387,15 +447,36 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         holes = __builtin_amdgcn_readfirstlane(red[4]);
         f16v sa[T::KB], sb[T::KB];  // scores of even and of odd tiles from t0 on
         int id = id_at(t0);
-        // the first keys, waited for alone, the first values and the second keys
-        issue(t0, id, kplane, kword, KX, 0);
-        issue(t0, id, vplane, vword, VX, 2 * T::BYTES);
-        if (t0 + 1 < t1) {
-            id = id_at(t0 + 1);
-            issue(t0 + 1, id, kplane, kword, KX, 0);
-            wait_vm<2 * (D / 32)>();
+        if constexpr (BITS == 16) {
+            // the first keys, waited for alone, the first values and the second keys
+            issue(t0, id, kplane, kword, KX, 0);
+            issue(t0, id, vplane, vword, VX, 2 * T::BYTES);
+            if (t0 + 1 < t1) {
+                id = id_at(t0 + 1);
+                issue(t0 + 1, id, kplane, kword, KX, 0);
+                wait_vm<2 * (D / 32)>();
+            } else {
+                wait_vm<D / 32>();
+            }
         } else {
-            wait_vm<D / 32>();
+            // they, and what the first turn spreads: the second values, the third keys
+            Raw<D> first;
+            fetch(t0, id, A.kp, first, false);
+            fetch(t0, id, A.vp, vraw, true);
+            if (t0 + 1 < t1) {
+                id = id_at(t0 + 1);
+                fetch(t0 + 1, id, A.kp, kraw, false);
+            }
+            spread(t0, first, false);
+            spread(t0, vraw, true);
+            if (t0 + 1 < t1) {
+                spread(t0 + 1, kraw, false);
+                fetch(t0 + 1, id, A.vp, vraw, true);
+                if (t0 + 2 < t1) {
+                    id = id_at(t0 + 2);
+                    fetch(t0 + 2, id, A.kp, kraw, false);
+                }
+            }
         }
         barrier();
         {
@@ -412,10 +493,27 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
         // tile t, whose scores are in sc; those of the next go to sn
         auto turn = [&](int t, f16v (&sc)[T::KB], f16v (&sn)[T::KB]) {
             const bool more = t + 1 < t1;
-            wait_vm<0>();
+            if constexpr (BITS == 16) wait_vm<0>();
             if (lo_all > hi_all) clear(t);
             barrier();
-            if (more) {
+            if constexpr (BITS != 16) {
+                if (more) {
+                    spread(t + 1, vraw, true);
+                    if (t + 2 < t1) {
+                        spread(t + 2, kraw, false);
+                        if (t + 3 < t1 && page_of(base + (t + 4) * T::KT - 1) - ids_from >= IDS) {
+                            fill_ids(page_of(base + (t + 1) * T::KT), std::false_type{});  // its mask looks them up
+                            __syncthreads();
+                            holes = __builtin_amdgcn_readfirstlane(red[4]);
+                        }
+                        fetch(t + 2, id, A.vp, vraw, true);
+                        if (t + 3 < t1) {
+                            id = id_at(t + 3);
+                            fetch(t + 3, id, A.kp, kraw, false);
+                        }
+                    }
+                }
+            } else if (more) {
                 issue(t + 1, id, vplane, vword, VX, 2 * T::BYTES);
                 if (t + 2 < t1) {
                     if (page_of(base + (t + 3) * T::KT - 1) - ids_from >= IDS) {
@@ -441,7 +539,7 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
             // ---- the next tile's scores beside the first half of the weights
             // (behind the last tile LDS holds older keys: not used)
             {
-                constexpr int N = T::KB * STEPS, AHEAD = 4, PAIRS = 4 * T::KB;
+                constexpr int N = T::KB * STEPS, AHEAD = BITS == 16 ? 4 : 2, PAIRS = 4 * T::KB;
                 const uint32_t kr = kread + (uint32_t)((t + 1) & 1) * T::BYTES;
                 h8 kf[AHEAD];
                 auto frag = [&](int i) { return kfrag(kr, i); };
@@ -580,8 +678,9 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 // to 4000 positions (524 MB) 107 / 146 us (4.9 TB/s), 128 of up to 500 27 / 33;
 // 128 full slots of 8192 (4.3 GB) 765 us with the join, 5.6 TB/s.  Values by
 // loads to registers and LDS writes: 127 and 36 us.
-constexpr int few_bufs(int D, int mode, int nb) { return mode == 0 && !(D == 128 && nb == 2) ? 1 : 2; }
-constexpr int few_wgs(int D, int mode, int nb) { return few_bufs(D, mode, nb) == 1 ? 4 : 2; }
+constexpr int few_wgs(int D, int mode, int nb) { return mode == 0 && !(D == 128 && nb == 2) ? 4 : 2; }
+// a quantised cache's tiles wait in registers as codes: one buffer of values
+constexpr int few_bufs(int D, int mode, int nb) { return BITS != 16 || few_wgs(D, mode, nb) == 4 ? 1 : 2; }
 constexpr int OWN_LEAST = 4;  // tiles that a part of an own task has at least, where there are
 template <int D, int NB, int BUFS>
 struct Few {
@@ -589,7 +688,7 @@ struct Few {
     static constexpr int OB = NB * (D / 16) * 64 * 16;     // of a wave's sums
     static constexpr int WAVE = BUFS * VT > OB ? BUFS * VT : OB;  // LDS of a wave
     static constexpr int LDS = 4 * WAVE + 4 * NB * 16 * 8;
-    static_assert(LDS <= (BUFS == 1 ? 40 : 80) * 1024, "workgroups to a CU");
+    static_assert(LDS <= (BUFS == 1 && BITS == 16 ? 40 : 80) * 1024, "workgroups to a CU");
 };
 template <int D, int NB, int BUFS>
 DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int plo, int phi, const int* trow, int part,
@@ -621,7 +720,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
         qrow[b] = (size_t)sj * A.q_heads + kvh * g + (rr - sj * g);
 #pragma unroll
         for (int i = 0; i < STEPS; i++)
-            qf[b][i] = *reinterpret_cast<const h8*>(A.q + qrow[b] * D + 32 * i + 8 * q4);
+            qf[b][i] = *reinterpret_cast<const h8*>(A.q + qrow[b] * D + (BITS == 16 ? 32 * i + 8 * q4 : D / 4 * q4 + 8 * i));
     }
     int lo_any = 0x7fffffff, hi_any = 0, lo_all = 0, hi_all = 0x7fffffff;
 #pragma unroll
@@ -664,6 +763,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
     const uint32_t vbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * F::WAVE;
     h8 kf[BUFS][2][STEPS];
     uint32_t gone[BUFS];  // bit u: group u of the tile has no page
+    Raw<D> kraw[2], vraw[2];
     auto issue = [&](int t, auto buf) {
         gone[buf] = 0;
 #pragma unroll
@@ -683,6 +783,13 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
                 for (int i = 0, p = p0; i < 16; i++, p++)
                     if (__ballot(live[0] && lo[0] <= p && p < hi[0])) seen |= 1u << i;
             }
+            if constexpr (BITS != 16) {
+                const int pk = min(max(p0 + li, lo_any), hi_any - 1) & (page - 1);
+                kraw[u].load(head_page<D>(A, A.kp, id, kvh), page, pk, q4);
+                vraw[u].load(head_page<D>(A, A.vp, id, kvh), page, pk, q4);
+                if (id < 0 || !(seen >> li & 1)) vraw[u].s = 0;
+                continue;
+            }
             const uint16_t* vsrc = id < 0 ? reinterpret_cast<const uint16_t*>(no_page) : A.vp + off;
             const int pk = min(max(p0 + li, lo_any), hi_any - 1) & (page - 1);
 #pragma unroll
@@ -700,27 +807,66 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
         }
     };
     auto step = [&](int t, auto buf) {
-        if constexpr (BUFS == 1) issue(t, buf);
-        wait_vm<0>();
-        if constexpr (BUFS == 2)
-            if (t + 4 < t1) issue(t + 4, std::integral_constant<int, 1 - buf>{});
+        f4 kq[NB][2];  // a quantised cache's scores
+        uint32_t now = 0;
+        auto none = [&]() -> uint32_t& {
+            if constexpr (BITS == 16) return gone[buf];
+            else return now;
+        };
+        if constexpr (BITS == 16) {
+            if constexpr (BUFS == 1) issue(t, buf);
+            wait_vm<0>();
+            if constexpr (BUFS == 2)
+                if (t + 4 < t1) issue(t + 4, std::integral_constant<int, 1 - buf>{});
+        } else {
+            now = gone[0];
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                const int f = D == 128 ? (li & 7) << 1 : (li >> 1 & 3) << 1;
+                uint8_t* to = lds + wave * F::WAVE + (16 * u + li) * D * 2;
+#pragma unroll
+                for (int i = 0; i < STEPS; i++) {
+                    *reinterpret_cast<h8*>(to + ((q4 * STEPS + i) ^ f) * 16) = vraw[u].get(i);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+#pragma unroll
+                for (int b = 0; b < NB; b++) kq[b][u] = f4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int i = 0; i < STEPS; i++) {
+                    const h8 k = kraw[u].get(i);
+#pragma unroll
+                    for (int b = 0; b < NB; b++)
+                        kq[b][u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(k, qf[b][i], kq[b][u], 0, 0, 0);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            }
+            if (t + 4 < t1) issue(t + 4, buf);
+            __builtin_amdgcn_sched_barrier(0);
+        }
         const int p0 = base + 32 * t;
-        __asm__ volatile("" : "+s"(gone[buf]));  // one path for the tile, by one test
+        __asm__ volatile("" : "+s"(none()));  // one path for the tile, by one test
         h8 pf[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
             f4 sc[2];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
+                if constexpr (BITS != 16) {
+                    sc[u] = kq[b][u];
+                    continue;
+                }
                 sc[u] = f4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
                 for (int i = 0; i < STEPS; i++)
                     sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[buf][u][i], qf[b][i], sc[u], 0, 0, 0);
             }
-            if (p0 < lo_all || p0 + 32 > hi_all || gone[buf]) {
+            if (p0 < lo_all || p0 + 32 > hi_all || none()) {
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const int end = gone[buf] >> u & 1 ? 0 : hi[b];
+                    const int end = none() >> u & 1 ? 0 : hi[b];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int p = p0 + 16 * u + 4 * q4 + i;
@@ -778,6 +924,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
     using B1 = std::integral_constant<int, 1>;
     int t = t0 + wave;
     if constexpr (BUFS == 1) {
+        if (BITS != 16 && t < t1) issue(t, B0{});
         for (; t < t1; t += 4) step(t, B0{});
     } else if (t < t1) {
         issue(t, B0{});
@@ -878,8 +1025,15 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
     few_task<D, NB, BUFS>(A, lds, kvh, s * rows + tile * 16 * NB, (s + 1) * rows, A.prefix_pages << A.page_shift, 0x7fffffff,
                     A.table + (size_t)s * A.table_stride, part, A.own_parts, A.prefix_parts + part, A.prefix_pages, OWN_LEAST, false);
 }
+#if CIMA_KV_BITS == 16
+#define ATTN_NAME(D, MODE, NB) cima_attn_paged_d##D##_m##MODE##_n##NB
+#elif CIMA_KV_BITS == 8
+#define ATTN_NAME(D, MODE, NB) cima_attn_paged_q8_d##D##_m##MODE##_n##NB
+#else
+#define ATTN_NAME(D, MODE, NB) cima_attn_paged_q4_d##D##_m##MODE##_n##NB
+#endif
 #define ATTN(D, MODE, NB)                                                                                            \
-    extern "C" __global__ __launch_bounds__(256, few_wgs(D, MODE, NB)) void cima_attn_paged_d##D##_m##MODE##_n##NB(const AttnArgs A) {  \
+    extern "C" __global__ __launch_bounds__(256, few_wgs(D, MODE, NB)) void ATTN_NAME(D, MODE, NB)(const AttnArgs A) {  \
         extern __shared__ __align__(1024) uint8_t lds[];                                                             \
         attn_body<D, MODE, NB>(A, lds);                                                                              \
     }
@@ -893,6 +1047,7 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
 ATTN_ALL(64)
 ATTN_ALL(128)
 
+#if CIMA_KV_BITS == 16  // the partial sums are the same for every cache
 // The parts of a row joined: out = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M)
 // l_c.  A workgroup takes 16 rows and 16 elements.  First all parts' {m, l} of
 // the rows are read together and become weights in LDS, and the parts that any
@@ -1013,3 +1168,4 @@ DEV void attn_join_body(const AttnArgs& A) {
 }
 extern "C" __global__ __launch_bounds__(256) void cima_attn_paged_join_d64(const AttnArgs A) { attn_join_body<64>(A); }
 extern "C" __global__ __launch_bounds__(256) void cima_attn_paged_join_d128(const AttnArgs A) { attn_join_body<128>(A); }
+#endif

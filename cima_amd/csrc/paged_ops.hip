@@ -1,8 +1,9 @@
 // Paged KV cache for gfx950 (CDNA4): the code object cima_paged.hsaco.  RoPE
-// with the append of a step's keys and values, and the operations on pages:
-// copy, reserve, fork, free, compact.  The cache's layout is cima_kv_pages in
-// include/cima_hip.h.
+// with the append of a step's keys and values, the read back, and the operations
+// on pages: copy, reserve, fork, free, compact.  The cache's layout is
+// cima_kv_pages in include/cima_hip.h.
 #include "gguf_formats.h"
+#include "kv_quant.h"
 
 // ---------------------------------------------------------- RoPE and append
 
@@ -82,6 +83,177 @@ DEV void rope_append_body(const uint16_t* __restrict__ qkv, uint16_t* __restrict
     }
 ROPE_APPEND(64)
 ROPE_APPEND(128)
+
+// The same into a quantised cache.  A row's keys are rotated in fp64 and rounded to
+// f16, what an f16 cache would hold, so that the codes do not hang on fp32's last
+// bits (with an fp32 rotation one key in 10^4 is off by an f16 step, and now and
+// then a code or its group's scale with it); queries as above.  A thread has eight
+// elements of a group, a quad the group: its extremes are two exchanges in the quad.
+template <int D, int BITS>
+DEV void rope_append_quant_body(const uint16_t* __restrict__ qkv, uint16_t* __restrict__ q, uint8_t* __restrict__ kp,
+                                uint8_t* __restrict__ vp, const int* __restrict__ table, const int* __restrict__ lens,
+                                int n_new, int q_heads, int kv_heads, int page_shift, int n_pages, int table_stride,
+                                int rotate, double log2_theta) {
+    using Q = KvQ<BITS>;
+    constexpr int H8 = D / 16;  // 8-pair words of a head
+    __shared__ float cs[D / 2], sn[D / 2];
+    __shared__ double cd[D / 2], sd[D / 2];
+    const int row = blockIdx.x, s = row / n_new, t = threadIdx.x;
+    const int len = lens[s];
+    if (len < 0) return;
+    const int pos = len + (row - s * n_new);
+    const int at = pos >> page_shift;
+    int id = -1;
+    if ((unsigned)at < (unsigned)table_stride) id = table[(size_t)s * table_stride + at];
+    if (t < D / 2) {
+        double sv = 0., cv = 1.;
+        if (rotate) {
+            const double turns = (double)pos * (exp2(log2_theta * (-2.0 * t / D)) * 0.15915494309189533577);
+            sincospi(2.0 * (turns - rint(turns)), &sv, &cv);
+        }
+        cs[t] = (float)cv, sn[t] = (float)sv;
+        cd[t] = cv, sd[t] = sv;
+    }
+    __syncthreads();
+    const uint16_t* x = qkv + (size_t)row * (q_heads + 2 * kv_heads) * D;
+    const bool keep = (unsigned)id < (unsigned)n_pages;
+    const int page = 1 << page_shift, r = pos & (page - 1);
+    // eight elements i, ... of head h: words of its page, and the group's scales
+    auto put = [&](uint8_t* plane, int h, int i, const uint32_t (&v)[4]) {
+        uint32_t w[Q::WORDS];
+        const uint32_t sc = kv_encode<BITS>(v, w);
+        uint8_t* head = plane + ((size_t)id * kv_heads + h) * page * Q::row(D);
+        uint32_t* c = reinterpret_cast<uint32_t*>(head + r * Q::codes(D) + i * BITS / 8);
+#pragma unroll
+        for (int k = 0; k < Q::WORDS; k++) c[k] = w[k];
+        if ((i & 31) == 0) {
+            uint8_t* z = head + page * Q::codes(D) + r * Q::scales(D) + i / 32 * Q::SCALE;
+            if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(z) = sc;
+            else *reinterpret_cast<uint16_t*>(z) = (uint16_t)sc;
+        }
+    };
+    for (int e = t; e < (q_heads + kv_heads) * H8; e += 256) {
+        const int h = e / H8, i = e % H8 * 8;
+        if (h >= q_heads && !keep) continue;
+        const uint4 a = *reinterpret_cast<const uint4*>(x + (size_t)h * D + i);
+        const uint4 b = *reinterpret_cast<const uint4*>(x + (size_t)h * D + D / 2 + i);
+        const uint32_t au[4] = {a.x, a.y, a.z, a.w}, bu[4] = {b.x, b.y, b.z, b.w};
+        uint32_t oa[4], ob[4];
+        if (h < q_heads) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const float a0 = h2f(au[j] & 0xffffu), a1 = h2f(au[j] >> 16);
+                const float b0 = h2f(bu[j] & 0xffffu), b1 = h2f(bu[j] >> 16);
+                const float c0 = cs[i + 2 * j], c1 = cs[i + 2 * j + 1], s0 = sn[i + 2 * j], s1 = sn[i + 2 * j + 1];
+                oa[j] = f2h2(a0 * c0 - b0 * s0, a1 * c1 - b1 * s1);
+                ob[j] = f2h2(a0 * s0 + b0 * c0, a1 * s1 + b1 * c1);
+            }
+            uint16_t* y = q + ((size_t)row * q_heads + h) * D;
+            *reinterpret_cast<uint4*>(y + i) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
+            *reinterpret_cast<uint4*>(y + D / 2 + i) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
+            continue;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const uint32_t sh = j & 1 ? 16 : 0;
+            const double p = h2f(au[j / 2] >> sh & 0xffffu), z = h2f(bu[j / 2] >> sh & 0xffffu);
+            const double c = cd[i + j], n = sd[i + j];
+            const uint32_t lo = d2h(fma(p, c, -(z * n))), hi = d2h(fma(p, n, z * c));
+            oa[j / 2] = j & 1 ? oa[j / 2] | lo << 16 : lo;
+            ob[j / 2] = j & 1 ? ob[j / 2] | hi << 16 : hi;
+        }
+        put(kp, h - q_heads, i, oa);
+        put(kp, h - q_heads, D / 2 + i, ob);
+    }
+    if (!keep) return;
+    for (int e = t; e < kv_heads * (D / 8); e += 256) {
+        const int h = e / (D / 8), i = e % (D / 8) * 8;
+        const uint4 a = *reinterpret_cast<const uint4*>(x + (size_t)(q_heads + kv_heads + h) * D + i);
+        const uint32_t au[4] = {a.x, a.y, a.z, a.w};
+        put(vp, h, i, au);
+    }
+}
+#define ROPE_APPEND_QUANT(D, BITS)                                                                                   \
+    extern "C" __global__ __launch_bounds__(256) void cima_rope_append_paged_q##BITS##_d##D(                         \
+        const uint16_t* __restrict__ qkv, uint16_t* __restrict__ q, uint8_t* __restrict__ kp,                        \
+        uint8_t* __restrict__ vp, const int* __restrict__ table, const int* __restrict__ lens, int n_new,            \
+        int q_heads, int kv_heads, int page_shift, int n_pages, int table_stride, int rotate,                        \
+        double log2_theta) {                                                                                         \
+        rope_append_quant_body<D, BITS>(qkv, q, kp, vp, table, lens, n_new, q_heads, kv_heads, page_shift, n_pages,  \
+                                        table_stride, rotate, log2_theta);                                           \
+    }
+ROPE_APPEND_QUANT(64, 4)
+ROPE_APPEND_QUANT(128, 4)
+ROPE_APPEND_QUANT(64, 8)
+ROPE_APPEND_QUANT(128, 8)
+
+// ---------------------------------------------------------------- read back
+
+// Positions first + j of slots as f16 rows [slot][head][max_seq][D]: a thread has
+// eight elements of READ_ROWS rows of the keys and of the values, whose loads go out
+// together.  Positions without a page are zeros.
+constexpr int READ_ROWS = 4;
+template <int D, int BITS>
+DEV void kv_read_body(const uint8_t* __restrict__ kp, const uint8_t* __restrict__ vp, const int* __restrict__ table,
+                      const int* __restrict__ slots, const int* __restrict__ first, uint16_t* __restrict__ k,
+                      uint16_t* __restrict__ v, int kv_heads, int page_shift, int n_pages, int table_stride,
+                      int max_seqs, int n, int blocks, long long max_seq) {
+    using Q = KvQ<BITS>;
+    constexpr int W8 = D / 8, PASS = 256 / W8;  // threads of a row, rows of a pass
+    const int b = blockIdx.x % blocks, sh = blockIdx.x / blocks, i = sh / kv_heads, h = sh % kv_heads;
+    const int slot = slots ? slots[i] : i;
+    const long long from = first ? first[i] : 0;
+    const int w8 = threadIdx.x % W8, page = 1 << page_shift;
+    const size_t out = (size_t)sh * max_seq * D + w8 * 8;
+    uint32_t w[2][READ_ROWS][Q::WORDS], sc[2][READ_ROWS];
+    bool has[READ_ROWS];
+#pragma unroll
+    for (int u = 0; u < READ_ROWS; u++) {
+        const int j = (b * READ_ROWS + u) * PASS + threadIdx.x / W8;
+        const long long pos = from + j, e = pos >> page_shift;
+        int id = -1;
+        if (j < n && pos >= 0 && e < table_stride && (unsigned)slot < (unsigned)max_seqs)
+            id = table[(size_t)slot * table_stride + e];
+        has[u] = (unsigned)id < (unsigned)n_pages;
+        const int r = (int)(pos & (page - 1));
+        const size_t head = ((size_t)(has[u] ? id : 0) * kv_heads + h) * page * Q::row(D);
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            const uint8_t* p = (c ? vp : kp) + head;
+            const uint32_t* at = reinterpret_cast<const uint32_t*>(p + (size_t)r * Q::codes(D)) + w8 * Q::WORDS;
+#pragma unroll
+            for (int x = 0; x < Q::WORDS; x++) w[c][u][x] = at[x];
+            sc[c][u] = Q::load_scale(p, page, D, r, w8 / 4);
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < READ_ROWS; u++) {
+        const int j = (b * READ_ROWS + u) * PASS + threadIdx.x / W8;
+        if (j >= n) break;
+#pragma unroll
+        for (int c = 0; c < 2; c++) {
+            uint32_t o[4];
+            Q::decode(w[c][u], sc[c][u], o);
+            const uint4 z = has[u] ? make_uint4(o[0], o[1], o[2], o[3]) : make_uint4(0, 0, 0, 0);
+            *reinterpret_cast<uint4*>((c ? v : k) + out + (size_t)j * D) = z;
+        }
+    }
+}
+#define KV_READ(D, BITS)                                                                                             \
+    extern "C" __global__ __launch_bounds__(256) void cima_kv_pages_read_b##BITS##_d##D(                             \
+        const uint8_t* __restrict__ kp, const uint8_t* __restrict__ vp, const int* __restrict__ table,               \
+        const int* __restrict__ slots, const int* __restrict__ first, uint16_t* __restrict__ k,                      \
+        uint16_t* __restrict__ v, int kv_heads, int page_shift, int n_pages, int table_stride, int max_seqs, int n,  \
+        int blocks, long long max_seq) {                                                                             \
+        kv_read_body<D, BITS>(kp, vp, table, slots, first, k, v, kv_heads, page_shift, n_pages, table_stride,        \
+                              max_seqs, n, blocks, max_seq);                                                         \
+    }
+KV_READ(64, 4)
+KV_READ(128, 4)
+KV_READ(64, 8)
+KV_READ(128, 8)
+KV_READ(64, 16)
+KV_READ(128, 16)
 
 // -------------------------------------------------------------- page copies
 
@@ -349,11 +521,11 @@ extern "C" __global__ __launch_bounds__(1024) void cima_kv_pages_fork(int* refs,
 }
 
 // Fork, second launch: workgroups [0, n) write the children's rows and count
-// the shared pages, the others copy the rows of the pages begun, one child
-// and plane each.
+// the shared pages, the others copy the rows of the pages begun (and a quantised
+// cache's scales of them), one child and plane each.
 extern "C" __global__ __launch_bounds__(256) void cima_kv_pages_fork_copy(
     uint4* pool, long long plane_words, int* refs, int n_pages, int* table, const int* __restrict__ lens,
-    int table_stride, int page_shift, int kv_heads, int row_words, const int* __restrict__ parents,
+    int table_stride, int page_shift, int kv_heads, int row_words, int scale_words, const int* __restrict__ parents,
     const int* __restrict__ children, int n, const int* __restrict__ status) {
     if (*status != 0) return;
     const int b = blockIdx.x, i = b % n;
@@ -377,12 +549,19 @@ extern "C" __global__ __launch_bounds__(256) void cima_kv_pages_fork_copy(
     const int src = from[full], dst = to[full];
     if ((unsigned)src >= (unsigned)n_pages || (unsigned)dst >= (unsigned)n_pages) return;
     uint4* plane = pool + (long long)(b / n - 1) * plane_words;
-    const int live = rest * row_words, head = row_words << page_shift;  // words copied and held per head
+    // 16-byte words of rows copied and held per head, behind them 4-byte words of
+    // rows' scales
+    const int live = rest * row_words, rows = row_words << page_shift, live4 = rest * scale_words;
+    const int head = rows + ((scale_words << page_shift) >> 2);
     const uint4* s = plane + (long long)src * kv_heads * head;
     uint4* d = plane + (long long)dst * kv_heads * head;
     for (int e = threadIdx.x; e < kv_heads * live; e += 256) {
         const int w = e / live * head + e % live;
         d[w] = s[w];
+    }
+    for (int e = threadIdx.x; e < kv_heads * live4; e += 256) {
+        const int w = (e / live4 * head + rows) * 4 + e % live4;
+        reinterpret_cast<uint32_t*>(d)[w] = reinterpret_cast<const uint32_t*>(s)[w];
     }
 }
 

@@ -28,7 +28,7 @@ LIBHIP = os.path.join(LIB_DIR, "libcima_hip.so")
 # writes them)
 CODE_OBJECTS = [os.path.join(LIB_DIR, f"cima_{n}.hsaco")
                 for n in ("gemv_a", "gemv_b", "gemv_c", "gemm", "dequant", "decode", "bnb4", "gemm_wide", "paged",
-                          "paged_attn", "sample")]
+                          "paged_attn", "paged_attn_q4", "paged_attn_q8", "sample")]
 
 # declared in include/cima_hip.h, in order
 EXPORTS = (
@@ -42,7 +42,7 @@ EXPORTS = (
     "cima_hip_rmsnorm", "cima_hip_rope", "cima_hip_kv_append", "cima_hip_attn_decode_split", "cima_hip_attn_reduce",
     "cima_hip_attn_decode_noalloc", "cima_hip_attn_decode", "cima_hip_attn_gguf_gemv", "cima_hip_gguf_gemv_argmax", "cima_hip_argmax",
     "cima_hip_argmax_to_ids", "cima_hip_pos_bump", "cima_hip_decode_step",
-    "cima_hip_rope_append_paged", "cima_hip_attn_paged", "cima_hip_kv_pages_copy", "cima_hip_kv_pages_reserve",
+    "cima_hip_rope_append_paged", "cima_hip_attn_paged", "cima_hip_kv_pages_read", "cima_hip_kv_pages_copy", "cima_hip_kv_pages_reserve",
     "cima_hip_kv_pages_fork", "cima_hip_kv_pages_free", "cima_hip_kv_pages_compact", "cima_hip_softmax_rows",
     "cima_hip_verify_drafts",
     "cima_hip_capture_begin", "cima_hip_capture_end", "cima_hip_graph_launch", "cima_hip_graph_destroy",
@@ -77,7 +77,7 @@ class KvPages(ctypes.Structure):
     _fields_ = ([("pool", ctypes.c_void_p), ("plane_elems", ctypes.c_longlong)]
                 + [(n, ctypes.c_void_p) for n in ("refs", "table", "lens")]
                 + [(n, ctypes.c_int) for n in ("n_planes", "n_pages", "kv_heads", "page", "head_dim", "max_seqs",
-                                               "table_stride")])
+                                               "table_stride", "ggml_type")])
 
 
 E_INVALID, E_FORMAT, E_NO_KERNEL, E_NOT_INIT, E_LIBRARY = -1, -2, -3, -4, -5
@@ -142,6 +142,7 @@ def load_library(path: str = LIBHIP) -> ctypes.CDLL:
     U = ctypes.c_ulonglong
     L.cima_hip_rope_append_paged.argtypes = [P, P, I, P, P, I, I, I, F]
     L.cima_hip_attn_paged.argtypes = [P, P, I, P, P, I, I, I, F, I, I, I, P, U]
+    L.cima_hip_kv_pages_read.argtypes = [P, P, I, P, P, P, P, I, I, I]
     L.cima_hip_kv_pages_copy.argtypes = [P, P, P, P, I]
     L.cima_hip_kv_pages_reserve.argtypes = [P, P, I, I, P]
     L.cima_hip_kv_pages_fork.argtypes = [P, P, P, P, I, P]
@@ -563,6 +564,19 @@ class HipCtx:
         self._check(self.lib.cima_hip_attn_paged(
             self.handle, self._kv(kv), layer, _ptr_of(q, _F16, n, "q", d), _ptr_of(out, _F16, n, "out", d), seqs, n_new,
             q_heads, scale, prefix_pages, prefix_slot, window, *self._slab(slab)))
+
+    def kv_pages_read(self, kv, layer: int, k, v, n_slots: int, n: int, slots=None, first=None,
+                      max_seq: Optional[int] = None) -> None:
+        """Positions ``first[i] + j`` (first None: from 0), ``j < n``, of slots
+        ``slots[i]`` (None: 0, 1, ...) as f16 rows ``j`` of ``k`` and ``v``
+        [n_slots, kv_heads, max_seq, head_dim]; rows from n on are left alone
+        (max_seq None: n)."""
+        d, room = self.device, n if max_seq is None else max_seq
+        size = n_slots * kv.kv_heads * room * kv.head_dim
+        self._check(self.lib.cima_hip_kv_pages_read(
+            self.handle, self._kv(kv), layer, _ptr_of(slots, _I32, n_slots, "slots", d),
+            _ptr_of(first, _I32, n_slots, "first", d), _ptr_of(k, _F16, size, "k", d), _ptr_of(v, _F16, size, "v", d),
+            n_slots, n, room))
 
     def kv_pages_copy(self, kv, src, dst, n: int) -> None:
         """Page ``dst[i]`` of every plane = page ``src[i]``."""

@@ -56,7 +56,8 @@ typedef struct cima_hip_ctx cima_hip_ctx;
  * selection, one non-blocking stream, then loading the prebuilt gfx950 code
  * objects (cima_gemv_a/b/c.hsaco, cima_gemm.hsaco, cima_gemm_wide.hsaco,
  * cima_dequant.hsaco, cima_decode.hsaco, cima_bnb4.hsaco, cima_paged.hsaco,
- * cima_paged_attn.hsaco, cima_sample.hsaco) with hipModuleLoad and resolving
+ * cima_paged_attn.hsaco, cima_paged_attn_q4.hsaco, cima_paged_attn_q8.hsaco,
+ * cima_sample.hsaco) with hipModuleLoad and resolving
  * every kernel (the reference JIT-compiles with NVRTC and resolves its
  * KernelSet, src/cuda.rs:808-877).
  * code_dir: directory holding the code objects, or NULL for the directory
@@ -418,7 +419,7 @@ int cima_hip_decode_step(cima_hip_ctx* ctx, const cima_decoder* d);
  * streams, other graphs in flight) need a slab each.
  * --------------------------------------------------------------------- */
 
-/* The cache.  A page is [kv_heads, page, head_dim] f16 in every plane, two
+/* The cache.  A page is [kv_heads, page, head_dim] in every plane, two
  * planes a layer: keys in plane 2 l, values in plane 2 l + 1.  Slot s holds
  * position t of its sequence in row t % page of page table[s * table_stride +
  * t / page]; unused entries are -1.  lens[s] is its number of cached tokens,
@@ -427,14 +428,29 @@ int cima_hip_decode_step(cima_hip_ctx* ctx, const cima_decoder* d);
  * most 1048576 pages, 4096 slots and 2^30 positions a slot; pool is 16-byte
  * aligned and plane_elems a multiple of 8.  A page that several slots hold is
  * full: cima_hip_kv_pages_fork copies one that is begun, so that no two slots
- * append to the same. */
+ * append to the same.
+ *
+ * ggml_type 0: the elements are f16.  CIMA_GGML_Q4_1 or CIMA_GGML_Q8_0: they are
+ * quantised as they are written, a row's head_dim in groups of 32 as in the GGUF
+ * block of that type, and stand for the f16 nearest to c d + m (codes c from 0 to
+ * 15, f16 scale d and least value m) or c d (codes from -127 to 127).  d is the
+ * least f16 that is not below (max - m) / 15 or max|x| / 127, c the code nearest to
+ * the quotient (half to even): a value is off by at most d / 2 and its own rounding.
+ * What is written has to be finite (a group that is not reads back as NaN), and of
+ * Q4_1 at most 65000, which the sum may pass by.  A head's page is 20 / 32 or 34 /
+ * 32 bytes an element: the codes of its rows, [page, head_dim], then the groups'
+ * scales, [page, head_dim / 32] of {d, m} or d.  Q8_0's codes are bytes with 128
+ * added; Q4_1's are in little-endian 32-bit words of eight elements, element 2 k in
+ * bits 4 k to 4 k + 3, element 2 k + 1 in bits 4 k + 16 to 4 k + 19. */
 typedef struct cima_kv_pages {
-    void* pool;             /* f16 planes of [n_pages, kv_heads, page, head_dim] */
-    long long plane_elems;  /* elements from one plane to the next */
+    void* pool;             /* planes of [n_pages, kv_heads, page, head_dim] */
+    long long plane_elems;  /* f16 elements from one plane to the next; of a quantised cache, a
+                             * multiple of 16 bytes */
     int* refs;              /* [n_pages] */
     int* table;             /* [max_seqs, table_stride] */
     int* lens;              /* [max_seqs] */
     int n_planes, n_pages, kv_heads, page, head_dim, max_seqs, table_stride;
+    int ggml_type;          /* 0 (f16), CIMA_GGML_Q4_1 or CIMA_GGML_Q8_0 */
 } cima_kv_pages;
 
 /* RoPE of a step's queries and keys, and the append of its keys and values:
@@ -446,7 +462,8 @@ typedef struct cima_kv_pages {
  * 100000 an fp32 angle is off by up to 0.008); theta 0 = no rotation.  lens is not changed: every layer of the step
  * appends at the same positions.  Slots not in use write nothing, neither q;
  * positions without a page (entry -1 or behind the row) write no key.  Less
- * than 2^24 rows.
+ * than 2^24 rows.  A quantised cache takes the rotated keys rounded to f16, as an
+ * f16 cache holds them, and the values.
  * qkv and q 16-byte aligned, not overlapping. */
 int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* qkv, void* q,
                                int seqs, int n_new, int q_heads, float theta);
@@ -475,6 +492,17 @@ int cima_hip_rope_append_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int l
 int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* q, void* out, int seqs,
                         int n_new, int q_heads, float scale, int prefix_pages, int prefix_slot, int window, void* slab,
                         unsigned long long slab_bytes);
+
+/* Keys and values of `layer` out of the pages, as f16 (a quantised cache's values
+ * as the attention takes them): position first[i] + j of slot slots[i] goes to row j
+ * of k and v [n_slots, kv_heads, max_seq, head_dim], i < n_slots, j < n; rows from n
+ * on are left as they are.  One slot's are the caches of cima_hip_kv_append and
+ * cima_hip_attn_decode.  slots NULL: slots 0, 1, ...; first NULL: from position 0.
+ * A position without a page, a negative one, or any of a slot outside [0, max_seqs),
+ * is zeros; lens is not looked at: a position that has a page is what the page holds.
+ * n <= max_seq; k and v 16-byte aligned, not overlapping. */
+int cima_hip_kv_pages_read(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const int* slots, const int* first,
+                           void* k, void* v, int n_slots, int n, int max_seq);
 
 /* Page dst[i] of every plane = page src[i], i < n; counts and tables stay.
  * Pairs with an id outside [0, n_pages) are skipped.  No page may be written

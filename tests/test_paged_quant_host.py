@@ -1,0 +1,83 @@
+"""The quantised paged cache without a device: descriptor, sizes, kernels in the
+code objects, and what PagedKV and a missing context refuse."""
+import ctypes
+
+import pytest
+
+from cima_amd import build as cbuild
+from cima_amd import hip as hipmod
+from cima_amd.gguf import DType
+from test_paged_fields import _OnDevice
+
+torch = pytest.importorskip("torch")
+
+
+def _tensors(t, planes=4, pages=6, heads=2, page=16, dim=64, slots=3, stride=5):
+    from cima_amd.paged import head_page_bytes
+
+    i32 = torch.int32
+    return [torch.zeros((planes, pages, heads, head_page_bytes(t, page, dim)), dtype=torch.uint8),
+            torch.zeros(pages, dtype=i32), torch.full((slots, stride), -1, dtype=i32), torch.full((slots,), -1, dtype=i32)]
+
+
+@pytest.mark.parametrize("t,page,dim,size", [(DType.Q4_1, 16, 64, 640), (DType.Q4_1, 256, 128, 20480),
+                                             (DType.Q8_0, 16, 64, 1088), (DType.Q8_0, 64, 128, 8704)])
+def test_sizes_and_descriptor(t, page, dim, size):
+    from cima_amd.paged import PagedKV, head_page_bytes
+
+    assert head_page_bytes(t, page, dim) == size and size % 16 == 0
+    kv = PagedKV(*(x.as_subclass(_OnDevice) for x in _tensors(t, page=page, dim=dim)), ggml_type=t, page=page,
+                 head_dim=dim)
+    d = kv.desc
+    assert (d.ggml_type, d.page, d.head_dim, d.kv_heads, d.n_planes, d.n_pages) == (t, page, dim, 2, 4, 6)
+    assert d.plane_elems == 6 * 2 * size and kv.layers == 2
+    assert ctypes.sizeof(hipmod.KvPages) == 72        # as large as it was without the type
+
+
+def test_paged_kv_refuses_wrong_tensors():
+    from cima_amd.paged import PagedKV, head_page_bytes
+
+    t = DType.Q4_1
+
+    def no(ts, text, **kw):
+        with pytest.raises(hipmod.EngineError, match=text) as e:
+            PagedKV(*ts, **{"ggml_type": t, "page": 16, "head_dim": 64, **kw})
+        assert e.value.code == hipmod.E_INVALID
+    good = _tensors(t)
+    no(good, "not on a HIP device")                   # all else is as it must be
+    no([good[0].half()] + good[1:], "pool")
+    no([good[0][:3]] + good[1:], "pool")
+    no([good[0][..., :-1]] + good[1:], "pool")
+    no([good[0][:, :, ::2]] + good[1:], "contiguous")
+    no(good, "pool", ggml_type=DType.Q8_0)
+    no(good, "pool", page=32)
+    no(good, "pool", head_dim=128)
+    no(good, "ggml type", ggml_type=DType.Q4_K)
+    no(good, "a page", page=0)
+    no(good, "a page", head_dim=48)
+    no(_tensors(t)[:1] + [good[1].long()] + good[2:], "refs")
+    with pytest.raises(hipmod.EngineError, match="ggml type"):
+        head_page_bytes(0, 16, 64)
+    # an f16 pool may name its sizes, if they are its own
+    f16 = [torch.zeros((4, 6, 2, 16, 64), dtype=torch.float16), *good[1:]]
+    no(f16, "not on a HIP device", ggml_type=0)
+    no(f16, "pages of", ggml_type=0, page=32)
+    no(f16, "pages of", ggml_type=0, head_dim=128)
+
+
+def test_code_objects_hold_every_kernel():
+    want = {"paged": [f"cima_rope_append_paged_q{b}_d{d}" for b in (4, 8) for d in (64, 128)]
+            + [f"cima_kv_pages_read_b{b}_d{d}" for b in (4, 8, 16) for d in (64, 128)]}
+    for b in (4, 8):
+        want[f"paged_attn_q{b}"] = [f"cima_attn_paged_q{b}_d{d}_m{m}_n{n}" for d in (64, 128) for m in (0, 1, 2)
+                                    for n in (1, 2)]
+    for name, kernels in want.items():
+        blob = open(cbuild.HSACOS[name], "rb").read()
+        for k in kernels:
+            assert k.encode() in blob, k
+
+
+def test_read_back_refuses_a_missing_context():
+    L = hipmod.load_library()
+    rc = L.cima_hip_kv_pages_read(None, ctypes.byref(hipmod.KvPages()), 0, None, None, None, None, 1, 1, 1)
+    assert rc == hipmod.E_NOT_INIT and b"not initialised" in L.cima_hip_last_error()
