@@ -677,6 +677,9 @@ int cima_hip_init(int device, const char* code_dir, cima_hip_ctx** out) {
     for (const char* t : kSampleTypes)
         for (const char* kn : {"stats_w2", "probs_w2", "stats_w8", "probs_w8", "t256_w2", "t256_w8", "t1024_w8"})
             if (!rc) rc = add(MOD_SAMPLE, std::string("cima_softmax_") + kn + "_" + t);
+    for (const char* t : kSampleTypes)
+        for (const char* kn : {"t256_w2", "t256_w8", "t1024_w8", "join"})
+            if (!rc) rc = add(MOD_SAMPLE, std::string("cima_logprobs_") + kn + "_" + t);
     if (rc) {
         unload(ctx);
         delete ctx;
@@ -1999,6 +2002,23 @@ namespace {
 // multiple of (VF_STEP) and most parts of a row
 const int kSoftmaxWord = 1024, kSoftmaxLongRows = 128, kVerifyStep = 2048, kVerifyParts = 64;
 
+// LP_TOP in sample_ops.hip
+const int kLogprobsTop = 32;
+
+// kernel-argument mirror of LpArgs in sample_ops.hip (same member order)
+struct LogprobsArgs {
+    const void* x;
+    const int* tokens;
+    float *logprob, *entropy;
+    int* top_ids;
+    float* top_logprobs;
+    const float* temp;
+    float* stats;
+    unsigned long long* keys;
+    int n, n_top, kept, rows_per_temp, parts;
+    float cap;
+};
+
 // kernel-argument mirror of VfArgs in sample_ops.hip (same member order)
 struct VerifyArgs {
     const float *p, *q;
@@ -2050,6 +2070,53 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
     snprintf(name, sizeof name, "cima_softmax_probs_w%d_%s", words, sfx);
     void* pargs[] = {&x, &y, &slab, &n, &temp, &rows_per_temp, &cap, &parts};
     return launch_named(ctx, name, (unsigned)(rows * parts), 256, pargs, api);
+}
+
+int cima_hip_logprobs_rows(cima_hip_ctx* ctx, const void* x, int rows, int n, const int* tokens, float* logprob,
+                           float* entropy, int n_top, int* top_ids, float* top_logprobs, const float* temp,
+                           int rows_per_temp, float cap, int x_dtype, void* slab, unsigned long long slab_bytes) {
+    const char* api = "cima_hip_logprobs_rows";
+    if (int rc = ready(ctx, api)) return rc;
+    if (rows < 0 || rows > kMaxGrid / 4 || n <= 0 || n > 0x3fffffff || n_top < 0 || n_top > kLogprobsTop ||
+        rows_per_temp <= 0 || !(cap >= 0.f && cap < INFINITY))
+        return fail(CIMA_E_INVALID, "%s: rows=%d n=%d n_top=%d (at most %d) rows_per_temp=%d cap=%g", api, rows, n, n_top,
+                    kLogprobsTop, rows_per_temp, cap);
+    if (x_dtype != CIMA_DT_F32 && x_dtype != CIMA_DT_F16)
+        return fail(CIMA_E_INVALID, "%s: x_dtype %d is not f32 or f16", api, x_dtype);
+    if (rows == 0) return 0;
+    if (!x || (logprob && !tokens) || (n_top && (!top_ids || !top_logprobs)))
+        return fail(CIMA_E_INVALID, "%s: null pointer (logprob takes tokens, n_top both of its outputs)", api);
+    if (!aligned(x, x_dtype == CIMA_DT_F32 ? 4 : 2) || !aligned(tokens, 4) || !aligned(logprob, 4) ||
+        !aligned(entropy, 4) || !aligned(top_ids, 4) || !aligned(top_logprobs, 4) || !aligned(temp, 4))
+        return fail(CIMA_E_INVALID, "%s: misaligned pointer", api);
+    const bool f32 = x_dtype == CIMA_DT_F32;
+    const char* sfx = kSampleTypes[(cap > 0.f ? 2 : 0) + (f32 ? 1 : 0)];
+    char name[64];
+    LogprobsArgs A{x, tokens, logprob, entropy, top_ids, top_logprobs, temp, nullptr, nullptr, n, n_top, std::max(n_top, 1),
+                   rows_per_temp, 1, cap};
+    void* args[] = {&A};
+    // rows that a workgroup holds, and rows in parts, as in cima_hip_softmax_rows
+    static const int shapes[][2] = {{256, 2}, {256, 8}, {1024, 8}};
+    for (const auto& sh : shapes)
+        if (n <= sh[0] * sh[1] * 4) {
+            snprintf(name, sizeof name, "cima_logprobs_t%d_w%d_%s", sh[0], sh[1], sfx);
+            return launch_named(ctx, name, (unsigned)rows, (unsigned)sh[0], args, api);
+        }
+    const auto parts_of = [&](int words) { return (n - 1) / (kSoftmaxWord * words) + 1; };
+    const unsigned long long each = 16 + 8ULL * A.kept;
+    int words = 8;
+    if ((long long)rows * parts_of(2) <= 4LL * ctx->num_cu && slab_bytes >= each * rows * parts_of(2)) words = 2;
+    A.parts = parts_of(words);
+    const long long all = (long long)rows * A.parts;
+    if (all > kMaxGrid || !slab || !aligned(slab, 8) || slab_bytes < each * all)
+        return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (8 B)", api,
+                    slab_bytes, each * all);
+    A.keys = (unsigned long long*)slab;
+    A.stats = (float*)slab + 2 * A.kept * all;
+    snprintf(name, sizeof name, "cima_logprobs_t256_w%d_%s", words, sfx);
+    if (int rc = launch_named(ctx, name, (unsigned)all, 256, args, api)) return rc;
+    snprintf(name, sizeof name, "cima_logprobs_join_%s", sfx);
+    return launch_named(ctx, name, (unsigned)rows, 256, args, api);
 }
 
 int cima_hip_verify_drafts(cima_hip_ctx* ctx, const float* p, const float* q, const int* drafts, const int* counts,

@@ -1,5 +1,6 @@
 // Sampling over rows of the vocabulary for gfx950 (CDNA4): the code object
-// cima_sample.hsaco.  Softmax of rows of logits at a temperature, and the
+// cima_sample.hsaco.  Softmax of rows of logits at a temperature, log probabilities
+// of given tokens with the rows' entropy and likeliest alternatives, and the
 // verification of drafted tokens.
 #include "gguf_formats.h"
 
@@ -272,6 +273,324 @@ SOFTMAX(cap_f32, true, true)
 SOFTMAX_WHOLE(f16, false, false, 1024, 16)
 SOFTMAX_WHOLE(f32, true, false, 1024, 16)
 
+// v of the lane that a DPP pattern names, 0 where there is none
+template <int CTRL, int ROWS>
+DEV double dpp_d(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)u, CTRL, ROWS, 0xf, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// inclusive running sum over the wave: within rows of 16, then from row to row
+DEV double wave_scan_d(double v) {
+    v += dpp_d<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
+    v += dpp_d<0x112, 0xf>(v);
+    v += dpp_d<0x114, 0xf>(v);
+    v += dpp_d<0x118, 0xf>(v);
+    v += dpp_d<0x142, 0xa>(v);  // row_bcast:15 into rows 1, 3
+    v += dpp_d<0x143, 0xc>(v);  // row_bcast:31 into rows 2, 3
+    return v;
+}
+DEV double lane_d(double v, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, lane), hi = __builtin_amdgcn_readlane((uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+// ------------------------------------------------------- log probabilities
+//
+// With z = (f(x) - m) / T and L = sum e^z over a row: a token's log probability is z -
+// ln L, the row's entropy ln L - sum e^z z / L.  One reading: a part's logits stay in
+// registers, first their largest, then the two sums.  The likeliest n_top of a part
+// are found from the threads' largest: each wave takes the n_top-th largest of its
+// lanes', which bounds the row's n_top-th from below, and the highest of these bounds
+// leaves the few logits that are looked at one by one, ranked by counting (value
+// first, then the lower id).  A second launch joins rows of several parts.  Parts
+// as in the softmax above; sums of parts are joined in fp64.
+constexpr int LP_TOP = 32;    // most alternatives
+constexpr int LP_LIST = 1024;  // logits looked at one by one
+
+struct LpArgs {
+    const void* x;
+    const int* tokens;
+    float* logprob;
+    float* entropy;
+    int* top_ids;
+    float* top_logprobs;
+    const float* temp;
+    float4* stats;                // [rows][parts]: m, l, sum of e^z z in log2's unit
+    unsigned long long* keys;     // [rows][parts][kept]
+    int n, n_top, kept, rows_per_temp, parts;  // kept: keys of a part, n_top or 1
+    float cap;
+};
+
+// logits in order as whole numbers; -0 as 0
+DEV uint32_t lp_order(float v) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, v + 0.f);
+    return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
+}
+DEV float lp_value(unsigned long long key) {
+    const uint32_t u = (uint32_t)(key >> 32);
+    return __builtin_bit_cast(float, u ^ (u >> 31 ? 0x80000000u : 0xffffffffu));
+}
+constexpr uint32_t LP_NONE = 0x007fffffu;  // of -inf: a token that may not be taken
+DEV unsigned long long lp_key(uint32_t order, int at) { return (unsigned long long)order << 32 | (uint32_t)~at; }
+DEV int lp_id(unsigned long long key) { return (int)~(uint32_t)key; }
+
+DEV unsigned long long wave_max_key(unsigned long long v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) {
+        const unsigned long long w = __shfl_xor(v, o);
+        v = w > v ? w : v;
+    }
+    return v;
+}
+template <int NT>
+struct LpTop {  // shared between the threads of a workgroup
+    unsigned long long list[LP_LIST], top[LP_TOP], best[NT / 64];
+    int count;
+};
+// the `kept` largest of the listed keys to S.top in order, zeros behind them;
+// each(f) calls f with every key of this thread, for lists that are too short
+template <int NT, typename E>
+DEV void lp_rank(LpTop<NT>& S, int kept, E each) {
+    __syncthreads();
+    const int count = S.count;
+    if (count <= LP_LIST) {
+        for (int i = threadIdx.x; i < count; i += NT) {
+            const unsigned long long k = S.list[i];
+            int rank = 0;
+            for (int j = 0; j < count; j++) rank += S.list[j] > k;
+            if (rank < kept) S.top[rank] = k;
+        }
+        if ((int)threadIdx.x >= count && (int)threadIdx.x < kept) S.top[threadIdx.x] = 0;
+    } else {  // more equal logits than the list holds: one after the other
+        unsigned long long last = ~0ull;
+        for (int i = 0; i < kept; i++) {
+            unsigned long long b = 0;
+            each([&](unsigned long long k) { b = k < last && k > b ? k : b; });
+            b = wave_max_key(b);
+            __syncthreads();
+            if ((threadIdx.x & 63) == 0) S.best[threadIdx.x >> 6] = b;
+            __syncthreads();
+#pragma unroll
+            for (int w = 0; w < NT / 64; w++) b = S.best[w] > b ? S.best[w] : b;
+            if (threadIdx.x == 0) S.top[i] = b;
+            last = b;
+            if (!b) last = 0;
+        }
+    }
+    __syncthreads();
+}
+// a row's results: largest f(x) m, sums L and H as in LpArgs, the best keys in top
+DEV void lp_finish(const LpArgs& A, int row, float T, float m, double L, double H, const unsigned long long* top, float xt,
+                   bool cap) {
+    const double ln = log(L);
+    auto logprob = [&](float x) -> float {
+        if (x == -INFINITY) return -INFINITY;
+        const float f = cap ? sm_f(x, A.cap) : x;
+        return (float)((double)(f - m) / (double)T - ln);
+    };
+    const bool one = !(T > 0.f);  // the largest logit alone
+    const int first = one && top[0] ? lp_id(top[0]) : -1;
+    const int t = threadIdx.x;
+    if (t == 0) {
+        const int id = A.tokens ? A.tokens[row] : -1;
+        const bool known = (unsigned)id < (unsigned)A.n;
+        if (A.logprob) A.logprob[row] = !known ? -INFINITY : one ? (id == first ? 0.f : -INFINITY) : logprob(xt);
+        if (A.entropy) A.entropy[row] = one || L == 0. ? 0.f : (float)(ln - 0.69314718055994530942 * H / L);
+    }
+    if (t < A.n_top) {
+        const unsigned long long k = top[t];
+        A.top_ids[(size_t)row * A.n_top + t] = k ? lp_id(k) : -1;
+        A.top_logprobs[(size_t)row * A.n_top + t] = !k ? -INFINITY : one ? (t ? -INFINITY : 0.f) : logprob(lp_value(k));
+    }
+}
+template <bool F32>
+DEV float lp_token_logit(const LpArgs& A, int row) {
+    const int id = A.tokens ? A.tokens[row] : -1;
+    if ((unsigned)id >= (unsigned)A.n) return -INFINITY;
+    const size_t at = (size_t)row * A.n + id;
+    if constexpr (F32) return ((const float*)A.x)[at];
+    else return h2f(((const uint16_t*)A.x)[at]);
+}
+
+// R words of V logits a thread
+template <bool F32, bool CAP, int NT, int R, int V>
+DEV void lp_part(const LpArgs& A) {
+    __shared__ LpTop<NT> S;
+    __shared__ float red[3][NT / 64];
+    __shared__ uint32_t bound[NT / 64];
+    constexpr int W = F32 ? V : V / 2;
+    const int row = blockIdx.x / A.parts, part = blockIdx.x % A.parts, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
+    const int base = part * NT * R * V + threadIdx.x * V;
+    uint32_t v[R][W];
+#pragma unroll
+    for (int r = 0; r < R; r++) sm_load<F32, V>(A.x, (size_t)row * A.n, base + r * NT * V, A.n, v[r]);
+    const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f;
+    const float xt = lp_token_logit<F32>(A, row);
+    auto get = [&](int r, int j) { return sm_get<F32, V>(v[r], j); };
+    // ---- the thread's and the part's largest
+    float mine = -INFINITY;
+    if constexpr (F32) {
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int j = 0; j < V; j++) mine = fmaxf(mine, get(r, j));
+    } else {
+        typedef _Float16 hp __attribute__((ext_vector_type(2)));
+        hp h = {(_Float16)-INFINITY, (_Float16)-INFINITY};
+#pragma unroll
+        for (int r = 0; r < R; r++)
+#pragma unroll
+            for (int k = 0; k < W; k++) h = __builtin_elementwise_max(h, __builtin_bit_cast(hp, v[r][k]));
+        mine = fmaxf((float)h[0], (float)h[1]);
+    }
+    float m = wave_max_u(mine);
+    if (lane == 0) red[0][w] = m;
+    const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
+    const uint32_t order = lp_order(mine);
+    if (kept) {
+        // the kept-th largest of the lanes' or less, by its bits from the highest on
+        // (f16 logits have no more than 19)
+        uint32_t t = 0;
+        for (int b = 31; b >= (F32 ? 0 : 13); b--) {
+            const int c = __popcll(__ballot(order >= (t | 1u << b)));
+            if (c >= kept) t |= 1u << b;
+            if (c == kept) break;
+        }
+        if (lane == 0) bound[w] = t;
+    }
+    if (threadIdx.x == 0) S.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NT / 64; k++) m = fmaxf(m, red[0][k]);
+    // ---- the sums
+    m = uniform(CAP ? sm_f(m, A.cap) : m);
+    const float c = m == -INFINITY ? 0.f : m, s = sm_scale(1.44269504088896340736f, T > 0.f ? T : 1.f);
+    float l = 0.f, h = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; r++) {
+        float pl = 0.f, ph = 0.f;
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const float x = get(r, j), z = ((CAP ? sm_f(x, A.cap) : x) - c) * s;
+            const float e = __builtin_amdgcn_exp2f(z);
+            pl += e;
+            ph = fmaf(e, fmaxf(z, -1e30f), ph);
+        }
+        l += pl, h += ph;
+    }
+    l = wave_sum_u(l), h = wave_sum_u(h);
+    if (lane == 0) red[1][w] = l, red[2][w] = h;
+    // ---- the part's likeliest
+    if (kept) {
+        uint32_t t = LP_NONE + 1;
+#pragma unroll
+        for (int k = 0; k < NT / 64; k++) t = max(t, bound[k]);
+        auto each = [&](auto f) {
+#pragma unroll
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int j = 0; j < V; j++) {
+                    const float x = get(r, j);
+                    const uint32_t o = lp_order(x);
+                    if (o >= t && x == x) f(lp_key(o, base + r * NT * V + j));
+                }
+        };
+        if (order >= t)
+            each([&](unsigned long long k) {
+                const int at = atomicAdd(&S.count, 1);
+                if (at < LP_LIST) S.list[at] = k;
+            });
+        lp_rank<NT>(S, kept, each);
+    } else {
+        __syncthreads();
+    }
+    l = red[1][0], h = red[2][0];
+#pragma unroll
+    for (int k = 1; k < NT / 64; k++) l += red[1][k], h += red[2][k];
+    if (A.parts == 1) {
+        lp_finish(A, row, T, m, l, h, S.top, xt, CAP);
+    } else {
+        if (threadIdx.x == 0) A.stats[blockIdx.x] = make_float4(m, l, h, 0.f);
+        if ((int)threadIdx.x < kept) A.keys[(size_t)blockIdx.x * A.kept + threadIdx.x] = S.top[threadIdx.x];
+    }
+}
+
+// A row's parts joined: their sums brought to the largest m, and of their keys those
+// that are not below the largest of the parts' last ones, which bounds the row's
+// last one.
+template <bool F32, bool CAP>
+DEV void lp_join(const LpArgs& A) {
+    constexpr int NT = 256;
+    __shared__ LpTop<NT> S;
+    __shared__ float red[4];
+    __shared__ double sums[2][4];
+    __shared__ unsigned long long bound[4];
+    const int row = blockIdx.x, t = threadIdx.x, w = t >> 6, lane = t & 63;
+    const float4* st = A.stats + (size_t)row * A.parts;
+    const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f;
+    const float xt = lp_token_logit<F32>(A, row);
+    const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
+    const unsigned long long* keys = A.keys + (size_t)row * A.parts * A.kept;
+    float m = -INFINITY;
+    unsigned long long last = 1;
+    for (int p = t; p < A.parts; p += NT) {
+        m = fmaxf(m, st[p].x);
+        if (kept) last = max(last, keys[(size_t)p * A.kept + kept - 1]);
+    }
+    m = wave_max_u(m);
+    last = wave_max_key(last);
+    if (lane == 0) red[w] = m, bound[w] = last;
+    if (t == 0) S.count = 0;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 4; k++) m = fmaxf(m, red[k]), last = max(last, bound[k]);
+    const float c = m == -INFINITY ? 0.f : m, s = sm_scale(1.44269504088896340736f, T > 0.f ? T : 1.f);
+    double L = 0, H = 0;
+    for (int p = t; p < A.parts; p += NT) {
+        const float4 q = st[p];
+        const float z = (q.x - c) * s, a = q.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(z);
+        L += (double)q.y * a;
+        H += a != 0.f ? a * ((double)q.z + (double)q.y * (q.x == -INFINITY ? 0.f : z)) : 0.;
+    }
+    L = lane_d(wave_scan_d(L), 63), H = lane_d(wave_scan_d(H), 63);
+    if (lane == 0) sums[0][w] = L, sums[1][w] = H;
+    if (kept) {
+        auto each = [&](auto f) {
+            for (long long i = t; i < (long long)A.parts * kept; i += NT) {
+                const unsigned long long k = keys[i / kept * A.kept + i % kept];
+                if (k >= last) f(k);
+            }
+        };
+        each([&](unsigned long long k) {
+            const int at = atomicAdd(&S.count, 1);
+            if (at < LP_LIST) S.list[at] = k;
+        });
+        lp_rank<NT>(S, kept, each);
+    } else {
+        __syncthreads();
+    }
+    L = (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]);
+    H = (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3]);
+    lp_finish(A, row, T, m, L, H, S.top, xt, CAP);
+}
+#define LOGPROBS_PART(NAME, F32, CAP, NT, R)                                                              \
+    extern "C" __global__ __launch_bounds__(NT) void cima_logprobs_t##NT##_w##R##_##NAME(const LpArgs A) { \
+        lp_part<F32, CAP, NT, F32 ? R : R / 2, F32 ? 4 : 8>(A);                                            \
+    }
+#define LOGPROBS(NAME, F32, CAP)                                                                          \
+    LOGPROBS_PART(NAME, F32, CAP, 256, 2)                                                                 \
+    LOGPROBS_PART(NAME, F32, CAP, 256, 8)                                                                 \
+    LOGPROBS_PART(NAME, F32, CAP, 1024, 8)                                                                \
+    extern "C" __global__ __launch_bounds__(256) void cima_logprobs_join_##NAME(const LpArgs A) {         \
+        lp_join<F32, CAP>(A);                                                                              \
+    }
+LOGPROBS(f16, false, false)
+LOGPROBS(f32, true, false)
+LOGPROBS(cap_f16, false, true)
+LOGPROBS(cap_f32, true, true)
+
 // ------------------------------------------------------------- verification
 //
 // Which drafts are kept needs one probability of p and q a draft; the token
@@ -371,29 +690,6 @@ DEV void vf_load(const VfRow& r, int i, int n, float (&v)[8]) {
         if (r.q) v[j] -= w[j];
         v[j] = v[j] > 0.f && i + j != r.one ? v[j] : 0.f;
     }
-}
-// v of the lane that a DPP pattern names, 0 where there is none
-template <int CTRL, int ROWS>
-DEV double dpp_d(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (uint32_t)u, CTRL, ROWS, 0xf, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (uint32_t)(u >> 32), CTRL, ROWS, 0xf, false);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
-}
-// inclusive running sum over the wave: within rows of 16, then from row to row
-DEV double wave_scan_d(double v) {
-    v += dpp_d<0x111, 0xf>(v);  // row_shr:1, 2, 4, 8
-    v += dpp_d<0x112, 0xf>(v);
-    v += dpp_d<0x114, 0xf>(v);
-    v += dpp_d<0x118, 0xf>(v);
-    v += dpp_d<0x142, 0xa>(v);  // row_bcast:15 into rows 1, 3
-    v += dpp_d<0x143, 0xc>(v);  // row_bcast:31 into rows 2, 3
-    return v;
-}
-DEV double lane_d(double v, int lane) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = __builtin_amdgcn_readlane((uint32_t)u, lane), hi = __builtin_amdgcn_readlane((uint32_t)(u >> 32), lane);
-    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 // sum of one part by the workgroup
 DEV double vf_part(const VfArgs& A, const VfRow& r, int part) {

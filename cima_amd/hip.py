@@ -44,7 +44,7 @@ EXPORTS = (
     "cima_hip_argmax_to_ids", "cima_hip_pos_bump", "cima_hip_decode_step",
     "cima_hip_rope_append_paged", "cima_hip_attn_paged", "cima_hip_kv_pages_read", "cima_hip_kv_pages_copy", "cima_hip_kv_pages_reserve",
     "cima_hip_kv_pages_fork", "cima_hip_kv_pages_free", "cima_hip_kv_pages_compact", "cima_hip_softmax_rows",
-    "cima_hip_verify_drafts",
+    "cima_hip_logprobs_rows", "cima_hip_verify_drafts",
     "cima_hip_capture_begin", "cima_hip_capture_end", "cima_hip_graph_launch", "cima_hip_graph_destroy",
     "cima_hip_nf4_dequant", "cima_hip_nf4_gemv", "cima_hip_set_nf4_tuning", "cima_hip_nf4_gemm_slab",
     "cima_hip_stream_read", "cima_hip_stream_read_cfg",
@@ -149,6 +149,7 @@ def load_library(path: str = LIBHIP) -> ctypes.CDLL:
     L.cima_hip_kv_pages_free.argtypes = [P, P, P, I]
     L.cima_hip_kv_pages_compact.argtypes = [P, P, P, P, P, P, U]
     L.cima_hip_softmax_rows.argtypes = [P, P, P, I, I, P, I, F, I, P, U]
+    L.cima_hip_logprobs_rows.argtypes = [P, P, I, I, P, P, P, I, P, P, P, I, F, I, P, U]
     L.cima_hip_verify_drafts.argtypes = [P] * 9 + [I, I, I, P, U]
     L.cima_hip_capture_begin.argtypes = [P]
     L.cima_hip_stream_read.argtypes = [P, P, LL, P]
@@ -624,6 +625,21 @@ class HipCtx:
         act, d = _act_of(x), self.device
         self._check(self.lib.cima_hip_softmax_rows(
             self.handle, _ptr_of(x, _F16 if act else _F32, rows * n, "x", d), _ptr_of(y, _F32, rows * n, "y", d), rows, n,
+            _ptr_of(temp, _F32, -(-rows // rows_per_temp), "temp", d), rows_per_temp, cap, act, *self._slab(slab)))
+
+    def logprobs_rows(self, x, rows: int, n: int, tokens=None, logprob=None, entropy=None, n_top: int = 0, top_ids=None,
+                      top_logprobs=None, temp=None, rows_per_temp: int = 1, cap: float = 0.0, slab=None) -> None:
+        """``logprob[r]`` of ``tokens[r]`` by the probabilities that ``softmax_rows``
+        gives of the same logits, the rows' ``entropy``, and the ``n_top`` likeliest
+        tokens with theirs (``top_ids``, ``top_logprobs`` [rows, n_top]); outputs that
+        are None are not written."""
+        if rows_per_temp <= 0:
+            raise EngineError("hip", E_INVALID, f"rows_per_temp is {rows_per_temp}")
+        act, d, k = _act_of(x), self.device, rows * n_top
+        self._check(self.lib.cima_hip_logprobs_rows(
+            self.handle, _ptr_of(x, _F16 if act else _F32, rows * n, "x", d), rows, n, _ptr_of(tokens, _I32, rows, "tokens", d),
+            _ptr_of(logprob, _F32, rows, "logprob", d), _ptr_of(entropy, _F32, rows, "entropy", d), n_top,
+            _ptr_of(top_ids, _I32, k, "top_ids", d), _ptr_of(top_logprobs, _F32, k, "top_logprobs", d),
             _ptr_of(temp, _F32, -(-rows // rows_per_temp), "temp", d), rows_per_temp, cap, act, *self._slab(slab)))
 
     def verify_drafts(self, p, q, drafts, counts, u, accepted, tokens, lens, seqs: int, n_draft: int, vocab: int,

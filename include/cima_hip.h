@@ -554,6 +554,24 @@ int cima_hip_kv_pages_compact(cima_hip_ctx* ctx, const cima_kv_pages* kv, int* r
 int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, int n, const float* temp,
                           int rows_per_temp, float cap, int x_dtype, void* slab, unsigned long long slab_bytes);
 
+/* Log probabilities of tokens by rows of logits, with what is as likely:
+ * logprob[r] = ln p[r][tokens[r]] of the probabilities p that cima_hip_softmax_rows
+ * gives of x, temp, rows_per_temp and cap, entropy[r] = -sum p ln p, and
+ * top_ids, top_logprobs [rows, n_top] the n_top likeliest tokens of a row and their
+ * log probabilities, the largest logit first, equal ones by the lower id.  All fp32.
+ * An id outside [0, n) has -inf, as has a token whose logit is -inf; such tokens are
+ * not among the likeliest, nor is NaN: entries that no token is left for are -1 and
+ * -inf.  A row that softmax_rows makes NaN has NaN for its entropy and its other log
+ * probabilities, one of -inf alone an entropy of 0.  Where temp <= 0 or NaN the largest
+ * logit has 0, all others -inf.
+ * tokens, logprob and entropy may be NULL (not wanted), as top_ids and top_logprobs
+ * with n_top 0; n_top at most 32, less than 2^22 rows.  slab (8-byte aligned): 24 + 8
+ * n_top bytes for each 8192 logits of a row (rounded up) and row; none is needed up to
+ * 32768 logits.  Four times as much makes few rows faster. */
+int cima_hip_logprobs_rows(cima_hip_ctx* ctx, const void* x, int rows, int n, const int* tokens, float* logprob,
+                           float* entropy, int n_top, int* top_ids, float* top_logprobs, const float* temp,
+                           int rows_per_temp, float cap, int x_dtype, void* slab, unsigned long long slab_bytes);
+
 /* Speculative sampling: which drafted tokens the target keeps, and the token
  * that follows, by given uniform numbers.  p f32 [seqs, n_draft + 1, vocab]
  * are the target's probabilities, q f32 [seqs, n_draft, vocab] the draft's
