@@ -74,8 +74,14 @@ struct KvQ {
 
 // ---------------------------------------------------------------- storing
 
-// fp64 -> f16 bits, rounded once (through fp32 it would be rounded twice)
-DEV uint32_t d2h(double v) { return (uint32_t)__builtin_bit_cast(uint16_t, (_Float16)v); }
+// fp64 -> f16 bits, rounded once: an fp32 that is not exact is made odd on the way,
+// and no odd one lies half way between two f16
+DEV uint32_t d2h(double v) {
+    const float f = (float)v;
+    uint32_t u = __builtin_bit_cast(uint32_t, f);
+    if ((double)f != v) u = (u - (fabs((double)f) > fabs(v) ? 1u : 0u)) | 1u;
+    return f2h(__builtin_bit_cast(float, u));
+}
 // max over the four lanes of a quad
 DEV float quad_max(float v) {
     v = fmaxf(v, dpp_xor1(v));
@@ -90,12 +96,17 @@ DEV uint32_t scale_up(double w, float steps) {
         if ((double)(h2f(c) * steps) < w) c++;
     return c;
 }
-// the code nearest to z = (x - m) / d, in 64 bits where fp32 does not tell which
-DEV int code_of(float x, float m, float d, float inv) {
+// the code nearest to (x - m) / d, by exact products in fp64 where the fp32 quotient
+// (off by less than `near`) lies that close to half way
+DEV float code_of(float x, float m, float d, float inv, float near) {
     const float z = (x - m) * inv;
     float r = rintf(z);
-    if (fabsf(z - r) > 0.499f) r = (float)rint(((double)x - (double)m) / (double)d);
-    return (int)r;
+    if (fabsf(z - r) > 0.5f - near) {
+        const float k = floorf(z);
+        const double two = 2. * ((double)x - (double)m), half = (2. * k + 1.) * (double)d;
+        r = two > half || (two == half && ((int)k & 1)) ? k + 1.f : k;
+    }
+    return r;
 }
 // Eight f16 elements of a group that a quad's lanes hold in order: their words, and
 // the group's scales (the same in all four lanes).  A group that is not finite
@@ -118,10 +129,12 @@ DEV uint32_t kv_encode(const uint32_t (&x)[4], uint32_t (&w)[KvQ<BITS>::WORDS]) 
     const float m = BITS == 4 ? lo : 0.f;
     const double width = BITS == 4 ? (double)hi - (double)lo : (double)fmaxf(hi, -lo);
     const uint32_t db = bad ? 0x7e00u : scale_up(width, STEPS);
-    const float d = h2f(db), inv = d > 0.f ? 1.f / d : 0.f;
+    const float d = h2f(db), inv = d > 0.f ? __builtin_amdgcn_rcpf(d) : 0.f;
+    // the quotient's fp32 roundings (the reciprocal's 2^-23) at its largest, 15 or 127
+    constexpr float NEAR = BITS == 4 ? 1e-5f : 1e-4f;
     int c[8];
 #pragma unroll
-    for (int i = 0; i < 8; i++) c[i] = d > 0.f ? code_of(v[i], m, d, inv) : 0;
+    for (int i = 0; i < 8; i++) c[i] = d > 0.f ? (int)code_of(v[i], m, d, inv, NEAR) : 0;
     if constexpr (BITS == 4) {
         w[0] = 0;
 #pragma unroll

@@ -118,11 +118,47 @@ DEV void rope_append_quant_body(const uint16_t* __restrict__ qkv, uint16_t* __re
     const uint16_t* x = qkv + (size_t)row * (q_heads + 2 * kv_heads) * D;
     const bool keep = (unsigned)id < (unsigned)n_pages;
     const int page = 1 << page_shift, r = pos & (page - 1);
-    // eight elements i, ... of head h: words of its page, and the group's scales
-    auto put = [&](uint8_t* plane, int h, int i, const uint32_t (&v)[4]) {
+    for (int e = t; e < q_heads * H8; e += 256) {
+        const int h = e / H8, i = e % H8 * 8;
+        const uint4 a = *reinterpret_cast<const uint4*>(x + (size_t)h * D + i);
+        const uint4 b = *reinterpret_cast<const uint4*>(x + (size_t)h * D + D / 2 + i);
+        const uint32_t au[4] = {a.x, a.y, a.z, a.w}, bu[4] = {b.x, b.y, b.z, b.w};
+        uint32_t oa[4], ob[4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const float a0 = h2f(au[j] & 0xffffu), a1 = h2f(au[j] >> 16);
+            const float b0 = h2f(bu[j] & 0xffffu), b1 = h2f(bu[j] >> 16);
+            const float c0 = cs[i + 2 * j], c1 = cs[i + 2 * j + 1], s0 = sn[i + 2 * j], s1 = sn[i + 2 * j + 1];
+            oa[j] = f2h2(a0 * c0 - b0 * s0, a1 * c1 - b1 * s1);
+            ob[j] = f2h2(a0 * s0 + b0 * c0, a1 * s1 + b1 * c1);
+        }
+        uint16_t* y = q + ((size_t)row * q_heads + h) * D;
+        *reinterpret_cast<uint4*>(y + i) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
+        *reinterpret_cast<uint4*>(y + D / 2 + i) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
+    }
+    if (!keep) return;
+    // keys, then values, eight elements a thread: 8 heads of 128 are one pass
+    for (int e = t; e < 2 * kv_heads * (D / 8); e += 256) {
+        const int h = e / (D / 8), i = e % (D / 8) * 8;
+        const uint16_t* from = x + (size_t)(q_heads + h) * D;
+        const uint4 own = *reinterpret_cast<const uint4*>(from + i);
+        uint32_t v[4] = {own.x, own.y, own.z, own.w};
+        if (h < kv_heads) {
+            const uint4 other = *reinterpret_cast<const uint4*>(from + (i ^ (D / 2)));
+            const uint32_t o[4] = {other.x, other.y, other.z, other.w};
+            const int at = i & (D / 2 - 1);
+            const double sign = i < D / 2 ? -1. : 1.;
+#pragma unroll
+            for (int j = 0; j < 4; j++) {
+                const double a0 = h2f(v[j] & 0xffffu), a1 = h2f(v[j] >> 16);
+                const double b0 = h2f(o[j] & 0xffffu), b1 = h2f(o[j] >> 16);
+                v[j] = d2h(fma(a0, cd[at + 2 * j], sign * b0 * sd[at + 2 * j])) |
+                       d2h(fma(a1, cd[at + 2 * j + 1], sign * b1 * sd[at + 2 * j + 1])) << 16;
+            }
+        }
         uint32_t w[Q::WORDS];
         const uint32_t sc = kv_encode<BITS>(v, w);
-        uint8_t* head = plane + ((size_t)id * kv_heads + h) * page * Q::row(D);
+        uint8_t* head = (h < kv_heads ? kp : vp) + ((size_t)id * kv_heads + (h < kv_heads ? h : h - kv_heads)) * page * Q::row(D);
         uint32_t* c = reinterpret_cast<uint32_t*>(head + r * Q::codes(D) + i * BITS / 8);
 #pragma unroll
         for (int k = 0; k < Q::WORDS; k++) c[k] = w[k];
@@ -131,46 +167,6 @@ DEV void rope_append_quant_body(const uint16_t* __restrict__ qkv, uint16_t* __re
             if constexpr (BITS == 4) *reinterpret_cast<uint32_t*>(z) = sc;
             else *reinterpret_cast<uint16_t*>(z) = (uint16_t)sc;
         }
-    };
-    for (int e = t; e < (q_heads + kv_heads) * H8; e += 256) {
-        const int h = e / H8, i = e % H8 * 8;
-        if (h >= q_heads && !keep) continue;
-        const uint4 a = *reinterpret_cast<const uint4*>(x + (size_t)h * D + i);
-        const uint4 b = *reinterpret_cast<const uint4*>(x + (size_t)h * D + D / 2 + i);
-        const uint32_t au[4] = {a.x, a.y, a.z, a.w}, bu[4] = {b.x, b.y, b.z, b.w};
-        uint32_t oa[4], ob[4];
-        if (h < q_heads) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const float a0 = h2f(au[j] & 0xffffu), a1 = h2f(au[j] >> 16);
-                const float b0 = h2f(bu[j] & 0xffffu), b1 = h2f(bu[j] >> 16);
-                const float c0 = cs[i + 2 * j], c1 = cs[i + 2 * j + 1], s0 = sn[i + 2 * j], s1 = sn[i + 2 * j + 1];
-                oa[j] = f2h2(a0 * c0 - b0 * s0, a1 * c1 - b1 * s1);
-                ob[j] = f2h2(a0 * s0 + b0 * c0, a1 * s1 + b1 * c1);
-            }
-            uint16_t* y = q + ((size_t)row * q_heads + h) * D;
-            *reinterpret_cast<uint4*>(y + i) = make_uint4(oa[0], oa[1], oa[2], oa[3]);
-            *reinterpret_cast<uint4*>(y + D / 2 + i) = make_uint4(ob[0], ob[1], ob[2], ob[3]);
-            continue;
-        }
-#pragma unroll
-        for (int j = 0; j < 8; j++) {
-            const uint32_t sh = j & 1 ? 16 : 0;
-            const double p = h2f(au[j / 2] >> sh & 0xffffu), z = h2f(bu[j / 2] >> sh & 0xffffu);
-            const double c = cd[i + j], n = sd[i + j];
-            const uint32_t lo = d2h(fma(p, c, -(z * n))), hi = d2h(fma(p, n, z * c));
-            oa[j / 2] = j & 1 ? oa[j / 2] | lo << 16 : lo;
-            ob[j / 2] = j & 1 ? ob[j / 2] | hi << 16 : hi;
-        }
-        put(kp, h - q_heads, i, oa);
-        put(kp, h - q_heads, D / 2 + i, ob);
-    }
-    if (!keep) return;
-    for (int e = t; e < kv_heads * (D / 8); e += 256) {
-        const int h = e / (D / 8), i = e % (D / 8) * 8;
-        const uint4 a = *reinterpret_cast<const uint4*>(x + (size_t)(q_heads + kv_heads + h) * D + i);
-        const uint32_t au[4] = {a.x, a.y, a.z, a.w};
-        put(vp, h, i, au);
     }
 }
 #define ROPE_APPEND_QUANT(D, BITS)                                                                                   \

@@ -65,6 +65,17 @@ DEV float sm_scale(float c, float T) { return fminf(fmaxf(c / T, 1e-37f), 1e38f)
 // share.
 DEV float sm_f(float x, float cap) { return __builtin_isinf(x) ? x : cap * tanhf(x / cap); }
 
+// a logit of a pair less c: of f16 logits as x * 1 - c, one instruction with the
+// conversion, the same number
+DEV float mix_less(uint32_t pair, bool high, float c) {
+    float d;
+    if (high)
+        __asm__("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(pair), "v"(c));
+    else
+        __asm__("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(pair), "v"(c));
+    return d;
+}
+
 // R words of V logits a thread of a row by NT threads: the maximum, the first place of it
 // (T <= 0) or the sum (T > 0).  CAP: f is applied when the logits are loaded,
 // which are fp32 from there on.
@@ -77,16 +88,9 @@ struct SmRow {
     int at;
 
     DEV float get(int r, int j) const { return sm_get<W32, V>(v[r], j); }
-    // a logit less c: of f16 logits as x * 1 - c, one instruction with the
-    // conversion, the same number
     DEV float less(int r, int j, float c) const {
         if constexpr (W32) return get(r, j) - c;
-        float d;
-        if (j & 1)
-            __asm__("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(v[r][j / 2]), "v"(c));
-        else
-            __asm__("v_fma_mix_f32 %0, %1, 1.0, -%2 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(v[r][j / 2]), "v"(c));
-        return d;
+        else return mix_less(v[r][j / 2], j & 1, c);
     }
     // keeps the compiler from holding all logits as fp32 from one pass to the next
     DEV void fresh() {
@@ -355,14 +359,28 @@ template <int NT, typename E>
 DEV void lp_rank(LpTop<NT>& S, int kept, E each) {
     __syncthreads();
     const int count = S.count;
-    if (count <= LP_LIST) {
+    if (count <= 64) {  // a lane each: no loads from list to list
+        if (threadIdx.x < 64) {
+            const unsigned long long k = (int)threadIdx.x < count ? S.list[threadIdx.x] : 0;
+            const uint32_t lo = (uint32_t)k, hi = (uint32_t)(k >> 32);
+            int rank = 0;
+            for (int j = 0; j < count; j++) {
+                const uint32_t a = __builtin_amdgcn_readlane(lo, j), b = __builtin_amdgcn_readlane(hi, j);
+                rank += ((unsigned long long)b << 32 | a) > k;
+            }
+            if ((int)threadIdx.x < count) {
+                if (rank < kept) S.top[rank] = k;
+            } else if ((int)threadIdx.x < kept) {
+                S.top[threadIdx.x] = 0;
+            }
+        }
+    } else if (count <= LP_LIST) {
         for (int i = threadIdx.x; i < count; i += NT) {
             const unsigned long long k = S.list[i];
             int rank = 0;
             for (int j = 0; j < count; j++) rank += S.list[j] > k;
             if (rank < kept) S.top[rank] = k;
         }
-        if ((int)threadIdx.x >= count && (int)threadIdx.x < kept) S.top[threadIdx.x] = 0;
     } else {  // more equal logits than the list holds: one after the other
         unsigned long long last = ~0ull;
         for (int i = 0; i < kept; i++) {
@@ -419,8 +437,9 @@ template <bool F32, bool CAP, int NT, int R, int V>
 DEV void lp_part(const LpArgs& A) {
     __shared__ LpTop<NT> S;
     __shared__ float red[3][NT / 64];
-    __shared__ uint32_t bound[NT / 64];
+    __shared__ uint32_t bound[2][NT / 64];
     constexpr int W = F32 ? V : V / 2;
+    static_assert(R * V == 32 || R * V == 8, "a bit for each logit of a thread");
     const int row = blockIdx.x / A.parts, part = blockIdx.x % A.parts, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
     const int base = part * NT * R * V + threadIdx.x * V;
     uint32_t v[R][W];
@@ -429,6 +448,12 @@ DEV void lp_part(const LpArgs& A) {
     const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f;
     const float xt = lp_token_logit<F32>(A, row);
     auto get = [&](int r, int j) { return sm_get<F32, V>(v[r], j); };
+    // f of a logit less c (SmRow::less)
+    auto less = [&](int r, int j, float c) {
+        if constexpr (CAP) return sm_f(get(r, j), A.cap) - c;
+        else if constexpr (F32) return get(r, j) - c;
+        else return mix_less(v[r][j / 2], j & 1, c);
+    };
     // ---- the thread's and the part's largest
     float mine = -INFINITY;
     if constexpr (F32) {
@@ -450,15 +475,21 @@ DEV void lp_part(const LpArgs& A) {
     const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
     const uint32_t order = lp_order(mine);
     if (kept) {
-        // the kept-th largest of the lanes' or less, by its bits from the highest on
+        // the need-th largest of the lanes' or less, by its bits from the highest on
         // (f16 logits have no more than 19)
-        uint32_t t = 0;
-        for (int b = 31; b >= (F32 ? 0 : 13); b--) {
-            const int c = __popcll(__ballot(order >= (t | 1u << b)));
-            if (c >= kept) t |= 1u << b;
-            if (c == kept) break;
-        }
-        if (lane == 0) bound[w] = t;
+        auto nth = [&](int need) {
+            uint32_t t = 0;
+            for (int b = 31; b >= (F32 ? 0 : 13); b--) {
+                const int c = __popcll(__ballot(order >= (t | 1u << b)));
+                if (c >= need) t |= 1u << b;
+                if (c == need) break;
+            }
+            return t;
+        };
+        // `kept` logits are not below any wave's kept-th, nor below the least of the
+        // waves' (kept / waves)-th, which is the higher where the waves are alike
+        const uint32_t a = nth(kept), b = nth((kept + NT / 64 - 1) / (NT / 64));
+        if (lane == 0) bound[0][w] = a, bound[1][w] = b;
     }
     if (threadIdx.x == 0) S.count = 0;
     __syncthreads();
@@ -473,8 +504,7 @@ DEV void lp_part(const LpArgs& A) {
         float pl = 0.f, ph = 0.f;
 #pragma unroll
         for (int j = 0; j < V; j++) {
-            const float x = get(r, j), z = ((CAP ? sm_f(x, A.cap) : x) - c) * s;
-            const float e = __builtin_amdgcn_exp2f(z);
+            const float z = less(r, j, c) * s, e = __builtin_amdgcn_exp2f(z);
             pl += e;
             ph = fmaf(e, fmaxf(z, -1e30f), ph);
         }
@@ -484,24 +514,34 @@ DEV void lp_part(const LpArgs& A) {
     if (lane == 0) red[1][w] = l, red[2][w] = h;
     // ---- the part's likeliest
     if (kept) {
-        uint32_t t = LP_NONE + 1;
+        uint32_t t = LP_NONE + 1, all = 0xffffffffu;
 #pragma unroll
-        for (int k = 0; k < NT / 64; k++) t = max(t, bound[k]);
-        auto each = [&](auto f) {
+        for (int k = 0; k < NT / 64; k++) t = max(t, bound[0][k]), all = min(all, bound[1][k]);
+        t = max(t, all);
+        const float least = lp_value((unsigned long long)t << 32);  // or NaN: more than any logit
+        // which of the thread's logits are not below the bound, then those few from
+        // memory once more
+        uint32_t some = 0;
+        if (order >= t) {
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float x = get(r, j);
-                    const uint32_t o = lp_order(x);
-                    if (o >= t && x == x) f(lp_key(o, base + r * NT * V + j));
-                }
+                for (int j = 0; j < V; j++) some |= get(r, j) >= least ? 1u << (r * V + j) : 0u;
+        }
+        auto each = [&](auto f) {
+            for (uint32_t left = some; left; left &= left - 1) {
+                const int i = __ffs(left) - 1, at = base + i / V * NT * V + i % V;
+                const size_t e = (size_t)row * A.n + at;
+                float x;
+                if constexpr (F32) x = ((const float*)A.x)[e];
+                else x = h2f(((const uint16_t*)A.x)[e]);
+                f(lp_key(lp_order(x), at));
+            }
         };
-        if (order >= t)
-            each([&](unsigned long long k) {
-                const int at = atomicAdd(&S.count, 1);
-                if (at < LP_LIST) S.list[at] = k;
-            });
+        each([&](unsigned long long k) {
+            const int at = atomicAdd(&S.count, 1);
+            if (at < LP_LIST) S.list[at] = k;
+        });
         lp_rank<NT>(S, kept, each);
     } else {
         __syncthreads();
@@ -513,7 +553,7 @@ DEV void lp_part(const LpArgs& A) {
         lp_finish(A, row, T, m, l, h, S.top, xt, CAP);
     } else {
         if (threadIdx.x == 0) A.stats[blockIdx.x] = make_float4(m, l, h, 0.f);
-        if ((int)threadIdx.x < kept) A.keys[(size_t)blockIdx.x * A.kept + threadIdx.x] = S.top[threadIdx.x];
+        if ((int)threadIdx.x < kept) A.keys[(size_t)blockIdx.x * kept + threadIdx.x] = S.top[threadIdx.x];
     }
 }
 
@@ -532,13 +572,23 @@ DEV void lp_join(const LpArgs& A) {
     const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f;
     const float xt = lp_token_logit<F32>(A, row);
     const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
-    const unsigned long long* keys = A.keys + (size_t)row * A.parts * A.kept;
+    const unsigned long long* keys = A.keys + (size_t)row * A.parts * kept;
+    // the first of a thread's stats and keys are fetched together
+    constexpr int U = 4;
+    const long long many = (long long)A.parts * kept;
+    const float4 mine = st[min(t, A.parts - 1)];
+    unsigned long long key[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) key[u] = t + u * NT < many ? keys[t + u * NT] : 0;
     float m = -INFINITY;
     unsigned long long last = 1;
-    for (int p = t; p < A.parts; p += NT) {
-        m = fmaxf(m, st[p].x);
-        if (kept) last = max(last, keys[(size_t)p * A.kept + kept - 1]);
-    }
+    for (int p = t; p < A.parts; p += NT) m = fmaxf(m, p == t ? mine.x : st[p].x);
+    // a key at a part's end
+#pragma unroll
+    for (int u = 0; u < U; u++)
+        if (t + u * NT < many && (t + u * NT) % kept == kept - 1) last = max(last, key[u]);
+    for (long long i = t + U * NT; i < many; i += NT)
+        if (i % kept == kept - 1) last = max(last, keys[i]);
     m = wave_max_u(m);
     last = wave_max_key(last);
     if (lane == 0) red[w] = m, bound[w] = last;
@@ -549,7 +599,7 @@ DEV void lp_join(const LpArgs& A) {
     const float c = m == -INFINITY ? 0.f : m, s = sm_scale(1.44269504088896340736f, T > 0.f ? T : 1.f);
     double L = 0, H = 0;
     for (int p = t; p < A.parts; p += NT) {
-        const float4 q = st[p];
+        const float4 q = p == t ? mine : st[p];
         const float z = (q.x - c) * s, a = q.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(z);
         L += (double)q.y * a;
         H += a != 0.f ? a * ((double)q.z + (double)q.y * (q.x == -INFINITY ? 0.f : z)) : 0.;
@@ -558,8 +608,11 @@ DEV void lp_join(const LpArgs& A) {
     if (lane == 0) sums[0][w] = L, sums[1][w] = H;
     if (kept) {
         auto each = [&](auto f) {
-            for (long long i = t; i < (long long)A.parts * kept; i += NT) {
-                const unsigned long long k = keys[i / kept * A.kept + i % kept];
+#pragma unroll
+            for (int u = 0; u < U; u++)
+                if (key[u] >= last) f(key[u]);
+            for (long long i = t + U * NT; i < many; i += NT) {
+                const unsigned long long k = keys[i];
                 if (k >= last) f(k);
             }
         };
