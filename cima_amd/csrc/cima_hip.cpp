@@ -678,7 +678,7 @@ int cima_hip_init(int device, const char* code_dir, cima_hip_ctx** out) {
         for (const char* kn : {"stats_w2", "probs_w2", "stats_w8", "probs_w8", "t256_w2", "t256_w8", "t1024_w8"})
             if (!rc) rc = add(MOD_SAMPLE, std::string("cima_softmax_") + kn + "_" + t);
     for (const char* t : kSampleTypes)
-        for (const char* kn : {"t256_w2", "t256_w8", "t1024_w8", "join"})
+        for (const char* kn : {"t256_w2", "t256_w8", "t1024_w8", "part_w2", "part_w8", "join_w2", "join_w8"})
             if (!rc) rc = add(MOD_SAMPLE, std::string("cima_logprobs_") + kn + "_" + t);
     if (rc) {
         unload(ctx);
@@ -2014,8 +2014,8 @@ struct LogprobsArgs {
     float* top_logprobs;
     const float* temp;
     float* stats;
-    unsigned long long* keys;
-    int n, n_top, kept, rows_per_temp, parts;
+    void* largest;
+    int n, n_top, rows_per_temp, parts, chunk_shift;
     float cap;
 };
 
@@ -2092,8 +2092,8 @@ int cima_hip_logprobs_rows(cima_hip_ctx* ctx, const void* x, int rows, int n, co
     const bool f32 = x_dtype == CIMA_DT_F32;
     const char* sfx = kSampleTypes[(cap > 0.f ? 2 : 0) + (f32 ? 1 : 0)];
     char name[64];
-    LogprobsArgs A{x, tokens, logprob, entropy, top_ids, top_logprobs, temp, nullptr, nullptr, n, n_top, std::max(n_top, 1),
-                   rows_per_temp, 1, cap};
+    LogprobsArgs A{x, tokens, logprob, entropy, top_ids, top_logprobs, temp, nullptr, nullptr, n, n_top, rows_per_temp, 1, 0,
+                   cap};
     void* args[] = {&A};
     // rows that a workgroup holds, and rows in parts, as in cima_hip_softmax_rows
     static const int shapes[][2] = {{256, 2}, {256, 8}, {1024, 8}};
@@ -2103,19 +2103,24 @@ int cima_hip_logprobs_rows(cima_hip_ctx* ctx, const void* x, int rows, int n, co
             return launch_named(ctx, name, (unsigned)rows, (unsigned)sh[0], args, api);
         }
     const auto parts_of = [&](int words) { return (n - 1) / (kSoftmaxWord * words) + 1; };
-    const unsigned long long each = 16 + 8ULL * A.kept;
+    // bytes of a chunk's sums and of its groups' largest logits, 256 of 8192 logits or
+    // 64 of 2048
+    const auto bytes_of = [&](int words) { return 16ULL + (words == 2 ? 64 : 256) * (f32 ? 4ULL : 2ULL); };
+    const auto need_of = [&](int words) { return (unsigned long long)rows * parts_of(words) * bytes_of(words); };
     int words = 8;
-    if ((long long)rows * parts_of(2) <= 4LL * ctx->num_cu && slab_bytes >= each * rows * parts_of(2)) words = 2;
-    A.parts = parts_of(words);
-    const long long all = (long long)rows * A.parts;
-    if (all > kMaxGrid || !slab || !aligned(slab, 8) || slab_bytes < each * all)
-        return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (8 B)", api,
-                    slab_bytes, each * all);
-    A.keys = (unsigned long long*)slab;
-    A.stats = (float*)slab + 2 * A.kept * all;
-    snprintf(name, sizeof name, "cima_logprobs_t256_w%d_%s", words, sfx);
-    if (int rc = launch_named(ctx, name, (unsigned)all, 256, args, api)) return rc;
-    snprintf(name, sizeof name, "cima_logprobs_join_%s", sfx);
+    if ((long long)rows * parts_of(2) <= 4LL * ctx->num_cu && slab_bytes >= need_of(2)) words = 2;
+    const long long chunks = (long long)rows * parts_of(words);
+    if (chunks > kMaxGrid || !slab || !aligned(slab, 16) || slab_bytes < need_of(words))
+        return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (16 B)", api,
+                    slab_bytes, need_of(words));
+    static int sh = getenv("LPSH") ? atoi(getenv("LPSH")) : 0;
+    A.chunk_shift = words == 8 ? sh : 0;
+    A.parts = ((parts_of(words) - 1) >> A.chunk_shift) + 1;
+    A.stats = (float*)slab;
+    A.largest = (char*)slab + 16 * chunks;
+    snprintf(name, sizeof name, "cima_logprobs_part_w%d_%s", words, sfx);
+    if (int rc = launch_named(ctx, name, (unsigned)(rows * A.parts), 256, args, api)) return rc;
+    snprintf(name, sizeof name, "cima_logprobs_join_w%d_%s", words, sfx);
     return launch_named(ctx, name, (unsigned)rows, 256, args, api);
 }
 

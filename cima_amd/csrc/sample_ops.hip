@@ -4,6 +4,8 @@
 // verification of drafted tokens.
 #include "gguf_formats.h"
 
+#include <type_traits>
+
 // ------------------------------------------------------------------ softmax
 //
 // A row's logits are read into registers: the maximum first, then the sum of
@@ -303,15 +305,20 @@ DEV double lane_d(double v, int lane) {
 // ------------------------------------------------------- log probabilities
 //
 // With z = (f(x) - m) / T and L = sum e^z over a row: a token's log probability is z -
-// ln L, the row's entropy ln L - sum e^z z / L.  One reading: a part's logits stay in
-// registers, first their largest, then the two sums.  The likeliest n_top of a part
-// are found from the threads' largest: each wave takes the n_top-th largest of its
-// lanes', which bounds the row's n_top-th from below, and the highest of these bounds
-// leaves the few logits that are looked at one by one, ranked by counting (value
-// first, then the lower id).  A second launch joins rows of several parts.  Parts
-// as in the softmax above; sums of parts are joined in fp64.
-constexpr int LP_TOP = 32;    // most alternatives
+// ln L, the row's entropy ln L - sum e^z z / L.  One reading of the logits, each thread
+// to its own running maximum and sums.  The likeliest n_top are found from the
+// largest logits of groups of 32 (a thread's, in a row of one workgroup): each wave
+// takes the (n_top / waves)-th largest of its lanes', so that the least of these
+// bounds the row's n_top-th from below, and what the few groups that reach it hold is
+// looked at one by one and ranked by counting (value first, then the lower id).
+// Rows up to 32768 logits go to a workgroup each, in one launch; of longer ones the
+// parts leave their sums and groups' largest, and a second launch joins them (in
+// fp64) and finds the likeliest: looked for in each part they took as long as the
+// sums did.
+
+constexpr int LP_TOP = 32;     // most alternatives
 constexpr int LP_LIST = 1024;  // logits looked at one by one
+constexpr int LP_GROUPS = 256;
 
 struct LpArgs {
     const void* x;
@@ -321,9 +328,9 @@ struct LpArgs {
     int* top_ids;
     float* top_logprobs;
     const float* temp;
-    float4* stats;                // [rows][parts]: m, l, sum of e^z z in log2's unit
-    unsigned long long* keys;     // [rows][parts][kept]
-    int n, n_top, kept, rows_per_temp, parts;  // kept: keys of a part, n_top or 1
+    float4* stats;  // [rows][parts]: m, l, sum of e^z z in log2's unit
+    void* largest;  // [rows][parts][groups of a part], f32 or f16 as the logits
+    int n, n_top, rows_per_temp, parts, chunk_shift;  // 2^chunk_shift chunks a part
     float cap;
 };
 
@@ -332,32 +339,25 @@ DEV uint32_t lp_order(float v) {
     const uint32_t u = __builtin_bit_cast(uint32_t, v + 0.f);
     return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
-DEV float lp_value(unsigned long long key) {
-    const uint32_t u = (uint32_t)(key >> 32);
-    return __builtin_bit_cast(float, u ^ (u >> 31 ? 0x80000000u : 0xffffffffu));
+DEV float lp_value(uint32_t order) {
+    return __builtin_bit_cast(float, order ^ (order >> 31 ? 0x80000000u : 0xffffffffu));
 }
 constexpr uint32_t LP_NONE = 0x007fffffu;  // of -inf: a token that may not be taken
 DEV unsigned long long lp_key(uint32_t order, int at) { return (unsigned long long)order << 32 | (uint32_t)~at; }
 DEV int lp_id(unsigned long long key) { return (int)~(uint32_t)key; }
+DEV int lanes_below(unsigned long long m) { return __popcll(m & ((1ull << (threadIdx.x & 63)) - 1)); }
 
-DEV unsigned long long wave_max_key(unsigned long long v) {
-#pragma unroll
-    for (int o = 32; o; o >>= 1) {
-        const unsigned long long w = __shfl_xor(v, o);
-        v = w > v ? w : v;
-    }
-    return v;
-}
 template <int NT>
 struct LpTop {  // shared between the threads of a workgroup
-    unsigned long long list[LP_LIST], top[LP_TOP], best[NT / 64];
-    int count;
+    unsigned long long list[LP_LIST + 8], top[LP_TOP];
+    int group[LP_GROUPS];
+    int count, groups, found[2][NT / 64], bits[32];
+    uint32_t bound[2][NT / 64];
 };
-// the `kept` largest of the listed keys to S.top in order, zeros behind them;
-// each(f) calls f with every key of this thread, for lists that are too short
-template <int NT, typename E>
-DEV void lp_rank(LpTop<NT>& S, int kept, E each) {
-    __syncthreads();
+// the `kept` largest of the listed keys to S.top in order, zeros behind them, while
+// the second wave does something else
+template <int NT, typename B>
+DEV void lp_rank(LpTop<NT>& S, int kept, B beside) {
     const int count = S.count;
     if (count <= 64) {  // a lane each: no loads from list to list
         if (threadIdx.x < 64) {
@@ -373,36 +373,137 @@ DEV void lp_rank(LpTop<NT>& S, int kept, E each) {
             } else if ((int)threadIdx.x < kept) {
                 S.top[threadIdx.x] = 0;
             }
+        } else if (threadIdx.x < 128) {
+            beside();
         }
-    } else if (count <= LP_LIST) {
+    } else {
+        if (threadIdx.x >= 64 && threadIdx.x < 128) beside();
+        if (threadIdx.x < 7) S.list[count + threadIdx.x] = 0;
+        __syncthreads();
         for (int i = threadIdx.x; i < count; i += NT) {
             const unsigned long long k = S.list[i];
             int rank = 0;
-            for (int j = 0; j < count; j++) rank += S.list[j] > k;
-            if (rank < kept) S.top[rank] = k;
-        }
-    } else {  // more equal logits than the list holds: one after the other
-        unsigned long long last = ~0ull;
-        for (int i = 0; i < kept; i++) {
-            unsigned long long b = 0;
-            each([&](unsigned long long k) { b = k < last && k > b ? k : b; });
-            b = wave_max_key(b);
-            __syncthreads();
-            if ((threadIdx.x & 63) == 0) S.best[threadIdx.x >> 6] = b;
-            __syncthreads();
+            for (int j = 0; j < count; j += 8)
 #pragma unroll
-            for (int w = 0; w < NT / 64; w++) b = S.best[w] > b ? S.best[w] : b;
-            if (threadIdx.x == 0) S.top[i] = b;
-            last = b;
-            if (!b) last = 0;
+                for (int u = 0; u < 8; u++) rank += S.list[j + u] > k;
+            if (rank < kept) S.top[rank] = k;
         }
     }
     __syncthreads();
 }
-// a row's results: largest f(x) m, sums L and H as in LpArgs, the best keys in top
-DEV void lp_finish(const LpArgs& A, int row, float T, float m, double L, double H, const unsigned long long* top, float xt,
-                   bool cap) {
-    const double ln = log(L);
+// The row's `kept` likeliest to S.top.  each_group(f): f(order of the largest, group)
+// for every group of this thread; index(g, e): the row's place of logit e of ONE of
+// group g; load(i): logit i of the row's n, -inf behind them; beside(): something
+// that the second wave has to do once.
+template <int NT, int ONE, typename G, typename I, typename L, typename B>
+DEV void lp_select(LpTop<NT>& S, int kept, int n, bool f32, G each_group, I index, L load, B beside) {
+    const int t = threadIdx.x, w = t >> 6, lane = t & 63;
+    uint32_t best = 0;
+    each_group([&](uint32_t o, int) { best = max(best, o); });
+    // the need-th largest of the lanes' or less, by its bits from the highest on (f16
+    // logits have no more than 19)
+    auto nth = [&](int need) {
+        uint32_t v = 0;
+        for (int b = 31; b >= (f32 ? 0 : 13); b--) {
+            const int c = __popcll(__ballot(best >= (v | 1u << b)));
+            if (c >= need) v |= 1u << b;
+            if (c == need) break;
+        }
+        return v;
+    };
+    uint32_t v = nth((kept + NT / 64 - 1) / (NT / 64));
+    if (lane == 0) S.bound[0][w] = v;
+    if (t == 0) S.count = S.groups = 0;
+    if (t < 32) S.bits[t] = 0;
+    __syncthreads();
+    v = 0xffffffffu;
+#pragma unroll
+    for (int k = 0; k < NT / 64; k++) v = min(v, S.bound[0][k]);
+    if (v <= LP_NONE) {  // a wave with few logits, or of tokens that may not be taken: any wave's kept-th
+        const uint32_t b = nth(kept);
+        if (lane == 0) S.bound[1][w] = b;
+        __syncthreads();
+        v = LP_NONE + 1;
+#pragma unroll
+        for (int k = 0; k < NT / 64; k++) v = max(v, S.bound[1][k]);
+    }
+    // logits of the groups whose largest is not below `least` that are not below it
+    // themselves to S.list (after a barrier), as far as there is room
+    auto look = [&](uint32_t least) {
+        if (best >= least) {
+            int mine = 0;
+            each_group([&](uint32_t o, int) { mine += o >= least; });
+            int to = atomicAdd(&S.groups, mine);
+            each_group([&](uint32_t o, int g) {
+                if (o >= least && to < LP_GROUPS) S.group[to++] = g;
+            });
+        }
+        __syncthreads();
+        const int many = min(S.groups, LP_GROUPS) * ONE;
+        constexpr int U = 4;
+        for (int i0 = 0; i0 < many; i0 += NT * U) {
+            int at[U];
+            float x[U];
+#pragma unroll
+            for (int u = 0; u < U; u++) {
+                const int i = i0 + NT * u + t;
+                at[u] = i < many ? index(S.group[i / ONE], i % ONE) : 0;
+                x[u] = i < many ? load(at[u]) : -INFINITY;
+            }
+            // a number's order is that of what is not less
+            int mine = 0;
+#pragma unroll
+            for (int u = 0; u < U; u++) mine += x[u] >= lp_value(least);
+            if (mine) {
+                int to = atomicAdd(&S.count, mine);
+#pragma unroll
+                for (int u = 0; u < U; u++)
+                    if (x[u] >= lp_value(least) && to < LP_LIST) S.list[to++] = lp_key(lp_order(x[u]), at[u]);
+            }
+        }
+        __syncthreads();
+    };
+    look(v);
+    if (S.groups <= LP_GROUPS && S.count <= LP_LIST) {
+        lp_rank<NT>(S, kept, beside);
+        return;
+    }
+    // Too many, such as equal ones: v = the kept-th largest of the groups' exactly.
+    // What is above it lies in less than `kept` groups; of its equals the first follow.
+    v = 0;
+    for (int b = 31; b >= 0; b--) {
+        int c = 0;
+        each_group([&](uint32_t o, int) { c += o >= (v | 1u << b); });
+        if (c) atomicAdd(&S.bits[b], c);
+        __syncthreads();
+        if (S.bits[b] >= kept) v |= 1u << b;
+    }
+    v = max(v, LP_NONE);
+    if (t == 0) S.count = S.groups = 0;
+    __syncthreads();
+    look(v + 1);
+    lp_rank<NT>(S, kept, beside);
+    int have = min(S.count, kept);
+    for (int i0 = 0, k = 0; i0 < n && have < kept && v > LP_NONE; i0 += NT, k ^= 1) {
+        const float x = load(i0 + t);
+        const unsigned long long hit = __ballot(lp_order(x) == v);
+        if (lane == 0) S.found[k][w] = __popcll(hit);
+        __syncthreads();
+        int to = have + lanes_below(hit), all = 0;
+#pragma unroll
+        for (int u = 0; u < NT / 64; u++) {
+            if (u < w) to += S.found[k][u];
+            all += S.found[k][u];
+        }
+        if (lp_order(x) == v && to < kept) S.top[to] = lp_key(v, i0 + t);
+        have += all;
+    }
+    __syncthreads();
+}
+// a row's results: largest f(x) m, sums L (and its logarithm) and H as in LpArgs, the
+// best keys in top
+DEV void lp_finish(const LpArgs& A, int row, float T, float m, double ln, double L, double H,
+                   const unsigned long long* top, float xt, bool cap) {
     auto logprob = [&](float x) -> float {
         if (x == -INFINITY) return -INFINITY;
         const float f = cap ? sm_f(x, A.cap) : x;
@@ -420,225 +521,253 @@ DEV void lp_finish(const LpArgs& A, int row, float T, float m, double L, double 
     if (t < A.n_top) {
         const unsigned long long k = top[t];
         A.top_ids[(size_t)row * A.n_top + t] = k ? lp_id(k) : -1;
-        A.top_logprobs[(size_t)row * A.n_top + t] = !k ? -INFINITY : one ? (t ? -INFINITY : 0.f) : logprob(lp_value(k));
+        A.top_logprobs[(size_t)row * A.n_top + t] =
+            !k ? -INFINITY : one ? (t ? -INFINITY : 0.f) : logprob(lp_value((uint32_t)(k >> 32)));
     }
 }
 template <bool F32>
-DEV float lp_token_logit(const LpArgs& A, int row) {
-    const int id = A.tokens ? A.tokens[row] : -1;
-    if ((unsigned)id >= (unsigned)A.n) return -INFINITY;
-    const size_t at = (size_t)row * A.n + id;
-    if constexpr (F32) return ((const float*)A.x)[at];
-    else return h2f(((const uint16_t*)A.x)[at]);
+DEV float lp_load(const LpArgs& A, size_t row0, int i) {
+    if ((unsigned)i >= (unsigned)A.n) return -INFINITY;
+    if constexpr (F32) return ((const float*)A.x)[row0 + i];
+    else return h2f(((const uint16_t*)A.x)[row0 + i]);
 }
 
-// R words of V logits a thread
-template <bool F32, bool CAP, int NT, int R, int V>
-DEV void lp_part(const LpArgs& A) {
-    __shared__ LpTop<NT> S;
-    __shared__ float red[3][NT / 64];
-    __shared__ uint32_t bound[2][NT / 64];
-    constexpr int W = F32 ? V : V / 2;
-    static_assert(R * V == 32 || R * V == 8, "a bit for each logit of a thread");
-    const int row = blockIdx.x / A.parts, part = blockIdx.x % A.parts, w = threadIdx.x >> 6, lane = threadIdx.x & 63;
-    const int base = part * NT * R * V + threadIdx.x * V;
+// A thread's running sums: R words of V logits at a time.
+template <bool F32, bool CAP, int R, int V>
+struct LpSums {
+    static constexpr int W = F32 ? V : V / 2;
     uint32_t v[R][W];
-#pragma unroll
-    for (int r = 0; r < R; r++) sm_load<F32, V>(A.x, (size_t)row * A.n, base + r * NT * V, A.n, v[r]);
-    const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f;
-    const float xt = lp_token_logit<F32>(A, row);
-    auto get = [&](int r, int j) { return sm_get<F32, V>(v[r], j); };
+    float mine = -INFINITY, c = 0.f, l = 0.f, h = 0.f;  // the largest, f of it (0: none), the sums
+
+    DEV float get(int r, int j) const { return sm_get<F32, V>(v[r], j); }
     // f of a logit less c (SmRow::less)
-    auto less = [&](int r, int j, float c) {
-        if constexpr (CAP) return sm_f(get(r, j), A.cap) - c;
+    DEV float less(int r, int j, float cap) const {
+        if constexpr (CAP) return sm_f(get(r, j), cap) - c;
         else if constexpr (F32) return get(r, j) - c;
         else return mix_less(v[r][j / 2], j & 1, c);
-    };
-    // ---- the thread's and the part's largest
-    float mine = -INFINITY;
-    if constexpr (F32) {
-#pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int j = 0; j < V; j++) mine = fmaxf(mine, get(r, j));
-    } else {
-        typedef _Float16 hp __attribute__((ext_vector_type(2)));
-        hp h = {(_Float16)-INFINITY, (_Float16)-INFINITY};
-#pragma unroll
-        for (int r = 0; r < R; r++)
-#pragma unroll
-            for (int k = 0; k < W; k++) h = __builtin_elementwise_max(h, __builtin_bit_cast(hp, v[r][k]));
-        mine = fmaxf((float)h[0], (float)h[1]);
     }
-    float m = wave_max_u(mine);
-    if (lane == 0) red[0][w] = m;
-    const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
-    const uint32_t order = lp_order(mine);
-    if (kept) {
-        // the need-th largest of the lanes' or less, by its bits from the highest on
-        // (f16 logits have no more than 19)
-        auto nth = [&](int need) {
-            uint32_t t = 0;
-            for (int b = 31; b >= (F32 ? 0 : 13); b--) {
-                const int c = __popcll(__ballot(order >= (t | 1u << b)));
-                if (c >= need) t |= 1u << b;
-                if (c == need) break;
-            }
-            return t;
-        };
-        // `kept` logits are not below any wave's kept-th, nor below the least of the
-        // waves' (kept / waves)-th, which is the higher where the waves are alike
-        const uint32_t a = nth(kept), b = nth((kept + NT / 64 - 1) / (NT / 64));
-        if (lane == 0) bound[0][w] = a, bound[1][w] = b;
-    }
-    if (threadIdx.x == 0) S.count = 0;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < NT / 64; k++) m = fmaxf(m, red[0][k]);
-    // ---- the sums
-    m = uniform(CAP ? sm_f(m, A.cap) : m);
-    const float c = m == -INFINITY ? 0.f : m, s = sm_scale(1.44269504088896340736f, T > 0.f ? T : 1.f);
-    float l = 0.f, h = 0.f;
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-        float pl = 0.f, ph = 0.f;
-#pragma unroll
-        for (int j = 0; j < V; j++) {
-            const float z = less(r, j, c) * s, e = __builtin_amdgcn_exp2f(z);
-            pl += e;
-            ph = fmaf(e, fmaxf(z, -1e30f), ph);
-        }
-        l += pl, h += ph;
-    }
-    l = wave_sum_u(l), h = wave_sum_u(h);
-    if (lane == 0) red[1][w] = l, red[2][w] = h;
-    // ---- the part's likeliest
-    if (kept) {
-        uint32_t t = LP_NONE + 1, all = 0xffffffffu;
-#pragma unroll
-        for (int k = 0; k < NT / 64; k++) t = max(t, bound[0][k]), all = min(all, bound[1][k]);
-        t = max(t, all);
-        const float least = lp_value((unsigned long long)t << 32);  // or NaN: more than any logit
-        // which of the thread's logits are not below the bound, then those few from
-        // memory once more
-        uint32_t some = 0;
-        if (order >= t) {
+    // the words' largest, that of numbers
+    DEV float largest() const {
+        float m = -INFINITY;
+        if constexpr (F32) {
 #pragma unroll
             for (int r = 0; r < R; r++)
 #pragma unroll
-                for (int j = 0; j < V; j++) some |= get(r, j) >= least ? 1u << (r * V + j) : 0u;
-        }
-        auto each = [&](auto f) {
-            for (uint32_t left = some; left; left &= left - 1) {
-                const int i = __ffs(left) - 1, at = base + i / V * NT * V + i % V;
-                const size_t e = (size_t)row * A.n + at;
-                float x;
-                if constexpr (F32) x = ((const float*)A.x)[e];
-                else x = h2f(((const uint16_t*)A.x)[e]);
-                f(lp_key(lp_order(x), at));
-            }
-        };
-        each([&](unsigned long long k) {
-            const int at = atomicAdd(&S.count, 1);
-            if (at < LP_LIST) S.list[at] = k;
-        });
-        lp_rank<NT>(S, kept, each);
-    } else {
-        __syncthreads();
-    }
-    l = red[1][0], h = red[2][0];
+                for (int j = 0; j < V; j++) m = fmaxf(m, get(r, j));
+        } else {
+            typedef _Float16 hp __attribute__((ext_vector_type(2)));
+            hp p = {(_Float16)-INFINITY, (_Float16)-INFINITY};
 #pragma unroll
-    for (int k = 1; k < NT / 64; k++) l += red[1][k], h += red[2][k];
-    if (A.parts == 1) {
-        lp_finish(A, row, T, m, l, h, S.top, xt, CAP);
-    } else {
-        if (threadIdx.x == 0) A.stats[blockIdx.x] = make_float4(m, l, h, 0.f);
-        if ((int)threadIdx.x < kept) A.keys[(size_t)blockIdx.x * kept + threadIdx.x] = S.top[threadIdx.x];
+            for (int r = 0; r < R; r++)
+#pragma unroll
+                for (int i = 0; i < W; i++) p = __builtin_elementwise_max(p, __builtin_bit_cast(hp, v[r][i]));
+            m = fmaxf((float)p[0], (float)p[1]);
+        }
+        return m;
     }
+    // to another largest
+    DEV void bring(float to, float s) {
+        const float z = mine == -INFINITY ? 0.f : (c - to) * s, a = __builtin_amdgcn_exp2f(z);
+        h = a * fmaf(fmaxf(z, -1e30f), l, h), l *= a;
+        c = to;
+    }
+    DEV void add(float m, float cap, float s) {
+        if (m > mine) {
+            bring(CAP ? sm_f(m, cap) : m, s);
+            mine = m;
+        }
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            float pl = 0.f, ph = 0.f;
+#pragma unroll
+            for (int j = 0; j < V; j++) {
+                const float z = less(r, j, cap) * s, e = __builtin_amdgcn_exp2f(z);
+                pl += e;
+                ph = fmaf(e, fmaxf(z, -1e30f), ph);
+            }
+            l += pl, h += ph;
+        }
+    }
+    // the workgroup's: *m is f of its largest
+    template <int NT>
+    DEV void join(float* m, float cap, float s) {
+        __shared__ float red[3][NT / 64];
+        const int w = threadIdx.x >> 6;
+        const float a = wave_max_u(mine);
+        if ((threadIdx.x & 63) == 0) red[0][w] = a;
+        __syncthreads();
+        float b = red[0][0];
+#pragma unroll
+        for (int k = 1; k < NT / 64; k++) b = fmaxf(b, red[0][k]);
+        *m = uniform(CAP ? sm_f(b, cap) : b);
+        bring(*m, s);
+        l = wave_sum_u(l), h = wave_sum_u(h);
+        if ((threadIdx.x & 63) == 0) red[1][w] = l, red[2][w] = h;
+        __syncthreads();
+        l = red[1][0], h = red[2][0];
+#pragma unroll
+        for (int k = 1; k < NT / 64; k++) l += red[1][k], h += red[2][k];
+    }
+};
+DEV float lp_scale(float T) { return sm_scale(1.44269504088896340736f, T > 0.f ? T : 1.f); }
+
+// a row in R words of V logits a thread
+template <bool F32, bool CAP, int NT, int R, int V>
+DEV void lp_whole(const LpArgs& A) {
+    __shared__ LpTop<NT> S;
+    const int row = blockIdx.x, t = threadIdx.x;
+    const size_t row0 = (size_t)row * A.n;
+    LpSums<F32, CAP, R, V> P;
+#pragma unroll
+    for (int r = 0; r < R; r++) sm_load<F32, V>(A.x, row0, t * V + r * NT * V, A.n, P.v[r]);
+    const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
+    const float xt = lp_load<F32>(A, row0, A.tokens ? A.tokens[row] : -1);
+    const float mine = P.largest();
+    P.add(mine, A.cap, s);
+    float m;
+    P.template join<NT>(&m, A.cap, s);
+    const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
+    if (kept)
+        lp_select<NT, R * V>(
+            S, kept, A.n, F32, [&](auto f) { f(lp_order(mine), t); },
+            [&](int g, int e) { return e / V * NT * V + g * V + e % V; }, [&](int i) { return lp_load<F32>(A, row0, i); },
+            [] {});
+    lp_finish(A, row, T, m, log((double)P.l), P.l, P.h, S.top, xt, CAP);
 }
 
-// A row's parts joined: their sums brought to the largest m, and of their keys those
-// that are not below the largest of the parts' last ones, which bounds the row's
-// last one.
-template <bool F32, bool CAP>
-DEV void lp_join(const LpArgs& A) {
-    constexpr int NT = 256;
-    __shared__ LpTop<NT> S;
-    __shared__ float red[4];
-    __shared__ double sums[2][4];
-    __shared__ unsigned long long bound[4];
-    const int row = blockIdx.x, t = threadIdx.x, w = t >> 6, lane = t & 63;
-    const float4* st = A.stats + (size_t)row * A.parts;
-    const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f;
-    const float xt = lp_token_logit<F32>(A, row);
-    const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
-    const unsigned long long* keys = A.keys + (size_t)row * A.parts * kept;
-    // the first of a thread's stats and keys are fetched together
-    constexpr int U = 4;
-    const long long many = (long long)A.parts * kept;
-    const float4 mine = st[min(t, A.parts - 1)];
-    unsigned long long key[U];
-#pragma unroll
-    for (int u = 0; u < U; u++) key[u] = t + u * NT < many ? keys[t + u * NT] : 0;
-    float m = -INFINITY;
-    unsigned long long last = 1;
-    for (int p = t; p < A.parts; p += NT) m = fmaxf(m, p == t ? mine.x : st[p].x);
-    // a key at a part's end
-#pragma unroll
-    for (int u = 0; u < U; u++)
-        if (t + u * NT < many && (t + u * NT) % kept == kept - 1) last = max(last, key[u]);
-    for (long long i = t + U * NT; i < many; i += NT)
-        if (i % kept == kept - 1) last = max(last, keys[i]);
-    m = wave_max_u(m);
-    last = wave_max_key(last);
-    if (lane == 0) red[w] = m, bound[w] = last;
-    if (t == 0) S.count = 0;
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < 4; k++) m = fmaxf(m, red[k]), last = max(last, bound[k]);
-    const float c = m == -INFINITY ? 0.f : m, s = sm_scale(1.44269504088896340736f, T > 0.f ? T : 1.f);
-    double L = 0, H = 0;
-    for (int p = t; p < A.parts; p += NT) {
-        const float4 q = p == t ? mine : st[p];
-        const float z = (q.x - c) * s, a = q.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(z);
-        L += (double)q.y * a;
-        H += a != 0.f ? a * ((double)q.z + (double)q.y * (q.x == -INFINITY ? 0.f : z)) : 0.;
+// Parts of rows: 256 threads, 2^chunk_shift chunks of 32 logits a thread, a group
+// each, or (QUAD) one chunk of 8, a group being four neighbours'.
+template <bool F32, bool QUAD>
+struct LpShape {
+    static constexpr int V = F32 ? 4 : 8, R = (QUAD ? 8 : 32) / V, CHUNK = 256 * R * V;
+    static constexpr int GROUPS = QUAD ? 64 : 256;  // of a chunk
+    using Largest = std::conditional_t<F32, float, uint16_t>;
+    // logit e of 32 of group g of a row
+    DEV static int index(int g, int e) {
+        const int chunk = g / GROUPS, i = g % GROUPS;
+        if constexpr (QUAD) return chunk * CHUNK + e / (4 * V) * (256 * V) + (4 * i + e / V % 4) * V + e % V;
+        else return chunk * CHUNK + e / V * (256 * V) + i * V + e % V;
     }
-    L = lane_d(wave_scan_d(L), 63), H = lane_d(wave_scan_d(H), 63);
-    if (lane == 0) sums[0][w] = L, sums[1][w] = H;
-    if (kept) {
-        auto each = [&](auto f) {
+};
+template <bool F32, bool CAP, bool QUAD>
+DEV void lp_part(const LpArgs& A) {
+    using P = LpShape<F32, QUAD>;
+    const int row = blockIdx.x / A.parts, part = blockIdx.x % A.parts, t = threadIdx.x;
+    const int first = part << A.chunk_shift, all = (A.n - 1) / P::CHUNK + 1, last = min(first + (1 << A.chunk_shift), all);
+    const size_t row0 = (size_t)row * A.n;
+    const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
+    const bool kept = A.n_top || !(T > 0.f);
+    typename P::Largest* to = (typename P::Largest*)A.largest + (size_t)row * all * P::GROUPS;
+    LpSums<F32, CAP, P::R, P::V> S;
+    uint32_t next[P::R][S.W];
+    auto load = [&](int k) {
 #pragma unroll
-            for (int u = 0; u < U; u++)
-                if (key[u] >= last) f(key[u]);
-            for (long long i = t + U * NT; i < many; i += NT) {
-                const unsigned long long k = keys[i];
-                if (k >= last) f(k);
+        for (int r = 0; r < P::R; r++) sm_load<F32, P::V>(A.x, row0, k * P::CHUNK + t * P::V + r * 256 * P::V, A.n, next[r]);
+    };
+    load(first);
+    for (int k = first; k < last; k++) {
+#pragma unroll
+        for (int r = 0; r < P::R; r++)
+#pragma unroll
+            for (int i = 0; i < S.W; i++) S.v[r][i] = next[r][i];
+        if (k + 1 < last) load(k + 1);
+        const float m = S.largest();
+        if (kept) {
+            float g = m;
+            if constexpr (QUAD) g = fmaxf(g, dpp_xor1(g)), g = fmaxf(g, dpp_xor2(g));
+            if (!QUAD || (t & 3) == 0) {
+                typename P::Largest* o = to + k * P::GROUPS + (QUAD ? t >> 2 : t);
+                if constexpr (F32) *o = g;
+                else *o = (uint16_t)f2h(g);
             }
-        };
-        each([&](unsigned long long k) {
-            const int at = atomicAdd(&S.count, 1);
-            if (at < LP_LIST) S.list[at] = k;
-        });
-        lp_rank<NT>(S, kept, each);
-    } else {
-        __syncthreads();
+        }
+        S.add(m, A.cap, s);
     }
-    L = (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]);
-    H = (sums[1][0] + sums[1][1]) + (sums[1][2] + sums[1][3]);
-    lp_finish(A, row, T, m, L, H, S.top, xt, CAP);
+    float m;
+    S.template join<256>(&m, A.cap, s);
+    if (t == 0) A.stats[blockIdx.x] = make_float4(m, S.l, S.h, 0.f);
 }
-#define LOGPROBS_PART(NAME, F32, CAP, NT, R)                                                              \
+
+// A row's parts joined: their sums brought to the largest m, its likeliest looked for.
+template <bool F32, bool CAP, bool QUAD>
+DEV void lp_join(const LpArgs& A) {
+    using P = LpShape<F32, QUAD>;
+    constexpr int NT = 256, VG = F32 ? 4 : 8;  // groups of a load
+    __shared__ LpTop<NT> S;
+    const int row = blockIdx.x, t = threadIdx.x, lane = t & 63;
+    const size_t row0 = (size_t)row * A.n;
+    const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
+    const float xt = lp_load<F32>(A, row0, A.tokens ? A.tokens[row] : -1);
+    const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
+    __shared__ double sums[3];
+    __shared__ float largest;
+    // the sums, by one wave
+    const float4* st = A.stats + (size_t)row * A.parts;
+    const float4 first = st[min(lane, A.parts - 1)];
+    auto join = [&] {
+        float m = -INFINITY;
+        for (int p = lane; p < A.parts; p += 64) m = fmaxf(m, p < 64 ? first.x : st[p].x);
+        m = wave_max_u(m);
+        const float c = m == -INFINITY ? 0.f : m;
+        double L = 0, H = 0;
+        for (int p = lane; p < A.parts; p += 64) {
+            const float4 q = p < 64 ? first : st[p];
+            const float z = (q.x - c) * s, a = q.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(z);
+            L += (double)q.y * a;
+            H += a != 0.f ? a * ((double)q.z + (double)q.y * (q.x == -INFINITY ? 0.f : z)) : 0.;
+        }
+        L = lane_d(wave_scan_d(L), 63), H = lane_d(wave_scan_d(H), 63);
+        sums[0] = log(L), sums[1] = L, sums[2] = H;
+        largest = m;
+    };
+    if (!kept) {
+        if (t >= 64) return;
+        join();
+    } else {
+        constexpr int K = 4;  // loads that a thread keeps: rows up to 1048576 / VG logits
+        const int loads = ((A.n - 1) / P::CHUNK + 1) * P::GROUPS / VG;
+        const uint4* from = (const uint4*)((const typename P::Largest*)A.largest + (size_t)row * loads * VG);
+        uint4 q[K];
+#pragma unroll
+        for (int u = 0; u < K; u++) q[u] = from[min(u * NT + t, loads - 1)];
+        lp_select<NT, 32>(
+            S, kept, A.n, F32,
+            [&](auto f) {
+                auto eight = [&](const uint4& v, int i) {
+                    const uint32_t a[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int k = 0; k < VG; k++) {
+                        const float x = F32 ? __builtin_bit_cast(float, a[k]) : h2f(k & 1 ? a[k / 2] >> 16 : a[k / 2] & 0xffffu);
+                        f(lp_order(x), i * VG + k);
+                    }
+                };
+#pragma unroll
+                for (int u = 0; u < K; u++)
+                    if (u * NT + t < loads) eight(q[u], u * NT + t);
+                for (int i = K * NT + t; i < loads; i += NT) eight(from[i], i);
+            },
+            P::index, [&](int i) { return lp_load<F32>(A, row0, i); }, join);
+        if (t >= 64) return;
+    }
+    lp_finish(A, row, T, largest, sums[0], sums[1], sums[2], S.top, xt, CAP);
+}
+#define LOGPROBS_WHOLE(NAME, F32, CAP, NT, R)                                                             \
     extern "C" __global__ __launch_bounds__(NT) void cima_logprobs_t##NT##_w##R##_##NAME(const LpArgs A) { \
-        lp_part<F32, CAP, NT, F32 ? R : R / 2, F32 ? 4 : 8>(A);                                            \
+        lp_whole<F32, CAP, NT, F32 ? R : R / 2, F32 ? 4 : 8>(A);                                           \
     }
-#define LOGPROBS(NAME, F32, CAP)                                                                          \
-    LOGPROBS_PART(NAME, F32, CAP, 256, 2)                                                                 \
-    LOGPROBS_PART(NAME, F32, CAP, 256, 8)                                                                 \
-    LOGPROBS_PART(NAME, F32, CAP, 1024, 8)                                                                \
-    extern "C" __global__ __launch_bounds__(256) void cima_logprobs_join_##NAME(const LpArgs A) {         \
-        lp_join<F32, CAP>(A);                                                                              \
+#define LOGPROBS_PARTS(NAME, F32, CAP, R, QUAD)                                                           \
+    extern "C" __global__ __launch_bounds__(256) void cima_logprobs_part_w##R##_##NAME(const LpArgs A) {  \
+        lp_part<F32, CAP, QUAD>(A);                                                                        \
+    }                                                                                                      \
+    extern "C" __global__ __launch_bounds__(256) void cima_logprobs_join_w##R##_##NAME(const LpArgs A) {  \
+        lp_join<F32, CAP, QUAD>(A);                                                                        \
     }
+#define LOGPROBS(NAME, F32, CAP)            \
+    LOGPROBS_WHOLE(NAME, F32, CAP, 256, 2)  \
+    LOGPROBS_WHOLE(NAME, F32, CAP, 256, 8)  \
+    LOGPROBS_WHOLE(NAME, F32, CAP, 1024, 8) \
+    LOGPROBS_PARTS(NAME, F32, CAP, 2, true) \
+    LOGPROBS_PARTS(NAME, F32, CAP, 8, false)
 LOGPROBS(f16, false, false)
 LOGPROBS(f32, true, false)
 LOGPROBS(cap_f16, false, true)

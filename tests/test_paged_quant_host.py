@@ -86,7 +86,7 @@ def test_read_back_refuses_a_missing_context():
 def test_logprobs_kernels_and_a_missing_context():
     blob = open(cbuild.HSACOS["sample"], "rb").read()
     for t in ("f16", "f32", "cap_f16", "cap_f32"):
-        for k in ("t256_w2", "t256_w8", "t1024_w8", "join"):
+        for k in ("t256_w2", "t256_w8", "t1024_w8", "part_w2", "part_w8", "join_w2", "join_w8"):
             assert f"cima_logprobs_{k}_{t}".encode() in blob
     L = hipmod.load_library()
     rc = L.cima_hip_logprobs_rows(None, None, 1, 1, None, None, None, 0, None, None, None, 1, 0.0, 0, None, 0)
