@@ -2113,8 +2113,10 @@ int cima_hip_logprobs_rows(cima_hip_ctx* ctx, const void* x, int rows, int n, co
     if (chunks > kMaxGrid || !slab || !aligned(slab, 16) || slab_bytes < need_of(words))
         return fail(CIMA_E_INVALID, "%s: the slab holds %llu of %llu bytes, or is null or misaligned (16 B)", api,
                     slab_bytes, need_of(words));
-    static int sh = getenv("LPSH") ? atoi(getenv("LPSH")) : 0;
-    A.chunk_shift = words == 8 ? sh : 0;
+    // Many f16 chunks four to a workgroup, whose loads run ahead of its sums: 384 rows of
+    // 128256 (6144) 22.9 us, one 24.4, two 23.8; but 2048 of them 11.2, 9.6, 10.7, and of
+    // 6144 f32 39.3, 35.9, 37.3, capped f16 49.8, 48.6, 49.3.
+    A.chunk_shift = words == 8 && !f32 && cap == 0.f && chunks >= 16LL * ctx->num_cu ? 2 : 0;
     A.parts = ((parts_of(words) - 1) >> A.chunk_shift) + 1;
     A.stats = (float*)slab;
     A.largest = (char*)slab + 16 * chunks;

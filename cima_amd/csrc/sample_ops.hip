@@ -78,6 +78,16 @@ DEV float mix_less(uint32_t pair, bool high, float c) {
     return d;
 }
 
+// a logit of a pair times s less c
+DEV float mix_fma(uint32_t pair, bool high, float s, float c) {
+    float d;
+    if (high)
+        __asm__("v_fma_mix_f32 %0, %1, %2, -%3 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(d) : "v"(pair), "v"(s), "v"(c));
+    else
+        __asm__("v_fma_mix_f32 %0, %1, %2, -%3 op_sel_hi:[1,0,0]" : "=v"(d) : "v"(pair), "v"(s), "v"(c));
+    return d;
+}
+
 // R words of V logits a thread of a row by NT threads: the maximum, the first place of it
 // (T <= 0) or the sum (T > 0).  CAP: f is applied when the logits are loaded,
 // which are fp32 from there on.
@@ -364,10 +374,12 @@ DEV void lp_rank(LpTop<NT>& S, int kept, B beside) {
             const unsigned long long k = (int)threadIdx.x < count ? S.list[threadIdx.x] : 0;
             const uint32_t lo = (uint32_t)k, hi = (uint32_t)(k >> 32);
             int rank = 0;
-            for (int j = 0; j < count; j++) {
-                const uint32_t a = __builtin_amdgcn_readlane(lo, j), b = __builtin_amdgcn_readlane(hi, j);
-                rank += ((unsigned long long)b << 32 | a) > k;
-            }
+            for (int j0 = 0; j0 < count; j0 += 4)
+#pragma unroll
+                for (int j = j0; j < j0 + 4; j++) {
+                    const uint32_t a = __builtin_amdgcn_readlane(lo, j), b = __builtin_amdgcn_readlane(hi, j);
+                    rank += ((unsigned long long)b << 32 | a) > k;
+                }
             if ((int)threadIdx.x < count) {
                 if (rank < kept) S.top[rank] = k;
             } else if ((int)threadIdx.x < kept) {
@@ -391,15 +403,14 @@ DEV void lp_rank(LpTop<NT>& S, int kept, B beside) {
     }
     __syncthreads();
 }
-// The row's `kept` likeliest to S.top.  each_group(f): f(order of the largest, group)
-// for every group of this thread; index(g, e): the row's place of logit e of ONE of
+// The row's `kept` likeliest to S.top.  each_group(f): f(largest, group) for every group
+// of this thread, `most` the largest of all of them; index(g, e): the row's place of logit e of ONE of
 // group g; load(i): logit i of the row's n, -inf behind them; beside(): something
 // that the second wave has to do once.
 template <int NT, int ONE, typename G, typename I, typename L, typename B>
-DEV void lp_select(LpTop<NT>& S, int kept, int n, bool f32, G each_group, I index, L load, B beside) {
+DEV void lp_select(LpTop<NT>& S, int kept, int n, bool f32, float most, G each_group, I index, L load, B beside) {
     const int t = threadIdx.x, w = t >> 6, lane = t & 63;
-    uint32_t best = 0;
-    each_group([&](uint32_t o, int) { best = max(best, o); });
+    const uint32_t best = lp_order(most);
     // the need-th largest of the lanes' or less, by its bits from the highest on (f16
     // logits have no more than 19)
     auto nth = [&](int need) {
@@ -429,15 +440,14 @@ DEV void lp_select(LpTop<NT>& S, int kept, int n, bool f32, G each_group, I inde
     }
     // logits of the groups whose largest is not below `least` that are not below it
     // themselves to S.list (after a barrier), as far as there is room
-    auto look = [&](uint32_t least) {
-        if (best >= least) {
-            int mine = 0;
-            each_group([&](uint32_t o, int) { mine += o >= least; });
-            int to = atomicAdd(&S.groups, mine);
-            each_group([&](uint32_t o, int g) {
-                if (o >= least && to < LP_GROUPS) S.group[to++] = g;
+    auto look = [&](float least) {
+        if (most >= least)
+            each_group([&](float x, int g) {
+                if (x >= least) {
+                    const int to = atomicAdd(&S.groups, 1);
+                    if (to < LP_GROUPS) S.group[to] = g;
+                }
             });
-        }
         __syncthreads();
         const int many = min(S.groups, LP_GROUPS) * ONE;
         constexpr int U = 4;
@@ -450,20 +460,19 @@ DEV void lp_select(LpTop<NT>& S, int kept, int n, bool f32, G each_group, I inde
                 at[u] = i < many ? index(S.group[i / ONE], i % ONE) : 0;
                 x[u] = i < many ? load(at[u]) : -INFINITY;
             }
-            // a number's order is that of what is not less
             int mine = 0;
 #pragma unroll
-            for (int u = 0; u < U; u++) mine += x[u] >= lp_value(least);
+            for (int u = 0; u < U; u++) mine += x[u] >= least;
             if (mine) {
                 int to = atomicAdd(&S.count, mine);
 #pragma unroll
                 for (int u = 0; u < U; u++)
-                    if (x[u] >= lp_value(least) && to < LP_LIST) S.list[to++] = lp_key(lp_order(x[u]), at[u]);
+                    if (x[u] >= least && to < LP_LIST) S.list[to++] = lp_key(lp_order(x[u]), at[u]);
             }
         }
         __syncthreads();
     };
-    look(v);
+    look(lp_value(v));
     if (S.groups <= LP_GROUPS && S.count <= LP_LIST) {
         lp_rank<NT>(S, kept, beside);
         return;
@@ -473,7 +482,7 @@ DEV void lp_select(LpTop<NT>& S, int kept, int n, bool f32, G each_group, I inde
     v = 0;
     for (int b = 31; b >= 0; b--) {
         int c = 0;
-        each_group([&](uint32_t o, int) { c += o >= (v | 1u << b); });
+        each_group([&](float x, int) { c += lp_order(x) >= (v | 1u << b); });
         if (c) atomicAdd(&S.bits[b], c);
         __syncthreads();
         if (S.bits[b] >= kept) v |= 1u << b;
@@ -481,7 +490,7 @@ DEV void lp_select(LpTop<NT>& S, int kept, int n, bool f32, G each_group, I inde
     v = max(v, LP_NONE);
     if (t == 0) S.count = S.groups = 0;
     __syncthreads();
-    look(v + 1);
+    look(lp_value(v + 1));
     lp_rank<NT>(S, kept, beside);
     int have = min(S.count, kept);
     for (int i0 = 0, k = 0; i0 < n && have < kept && v > LP_NONE; i0 += NT, k ^= 1) {
@@ -500,13 +509,19 @@ DEV void lp_select(LpTop<NT>& S, int kept, int n, bool f32, G each_group, I inde
     }
     __syncthreads();
 }
+// f of a logit as sm_f, cap - 2 cap / (1 + e^(2 x / cap)): off by cap 2^-21 at most, which
+// is all that a log probability asks of it (384 rows of 128256 48.6 -> 35.6 us)
+DEV float lp_f(float x, float cap) {
+    const float e = __builtin_amdgcn_exp2f(x * (2.88539008177792681472f / cap));
+    return __builtin_isinf(x) ? x : fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + e), cap);
+}
 // a row's results: largest f(x) m, sums L (and its logarithm) and H as in LpArgs, the
 // best keys in top
 DEV void lp_finish(const LpArgs& A, int row, float T, float m, double ln, double L, double H,
                    const unsigned long long* top, float xt, bool cap) {
     auto logprob = [&](float x) -> float {
         if (x == -INFINITY) return -INFINITY;
-        const float f = cap ? sm_f(x, A.cap) : x;
+        const float f = cap ? lp_f(x, A.cap) : x;
         return (float)((double)(f - m) / (double)T - ln);
     };
     const bool one = !(T > 0.f);  // the largest logit alone
@@ -532,48 +547,53 @@ DEV float lp_load(const LpArgs& A, size_t row0, int i) {
     else return h2f(((const uint16_t*)A.x)[row0 + i]);
 }
 
-// A thread's running sums: R words of V logits at a time.
+// the largest number of W words
+template <bool F32, int W>
+DEV float lp_largest(const uint32_t (&v)[W]) {
+    if constexpr (F32) {
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < W; i++) m = fmaxf(m, __builtin_bit_cast(float, v[i]));
+        return m;
+    } else {
+        typedef _Float16 hp __attribute__((ext_vector_type(2)));
+        uint32_t p = 0xfc00fc00u;
+#pragma unroll
+        for (int i = 0; i < W; i++) __asm__("v_pk_max_f16 %0, %0, %1" : "+v"(p) : "v"(v[i]));
+        const hp h = __builtin_bit_cast(hp, p);
+        return fmaxf((float)h[0], (float)h[1]);
+    }
+}
+// A thread's running sums of 2^z and 2^z z, R words of V logits at a time: z = (f(x) -
+// c) s, c f of the largest so far (0: none); FAST, of f16 logits, z = x s - b in one
+// instruction, b = c s as fp32 holds it, which the end puts right.  It takes |c s| up
+// to 2^20, so that b is near enough: s up to LP_FAST.
+constexpr float LP_FAST = 16.f;
 template <bool F32, bool CAP, int R, int V>
 struct LpSums {
     static constexpr int W = F32 ? V : V / 2;
-    uint32_t v[R][W];
-    float mine = -INFINITY, c = 0.f, l = 0.f, h = 0.f;  // the largest, f of it (0: none), the sums
+    using Words = uint32_t[R][W];
+    float mine = -INFINITY, c = 0.f, b = 0.f, l = 0.f, h = 0.f;
 
-    DEV float get(int r, int j) const { return sm_get<F32, V>(v[r], j); }
-    // f of a logit less c (SmRow::less)
-    DEV float less(int r, int j, float cap) const {
-        if constexpr (CAP) return sm_f(get(r, j), cap) - c;
-        else if constexpr (F32) return get(r, j) - c;
-        else return mix_less(v[r][j / 2], j & 1, c);
-    }
-    // the words' largest, that of numbers
-    DEV float largest() const {
-        float m = -INFINITY;
-        if constexpr (F32) {
+    DEV static float largest(const Words& v) {
+        uint32_t a[R * W];
 #pragma unroll
-            for (int r = 0; r < R; r++)
-#pragma unroll
-                for (int j = 0; j < V; j++) m = fmaxf(m, get(r, j));
-        } else {
-            typedef _Float16 hp __attribute__((ext_vector_type(2)));
-            hp p = {(_Float16)-INFINITY, (_Float16)-INFINITY};
-#pragma unroll
-            for (int r = 0; r < R; r++)
-#pragma unroll
-                for (int i = 0; i < W; i++) p = __builtin_elementwise_max(p, __builtin_bit_cast(hp, v[r][i]));
-            m = fmaxf((float)p[0], (float)p[1]);
-        }
-        return m;
+        for (int i = 0; i < R * W; i++) a[i] = v[i / W][i % W];
+        return lp_largest<F32, R * W>(a);
     }
     // to another largest
+    template <bool FAST>
     DEV void bring(float to, float s) {
-        const float z = mine == -INFINITY ? 0.f : (c - to) * s, a = __builtin_amdgcn_exp2f(z);
+        const float nb = to * s, z = mine == -INFINITY ? 0.f : FAST ? b - nb : (c - to) * s;
+        const float a = __builtin_amdgcn_exp2f(z);
         h = a * fmaf(fmaxf(z, -1e30f), l, h), l *= a;
-        c = to;
+        c = to, b = nb;
     }
-    DEV void add(float m, float cap, float s) {
+    // words whose largest is m
+    template <bool FAST>
+    DEV void add(const Words& v, float m, float cap, float s) {
         if (m > mine) {
-            bring(CAP ? sm_f(m, cap) : m, s);
+            bring<FAST>(CAP ? lp_f(m, cap) : m, s);
             mine = m;
         }
 #pragma unroll
@@ -581,7 +601,12 @@ struct LpSums {
             float pl = 0.f, ph = 0.f;
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                const float z = less(r, j, cap) * s, e = __builtin_amdgcn_exp2f(z);
+                float z;
+                if constexpr (FAST) z = mix_fma(v[r][j / 2], j & 1, s, b);
+                else if constexpr (CAP) z = (lp_f(sm_get<F32, V>(v[r], j), cap) - c) * s;
+                else if constexpr (F32) z = (sm_get<F32, V>(v[r], j) - c) * s;
+                else z = mix_less(v[r][j / 2], j & 1, c) * s;
+                const float e = __builtin_amdgcn_exp2f(z);
                 pl += e;
                 ph = fmaf(e, fmaxf(z, -1e30f), ph);
             }
@@ -589,24 +614,28 @@ struct LpSums {
         }
     }
     // the workgroup's: *m is f of its largest
-    template <int NT>
+    template <int NT, bool FAST>
     DEV void join(float* m, float cap, float s) {
         __shared__ float red[3][NT / 64];
         const int w = threadIdx.x >> 6;
         const float a = wave_max_u(mine);
         if ((threadIdx.x & 63) == 0) red[0][w] = a;
         __syncthreads();
-        float b = red[0][0];
+        float g = red[0][0];
 #pragma unroll
-        for (int k = 1; k < NT / 64; k++) b = fmaxf(b, red[0][k]);
-        *m = uniform(CAP ? sm_f(b, cap) : b);
-        bring(*m, s);
+        for (int k = 1; k < NT / 64; k++) g = fmaxf(g, red[0][k]);
+        *m = uniform(CAP ? lp_f(g, cap) : g);
+        bring<FAST>(*m, s);
         l = wave_sum_u(l), h = wave_sum_u(h);
         if ((threadIdx.x & 63) == 0) red[1][w] = l, red[2][w] = h;
         __syncthreads();
         l = red[1][0], h = red[2][0];
 #pragma unroll
         for (int k = 1; k < NT / 64; k++) l += red[1][k], h += red[2][k];
+        if (FAST && *m != -INFINITY) {  // z less what b was rounded by
+            const float off = -fmaf(*m, s, -b), e = __builtin_amdgcn_exp2f(off);
+            h = e * fmaf(off, l, h), l *= e;
+        }
     }
 };
 DEV float lp_scale(float T) { return sm_scale(1.44269504088896340736f, T > 0.f ? T : 1.f); }
@@ -618,18 +647,19 @@ DEV void lp_whole(const LpArgs& A) {
     const int row = blockIdx.x, t = threadIdx.x;
     const size_t row0 = (size_t)row * A.n;
     LpSums<F32, CAP, R, V> P;
+    typename decltype(P)::Words v;
 #pragma unroll
-    for (int r = 0; r < R; r++) sm_load<F32, V>(A.x, row0, t * V + r * NT * V, A.n, P.v[r]);
+    for (int r = 0; r < R; r++) sm_load<F32, V>(A.x, row0, t * V + r * NT * V, A.n, v[r]);
     const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
     const float xt = lp_load<F32>(A, row0, A.tokens ? A.tokens[row] : -1);
-    const float mine = P.largest();
-    P.add(mine, A.cap, s);
+    const float mine = P.largest(v);
+    P.template add<false>(v, mine, A.cap, s);
     float m;
-    P.template join<NT>(&m, A.cap, s);
+    P.template join<NT, false>(&m, A.cap, s);
     const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
     if (kept)
         lp_select<NT, R * V>(
-            S, kept, A.n, F32, [&](auto f) { f(lp_order(mine), t); },
+            S, kept, A.n, F32, mine, [&](auto f) { f(mine, t); },
             [&](int g, int e) { return e / V * NT * V + g * V + e % V; }, [&](int i) { return lp_load<F32>(A, row0, i); },
             [] {});
     lp_finish(A, row, T, m, log((double)P.l), P.l, P.h, S.top, xt, CAP);
@@ -659,33 +689,55 @@ DEV void lp_part(const LpArgs& A) {
     const bool kept = A.n_top || !(T > 0.f);
     typename P::Largest* to = (typename P::Largest*)A.largest + (size_t)row * all * P::GROUPS;
     LpSums<F32, CAP, P::R, P::V> S;
-    uint32_t next[P::R][S.W];
-    auto load = [&](int k) {
+    using Words = typename decltype(S)::Words;
+    auto load = [&](int k, Words& v) {
+        if ((k + 1) * P::CHUNK <= A.n) {
+            const size_t at = row0 + (size_t)k * P::CHUNK + t * P::V;
+            // past the caches: read once (777 rows of 151936 46.6 -> 42.0 us)
+            typedef uint32_t word4 __attribute__((ext_vector_type(4), aligned(2)));
 #pragma unroll
-        for (int r = 0; r < P::R; r++) sm_load<F32, P::V>(A.x, row0, k * P::CHUNK + t * P::V + r * 256 * P::V, A.n, next[r]);
-    };
-    load(first);
-    for (int k = first; k < last; k++) {
+            for (int r = 0; r < P::R; r++) {
+                word4 q;
+                if constexpr (F32) q = __builtin_nontemporal_load((const word4*)((const float*)A.x + at + r * 256 * P::V));
+                else q = __builtin_nontemporal_load((const word4*)((const uint16_t*)A.x + at + r * 256 * P::V));
 #pragma unroll
-        for (int r = 0; r < P::R; r++)
-#pragma unroll
-            for (int i = 0; i < S.W; i++) S.v[r][i] = next[r][i];
-        if (k + 1 < last) load(k + 1);
-        const float m = S.largest();
-        if (kept) {
-            float g = m;
-            if constexpr (QUAD) g = fmaxf(g, dpp_xor1(g)), g = fmaxf(g, dpp_xor2(g));
-            if (!QUAD || (t & 3) == 0) {
-                typename P::Largest* o = to + k * P::GROUPS + (QUAD ? t >> 2 : t);
-                if constexpr (F32) *o = g;
-                else *o = (uint16_t)f2h(g);
+                for (int i = 0; i < 4; i++) v[r][i] = q[i];
             }
+        } else {
+#pragma unroll
+            for (int r = 0; r < P::R; r++) sm_load<F32, P::V>(A.x, row0, k * P::CHUNK + t * P::V + r * 256 * P::V, A.n, v[r]);
         }
-        S.add(m, A.cap, s);
-    }
-    float m;
-    S.template join<256>(&m, A.cap, s);
-    if (t == 0) A.stats[blockIdx.x] = make_float4(m, S.l, S.h, 0.f);
+    };
+    auto all_chunks = [&](auto fast) {
+        auto add = [&](int k, const Words& v) {
+            const float m = S.largest(v);
+            if (kept) {
+                float g = m;
+                if constexpr (QUAD) g = fmaxf(g, dpp_xor1(g)), g = fmaxf(g, dpp_xor2(g));
+                if (!QUAD || (t & 3) == 0) {
+                    typename P::Largest* o = to + k * P::GROUPS + (QUAD ? t >> 2 : t);
+                    if constexpr (F32) *o = g;
+                    else *o = (uint16_t)f2h(g);
+                }
+            }
+            S.template add<fast>(v, m, A.cap, s);
+        };
+        Words v, next;
+        load(first, v);
+        for (int k = first; k < last; k += 2) {
+            if (k + 1 < last) load(k + 1, next);
+            add(k, v);
+            if (k + 1 == last) break;
+            if (k + 2 < last) load(k + 2, v);
+            add(k + 1, next);
+        }
+        float m;
+        S.template join<256, fast>(&m, A.cap, s);
+        if (t == 0) A.stats[blockIdx.x] = make_float4(m, S.l, S.h, 0.f);
+    };
+    if constexpr (F32 || CAP) all_chunks(std::false_type{});
+    else if (s <= LP_FAST) all_chunks(std::true_type{});
+    else all_chunks(std::false_type{});
 }
 
 // A row's parts joined: their sums brought to the largest m, its likeliest looked for.
@@ -729,16 +781,31 @@ DEV void lp_join(const LpArgs& A) {
         const uint4* from = (const uint4*)((const typename P::Largest*)A.largest + (size_t)row * loads * VG);
         uint4 q[K];
 #pragma unroll
-        for (int u = 0; u < K; u++) q[u] = from[min(u * NT + t, loads - 1)];
+        for (int u = 0; u < K; u++) {
+            constexpr uint32_t NONE = F32 ? 0xff800000u : 0xfc00fc00u;
+            q[u] = u * NT + t < loads ? from[u * NT + t] : make_uint4(NONE, NONE, NONE, NONE);
+        }
+        float most = -INFINITY;
+        {
+            uint32_t a[K * 4];
+#pragma unroll
+            for (int u = 0; u < K; u++) a[4 * u] = q[u].x, a[4 * u + 1] = q[u].y, a[4 * u + 2] = q[u].z, a[4 * u + 3] = q[u].w;
+            most = lp_largest<F32, K * 4>(a);
+            for (int i = K * NT + t; i < loads; i += NT) {
+                const uint4 z = from[i];
+                const uint32_t b[4] = {z.x, z.y, z.z, z.w};
+                most = fmaxf(most, lp_largest<F32, 4>(b));
+            }
+        }
         lp_select<NT, 32>(
-            S, kept, A.n, F32,
+            S, kept, A.n, F32, most,
             [&](auto f) {
                 auto eight = [&](const uint4& v, int i) {
                     const uint32_t a[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
                     for (int k = 0; k < VG; k++) {
                         const float x = F32 ? __builtin_bit_cast(float, a[k]) : h2f(k & 1 ? a[k / 2] >> 16 : a[k / 2] & 0xffffu);
-                        f(lp_order(x), i * VG + k);
+                        f(x, i * VG + k);
                     }
                 };
 #pragma unroll
