@@ -317,9 +317,10 @@ DEV double lane_d(double v, int lane) {
 // With z = (f(x) - m) / T and L = sum e^z over a row: a token's log probability is z -
 // ln L, the row's entropy ln L - sum e^z z / L.  One reading of the logits, each thread
 // to its own running maximum and sums.  The likeliest n_top are found from the
-// largest logits of groups of 32 (a thread's, in a row of one workgroup): each wave
-// takes the (n_top / waves)-th largest of its lanes', so that the least of these
-// bounds the row's n_top-th from below, and what the few groups that reach it hold is
+// largest logits of groups of 32 (neighbours, or a thread's in a row of one workgroup):
+// each wave
+// takes the (n_top / waves)-th largest of its lanes', so that the least of these bounds
+// the row's n_top-th from below, and what the few groups that reach it hold is
 // looked at one by one and ranked by counting (value first, then the lower id).
 // Rows up to 32768 logits go to a workgroup each, in one launch; of longer ones the
 // parts leave their sums and groups' largest, and a second launch joins them (in
@@ -355,6 +356,12 @@ DEV float lp_value(uint32_t order) {
 constexpr uint32_t LP_NONE = 0x007fffffu;  // of -inf: a token that may not be taken
 DEV unsigned long long lp_key(uint32_t order, int at) { return (unsigned long long)order << 32 | (uint32_t)~at; }
 DEV int lp_id(unsigned long long key) { return (int)~(uint32_t)key; }
+template <bool F32>
+DEV float lp_load(const void* x, size_t row0, int i, int n) {
+    if ((unsigned)i >= (unsigned)n) return -INFINITY;
+    if constexpr (F32) return ((const float*)x)[row0 + i];
+    else return h2f(((const uint16_t*)x)[row0 + i]);
+}
 DEV int lanes_below(unsigned long long m) { return __popcll(m & ((1ull << (threadIdx.x & 63)) - 1)); }
 
 template <int NT>
@@ -404,18 +411,18 @@ DEV void lp_rank(LpTop<NT>& S, int kept, B beside) {
     __syncthreads();
 }
 // The row's `kept` likeliest to S.top.  each_group(f): f(largest, group) for every group
-// of this thread, `most` the largest of all of them; index(g, e): the row's place of logit e of ONE of
-// group g; load(i): logit i of the row's n, -inf behind them; beside(): something
-// that the second wave has to do once.
-template <int NT, int ONE, typename G, typename I, typename L, typename B>
-DEV void lp_select(LpTop<NT>& S, int kept, int n, bool f32, float most, G each_group, I index, L load, B beside) {
+// of this thread, `most` the largest of all of them; place(g, p): where in the row
+// piece p of PIECES of V logits of group g begins; beside(): something that the second
+// wave has to do once.
+template <int NT, bool F32, int V, int PIECES, typename G, typename P, typename B>
+DEV void lp_select(LpTop<NT>& S, int kept, const void* x, size_t row0, int n, float most, G each_group, P place, B beside) {
     const int t = threadIdx.x, w = t >> 6, lane = t & 63;
     const uint32_t best = lp_order(most);
     // the need-th largest of the lanes' or less, by its bits from the highest on (f16
     // logits have no more than 19)
     auto nth = [&](int need) {
         uint32_t v = 0;
-        for (int b = 31; b >= (f32 ? 0 : 13); b--) {
+        for (int b = 31; b >= (F32 ? 0 : 13); b--) {
             const int c = __popcll(__ballot(best >= (v | 1u << b)));
             if (c >= need) v |= 1u << b;
             if (c == need) break;
@@ -449,25 +456,21 @@ DEV void lp_select(LpTop<NT>& S, int kept, int n, bool f32, float most, G each_g
                 }
             });
         __syncthreads();
-        const int many = min(S.groups, LP_GROUPS) * ONE;
-        constexpr int U = 4;
-        for (int i0 = 0; i0 < many; i0 += NT * U) {
-            int at[U];
-            float x[U];
-#pragma unroll
-            for (int u = 0; u < U; u++) {
-                const int i = i0 + NT * u + t;
-                at[u] = i < many ? index(S.group[i / ONE], i % ONE) : 0;
-                x[u] = i < many ? load(at[u]) : -INFINITY;
-            }
+        const int many = min(S.groups, LP_GROUPS) * PIECES;
+        for (int i = t; i < many; i += NT) {
+            const int at = place(S.group[i / PIECES], i % PIECES);
+            uint32_t v[F32 ? V : V / 2];
+            sm_load<F32, V>(x, row0, at, n, v);
             int mine = 0;
 #pragma unroll
-            for (int u = 0; u < U; u++) mine += x[u] >= least;
+            for (int j = 0; j < V; j++) mine += sm_get<F32, V>(v, j) >= least;
             if (mine) {
                 int to = atomicAdd(&S.count, mine);
 #pragma unroll
-                for (int u = 0; u < U; u++)
-                    if (x[u] >= least && to < LP_LIST) S.list[to++] = lp_key(lp_order(x[u]), at[u]);
+                for (int j = 0; j < V; j++) {
+                    const float y = sm_get<F32, V>(v, j);
+                    if (y >= least && to < LP_LIST) S.list[to++] = lp_key(lp_order(y), at + j);
+                }
             }
         }
         __syncthreads();
@@ -494,8 +497,8 @@ DEV void lp_select(LpTop<NT>& S, int kept, int n, bool f32, float most, G each_g
     lp_rank<NT>(S, kept, beside);
     int have = min(S.count, kept);
     for (int i0 = 0, k = 0; i0 < n && have < kept && v > LP_NONE; i0 += NT, k ^= 1) {
-        const float x = load(i0 + t);
-        const unsigned long long hit = __ballot(lp_order(x) == v);
+        const float y = lp_load<F32>(x, row0, i0 + t, n);
+        const unsigned long long hit = __ballot(lp_order(y) == v);
         if (lane == 0) S.found[k][w] = __popcll(hit);
         __syncthreads();
         int to = have + lanes_below(hit), all = 0;
@@ -504,7 +507,7 @@ DEV void lp_select(LpTop<NT>& S, int kept, int n, bool f32, float most, G each_g
             if (u < w) to += S.found[k][u];
             all += S.found[k][u];
         }
-        if (lp_order(x) == v && to < kept) S.top[to] = lp_key(v, i0 + t);
+        if (lp_order(y) == v && to < kept) S.top[to] = lp_key(v, i0 + t);
         have += all;
     }
     __syncthreads();
@@ -540,29 +543,36 @@ DEV void lp_finish(const LpArgs& A, int row, float T, float m, double ln, double
             !k ? -INFINITY : one ? (t ? -INFINITY : 0.f) : logprob(lp_value((uint32_t)(k >> 32)));
     }
 }
-template <bool F32>
-DEV float lp_load(const LpArgs& A, size_t row0, int i) {
-    if ((unsigned)i >= (unsigned)A.n) return -INFINITY;
-    if constexpr (F32) return ((const float*)A.x)[row0 + i];
-    else return h2f(((const uint16_t*)A.x)[row0 + i]);
-}
 
-// the largest number of W words
+// The largest number of W words, of f16 that of their lower halves beside that of
+// their upper ones
 template <bool F32, int W>
-DEV float lp_largest(const uint32_t (&v)[W]) {
-    if constexpr (F32) {
-        float m = -INFINITY;
+DEV uint32_t lp_largest(const uint32_t* v) {
+    uint32_t p = v[0];
 #pragma unroll
-        for (int i = 0; i < W; i++) m = fmaxf(m, __builtin_bit_cast(float, v[i]));
-        return m;
-    } else {
-        typedef _Float16 hp __attribute__((ext_vector_type(2)));
-        uint32_t p = 0xfc00fc00u;
-#pragma unroll
-        for (int i = 0; i < W; i++) __asm__("v_pk_max_f16 %0, %0, %1" : "+v"(p) : "v"(v[i]));
-        const hp h = __builtin_bit_cast(hp, p);
-        return fmaxf((float)h[0], (float)h[1]);
+    for (int i = 1; i < W; i++) {
+        if constexpr (F32) p = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, p), __builtin_bit_cast(float, v[i])));
+        else __asm__("v_pk_max_f16 %0, %0, %1" : "+v"(p) : "v"(v[i]));
     }
+    return p;
+}
+// (NaN alone: -inf)
+template <bool F32>
+DEV float lp_of(uint32_t p) {
+    if constexpr (F32) return fmaxf(__builtin_bit_cast(float, p), -INFINITY);
+    else return fmaxf(fmaxf(h2f(p & 0xffffu), h2f(p >> 16)), -INFINITY);
+}
+// the largest of aligned groups of 4 or 8 lanes
+template <bool F32, int LANES>
+DEV uint32_t lp_lanes(uint32_t p) {
+    auto other = [&](uint32_t q) {
+        const uint32_t both[2] = {p, q};
+        p = lp_largest<F32, 2>(both);
+    };
+    other(__builtin_amdgcn_mov_dpp(p, 0xB1, 0xf, 0xf, false));
+    other(__builtin_amdgcn_mov_dpp(p, 0x4E, 0xf, 0xf, false));
+    if constexpr (LANES == 8) other(__builtin_amdgcn_mov_dpp(p, 0x141, 0xf, 0xf, false));
+    return p;
 }
 // A thread's running sums of 2^z and 2^z z, R words of V logits at a time: z = (f(x) -
 // c) s, c f of the largest so far (0: none); FAST, of f16 logits, z = x s - b in one
@@ -575,12 +585,6 @@ struct LpSums {
     using Words = uint32_t[R][W];
     float mine = -INFINITY, c = 0.f, b = 0.f, l = 0.f, h = 0.f;
 
-    DEV static float largest(const Words& v) {
-        uint32_t a[R * W];
-#pragma unroll
-        for (int i = 0; i < R * W; i++) a[i] = v[i / W][i % W];
-        return lp_largest<F32, R * W>(a);
-    }
     // to another largest
     template <bool FAST>
     DEV void bring(float to, float s) {
@@ -651,37 +655,36 @@ DEV void lp_whole(const LpArgs& A) {
 #pragma unroll
     for (int r = 0; r < R; r++) sm_load<F32, V>(A.x, row0, t * V + r * NT * V, A.n, v[r]);
     const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
-    const float xt = lp_load<F32>(A, row0, A.tokens ? A.tokens[row] : -1);
-    const float mine = P.largest(v);
+    const float xt = lp_load<F32>(A.x, row0, A.tokens ? A.tokens[row] : -1, A.n);
+    const float mine = lp_of<F32>(lp_largest<F32, R * P.W>(&v[0][0]));
     P.template add<false>(v, mine, A.cap, s);
     float m;
     P.template join<NT, false>(&m, A.cap, s);
     const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
     if (kept)
-        lp_select<NT, R * V>(
-            S, kept, A.n, F32, mine, [&](auto f) { f(mine, t); },
-            [&](int g, int e) { return e / V * NT * V + g * V + e % V; }, [&](int i) { return lp_load<F32>(A, row0, i); },
-            [] {});
+        lp_select<NT, F32, V, R>(
+            S, kept, A.x, row0, A.n, mine, [&](auto f) { f(mine, t); },
+            [&](int g, int p) { return p * NT * V + g * V; }, [] {});
     lp_finish(A, row, T, m, log((double)P.l), P.l, P.h, S.top, xt, CAP);
 }
 
-// Parts of rows: 256 threads, 2^chunk_shift chunks of 32 logits a thread, a group
-// each, or (QUAD) one chunk of 8, a group being four neighbours'.
-template <bool F32, bool QUAD>
+// Parts of rows: 256 threads, 2^chunk_shift chunks of 32 logits a thread (SMALL: one
+// of 8).  A group is 32 logits that lie together, a word of LANES threads: what is
+// looked at again is a line of memory, not four.
+template <bool F32, bool SMALL>
 struct LpShape {
-    static constexpr int V = F32 ? 4 : 8, R = (QUAD ? 8 : 32) / V, CHUNK = 256 * R * V;
-    static constexpr int GROUPS = QUAD ? 64 : 256;  // of a chunk
+    static constexpr int V = F32 ? 4 : 8, R = (SMALL ? 8 : 32) / V, CHUNK = 256 * R * V, LANES = 32 / V;
+    static constexpr int GROUPS = CHUNK / 32;  // of a chunk; that of word r of threads LANES i, ... is R i + r
+    static_assert(R <= LANES, "a thread for each word");
     using Largest = std::conditional_t<F32, float, uint16_t>;
-    // logit e of 32 of group g of a row
-    DEV static int index(int g, int e) {
+    DEV static int place(int g, int piece) {
         const int chunk = g / GROUPS, i = g % GROUPS;
-        if constexpr (QUAD) return chunk * CHUNK + e / (4 * V) * (256 * V) + (4 * i + e / V % 4) * V + e % V;
-        else return chunk * CHUNK + e / V * (256 * V) + i * V + e % V;
+        return chunk * CHUNK + i % R * (256 * V) + i / R * 32 + piece * V;
     }
 };
-template <bool F32, bool CAP, bool QUAD>
+template <bool F32, bool CAP, bool SMALL>
 DEV void lp_part(const LpArgs& A) {
-    using P = LpShape<F32, QUAD>;
+    using P = LpShape<F32, SMALL>;
     const int row = blockIdx.x / A.parts, part = blockIdx.x % A.parts, t = threadIdx.x;
     const int first = part << A.chunk_shift, all = (A.n - 1) / P::CHUNK + 1, last = min(first + (1 << A.chunk_shift), all);
     const size_t row0 = (size_t)row * A.n;
@@ -710,14 +713,22 @@ DEV void lp_part(const LpArgs& A) {
     };
     auto all_chunks = [&](auto fast) {
         auto add = [&](int k, const Words& v) {
-            const float m = S.largest(v);
+            uint32_t word[P::R];
+#pragma unroll
+            for (int r = 0; r < P::R; r++) word[r] = lp_largest<F32, S.W>(v[r]);
+            const float m = lp_of<F32>(lp_largest<F32, P::R>(word));
             if (kept) {
-                float g = m;
-                if constexpr (QUAD) g = fmaxf(g, dpp_xor1(g)), g = fmaxf(g, dpp_xor2(g));
-                if (!QUAD || (t & 3) == 0) {
-                    typename P::Largest* o = to + k * P::GROUPS + (QUAD ? t >> 2 : t);
-                    if constexpr (F32) *o = g;
-                    else *o = (uint16_t)f2h(g);
+                const int i = t % P::LANES;
+                uint32_t g = 0;
+#pragma unroll
+                for (int r = 0; r < P::R; r++) {
+                    const uint32_t p = lp_lanes<F32, P::LANES>(word[r]);
+                    g = i == r ? p : g;
+                }
+                typename P::Largest* o = to + k * P::GROUPS + t / P::LANES * P::R + i;
+                if (i < P::R) {
+                    if constexpr (F32) *o = lp_of<F32>(g);
+                    else *o = (uint16_t)f2h(lp_of<F32>(g));
                 }
             }
             S.template add<fast>(v, m, A.cap, s);
@@ -741,15 +752,15 @@ DEV void lp_part(const LpArgs& A) {
 }
 
 // A row's parts joined: their sums brought to the largest m, its likeliest looked for.
-template <bool F32, bool CAP, bool QUAD>
+template <bool F32, bool CAP, bool SMALL>
 DEV void lp_join(const LpArgs& A) {
-    using P = LpShape<F32, QUAD>;
+    using P = LpShape<F32, SMALL>;
     constexpr int NT = 256, VG = F32 ? 4 : 8;  // groups of a load
     __shared__ LpTop<NT> S;
     const int row = blockIdx.x, t = threadIdx.x, lane = t & 63;
     const size_t row0 = (size_t)row * A.n;
     const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
-    const float xt = lp_load<F32>(A, row0, A.tokens ? A.tokens[row] : -1);
+    const float xt = lp_load<F32>(A.x, row0, A.tokens ? A.tokens[row] : -1, A.n);
     const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
     __shared__ double sums[3];
     __shared__ float largest;
@@ -785,20 +796,17 @@ DEV void lp_join(const LpArgs& A) {
             constexpr uint32_t NONE = F32 ? 0xff800000u : 0xfc00fc00u;
             q[u] = u * NT + t < loads ? from[u * NT + t] : make_uint4(NONE, NONE, NONE, NONE);
         }
-        float most = -INFINITY;
-        {
-            uint32_t a[K * 4];
+        uint32_t a[K * 4];
 #pragma unroll
-            for (int u = 0; u < K; u++) a[4 * u] = q[u].x, a[4 * u + 1] = q[u].y, a[4 * u + 2] = q[u].z, a[4 * u + 3] = q[u].w;
-            most = lp_largest<F32, K * 4>(a);
-            for (int i = K * NT + t; i < loads; i += NT) {
-                const uint4 z = from[i];
-                const uint32_t b[4] = {z.x, z.y, z.z, z.w};
-                most = fmaxf(most, lp_largest<F32, 4>(b));
-            }
+        for (int u = 0; u < K; u++) a[4 * u] = q[u].x, a[4 * u + 1] = q[u].y, a[4 * u + 2] = q[u].z, a[4 * u + 3] = q[u].w;
+        float most = lp_of<F32>(lp_largest<F32, K * 4>(a));
+        for (int i = K * NT + t; i < loads; i += NT) {
+            const uint4 z = from[i];
+            const uint32_t b[4] = {z.x, z.y, z.z, z.w};
+            most = fmaxf(most, lp_of<F32>(lp_largest<F32, 4>(b)));
         }
-        lp_select<NT, 32>(
-            S, kept, A.n, F32, most,
+        lp_select<NT, F32, P::V, P::LANES>(
+            S, kept, A.x, row0, A.n, most,
             [&](auto f) {
                 auto eight = [&](const uint4& v, int i) {
                     const uint32_t a[4] = {v.x, v.y, v.z, v.w};
@@ -813,7 +821,7 @@ DEV void lp_join(const LpArgs& A) {
                     if (u * NT + t < loads) eight(q[u], u * NT + t);
                 for (int i = K * NT + t; i < loads; i += NT) eight(from[i], i);
             },
-            P::index, [&](int i) { return lp_load<F32>(A, row0, i); }, join);
+            P::place, join);
         if (t >= 64) return;
     }
     lp_finish(A, row, T, largest, sums[0], sums[1], sums[2], S.top, xt, CAP);
@@ -822,12 +830,12 @@ DEV void lp_join(const LpArgs& A) {
     extern "C" __global__ __launch_bounds__(NT) void cima_logprobs_t##NT##_w##R##_##NAME(const LpArgs A) { \
         lp_whole<F32, CAP, NT, F32 ? R : R / 2, F32 ? 4 : 8>(A);                                           \
     }
-#define LOGPROBS_PARTS(NAME, F32, CAP, R, QUAD)                                                           \
+#define LOGPROBS_PARTS(NAME, F32, CAP, R, SMALL)                                                           \
     extern "C" __global__ __launch_bounds__(256) void cima_logprobs_part_w##R##_##NAME(const LpArgs A) {  \
-        lp_part<F32, CAP, QUAD>(A);                                                                        \
+        lp_part<F32, CAP, SMALL>(A);                                                                        \
     }                                                                                                      \
     extern "C" __global__ __launch_bounds__(256) void cima_logprobs_join_w##R##_##NAME(const LpArgs A) {  \
-        lp_join<F32, CAP, QUAD>(A);                                                                        \
+        lp_join<F32, CAP, SMALL>(A);                                                                        \
     }
 #define LOGPROBS(NAME, F32, CAP)            \
     LOGPROBS_WHOLE(NAME, F32, CAP, 256, 2)  \
