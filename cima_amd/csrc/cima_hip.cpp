@@ -1691,7 +1691,9 @@ struct PagedAttnArgs {
 };
 
 // few_wgs in paged_attn.hip: workgroups to a CU
-int paged_few_wgs(int dim, int mode, int nb) { return mode == 0 && !(dim == 128 && nb == 2) ? 4 : 2; }
+int paged_few_wgs(int bits, int dim, int mode, int nb) {
+    return mode || (dim == 128 && nb == 2) ? 2 : bits == 8 && (dim == 128 || nb == 2) ? 3 : 4;
+}
 // LDS of Few<dim, nb, bufs> and of Tile<dim, 2 or 4, 2 or 1> in paged_attn.hip
 unsigned paged_few_lds(int dim, int nb, int bufs) {
     return (unsigned)(4 * std::max(bufs * 32 * dim * 2, nb * (dim / 16) * 64 * 16) + 4 * nb * 16 * 8);
@@ -1806,7 +1808,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     // 19.0, 80 rows 20.3 / 20.4, 63 rows of 64 17.2 / 18.7.
     const bool few = prefix_pages && head_rows <= 16;
     const int mode = !prefix_pages || few ? 0 : head_rows <= 64 ? 1 : 2;
-    const int wgs = paged_few_wgs(dim, mode, nb);
+    const int wgs = paged_few_wgs(kv_bits(kv), dim, mode, nb);
     // Parts of own tasks: as many as have 128 positions in a full table, in at most
     // two rounds of the chip.  A slot's positions are shared by all of them (128 at
     // least), so that slots of any length load the XCDs, which take workgroups in
@@ -1900,7 +1902,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     else snprintf(name, sizeof name, "cima_attn_paged_d%d_m%d_n%d", dim, kind, nb);
     if (int rc = get_fn(ctx, name, &f)) return rc;
     void* args[] = {&A};
-    const int bufs = kv->ggml_type || paged_few_wgs(dim, kind, nb) == 4 ? 1 : 2;
+    const int bufs = kv->ggml_type || paged_few_wgs(16, dim, kind, nb) == 4 ? 1 : 2;
     const unsigned lds = std::max(paged_few_lds(dim, nb, bufs), mode ? paged_attn_lds(dim) : 0u);
     if (int rc = launch(ctx, f, (unsigned)grid, 256, args, api, lds)) return rc;
     if (all == 1) return 0;

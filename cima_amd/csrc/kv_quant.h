@@ -42,11 +42,14 @@ struct KvQ {
                 const kvh2 off = {(_Float16)-1024.f, (_Float16)-1024.f}, off4 = {(_Float16)-64.f, (_Float16)-64.f};
                 const kvh2 down4 = {(_Float16)0.0625f, (_Float16)0.0625f};
                 const uint32_t v = w[0] >> 8;
+                // in a vector register: and, or in one instruction, which takes one scalar
+                uint32_t one = 0x64006400u;
+                __asm__("" : "+v"(one));
                 kvh2 c[4];
-                c[0] = __builtin_bit_cast(kvh2, (w[0] & 0x000f000fu) | 0x64006400u) + off;
-                c[1] = __builtin_elementwise_fma(__builtin_bit_cast(kvh2, (w[0] & 0x00f000f0u) | 0x64006400u), down4, off4);
-                c[2] = __builtin_bit_cast(kvh2, (v & 0x000f000fu) | 0x64006400u) + off;
-                c[3] = __builtin_elementwise_fma(__builtin_bit_cast(kvh2, (v & 0x00f000f0u) | 0x64006400u), down4, off4);
+                c[0] = __builtin_bit_cast(kvh2, (w[0] & 0x000f000fu) | one) + off;
+                c[1] = __builtin_elementwise_fma(__builtin_bit_cast(kvh2, (w[0] & 0x00f000f0u) | one), down4, off4);
+                c[2] = __builtin_bit_cast(kvh2, (v & 0x000f000fu) | one) + off;
+                c[3] = __builtin_elementwise_fma(__builtin_bit_cast(kvh2, (v & 0x00f000f0u) | one), down4, off4);
 #pragma unroll
                 for (int i = 0; i < 4; i++)
                     o[i] = __builtin_bit_cast(uint32_t, __builtin_elementwise_fma(c[i], d, m));

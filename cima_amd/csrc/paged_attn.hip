@@ -678,9 +678,19 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 // to 4000 positions (524 MB) 107 / 146 us (4.9 TB/s), 128 of up to 500 27 / 33;
 // 128 full slots of 8192 (4.3 GB) 765 us with the join, 5.6 TB/s.  Values by
 // loads to registers and LDS writes: 127 and 36 us.
-constexpr int few_wgs(int D, int mode, int nb) { return mode == 0 && !(D == 128 && nb == 2) ? 4 : 2; }
+constexpr int few_wgs(int D, int mode, int nb) {
+    return mode || (D == 128 && nb == 2) ? 2 : BITS == 8 && (D == 128 || nb == 2) ? 3 : 4;
+}
 // a quantised cache's tiles wait in registers as codes: one buffer of values
 constexpr int few_bufs(int D, int mode, int nb) { return BITS != 16 || few_wgs(D, mode, nb) == 4 ? 1 : 2; }
+// Word w of a row of values is stored as word w ^ f: with it neither the transposing
+// reads (four rows, two words each) nor what writes the row (a direct copy; of a
+// quantised cache eight rows' lanes, a word each) meet bank conflicts.
+template <int D>
+DEV int few_flip(int row) {
+    if constexpr (BITS != 16) return (row & 3) << 1 | (row >> 2 & 1);
+    return D == 128 ? (row & 7) << 1 : (row >> 1 & 3) << 1;
+}
 constexpr int OWN_LEAST = 4;  // tiles that a part of an own task has at least, where there are
 template <int D, int NB, int BUFS>
 struct Few {
@@ -799,7 +809,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
             for (int c = 0; c < D / 32; c++) {
                 const int row = c * (64 / CH) + lane / CH, w = lane % CH;
                 const int p = min(max(p0 + row, lo_any), hi_any - 1) & (page - 1);
-                const int f = D == 128 ? (row & 7) << 1 : (row >> 1 & 3) << 1;
+                const int f = few_flip<D>(row);
                 const uint16_t* at = vsrc + (size_t)p * D;
                 if (slots && !(seen >> row & 1)) at = reinterpret_cast<const uint16_t*>(no_page);
                 dma16(at + 8 * (w ^ f), vbase + buf * F::VT + u * 16 * D * 2 + c * 1024);
@@ -822,7 +832,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
             now = gone[0];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
-                const int f = D == 128 ? (li & 7) << 1 : (li >> 1 & 3) << 1;
+                const int f = few_flip<D>(li);
                 uint8_t* to = lds + wave * F::WAVE + (16 * u + li) * D * 2;
 #pragma unroll
                 for (int i = 0; i < STEPS; i++) {
@@ -908,7 +918,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int row = 16 * u + 4 * q4 + (li >> 2), w = 2 * x + ((li & 3) >> 1);
-                const int f = D == 128 ? (row & 7) << 1 : (row >> 1 & 3) << 1;
+                const int f = few_flip<D>(row);
                 vv[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                     (lp)(uintptr_t)(vbase + buf * F::VT + row * D * 2 + (w ^ f) * 16 + (li & 1) * 8));
             }
