@@ -666,7 +666,7 @@ int cima_hip_init(int device, const char* code_dir, cima_hip_ctx** out) {
             if (!rc) rc = add(MOD_PAGED_ATTN, name);
         }
         for (int bits : {4, 8})
-            for (int mode : {0, 1, 2})
+            for (int mode : {0, 1, 2, 3})
                 for (int nb : {1, 2}) {
                     snprintf(name, sizeof name, "cima_attn_paged_q%d_d%d_m%d_n%d", bits, dim, mode, nb);
                     if (!rc) rc = add(bits == 4 ? MOD_PAGED_ATTN_Q4 : MOD_PAGED_ATTN_Q8, name);
@@ -1692,7 +1692,8 @@ struct PagedAttnArgs {
 
 // few_wgs in paged_attn.hip: workgroups to a CU
 int paged_few_wgs(int bits, int dim, int mode, int nb) {
-    return mode || (dim == 128 && nb == 2) ? 2 : bits == 8 && (dim == 128 || nb == 2) ? 3 : 4;
+    if (mode == 3 && nb == 1) return paged_few_wgs(bits, dim, 0, 2);
+    return (mode && mode != 3) || (dim == 128 && nb == 2) ? 2 : bits == 8 && (dim == 128 || nb == 2) ? 3 : 4;
 }
 // LDS of Few<dim, nb, bufs> and of Tile<dim, 2 or 4, 2 or 1> in paged_attn.hip
 unsigned paged_few_lds(int dim, int nb, int bufs) {
@@ -1806,8 +1807,15 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     // one side / the other: 16 rows of 128, 8000 positions 14.8 / 17.4, 8 rows, 512
     // 9.0 / 10.0, 24 rows, 8000 20.9 / 16.6; 64 rows a tile / 128: 40 rows 17.8 /
     // 19.0, 80 rows 20.3 / 20.4, 63 rows of 64 17.2 / 18.7.
-    const bool few = prefix_pages && head_rows <= 16;
-    const int mode = !prefix_pages || few ? 0 : head_rows <= 64 ? 1 : 2;
+    // Of quantised pages few-row tasks take 32 rows at a time and more of them: they
+    // wait for nothing, where the tiles' waves wait for each other's decoding.  Q4_1,
+    // tiles / few-row tasks, us, over 4096 and 30016: 32 rows of 128 14.6 / 13.5, 29.6 /
+    // 23.1, 64 rows 15.3 / 13.7, 32.1 / 30.2, 128 rows 18.8 / 16.7, 40.3 / 44.3; 56 rows of 64
+    // 11.6 / 10.8, 19.5 / 15.1, 224 rows 13.4 / 11.3, 23.4 / 22.3, 896 rows 17.2 / 17.6, 40.9 /
+    // 47.8; Q8_0, 64 rows of 128 16.1 / 14.8, 35.3 / 33.7.
+    const int few_rows = !kv->ggml_type ? 16 : dim == 64 ? 256 : 64;
+    const bool few = prefix_pages && head_rows <= few_rows;
+    const int mode = !prefix_pages || (few && head_rows <= 16) ? 0 : few ? 3 : head_rows <= 64 ? 1 : 2;
     const int wgs = paged_few_wgs(kv_bits(kv), dim, mode, nb);
     // Parts of own tasks: as many as have 128 positions in a full table, in at most
     // two rounds of the chip.  A slot's positions are shared by all of them (128 at
@@ -1831,15 +1839,29 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     // 9.6; beside few-row tasks 2 of 32/8 of 128 13.5 / 12.1.
     long long own = (own_room + 127) / 128;
     while (own > 1 && own_base * own > 2LL * wgs * ctx->num_cu) own = (own + 1) / 2;
-    if (prefix_pages ? (own_room <= (dim == 64 ? 640 : 512) && 3 * own_base >= ctx->num_cu) || (mode && own_room <= 256)
+    if (kv->ggml_type) {
+        // Quantised: the tasks are shorter, their joins not.  Parts of 256 positions up to
+        // four to a CU, of 750 up to sixteen where the tasks alone are more than one to a
+        // CU; one where they are one for each 1024 positions.  32/8 heads of 128, Q4_1, us
+        // by parts 1 / 2 / 4 / 8 / 16: 8 slots of up to 2000 24 / 17 / 12.5 / 11.5 / 12.9,
+        // 32 of up to 700 11.9 / 13.3 / 13.3 / 17 / 28, of 6000 65 / 46 / 38 / 40 / 45, 64 of
+        // 2000 30 / 29 / 30 / 36 / 53, of 6000 80 / 71 / 70 / 69 / 82, 128 of 2000 47 / 52 /
+        // 54 / 65 / 99, of 6000 125 / 123 / 120 / 128 / 153, 256 of 6000 219 / 217 / 224 / 242 /
+        // 271; Q8_0, 64 of 6000 107 / 109 / 102 / 102 / 114, 128 of 6000 197 / 187 / 180 / 192 /
+        // 217; 14/2 of 64, 32 slots of 4000 30 / 20 / 14 / 12 / 12.  Behind a prefix of 4096, 1 /
+        // 2 / 4 / 8: 8 slots of 1000 20.5 / 16.3 / 14.4 / 16.3, 128 of 1000 49 / 51 / 60 / 88.
+        const bool few = own_base <= ctx->num_cu;
+        own = std::min(own_room / (few ? 256 : 750), ((few ? 4LL : 16LL) * ctx->num_cu + own_base - 1) / own_base);
+        if (own_room <= brief || own_base * 1024 >= own_room * ctx->num_cu) own = 1;
+    } else if (prefix_pages ? (own_room <= (dim == 64 ? 640 : 512) && 3 * own_base >= ctx->num_cu) || (mode && own_room <= 256)
                      : own_room <= brief || own_base * 1024 >= std::min(own_room, 2048LL) * ctx->num_cu)
         own = 1;
     own = std::max(1LL, std::min(own, 64LL));
     int tiles = 0;
     long long pre = 0;
     if (prefix_pages) {
-        const int per = 64 * mode;  // rows of a tile
-        tiles = few ? 1 : (head_rows + per - 1) / per;
+        const int per = mode == 0 ? 16 : mode == 3 ? 32 : 64 * mode;  // rows of a tile
+        tiles = (head_rows + per - 1) / per;
         const long long base = (long long)kv->kv_heads * tiles, len = (long long)prefix_pages * kv->page;
         // a workgroup to a CU; two where each still has 512 positions, half of one
         // where the own tasks have much to read (256 KB a CU in full tables).  With
@@ -1885,7 +1907,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     A.own_parts = (int)own;
     A.row_tiles = tiles;
     A.scale2 = scale * 1.44269504088896340736f;
-    A.prefix_tile = few ? 16 : 32;
+    A.prefix_tile = mode == 0 ? 16 : 32;
     A.own_tile = 16 * nb;
     char name[64];
     hipFunction_t f;
@@ -1903,7 +1925,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     if (int rc = get_fn(ctx, name, &f)) return rc;
     void* args[] = {&A};
     const int bufs = kv->ggml_type || paged_few_wgs(16, dim, kind, nb) == 4 ? 1 : 2;
-    const unsigned lds = std::max(paged_few_lds(dim, nb, bufs), mode ? paged_attn_lds(dim) : 0u);
+    const unsigned lds = std::max(paged_few_lds(dim, mode == 3 ? 2 : nb, bufs), mode == 1 || mode == 2 ? paged_attn_lds(dim) : 0u);
     if (int rc = launch(ctx, f, (unsigned)grid, 256, args, api, lds)) return rc;
     if (all == 1) return 0;
     const long long join = (long long)kv->kv_heads * ((head_rows + 15) / 16) * (dim / 16);

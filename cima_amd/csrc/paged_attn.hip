@@ -678,8 +678,10 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 // to 4000 positions (524 MB) 107 / 146 us (4.9 TB/s), 128 of up to 500 27 / 33;
 // 128 full slots of 8192 (4.3 GB) 765 us with the join, 5.6 TB/s.  Values by
 // loads to registers and LDS writes: 127 and 36 us.
+constexpr int prefix_nb(int mode) { return mode == 3 ? 2 : 1; }  // 16-row blocks of a few-row prefix task
 constexpr int few_wgs(int D, int mode, int nb) {
-    return mode || (D == 128 && nb == 2) ? 2 : BITS == 8 && (D == 128 || nb == 2) ? 3 : 4;
+    if (mode == 3 && nb == 1) return few_wgs(D, 0, 2);
+    return (mode && mode != 3) || (D == 128 && nb == 2) ? 2 : BITS == 8 && (D == 128 || nb == 2) ? 3 : 4;
 }
 // a quantised cache's tiles wait in registers as codes: one buffer of values
 constexpr int few_bufs(int D, int mode, int nb) { return BITS != 16 || few_wgs(D, mode, nb) == 4 ? 1 : 2; }
@@ -790,8 +792,12 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
             uint32_t seen = 0xffff;  // bit i: position p0 + i
             if (slots && lo_all > hi_all) {
                 seen = 0;
-                for (int i = 0, p = p0; i < 16; i++, p++)
-                    if (__ballot(live[0] && lo[0] <= p && p < hi[0])) seen |= 1u << i;
+                for (int i = 0, p = p0; i < 16; i++, p++) {
+                    bool any = live[0] && lo[0] <= p && p < hi[0];
+#pragma unroll
+                    for (int b = 1; b < NB; b++) any |= live[b] && lo[b] <= p && p < hi[b];
+                    if (__ballot(any)) seen |= 1u << i;
+                }
             }
             if constexpr (BITS != 16) {
                 const int pk = min(max(p0 + li, lo_any), hi_any - 1) & (page - 1);
@@ -1016,9 +1022,10 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
         if (grp >= A.kv_heads * A.prefix_parts) return;
         const int kvh = grp / A.prefix_parts, part = grp % A.prefix_parts, phi = A.prefix_pages << A.page_shift;
         const int* trow = A.table + (size_t)A.prefix_slot * A.table_stride;
-        if constexpr (MODE == 0 && NB == 1)
-            few_task<D, NB, BUFS>(A, lds, kvh, 0, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
-                            ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1, true);
+        if constexpr ((MODE == 0 && NB == 1) || MODE >= 3)
+            few_task<D, prefix_nb(MODE), BUFS>(
+                A, lds, kvh, tile * 16 * prefix_nb(MODE), A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
+                ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1, true);
         else if constexpr (MODE == 1)
             attn_task<D, 2, 2>(A, lds, kvh, tile * 64, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
         else if constexpr (MODE == 2)
@@ -1056,6 +1063,12 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
     ATTN(D, 2, 2)
 ATTN_ALL(64)
 ATTN_ALL(128)
+#if CIMA_KV_BITS != 16
+ATTN(64, 3, 1)
+ATTN(64, 3, 2)
+ATTN(128, 3, 1)
+ATTN(128, 3, 2)
+#endif
 
 #if CIMA_KV_BITS == 16  // the partial sums are the same for every cache
 // The parts of a row joined: out = sum_c 2^(m_c - M) acc_c / sum_c 2^(m_c - M)
