@@ -410,11 +410,17 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
                 if (ids[page_of(p0 + kw + 16 * j) - ids_from] < 0) end[j] = 0;
         }
         float mx = -INFINITY;
+        int first = 0;
+        if constexpr (BITS != 16) {
+            first = p0 + kw + 4 * half;
+            __asm__ volatile("" : "+v"(first));  // no part of the sums kept from tile to tile
+        }
 #pragma unroll
         for (int b = 0; b < T::KB; b++)
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const int p = p0 + kw + 32 * b + (i & 3) + 8 * (i >> 2) + 4 * half;
+                const int p = BITS == 16 ? p0 + kw + 32 * b + (i & 3) + 8 * (i >> 2) + 4 * half
+                                         : first + 32 * b + (i & 3) + 8 * (i >> 2);
                 sc[b][i] = p >= lo && p < end[2 * b + (i >> 3)] ? sc[b][i] : -INFINITY;
                 mx = fmaxf(mx, sc[b][i]);
             }
@@ -678,7 +684,6 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 // to 4000 positions (524 MB) 107 / 146 us (4.9 TB/s), 128 of up to 500 27 / 33;
 // 128 full slots of 8192 (4.3 GB) 765 us with the join, 5.6 TB/s.  Values by
 // loads to registers and LDS writes: 127 and 36 us.
-constexpr int prefix_nb(int mode) { return mode == 3 ? 2 : 1; }  // 16-row blocks of a few-row prefix task
 constexpr int few_wgs(int D, int mode, int nb) {
     if (mode == 3 && nb == 1) return few_wgs(D, 0, 2);
     return (mode && mode != 3) || (D == 128 && nb == 2) ? 2 : BITS == 8 && (D == 128 || nb == 2) ? 3 : 4;
@@ -732,7 +737,8 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
         qrow[b] = (size_t)sj * A.q_heads + kvh * g + (rr - sj * g);
 #pragma unroll
         for (int i = 0; i < STEPS; i++)
-            qf[b][i] = *reinterpret_cast<const h8*>(A.q + qrow[b] * D + (BITS == 16 ? 32 * i + 8 * q4 : D / 4 * q4 + 8 * i));
+            if constexpr (BITS == 16) qf[b][i] = *reinterpret_cast<const h8*>(A.q + qrow[b] * D + 32 * i + 8 * q4);
+            else qf[b][i] = *reinterpret_cast<const h8*>(A.q + qrow[b] * D + D / 4 * q4 + 8 * i);
     }
     int lo_any = 0x7fffffff, hi_any = 0, lo_all = 0, hi_all = 0x7fffffff;
 #pragma unroll
@@ -774,7 +780,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
     const int page = 1 << A.page_shift;
     const uint32_t vbase = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint8_t*)lds + wave * F::WAVE;
     h8 kf[BUFS][2][STEPS];
-    uint32_t gone[BUFS];  // bit u: group u of the tile has no page
+    uint32_t gone[BITS == 16 ? BUFS : 2];  // bit u: group u of the tile has no page
     Raw<D> kraw[2], vraw[2];
     auto issue = [&](int t, auto buf) {
         gone[buf] = 0;
@@ -824,18 +830,14 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
     };
     auto step = [&](int t, auto buf) {
         f4 kq[NB][2];  // a quantised cache's scores
-        uint32_t now = 0;
-        auto none = [&]() -> uint32_t& {
-            if constexpr (BITS == 16) return gone[buf];
-            else return now;
-        };
+        constexpr int NOW = BITS == 16 ? (int)decltype(buf)::value : 1;
         if constexpr (BITS == 16) {
             if constexpr (BUFS == 1) issue(t, buf);
             wait_vm<0>();
             if constexpr (BUFS == 2)
                 if (t + 4 < t1) issue(t + 4, std::integral_constant<int, 1 - buf>{});
         } else {
-            now = gone[0];
+            gone[1] = gone[0];
 #pragma unroll
             for (int u = 0; u < 2; u++) {
                 const int f = few_flip<D>(li);
@@ -863,7 +865,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
             __builtin_amdgcn_sched_barrier(0);
         }
         const int p0 = base + 32 * t;
-        __asm__ volatile("" : "+s"(none()));  // one path for the tile, by one test
+        __asm__ volatile("" : "+s"(gone[NOW]));  // one path for the tile, by one test
         h8 pf[NB];
 #pragma unroll
         for (int b = 0; b < NB; b++) {
@@ -879,10 +881,10 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
                 for (int i = 0; i < STEPS; i++)
                     sc[u] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kf[buf][u][i], qf[b][i], sc[u], 0, 0, 0);
             }
-            if (p0 < lo_all || p0 + 32 > hi_all || none()) {
+            if (p0 < lo_all || p0 + 32 > hi_all || gone[NOW]) {
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const int end = none() >> u & 1 ? 0 : hi[b];
+                    const int end = gone[NOW] >> u & 1 ? 0 : hi[b];
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const int p = p0 + 16 * u + 4 * q4 + i;
@@ -1022,10 +1024,12 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
         if (grp >= A.kv_heads * A.prefix_parts) return;
         const int kvh = grp / A.prefix_parts, part = grp % A.prefix_parts, phi = A.prefix_pages << A.page_shift;
         const int* trow = A.table + (size_t)A.prefix_slot * A.table_stride;
-        if constexpr ((MODE == 0 && NB == 1) || MODE >= 3)
-            few_task<D, prefix_nb(MODE), BUFS>(
-                A, lds, kvh, tile * 16 * prefix_nb(MODE), A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
-                ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1, true);
+        if constexpr (MODE == 0 && NB == 1)
+            few_task<D, NB, BUFS>(A, lds, kvh, 0, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
+                            ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1, true);
+        else if constexpr (MODE == 3)
+            few_task<D, 2, BUFS>(A, lds, kvh, tile * 32, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
+                            ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1, true);
         else if constexpr (MODE == 1)
             attn_task<D, 2, 2>(A, lds, kvh, tile * 64, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
         else if constexpr (MODE == 2)
