@@ -77,6 +77,18 @@ def test_code_objects_hold_every_kernel():
             assert k.encode() in blob, k
 
 
+def test_quantised_kernels_do_not_spill():
+    """Attention, append, read back and log probabilities keep every value in registers."""
+    from test_abi import _kernel_notes
+
+    notes = {}
+    for name in ("paged", "paged_attn_q4", "paged_attn_q8", "sample"):
+        notes.update(_kernel_notes(cbuild.HSACOS[name]))
+    mine = {k: v for k, v in notes.items() if "paged_q" in k or "kv_pages_read" in k or "logprobs" in k}
+    assert len(mine) == 2 * 16 + 4 + 6 + 28
+    assert not {k: v for k, v in mine.items() if v[1] > 0}
+
+
 def test_read_back_refuses_a_missing_context():
     L = hipmod.load_library()
     rc = L.cima_hip_kv_pages_read(None, ctypes.byref(hipmod.KvPages()), 0, None, None, None, None, 1, 1, 1)
