@@ -920,6 +920,34 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
         }
         typedef __attribute__((address_space(3))) s4* lp;
         typedef short s8 __attribute__((ext_vector_type(8)));
+        if constexpr (BITS != 16) {
+            // read two products ahead: a short task waits for its own reads alone (32 slots
+            // of up to 700 11.6 -> 10.8 us; long ones, whose waves cover each other, the same)
+            constexpr int AHEAD = 2;
+            s8 vf[AHEAD];
+            auto frag = [&](int x) {
+                s4 vv[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const int row = 16 * u + 4 * q4 + (li >> 2), w = 2 * x + ((li & 3) >> 1);
+                    vv[u] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lp)(uintptr_t)(vbase + row * D * 2 + (w ^ few_flip<D>(row)) * 16 + (li & 1) * 8));
+                }
+                return __builtin_shufflevector(vv[0], vv[1], 0, 1, 2, 3, 4, 5, 6, 7);
+            };
+#pragma unroll
+            for (int x = 0; x < AHEAD; x++) vf[x] = frag(x);
+            __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+            for (int x = 0; x < XT; x++) {
+#pragma unroll
+                for (int b = 0; b < NB; b++)
+                    o[b][x] = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, vf[x % AHEAD]), pf[b], o[b][x], 0, 0, 0);
+                if (x + AHEAD < XT) vf[x % AHEAD] = frag(x + AHEAD);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+            return;
+        }
 #pragma unroll
         for (int x = 0; x < XT; x++) {
             s4 vv[2];
