@@ -10,7 +10,7 @@ q is rounded once more); log probabilities as in test_gpu_logprobs.py.
 import numpy as np
 import pytest
 from test_gpu_logprobs import _near, _want
-from test_gpu_paged import EPS16, THETA, _attend, _check, _i32
+from test_gpu_paged import EPS16, THETA, Batch, _attend, _check, _i32
 from test_gpu_paged_quant import TYPES, QBatch, quantise, values
 
 torch = pytest.importorskip("torch")
@@ -275,3 +275,23 @@ def test_attention_of_many_slots(hip, t):
     q = b.r.standard_normal((b.rows, b.q_heads, b.D)).astype(np.float16)
     got = _attend(hip, b, q)
     assert not got[np.array(lens) < 0].any()
+
+
+@pytest.mark.parametrize("t", [0, *TYPES], ids=str)
+@pytest.mark.parametrize("heads", [(14, 2, 64), (32, 8, 128)], ids=str)
+def test_a_slot_handed_to_the_single_sequence_attention(hip, t, heads):
+    """A slot read out of the pages is the contiguous cache of attn_decode: both
+    attentions are within their bound of the same 64-bit result."""
+    Q, H, D = heads
+    lens, room, csz = [40, 333], 512, 128
+    b = QBatch(t, lens, 1, heads, 16, seed=33) if t else Batch(lens, 1, heads, 16, seed=33)
+    q = b.r.standard_normal((b.rows, Q, D)).astype(np.float16)
+    qd = torch.from_numpy(q).cuda()
+    k, v = (torch.zeros((1, H, room, D), dtype=torch.float16, device="cuda") for _ in range(2))
+    out = torch.empty((Q, D), dtype=torch.float16, device="cuda")
+    hip.kv_pages_read(b.kv, 0, k, v, 1, 334, slots=_i32([1]), max_seq=room)
+    hip.attn_decode_noalloc(qd[1], k, v, out, Q, H, D, 334, room, csz, -(-room // csz), 1 / np.sqrt(D))
+    paged = _attend(hip, b, q)[1]
+    want, tol = (x[1] for x in b.want(q, 1 / np.sqrt(D), 0))
+    assert (np.abs(paged - want) <= tol).all()
+    assert (np.abs(out.cpu().numpy().astype(np.float64) - want) <= tol).all()
