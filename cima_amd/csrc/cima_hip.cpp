@@ -1688,6 +1688,7 @@ struct PagedAttnArgs {
     int prefix_pages, prefix_slot, window;
     int prefix_parts, own_parts, row_tiles, prefix_tile, own_tile, prefix_wgs;
     float scale2;
+    int by_length;
 };
 
 // few_wgs in paged_attn.hip: workgroups to a CU
@@ -1840,19 +1841,24 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     long long own = (own_room + 127) / 128;
     while (own > 1 && own_base * own > 2LL * wgs * ctx->num_cu) own = (own + 1) / 2;
     if (kv->ggml_type) {
-        // Quantised: the tasks are shorter, their joins not.  Parts of 256 positions up to
-        // four to a CU, of 750 up to sixteen where the tasks alone are more than one to a
-        // CU; one where they are one for each 1024 positions.  32/8 heads of 128, Q4_1, us
-        // by parts 1 / 2 / 4 / 8 / 16: 8 slots of up to 2000 24 / 17 / 12.5 / 11.5 / 12.9,
-        // 32 of up to 700 11.9 / 13.3 / 13.3 / 17 / 28, of 6000 65 / 46 / 38 / 40 / 45, 64 of
-        // 2000 30 / 29 / 30 / 36 / 53, of 6000 80 / 71 / 70 / 69 / 82, 128 of 2000 47 / 52 /
-        // 54 / 65 / 99, of 6000 125 / 123 / 120 / 128 / 153, 256 of 6000 219 / 217 / 224 / 242 /
-        // 271; Q8_0, 64 of 6000 107 / 109 / 102 / 102 / 114, 128 of 6000 197 / 187 / 180 / 192 /
-        // 217; 14/2 of 64, 32 slots of 4000 30 / 20 / 14 / 12 / 12.  Behind a prefix of 4096, 1 /
-        // 2 / 4 / 8: 8 slots of 1000 20.5 / 16.3 / 14.4 / 16.3, 128 of 1000 49 / 51 / 60 / 88.
+        // Quantised: the tasks are shorter, their joins not, and taken by their lengths
+        // (below) few parts do.  Parts of 256 positions up to four to a CU; where the tasks
+        // alone are more than one to a CU of 750 up to two rounds of the chip, behind a
+        // prefix up to sixteen to a CU; one where they are one for each 1024 positions (two
+        // for tasks of 32 rows without one).  32/8 heads of 128, Q4_1, us by parts 1 / 2 / 3 / 4 / 8 / 16: 32
+        // slots of up to 700 11.5 / 13 / 13 / 13 / 21 / 34, of 2000 21.6 / 20 / 18.6 / 18 / 23 / 35, 64
+        // of 6000 80 / 70 / 63 / 62 / 68 / 87, of 12000 154 / 126 / 112 / 109 / 112 / 128, 128 of 2000
+        // 45 / 49 / 52 / 57 / 78 / 129, of 6000 122 / 110 / 110 / 115 / 129 / 169, 256 of 6000 191 /
+        // 202 / 208 / 217 / 254 / 317; Q8_0, 64 of 6000 107 / 92 / 90 / 91 / 100 / 125, 128 of 6000
+        // 160 / 164 / 166 / 173 / 193 / 245; 14/2 of 64, 64 slots of 4000 28 / 19 / 18 / 15 / 15 / 19;
+        // 128 slots x 5 tokens of 28/4 heads, of 4000 85 / 103 / 113 / 125 / 159 / 160.  Behind a
+        // prefix of 4096, 1 / 2 / 4 / 8: 8 slots of 1000 20.5 / 16.3 / 14.4 / 16.3, 128 of 1000 49 /
+        // 51 / 60 / 88.
         const bool few = own_base <= ctx->num_cu;
-        own = std::min(own_room / (few ? 256 : 750), ((few ? 4LL : 16LL) * ctx->num_cu + own_base - 1) / own_base);
-        if (own_room <= brief || own_base * 1024 >= own_room * ctx->num_cu) own = 1;
+        own = few           ? std::min(own_room / 256, (4LL * ctx->num_cu + own_base - 1) / own_base)
+              : prefix_pages ? std::min(own_room / 750, (16LL * ctx->num_cu + own_base - 1) / own_base)
+                             : std::min(own_room / 750, 2LL * wgs * ctx->num_cu / own_base);
+        if (own_room <= brief || own_base * (prefix_pages ? 1 : nb) * 1024 >= own_room * ctx->num_cu) own = 1;
     } else if (prefix_pages ? (own_room <= (dim == 64 ? 640 : 512) && 3 * own_base >= ctx->num_cu) || (mode && own_room <= 256)
                      : own_room <= brief || own_base * 1024 >= std::min(own_room, 2048LL) * ctx->num_cu)
         own = 1;
@@ -1916,6 +1922,14 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     if (grid > kMaxGrid)
         return fail(CIMA_E_INVALID, "%s: %lld workgroups (less than 2^24: %d slots of %d rows, %d kv heads)", api, grid,
                     seqs, own_rows, kv->kv_heads);
+    // Slots taken by their lengths, which every wave has to look up first: where they are
+    // two tasks to a CU, or have 2048 positions to a CU.  us, by number / by length: 64
+    // slots of 8 heads of 128 of up to 700 14.0 / 12.5, 32 of 2000 18.0 / 17.5, of 6000 37.8 /
+    // 34.2, 16 of 12000 36.5 / 34.0; but 4 of 12000 15.6 / 17.1, 8 of 3000 13.6 / 14.2, 128 of
+    // 2 heads of 64 of 1000 12.4 / 13.6.  Not beside prefix tasks: 64 slots of 4000 behind
+    // 4096 65 / 67, 64 of 6000 behind 8192 92 / 100.
+    A.by_length = kv->ggml_type && !pre && seqs > 1 && seqs <= 256 &&
+                  (own_base >= 2LL * ctx->num_cu || own_base * own_room >= 2048LL * ctx->num_cu);
     // Own tasks of f16 alone, no more than two to a CU, run in a kernel that has two of
     // their tiles in flight.  us, one / two: 16 slots of 8 heads of 128 up to 300 7.9 /
     // 7.5, 32 of them 9.2 / 8.7, 4 slots of 14/2 heads of 64 over 573 7.7 / 7.3.
