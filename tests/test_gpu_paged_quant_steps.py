@@ -295,3 +295,63 @@ def test_a_slot_handed_to_the_single_sequence_attention(hip, t, heads):
     want, tol = (x[1] for x in b.want(q, 1 / np.sqrt(D), 0))
     assert (np.abs(paged - want) <= tol).all()
     assert (np.abs(out.cpu().numpy().astype(np.float64) - want) <= tol).all()
+
+
+# --------------------------------------------- slots in the order of their lengths
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("seqs,n_new,window", [(130, 1, 0), (256, 1, 0), (257, 1, 0), (129, 5, 0), (150, 1, 40)])
+def test_attention_of_slots_taken_by_length(hip, t, seqs, n_new, window):
+    """Lengths of every kind and number: each slot is served once."""
+    r = np.random.default_rng(seqs)
+    for lens in (r.integers(-1, 200, seqs), np.full(seqs, 37), np.where(np.arange(seqs) == seqs - 1, 600, -1),
+                 np.arange(seqs) * 2, np.zeros(seqs)):
+        _check(hip, QBatch(t, [int(n) for n in lens], n_new, (8, 4, 64), 32, seed=34), window)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_lengths_out_of_range_do_no_harm(hip, t):
+    """Lengths behind the table and below -1: the other slots' results are what they
+    are alone, slots of negative lengths have zeros."""
+    b = QBatch(t, [70 + 3 * i for i in range(140)], 1, (8, 4, 64), 32, seed=35)
+    q = b.r.standard_normal((b.rows, 8, 64)).astype(np.float16)
+    want = _attend(hip, b, q)
+    odd = {3: 2 ** 31 - 2, 64: -2 ** 31, 90: -7, 139: 2 ** 30}
+    for s, n in odd.items():
+        b.kv.lens[s] = n
+    got = _attend(hip, b, q)
+    rest = [s for s in range(140) if s not in odd]
+    assert np.array_equal(got[rest], want[rest])
+    assert not got[[64, 90]].any()
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+def test_a_captured_batch_of_slots_whose_lengths_change(hip, t):
+    """A captured call replayed with lengths that rise, fall and end, against the eager one."""
+    b = QBatch(t, [400] * 136, 1, (8, 4, 64), 32, seed=36)
+    r = np.random.default_rng(37)
+    q = torch.from_numpy(r.standard_normal((136, 8, 64)).astype(np.float16)).cuda()
+    out, eager = (torch.zeros((136, 8, 64), dtype=torch.float16, device="cuda") for _ in range(2))
+    slabs = [torch.empty(8 << 20, dtype=torch.uint8, device="cuda") for _ in range(2)]
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    hip.set_stream(s)
+    try:
+        hip.capture_begin()
+        try:
+            hip.attn_paged(b.kv, 0, q, out, 136, 1, 8, 0.125, slabs[0])
+        finally:
+            g = hip.capture_end()
+    finally:
+        hip.use_torch_stream()
+    for _ in range(4):
+        b.kv.lens.copy_(_i32(r.integers(-1, 400, 136)))
+        torch.cuda.synchronize()
+        g.launch()
+        torch.cuda.synchronize()
+        hip.attn_paged(b.kv, 0, q, eager, 136, 1, 8, 0.125, slabs[1])
+        torch.cuda.synchronize()
+        assert torch.equal(out, eager) and torch.isfinite(out).all()
+        b.lens = b.kv.lens.tolist()
+        want, tol = b.want(q.cpu().numpy(), 0.125, 0)
+        assert (np.abs(out.cpu().numpy() - want) <= tol).all()
