@@ -2133,18 +2133,24 @@ int cima_hip_logprobs_rows(cima_hip_ctx* ctx, const void* x, int rows, int n, co
     LogprobsArgs A{x, tokens, logprob, entropy, top_ids, top_logprobs, temp, nullptr, nullptr, n, n_top, rows_per_temp, 1, 0,
                    cap};
     void* args[] = {&A};
-    // rows that a workgroup holds, and rows in parts, as in cima_hip_softmax_rows
+    // bytes of a chunk's sums and of its groups' largest logits, 256 of 8192 logits or
+    // 64 of 2048
+    const auto parts_of = [&](int words) { return (n - 1) / (kSoftmaxWord * words) + 1; };
+    const auto bytes_of = [&](int words) { return 16ULL + (words == 2 ? 64 : 256) * (f32 ? 4ULL : 2ULL); };
+    const auto need_of = [&](int words) { return (unsigned long long)rows * parts_of(words) * bytes_of(words); };
+    // Rows that a workgroup holds, and rows in parts, as in cima_hip_softmax_rows.  A
+    // workgroup of 1024 threads has a CU to itself: more of them than CUs are parts where
+    // the slab holds them.  384 rows with 20 alternatives, us, whole / in parts: of 12000
+    // 18.0 / 13.6, of 32000 19.1 / 16.0, f32 20.5 / 17.9; 64 rows of 32000 9.2 / 11.4.
     static const int shapes[][2] = {{256, 2}, {256, 8}, {1024, 8}};
     for (const auto& sh : shapes)
         if (n <= sh[0] * sh[1] * 4) {
+            if (sh[0] == 1024 && rows > ctx->num_cu && (long long)rows * parts_of(8) <= kMaxGrid && slab &&
+                aligned(slab, 16) && slab_bytes >= need_of(8))
+                break;
             snprintf(name, sizeof name, "cima_logprobs_t%d_w%d_%s", sh[0], sh[1], sfx);
             return launch_named(ctx, name, (unsigned)rows, (unsigned)sh[0], args, api);
         }
-    const auto parts_of = [&](int words) { return (n - 1) / (kSoftmaxWord * words) + 1; };
-    // bytes of a chunk's sums and of its groups' largest logits, 256 of 8192 logits or
-    // 64 of 2048
-    const auto bytes_of = [&](int words) { return 16ULL + (words == 2 ? 64 : 256) * (f32 ? 4ULL : 2ULL); };
-    const auto need_of = [&](int words) { return (unsigned long long)rows * parts_of(words) * bytes_of(words); };
     int words = 8;
     if ((long long)rows * parts_of(2) <= 4LL * ctx->num_cu && slab_bytes >= need_of(2)) words = 2;
     const long long chunks = (long long)rows * parts_of(words);

@@ -318,14 +318,18 @@ DEV double lane_d(double v, int lane) {
 // ln L, the row's entropy ln L - sum e^z z / L.  One reading of the logits, each thread
 // to its own running maximum and sums.  The likeliest n_top are found from the
 // largest logits of groups of 32 (neighbours, or a thread's in a row of one workgroup):
-// each wave
-// takes the (n_top / waves)-th largest of its lanes', so that the least of these bounds
+// the n_top-th of 64 samples, each the largest of a 64th of the threads' groups, bounds
 // the row's n_top-th from below, and what the few groups that reach it hold is
 // looked at one by one and ranked by counting (value first, then the lower id).
 // Rows up to 32768 logits go to a workgroup each, in one launch; of longer ones the
 // parts leave their sums and groups' largest, and a second launch joins them (in
 // fp64) and finds the likeliest: looked for in each part they took as long as the
-// sums did.
+// sums did.  Measured on MI355X: 384 rows of 128256 f16 with 20 alternatives 21 us (4.7
+// TB/s) and 8.4 for the join; 777 rows of 151936 without 41.5 (5.7 TB/s) and 4.6; one of
+// them with 5 3.3 and 6.8, a chain of three loads, a search by bits and a ranking; 384
+// rows of 2000 in one launch 6.8.  Bound by vector instructions: a logit is a fused
+// multiply-add, an exponential at half rate, a maximum, an addition and another
+// multiply-add, and a share of finding its group's largest.
 
 constexpr int LP_TOP = 32;     // most alternatives
 constexpr int LP_LIST = 1024;  // logits looked at one by one
@@ -369,7 +373,7 @@ struct LpTop {  // shared between the threads of a workgroup
     unsigned long long list[LP_LIST + 8], top[LP_TOP];
     int group[LP_GROUPS];
     int count, groups, found[2][NT / 64], bits[32];
-    uint32_t bound[2][NT / 64];
+    uint32_t sample[64], bound[NT / 64];
 };
 // the `kept` largest of the listed keys to S.top in order, zeros behind them, while
 // the second wave does something else
@@ -410,91 +414,111 @@ DEV void lp_rank(LpTop<NT>& S, int kept, B beside) {
     }
     __syncthreads();
 }
-// The row's `kept` likeliest to S.top.  each_group(f): f(largest, group) for every group
-// of this thread, `most` the largest of all of them; place(g, p): where in the row
-// piece p of PIECES of V logits of group g begins; beside(): something that the second
-// wave has to do once.
-template <int NT, bool F32, int V, int PIECES, typename G, typename P, typename B>
-DEV void lp_select(LpTop<NT>& S, int kept, const void* x, size_t row0, int n, float most, G each_group, P place, B beside) {
+// those of R words of V logits, `step` apart from `at` of the row on, that are not below
+// `least` to S.list, as far as there is room
+template <int NT, bool F32, int V, int R>
+DEV void lp_list(LpTop<NT>& S, const uint32_t (&v)[R][F32 ? V : V / 2], int at, int step, float least) {
+    int mine = 0;
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < V; j++) mine += sm_get<F32, V>(v[r], j) >= least;
+    if (!mine) return;
+    int to = atomicAdd(&S.count, mine);
+#pragma unroll
+    for (int r = 0; r < R; r++)
+#pragma unroll
+        for (int j = 0; j < V; j++) {
+            const float y = sm_get<F32, V>(v[r], j);
+            if (y >= least && to < LP_LIST) S.list[to++] = lp_key(lp_order(y), at + r * step + j);
+        }
+}
+// The same of every group whose largest is not below `least`: each_group(f): f(largest,
+// group) for every group of this thread, `most` the largest of them; place(g, p): where
+// in the row piece p of PIECES of V logits of group g begins.  A barrier is behind it.
+template <int NT, bool F32, int V, int PIECES, typename G, typename P>
+DEV void lp_gather(LpTop<NT>& S, const void* x, size_t row0, int n, float least, G each_group, float most, P place) {
+    if (most >= least)
+        each_group([&](float y, int g) {
+            if (y >= least) {
+                const int to = atomicAdd(&S.groups, 1);
+                if (to < LP_GROUPS) S.group[to] = g;
+            }
+        });
+    __syncthreads();
+    const int many = min(S.groups, LP_GROUPS) * PIECES;
+    for (int i = threadIdx.x; i < many; i += NT) {
+        const int at = place(S.group[i / PIECES], i % PIECES);
+        uint32_t v[1][F32 ? V : V / 2];
+        sm_load<F32, V>(x, row0, at, n, v[0]);
+        lp_list<NT, F32, V>(S, v, at, 0, least);
+    }
+    __syncthreads();
+}
+// The row's `kept` likeliest to S.top.  `most`: the largest of this thread's groups;
+// gather(least): logits of the groups whose largest is not below `least` that are not
+// below it themselves to S.list, with a barrier behind; each_group(f): f(largest) for
+// every group of this thread; beside(): something that the second wave has to do once.
+template <int NT, bool F32, typename L, typename G, typename B>
+DEV void lp_select(LpTop<NT>& S, int kept, const void* x, size_t row0, int n, float most, L gather, G each_group, B beside) {
     const int t = threadIdx.x, w = t >> 6, lane = t & 63;
     const uint32_t best = lp_order(most);
-    // the need-th largest of the lanes' or less, by its bits from the highest on (f16
-    // logits have no more than 19)
-    auto nth = [&](int need) {
+    // the kept-th largest of the lanes' or less, by its bits from the highest on (f16
+    // logits have no more than 19) until as many are left and an eighth of it is known
+    auto nth = [&](uint32_t of) {
         uint32_t v = 0;
         for (int b = 31; b >= (F32 ? 0 : 13); b--) {
-            const int c = __popcll(__ballot(best >= (v | 1u << b)));
-            if (c >= need) v |= 1u << b;
-            if (c == need) break;
+            const int c = __popcll(__ballot(of >= (v | 1u << b)));
+            if (c >= kept) v |= 1u << b;
+            if (c == kept && b <= 20) break;
         }
         return v;
     };
-    uint32_t v = nth((kept + NT / 64 - 1) / (NT / 64));
-    if (lane == 0) S.bound[0][w] = v;
+    constexpr int LANES = NT / 64;  // that are one of 64 samples
+    static_assert(LANES == 4 || LANES == 16, "a quad or a row of lanes");
+    uint32_t many = best;
+    many = max(many, (uint32_t)__builtin_amdgcn_mov_dpp((int)many, 0xB1, 0xf, 0xf, false));
+    many = max(many, (uint32_t)__builtin_amdgcn_mov_dpp((int)many, 0x4E, 0xf, 0xf, false));
+    if constexpr (LANES == 16) {
+        many = max(many, (uint32_t)__builtin_amdgcn_mov_dpp((int)many, 0x141, 0xf, 0xf, false));
+        many = max(many, (uint32_t)__builtin_amdgcn_mov_dpp((int)many, 0x140, 0xf, 0xf, false));
+    }
+    if (t % LANES == 0) S.sample[t / LANES] = many;
     if (t == 0) S.count = S.groups = 0;
     if (t < 32) S.bits[t] = 0;
     __syncthreads();
-    v = 0xffffffffu;
-#pragma unroll
-    for (int k = 0; k < NT / 64; k++) v = min(v, S.bound[0][k]);
-    if (v <= LP_NONE) {  // a wave with few logits, or of tokens that may not be taken: any wave's kept-th
-        const uint32_t b = nth(kept);
-        if (lane == 0) S.bound[1][w] = b;
+    uint32_t v = nth(S.sample[lane]);
+    if (v <= LP_NONE) {  // few logits, or of tokens that may not be taken: any wave's kept-th
+        const uint32_t b = nth(best);
+        if (lane == 0) S.bound[w] = b;
         __syncthreads();
         v = LP_NONE + 1;
 #pragma unroll
-        for (int k = 0; k < NT / 64; k++) v = max(v, S.bound[1][k]);
+        for (int k = 0; k < NT / 64; k++) v = max(v, S.bound[k]);
     }
-    // logits of the groups whose largest is not below `least` that are not below it
-    // themselves to S.list (after a barrier), as far as there is room
-    auto look = [&](float least) {
-        if (most >= least)
-            each_group([&](float x, int g) {
-                if (x >= least) {
-                    const int to = atomicAdd(&S.groups, 1);
-                    if (to < LP_GROUPS) S.group[to] = g;
-                }
-            });
-        __syncthreads();
-        const int many = min(S.groups, LP_GROUPS) * PIECES;
-        for (int i = t; i < many; i += NT) {
-            const int at = place(S.group[i / PIECES], i % PIECES);
-            uint32_t v[F32 ? V : V / 2];
-            sm_load<F32, V>(x, row0, at, n, v);
-            int mine = 0;
-#pragma unroll
-            for (int j = 0; j < V; j++) mine += sm_get<F32, V>(v, j) >= least;
-            if (mine) {
-                int to = atomicAdd(&S.count, mine);
-#pragma unroll
-                for (int j = 0; j < V; j++) {
-                    const float y = sm_get<F32, V>(v, j);
-                    if (y >= least && to < LP_LIST) S.list[to++] = lp_key(lp_order(y), at + j);
-                }
-            }
+    // Logits that are not below v, from the groups whose largest is not, to S.list.  Where
+    // there are too many, such as equal ones, once more from v + 1 on, v then the kept-th
+    // largest of the groups' exactly: what is above it lies in less than `kept` groups.
+    bool exact = false;
+    while (true) {
+        gather(lp_value(exact ? v + 1 : v));
+        if (exact || (S.groups <= LP_GROUPS && S.count <= LP_LIST)) break;
+        v = 0;
+        for (int b = 31; b >= 0; b--) {
+            int c = 0;
+            each_group([&](float x) { c += lp_order(x) >= (v | 1u << b); });
+            if (c) atomicAdd(&S.bits[b], c);
+            __syncthreads();
+            if (S.bits[b] >= kept) v |= 1u << b;
         }
+        v = max(v, LP_NONE);
+        if (t == 0) S.count = S.groups = 0;
         __syncthreads();
-    };
-    look(lp_value(v));
-    if (S.groups <= LP_GROUPS && S.count <= LP_LIST) {
-        lp_rank<NT>(S, kept, beside);
-        return;
+        exact = true;
     }
-    // Too many, such as equal ones: v = the kept-th largest of the groups' exactly.
-    // What is above it lies in less than `kept` groups; of its equals the first follow.
-    v = 0;
-    for (int b = 31; b >= 0; b--) {
-        int c = 0;
-        each_group([&](float x, int) { c += lp_order(x) >= (v | 1u << b); });
-        if (c) atomicAdd(&S.bits[b], c);
-        __syncthreads();
-        if (S.bits[b] >= kept) v |= 1u << b;
-    }
-    v = max(v, LP_NONE);
-    if (t == 0) S.count = S.groups = 0;
-    __syncthreads();
-    look(lp_value(v + 1));
     lp_rank<NT>(S, kept, beside);
+    if (!exact) return;
+    // of v's equals the first follow
     int have = min(S.count, kept);
     for (int i0 = 0, k = 0; i0 < n && have < kept && v > LP_NONE; i0 += NT, k ^= 1) {
         const float y = lp_load<F32>(x, row0, i0 + t, n);
@@ -552,7 +576,11 @@ DEV uint32_t lp_largest(const uint32_t* v) {
 #pragma unroll
     for (int i = 1; i < W; i++) {
         if constexpr (F32) p = __builtin_bit_cast(uint32_t, fmaxf(__builtin_bit_cast(float, p), __builtin_bit_cast(float, v[i])));
-        else __asm__("v_pk_max_f16 %0, %0, %1" : "+v"(p) : "v"(v[i]));
+        else {
+            uint32_t q;  // a register of its own: no copy of v[0] before it
+            __asm__("v_pk_max_f16 %0, %1, %2" : "=v"(q) : "v"(p), "v"(v[i]));
+            p = q;
+        }
     }
     return p;
 }
@@ -600,19 +628,22 @@ struct LpSums {
             bring<FAST>(CAP ? lp_f(m, cap) : m, s);
             mine = m;
         }
+        const float least = -1e30f;  // for a product with 0
 #pragma unroll
         for (int r = 0; r < R; r++) {
-            float pl = 0.f, ph = 0.f;
+            float pl, ph;
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                float z;
+                float z, y;
                 if constexpr (FAST) z = mix_fma(v[r][j / 2], j & 1, s, b);
                 else if constexpr (CAP) z = (lp_f(sm_get<F32, V>(v[r], j), cap) - c) * s;
                 else if constexpr (F32) z = (sm_get<F32, V>(v[r], j) - c) * s;
                 else z = mix_less(v[r][j / 2], j & 1, c) * s;
                 const float e = __builtin_amdgcn_exp2f(z);
-                pl += e;
-                ph = fmaf(e, fmaxf(z, -1e30f), ph);
+                // (fmaxf of what an asm returns is two instructions, the first for NaN, which e has)
+                __asm__("v_max_f32 %0, %1, %2" : "=v"(y) : "s"(least), "v"(z));
+                pl = j ? pl + e : e;
+                ph = j ? fmaf(e, y, ph) : e * y;
             }
             l += pl, h += ph;
         }
@@ -662,9 +693,21 @@ DEV void lp_whole(const LpArgs& A) {
     P.template join<NT, false>(&m, A.cap, s);
     const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
     if (kept)
-        lp_select<NT, F32, V, R>(
-            S, kept, A.x, row0, A.n, mine, [&](auto f) { f(mine, t); },
-            [&](int g, int p) { return p * NT * V + g * V; }, [] {});
+        lp_select<NT, F32>(
+            S, kept, A.x, row0, A.n, mine,
+            [&](float least) {  // a thread's logits are its group
+                // few are listed from the registers (2000 logits, 20 alternatives 7.1 -> 6.2
+                // us), more read again by many threads (8000 7.6, from the registers 8.4)
+                if constexpr (R * V <= 8) {
+                    if (mine >= least) lp_list<NT, F32, V>(S, v, t * V, NT * V, least);
+                    __syncthreads();
+                } else {
+                    lp_gather<NT, F32, V, R>(
+                        S, A.x, row0, A.n, least, [&](auto f) { f(mine, t); }, mine,
+                        [&](int g, int p) { return p * NT * V + g * V; });
+                }
+            },
+            [&](auto f) { f(mine); }, [] {});
     lp_finish(A, row, T, m, log((double)P.l), P.l, P.h, S.top, xt, CAP);
 }
 
@@ -805,23 +848,26 @@ DEV void lp_join(const LpArgs& A) {
             const uint32_t b[4] = {z.x, z.y, z.z, z.w};
             most = fmaxf(most, lp_of<F32>(lp_largest<F32, 4>(b)));
         }
-        lp_select<NT, F32, P::V, P::LANES>(
+        auto each_group = [&](auto f) {
+            auto eight = [&](const uint4& v, int i) {
+                const uint32_t a[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                for (int k = 0; k < VG; k++) {
+                    const float x = F32 ? __builtin_bit_cast(float, a[k]) : h2f(k & 1 ? a[k / 2] >> 16 : a[k / 2] & 0xffffu);
+                    f(x, i * VG + k);
+                }
+            };
+#pragma unroll
+            for (int u = 0; u < K; u++)
+                if (u * NT + t < loads) eight(q[u], u * NT + t);
+            for (int i = K * NT + t; i < loads; i += NT) eight(from[i], i);
+        };
+        lp_select<NT, F32>(
             S, kept, A.x, row0, A.n, most,
-            [&](auto f) {
-                auto eight = [&](const uint4& v, int i) {
-                    const uint32_t a[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                    for (int k = 0; k < VG; k++) {
-                        const float x = F32 ? __builtin_bit_cast(float, a[k]) : h2f(k & 1 ? a[k / 2] >> 16 : a[k / 2] & 0xffffu);
-                        f(x, i * VG + k);
-                    }
-                };
-#pragma unroll
-                for (int u = 0; u < K; u++)
-                    if (u * NT + t < loads) eight(q[u], u * NT + t);
-                for (int i = K * NT + t; i < loads; i += NT) eight(from[i], i);
+            [&](float least) {
+                lp_gather<NT, F32, P::V, P::LANES>(S, A.x, row0, A.n, least, each_group, most, P::place);
             },
-            P::place, join);
+            [&](auto f) { each_group([&](float x, int) { f(x); }); }, join);
         if (t >= 64) return;
     }
     lp_finish(A, row, T, largest, sums[0], sums[1], sums[2], S.top, xt, CAP);

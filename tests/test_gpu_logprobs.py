@@ -246,6 +246,34 @@ def test_many_rows_and_a_replayed_graph(hip):
         hip.use_torch_stream()
 
 
+@pytest.mark.parametrize("n", [2000, 8000, 20000, 60000, 151936])
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+def test_a_few_neighbours_may_be_taken(hip, dtype, n):
+    """Rows of which one run of tokens is left, all of one sign, or as many as are
+    wanted and one more or less."""
+    r = np.random.default_rng(n)
+    x = np.full((8, n), -np.inf)
+    for i, (a, m) in enumerate(((0, 1000), (n // 3, 1500), (n - 31, 31), (5, 32), (n // 2, 33), (n // 2, 20), (7, 1993),
+                                (0, n))):
+        m = min(m, n - a)
+        x[i, a:a + m] = -1 - np.abs(r.standard_normal(m)) * 3 if i % 2 else 100 + np.abs(r.standard_normal(m))
+    x = x.astype(dtype)
+    for top in (20, 32):
+        _check(hip, x, np.full(8, 0.8, np.float32), 0.0, np.argmax(x, 1), top, slabs=(1 << 20,))
+
+
+@pytest.mark.parametrize("dtype", [np.float16, np.float32])
+@pytest.mark.parametrize("n", [8193, 12001, 32768])
+def test_more_rows_than_compute_units(hip, dtype, n):
+    """With a slab that holds their parts, one that does not and none."""
+    r = np.random.default_rng(n)
+    x = (r.standard_normal((270, n)) * 3).astype(dtype)
+    x[5:100, ::2] = -np.inf
+    temp = r.uniform(0.3, 1.5, 270).astype(np.float32)
+    need = (16 + 256 * x.itemsize) * 270 * -(-n // 8192)
+    _check(hip, x, temp, 0.0, r.integers(0, n, 270), 20, slabs=(need, need - 16, 0))
+
+
 def test_refusals(hip):
     n = 40000
     x = torch.zeros((2, n), device="cuda")
