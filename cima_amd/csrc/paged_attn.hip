@@ -204,7 +204,9 @@ struct Tile {
 // bounds it: of 155 us, without the copies 133, without reads from LDS 123, without
 // the weights 138, with the products alone 85; reading fragments 2 to 8 products
 // ahead changes nothing.  One workgroup of eight waves and 256 rows, which copies half
-// as much: 176; 64 rows a wave: 572, its registers spill.
+// as much: 176; 64 rows a wave: 572, its registers spill.  The same over Q4_1 with up to
+// 500 own positions 195 us, f16 174: each of the four row tiles decodes the page, beside
+// the products as far as the vector units, 0.51 busy, let it.
 template <int D, int WR, int WK>
 DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int plo, int phi, const int* trow,
                    int part, int parts, int col) {
@@ -685,6 +687,13 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 // to 4000 positions (524 MB) 107 / 146 us (4.9 TB/s), 128 of up to 500 27 / 33;
 // 128 full slots of 8192 (4.3 GB) 765 us with the join, 5.6 TB/s.  Values by
 // loads to registers and LDS writes: 127 and 36 us.
+//
+// Quantised, bound by vector instructions: of some 330 a wave and tile of 32 positions
+// of 128 208 are the elements' (13 for 8 of Q4_1, 12 of Q8_0; all others beside the
+// softmax are addresses and the task's begin and end).  8 kv heads of 128, 64 slots of
+// up to 12000: Q4_1 (493 MB) 99 us, 5.0 TB/s, the vector units busy 0.63 of the time; 40
+// slots of 4 heads of up to 6001, Q8_0 (131 MB) 33.  The values' loads sent before the
+// keys are decoded: 118 -> 121 us.
 constexpr int few_wgs(int D, int mode, int nb) {
     if (mode == 3 && nb == 1) return few_wgs(D, 0, 2);
     return (mode && mode != 3) || (D == 128 && nb == 2) ? 2 : BITS == 8 && (D == 128 || nb == 2) ? 3 : 4;
@@ -1079,7 +1088,7 @@ DEV int nth_longest(const AttnArgs& A, int r) {
     return 0;
 }
 // One launch: first the prefix tasks (MODE 0: as few-row tasks, up to 16 rows; 1
-// and 2: tiles of 64 and 128 rows), then the own tasks, one slot's rows 16 NB at
+// and 2: tiles of 64 and 128 rows; 3, of a quantised cache: few-row tasks of 32), then the own tasks, one slot's rows 16 NB at
 // a time, so that they fill what the prefix tasks leave.  Workgroups go to the XCDs in turn; the row tiles
 // of one range of one kv head follow each other on the same XCD, so that all but
 // the first find its pages in that XCD's L2.
