@@ -666,7 +666,7 @@ int cima_hip_init(int device, const char* code_dir, cima_hip_ctx** out) {
             if (!rc) rc = add(MOD_PAGED_ATTN, name);
         }
         for (int bits : {4, 8})
-            for (int mode : {0, 1, 2, 3})
+            for (int mode : {0, 2, 3})
                 for (int nb : {1, 2}) {
                     snprintf(name, sizeof name, "cima_attn_paged_q%d_d%d_m%d_n%d", bits, dim, mode, nb);
                     if (!rc) rc = add(bits == 4 ? MOD_PAGED_ATTN_Q4 : MOD_PAGED_ATTN_Q8, name);

@@ -1108,7 +1108,7 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
         else if constexpr (MODE == 3)
             few_task<D, 2, BUFS>(A, lds, kvh, tile * 32, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
                             ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1, true);
-        else if constexpr (MODE == 1)
+        else if constexpr (MODE == 1)  // of f16
             attn_task<D, 2, 2>(A, lds, kvh, tile * 64, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
         else if constexpr (MODE == 2)
             attn_task<D, 4, 1>(A, lds, kvh, tile * 128, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
@@ -1139,20 +1139,17 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
         extern __shared__ __align__(1024) uint8_t lds[];                                                             \
         attn_body<D, MODE, NB>(A, lds);                                                                              \
     }
-#define ATTN_ALL(D) \
-    ATTN(D, 0, 1)   \
-    ATTN(D, 1, 1)   \
-    ATTN(D, 2, 1)   \
-    ATTN(D, 0, 2)   \
-    ATTN(D, 1, 2)   \
-    ATTN(D, 2, 2)
-ATTN_ALL(64)
-ATTN_ALL(128)
-#if CIMA_KV_BITS != 16
-ATTN(64, 3, 1)
-ATTN(64, 3, 2)
-ATTN(128, 3, 1)
-ATTN(128, 3, 2)
+#define ATTN_MODE(MODE) \
+    ATTN(64, MODE, 1)   \
+    ATTN(64, MODE, 2)   \
+    ATTN(128, MODE, 1)  \
+    ATTN(128, MODE, 2)
+ATTN_MODE(0)
+ATTN_MODE(2)
+#if CIMA_KV_BITS == 16
+ATTN_MODE(1)
+#else
+ATTN_MODE(3)
 #endif
 
 #if CIMA_KV_BITS == 16  // the partial sums are the same for every cache

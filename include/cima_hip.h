@@ -567,7 +567,7 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
  * tokens, logprob and entropy may be NULL (not wanted), as top_ids and top_logprobs
  * with n_top 0; n_top at most 32, less than 2^22 rows.  slab (16-byte aligned): 528
  * bytes (f32 1040) for each 8192 logits of a row (rounded up) and row; none is needed
- * up to 32768 logits, where it makes some hundreds of rows faster.  One of 1200 KB or
+ * up to 32768 logits, where it makes some hundreds of rows faster.  One of 280 KB or
  * more makes few long rows faster.  A signalling NaN may hide other tokens of its row
  * from the likeliest. */
 int cima_hip_logprobs_rows(cima_hip_ctx* ctx, const void* x, int rows, int n, const int* tokens, float* logprob,
