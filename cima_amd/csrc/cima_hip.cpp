@@ -208,7 +208,9 @@ const char* const kPagedKernels[] = {
     "cima_kv_pages_compact_move", "cima_rope_append_paged_q4_d64", "cima_rope_append_paged_q4_d128",
     "cima_rope_append_paged_q8_d64", "cima_rope_append_paged_q8_d128", "cima_kv_pages_read_b4_d64",
     "cima_kv_pages_read_b4_d128", "cima_kv_pages_read_b8_d64", "cima_kv_pages_read_b8_d128",
-    "cima_kv_pages_read_b16_d64", "cima_kv_pages_read_b16_d128"};
+    "cima_kv_pages_read_b16_d64", "cima_kv_pages_read_b16_d128", "cima_kv_pages_read_few_b4_d64",
+    "cima_kv_pages_read_few_b4_d128", "cima_kv_pages_read_few_b8_d64", "cima_kv_pages_read_few_b8_d128",
+    "cima_kv_pages_read_few_b16_d64", "cima_kv_pages_read_few_b16_d128"};
 const char* const kSampleTypes[] = {"f16", "f32", "cap_f16", "cap_f32"};
 const char* const kSampleKernels[] = {"cima_softmax_t1024_w16_f16", "cima_softmax_t1024_w16_f32", "cima_verify_sums",
                                       "cima_verify_draw"};
@@ -1749,10 +1751,14 @@ int cima_hip_kv_pages_read(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer
     const void* vp = (const char*)kp + kv_plane_bytes(kv);
     const int* table = kv->table;
     int kvh = kv->kv_heads, shift = log2i(kv->page), np = kv->n_pages, stride = kv->table_stride, seqs = kv->max_seqs;
-    void* args[] = {&kp, &vp, &table, &slots, &first, &k, &v, &kvh, &shift, &np, &stride, &seqs, &n, &blocks, &mine};
+    // few rows: one a thread, up to eight workgroups a CU (both sides at kv_read_body)
+    const long long total = (long long)n_slots * kvh * n;
+    const bool few = total <= 8LL * ctx->num_cu * (rows / 4);
+    int all = few ? (int)total : 0;
+    void* args[] = {&kp, &vp, &table, &slots, &first, &k, &v, &kvh, &shift, &np, &stride, &seqs, &n, &blocks, &all, &mine};
     char name[64];
-    snprintf(name, sizeof name, "cima_kv_pages_read_b%d_d%d", kv_bits(kv), kv->head_dim);
-    return launch_named(ctx, name, (unsigned)(n_slots * kvh * blocks), 256, args, api);
+    snprintf(name, sizeof name, "cima_kv_pages_read%s_b%d_d%d", few ? "_few" : "", kv_bits(kv), kv->head_dim);
+    return launch_named(ctx, name, few ? (all - 1) / (rows / 4) + 1 : n_slots * kvh * blocks, 256, args, api);
 }
 
 int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const void* q, void* out, int seqs,

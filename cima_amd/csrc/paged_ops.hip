@@ -188,29 +188,41 @@ ROPE_APPEND_QUANT(128, 8)
 // ---------------------------------------------------------------- read back
 
 // Positions first + j of slots as f16 rows [slot][head][max_seq][D]: a thread has
-// eight elements of READ_ROWS rows of the keys and of the values, whose loads go out
+// eight elements of ROWS rows of the keys and of the values, whose loads go out
 // together.  Positions without a page are zeros.  Bound by memory, past the caches
 // both ways: 24 slots of 5000 positions, 8 heads of 128, Q4_1 (154 MB read, 491
 // written) 115 us on MI355X, 5.6 TB/s, Q8_0 133; through the caches 127 and 145.
+// Where there are few rows (`all`, of all heads one after the other) a
+// thread has one: one slot of 4003, 2 heads of 64, Q8_0 4.1 -> 3.3 us, 8 rows of 256 slots
+// 5.9 -> 5.0; but the 24 slots 133.
 constexpr int READ_ROWS = 4;
 typedef uint32_t word4 __attribute__((ext_vector_type(4)));
-template <int D, int BITS>
+template <int D, int BITS, int ROWS>
 DEV void kv_read_body(const uint8_t* __restrict__ kp, const uint8_t* __restrict__ vp, const int* __restrict__ table,
                       const int* __restrict__ slots, const int* __restrict__ first, uint16_t* __restrict__ k,
                       uint16_t* __restrict__ v, int kv_heads, int page_shift, int n_pages, int table_stride,
-                      int max_seqs, int n, int blocks, long long max_seq) {
+                      int max_seqs, int n, int blocks, int all, long long max_seq) {
     using Q = KvQ<BITS>;
     constexpr int W8 = D / 8, PASS = 256 / W8;  // threads of a row, rows of a pass
-    const int b = blockIdx.x % blocks, sh = blockIdx.x / blocks, i = sh / kv_heads, h = sh % kv_heads;
+    const int row = threadIdx.x / W8, w8 = threadIdx.x % W8, page = 1 << page_shift;
+    // the head, and the first row's position less the slot's first
+    int sh, j0;
+    if constexpr (ROWS == 1) {
+        const int at = blockIdx.x * PASS + row;
+        if (at >= all) return;
+        sh = (int)((uint32_t)at / (uint32_t)n), j0 = at - sh * n;
+    } else {
+        sh = blockIdx.x / blocks, j0 = blockIdx.x % blocks * ROWS * PASS + row;
+    }
+    const int i = sh / kv_heads, h = sh % kv_heads;
     const int slot = slots ? slots[i] : i;
     const long long from = first ? first[i] : 0;
-    const int w8 = threadIdx.x % W8, page = 1 << page_shift;
     const size_t out = (size_t)sh * max_seq * D + w8 * 8;
-    uint32_t w[2][READ_ROWS][Q::WORDS], sc[2][READ_ROWS];
-    bool has[READ_ROWS];
+    uint32_t w[2][ROWS][Q::WORDS], sc[2][ROWS];
+    bool has[ROWS];
 #pragma unroll
-    for (int u = 0; u < READ_ROWS; u++) {
-        const int j = (b * READ_ROWS + u) * PASS + threadIdx.x / W8;
+    for (int u = 0; u < ROWS; u++) {
+        const int j = j0 + u * PASS;
         const long long pos = from + j, e = pos >> page_shift;
         int id = -1;
         if (j < n && pos >= 0 && e < table_stride && (unsigned)slot < (unsigned)max_seqs)
@@ -228,8 +240,8 @@ DEV void kv_read_body(const uint8_t* __restrict__ kp, const uint8_t* __restrict_
         }
     }
 #pragma unroll
-    for (int u = 0; u < READ_ROWS; u++) {
-        const int j = (b * READ_ROWS + u) * PASS + threadIdx.x / W8;
+    for (int u = 0; u < ROWS; u++) {
+        const int j = j0 + u * PASS;
         if (j >= n) break;
 #pragma unroll
         for (int c = 0; c < 2; c++) {
@@ -240,15 +252,18 @@ DEV void kv_read_body(const uint8_t* __restrict__ kp, const uint8_t* __restrict_
         }
     }
 }
-#define KV_READ(D, BITS)                                                                                             \
-    extern "C" __global__ __launch_bounds__(256) void cima_kv_pages_read_b##BITS##_d##D(                             \
+#define KV_READ_AS(NAME, D, BITS, ROWS)                                                                              \
+    extern "C" __global__ __launch_bounds__(256) void cima_kv_pages_##NAME##_b##BITS##_d##D(                         \
         const uint8_t* __restrict__ kp, const uint8_t* __restrict__ vp, const int* __restrict__ table,               \
         const int* __restrict__ slots, const int* __restrict__ first, uint16_t* __restrict__ k,                      \
         uint16_t* __restrict__ v, int kv_heads, int page_shift, int n_pages, int table_stride, int max_seqs, int n,  \
-        int blocks, long long max_seq) {                                                                             \
-        kv_read_body<D, BITS>(kp, vp, table, slots, first, k, v, kv_heads, page_shift, n_pages, table_stride,        \
-                              max_seqs, n, blocks, max_seq);                                                         \
+        int blocks, int all, long long max_seq) {                                                                    \
+        kv_read_body<D, BITS, ROWS>(kp, vp, table, slots, first, k, v, kv_heads, page_shift, n_pages, table_stride,  \
+                                    max_seqs, n, blocks, all, max_seq);                                              \
     }
+#define KV_READ(D, BITS)                  \
+    KV_READ_AS(read, D, BITS, READ_ROWS)  \
+    KV_READ_AS(read_few, D, BITS, 1)
 KV_READ(64, 4)
 KV_READ(128, 4)
 KV_READ(64, 8)

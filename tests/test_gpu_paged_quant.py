@@ -395,6 +395,33 @@ def test_read_back(hip, t, heads, page):
         assert np.array_equal(k.cpu().numpy(), want[0]) and np.array_equal(v.cpu().numpy(), want[1])
 
 
+@pytest.mark.parametrize("t", [0, *TYPES], ids=str)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_read_back_of_many_rows(hip, t, dim):
+    """As many rows as are read one a thread, one more of each head, and more: slots again and
+    again, from positions before the first and behind the last."""
+    lens, page, H = [700, 33, -1, 512], 64, 8
+    b = QBatch(t, lens, 1, (8, H, dim), page, seed=38) if t else Batch(lens, 1, (8, H, dim), page, seed=38)
+    most = 8 * torch.cuda.get_device_properties(0).multi_processor_count * 256 // (dim // 8)
+    r = np.random.default_rng(39)
+    for n in (most // (8 * H), most // (8 * H) + 1, 1300):
+        slots, first = r.integers(-1, 5, 8), r.integers(-200, 300, 8)
+        k, v = (torch.full((8, H, n + 3, dim), 7.0, dtype=torch.float16, device="cuda") for _ in range(2))
+        hip.kv_pages_read(b.kv, 0, k, v, 8, n, slots=_i32(slots), first=_i32(first), max_seq=n + 3)
+        torch.cuda.synchronize()
+        want = np.zeros((2, 8, H, n + 3, dim), np.float16)
+        want[:, :, :, n:] = 7.0
+        for i, (s, f) in enumerate(zip(slots, first)):
+            if not 0 <= s < 4:
+                continue
+            p = f + np.arange(n)
+            ok = (p >= 0) & (p < b.table.shape[1] * page)
+            e = np.where(ok, b.table[s, np.where(ok, p, 0) // page], -1)
+            ok &= e >= 0
+            want[:, i][:, :, np.flatnonzero(ok)] = b.pool[:, e[ok], :, p[ok] % page].transpose(1, 2, 0, 3)
+        assert np.array_equal(k.cpu().numpy(), want[0]) and np.array_equal(v.cpu().numpy(), want[1])
+
+
 @pytest.mark.parametrize("t", TYPES, ids=str)
 def test_far_positions_and_pages_behind_4_gib(hip, t):
     """A pool of which a page lies behind 2^32 bytes: append, read back and attention find it."""
