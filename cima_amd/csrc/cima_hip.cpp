@@ -668,7 +668,7 @@ int cima_hip_init(int device, const char* code_dir, cima_hip_ctx** out) {
             if (!rc) rc = add(MOD_PAGED_ATTN, name);
         }
         for (int bits : {4, 8})
-            for (int mode : {0, 2, 3})
+            for (int mode : {0, 2, 3, 4})
                 for (int nb : {1, 2}) {
                     snprintf(name, sizeof name, "cima_attn_paged_q%d_d%d_m%d_n%d", bits, dim, mode, nb);
                     if (!rc) rc = add(bits == 4 ? MOD_PAGED_ATTN_Q4 : MOD_PAGED_ATTN_Q8, name);
@@ -1699,8 +1699,8 @@ int paged_few_wgs(int bits, int dim, int mode, int nb) {
     return (mode && mode != 3) || (dim == 128 && nb == 2) ? 2 : bits == 8 && (dim == 128 || nb == 2) ? 3 : 4;
 }
 // LDS of Few<dim, nb, bufs> and of Tile<dim, 2 or 4, 2 or 1> in paged_attn.hip
-unsigned paged_few_lds(int dim, int nb, int bufs) {
-    return (unsigned)(4 * std::max(bufs * 32 * dim * 2, nb * (dim / 16) * 64 * 16) + 4 * nb * 16 * 8);
+unsigned paged_few_lds(int dim, int nb, int bufs, int waves) {
+    return (unsigned)(waves * (std::max(bufs * 32 * dim * 2, nb * (dim / 16) * 64 * 16) + nb * 16 * 8));
 }
 unsigned paged_attn_lds(int dim) { return (unsigned)(4 * 64 * dim * 2 + 1024 * 4 + 4 * 32 + 128 * 8); }
 
@@ -1807,7 +1807,17 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     // 9.8 / 9.2, 9.9 / 10.8.
     const long long brief = dim == 64 ? (nb == 1 ? 768 : 640) : (nb == 1 ? 512 : 384);
     const long long room = (long long)kv->table_stride * kv->page;
-    if (room <= brief && nb == 1 && own_base <= ctx->num_cu) prefix_pages = 0;
+    // Quantised tasks that have a CU to themselves are run by eight waves (below), and so
+    // are those of longer tables.  us, one launch / split and joined: 8 slots of 14/2 heads
+    // of 64 in tables of 800, 1136, 1440, 1840 positions 7.4 / 9.5, 8.1 / 9.7, 9.2 / 9.7, 10.7 / 9.5, x 5
+    // tokens of 768, 1088 9.2 / 10.0, 10.2 / 10.0, of 32/8 heads of 128 of 672, 864, 1088 8.2 / 10.6,
+    // 9.2 / 10.3, 10.3 / 9.9, of 8 bits 9.7 / 11.7, 11.1 / 11.4, 12.8 / 11.1, x 5 tokens of 28/4 of 576, 768
+    // 10.7 / 11.8, 12.3 / 12.1; 4 behind 768 of 64 7.3 / 9.4, of 128 9.4 / 9.4, behind 1024 8.2 / 9.6,
+    // 10.6 / 9.8, x 4 tokens behind 512 and 768 of 64 8.4 / 9.4, 9.4 / 9.2.
+    const bool wide = kv->ggml_type && own_base <= ctx->num_cu;
+    const long long once = !wide ? brief : dim == 64 ? (nb == 1 ? 1536 : 1024) : (nb == 1 ? 896 : 640);
+    if (wide ? room <= (nb == 1 ? once : dim == 64 ? 768 : 0) : room <= brief && nb == 1 && own_base <= ctx->num_cu)
+        prefix_pages = 0;
     const long long own_room = room - (long long)prefix_pages * kv->page;
     // Up to 16 rows the prefix runs in the own tasks' kernel, whose waves fetch
     // for themselves; above, in tiles of 64 rows, from 65 rows on of 128.  us,
@@ -1850,8 +1860,10 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
         // Quantised: the tasks are shorter, their joins not, and taken by their lengths
         // (below) few parts do.  Parts of 256 positions up to four to a CU; where the tasks
         // alone are more than one to a CU of 750 up to two rounds of the chip, behind a
-        // prefix up to sixteen to a CU; one where they are one for each 1024 positions (two
-        // for tasks of 32 rows without one).  32/8 heads of 128, Q4_1, us by parts 1 / 2 / 3 / 4 / 8 / 16: 32
+        // prefix up to sixteen to a CU; one where they are one for each 1024 positions, for
+        // each 2048 where eight waves take them or, without a prefix, 32 rows: 32 slots of
+        // 8 heads of 128 of 1000, 1600, 2400 11.2 / 13.8, 14.6 / 16.5, 19.3 / 18.6, of 8 bits 13.6 / 18.2,
+        // 18.3 / 22.0, 25.2 / 27.4.  32/8 heads of 128, Q4_1, us by parts 1 / 2 / 3 / 4 / 8 / 16: 32
         // slots of up to 700 11.5 / 13 / 13 / 13 / 21 / 34, of 2000 21.6 / 20 / 18.6 / 18 / 23 / 35, 64
         // of 6000 80 / 70 / 63 / 62 / 68 / 87, of 12000 154 / 126 / 112 / 109 / 112 / 128, 128 of 2000
         // 45 / 49 / 52 / 57 / 78 / 129, of 6000 122 / 110 / 110 / 115 / 129 / 169, 256 of 6000 191 /
@@ -1864,7 +1876,9 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
         own = few           ? std::min(own_room / 256, (4LL * ctx->num_cu + own_base - 1) / own_base)
               : prefix_pages ? std::min(own_room / 750, (16LL * ctx->num_cu + own_base - 1) / own_base)
                              : std::min(own_room / 750, 2LL * wgs * ctx->num_cu / own_base);
-        if (own_room <= brief || own_base * (prefix_pages ? 1 : nb) * 1024 >= own_room * ctx->num_cu) own = 1;
+        if (prefix_pages ? own_room <= brief || own_base * 1024 >= own_room * ctx->num_cu
+                         : own_room <= once || own_base * (wide ? 2 : nb) * 1024 >= own_room * ctx->num_cu)
+            own = 1;
     } else if (prefix_pages ? (own_room <= (dim == 64 ? 640 : 512) && 3 * own_base >= ctx->num_cu) || (mode && own_room <= 256)
                      : own_room <= brief || own_base * 1024 >= std::min(own_room, 2048LL) * ctx->num_cu)
         own = 1;
@@ -1939,14 +1953,22 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     // Own tasks of f16 alone, no more than two to a CU, run in a kernel that has two of
     // their tiles in flight.  us, one / two: 16 slots of 8 heads of 128 up to 300 7.9 /
     // 7.5, 32 of them 9.2 / 8.7, 4 slots of 14/2 heads of 64 over 573 7.7 / 7.3.
-    const int kind = !pre && !kv->ggml_type && own_base * own <= 2LL * ctx->num_cu ? 1 : mode;
+    // Quantised tasks that have a CU to themselves and more than 256 positions (of 32 rows
+    // 384): eight waves.
+    // us, four / eight: 4 slots of 14/2 heads of 64 over 573 7.2 / 6.4, 8 of 32/8 of 128 of up
+    // to 400 8.1 / 7.6, of 8 bits 9.5 / 8.6, 32 of 700 11.1 / 9.8, 32 x 5 tokens of 28/4 of 1000 19.4 /
+    // 17.1; but 64 slots of 32/8 heads 10.0 / 10.5, of 8 bits 12.2 / 15.7, 3 slots x 5 tokens of
+    // 28/4 of 200 8.0 / 8.6.  Sixteen waves: 7.5, 8.9, 11.4, 10.3.
+    const int kind = !kv->ggml_type ? (!pre && own_base * own <= 2LL * ctx->num_cu ? 1 : mode)
+                     : all == 1 && !pre && wide && own_room > (nb == 1 ? 256 : 384) ? 4 : mode;
+    const int waves = kind == 4 ? 8 : 4;
     if (kv->ggml_type) snprintf(name, sizeof name, "cima_attn_paged_q%d_d%d_m%d_n%d", kv_bits(kv), dim, kind, nb);
     else snprintf(name, sizeof name, "cima_attn_paged_d%d_m%d_n%d", dim, kind, nb);
     if (int rc = get_fn(ctx, name, &f)) return rc;
     void* args[] = {&A};
     const int bufs = kv->ggml_type || paged_few_wgs(16, dim, kind, nb) == 4 ? 1 : 2;
-    const unsigned lds = std::max(paged_few_lds(dim, mode == 3 ? 2 : nb, bufs), mode == 1 || mode == 2 ? paged_attn_lds(dim) : 0u);
-    if (int rc = launch(ctx, f, (unsigned)grid, 256, args, api, lds)) return rc;
+    const unsigned lds = std::max(paged_few_lds(dim, mode == 3 ? 2 : nb, bufs, waves), mode == 1 || mode == 2 ? paged_attn_lds(dim) : 0u);
+    if (int rc = launch(ctx, f, (unsigned)grid, 64 * waves, args, api, lds)) return rc;
     if (all == 1) return 0;
     const long long join = (long long)kv->kv_heads * ((head_rows + 15) / 16) * (dim / 16);
     return launch_named(ctx, dim == 64 ? "cima_attn_paged_join_d64" : "cima_attn_paged_join_d128", (unsigned)join, 256,

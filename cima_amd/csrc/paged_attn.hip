@@ -694,6 +694,9 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 // up to 12000: Q4_1 (493 MB) 99 us, 5.0 TB/s, the vector units busy 0.63 of the time; 40
 // slots of 4 heads of up to 6001, Q8_0 (131 MB) 33.  The values' loads sent before the
 // keys are decoded: 118 -> 121 us.
+// waves of a task: 8 where a quantised cache's has a CU to itself (mode 4): a wave alone on
+// its SIMD takes 1 us for a tile, most of it the decoding's chain
+constexpr int few_waves(int mode) { return mode == 4 ? 8 : 4; }
 constexpr int few_wgs(int D, int mode, int nb) {
     if (mode == 3 && nb == 1) return few_wgs(D, 0, 2);
     return (mode && mode != 3) || (D == 128 && nb == 2) ? 2 : BITS == 8 && (D == 128 || nb == 2) ? 3 : 4;
@@ -709,18 +712,18 @@ DEV int few_flip(int row) {
     return D == 128 ? (row & 7) << 1 : (row >> 1 & 3) << 1;
 }
 constexpr int OWN_LEAST = 4;  // tiles that a part of an own task has at least, where there are
-template <int D, int NB, int BUFS>
+template <int D, int NB, int BUFS, int W>
 struct Few {
     static constexpr int VT = 32 * D * 2;                  // bytes of a tile's values
     static constexpr int OB = NB * (D / 16) * 64 * 16;     // of a wave's sums
     static constexpr int WAVE = BUFS * VT > OB ? BUFS * VT : OB;  // LDS of a wave
-    static constexpr int LDS = 4 * WAVE + 4 * NB * 16 * 8;
-    static_assert(LDS <= (BUFS == 1 && BITS == 16 ? 40 : 80) * 1024, "workgroups to a CU");
+    static constexpr int LDS = W * WAVE + W * NB * 16 * 8;
+    static_assert(LDS <= (W > 4 ? 160 : BUFS == 1 && BITS == 16 ? 40 : 80) * 1024, "workgroups to a CU");
 };
-template <int D, int NB, int BUFS>
+template <int D, int NB, int BUFS, int W>
 DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int plo, int phi, const int* trow, int part,
                   int parts, int col, int guess, int least, bool slots) {
-    using F = Few<D, NB, BUFS>;
+    using F = Few<D, NB, BUFS, W>;
     constexpr int STEPS = D / 32, XT = D / 16, CH = D / 8;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int li = lane & 15, q4 = lane >> 4;
@@ -845,7 +848,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
             if constexpr (BUFS == 1) issue(t, buf);
             wait_vm<0>();
             if constexpr (BUFS == 2)
-                if (t + 4 < t1) issue(t + 4, std::integral_constant<int, 1 - buf>{});
+                if (t + W < t1) issue(t + W, std::integral_constant<int, 1 - buf>{});
         } else {
             gone[1] = gone[0];
 #pragma unroll
@@ -871,7 +874,7 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
                     __builtin_amdgcn_sched_barrier(0);
                 }
             }
-            if (t + 4 < t1) issue(t + 4, buf);
+            if (t + W < t1) issue(t + W, buf);
             __builtin_amdgcn_sched_barrier(0);
         }
         const int p0 = base + 32 * t;
@@ -985,18 +988,18 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
     int t = t0 + wave;
     if constexpr (BUFS == 1) {
         if (BITS != 16 && t < t1) issue(t, B0{});
-        for (; t < t1; t += 4) step(t, B0{});
+        for (; t < t1; t += W) step(t, B0{});
     } else if (t < t1) {
         issue(t, B0{});
         while (true) {
             step(t, B0{});
-            if ((t += 4) >= t1) break;
+            if ((t += W) >= t1) break;
             step(t, B1{});
-            if ((t += 4) >= t1) break;
+            if ((t += W) >= t1) break;
         }
     }
     // ---- the waves' sums, brought to the largest maximum
-    f2* rm = reinterpret_cast<f2*>(lds + 4 * F::WAVE);
+    f2* rm = reinterpret_cast<f2*>(lds + W * F::WAVE);
 #pragma unroll
     for (int b = 0; b < NB; b++) {
         l[b] = quarters_sum(l[b]);
@@ -1009,9 +1012,9 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
     for (int b = 0; b < NB; b++) {
         M[b] = LOWEST, L[b] = 0.f;
 #pragma unroll
-        for (int w = 0; w < 4; w++) M[b] = fmaxf(M[b], rm[(w * NB + b) * 16 + li][0]);
+        for (int w = 0; w < W; w++) M[b] = fmaxf(M[b], rm[(w * NB + b) * 16 + li][0]);
 #pragma unroll
-        for (int w = 0; w < 4; w++) {
+        for (int w = 0; w < W; w++) {
             const f2 v = rm[(w * NB + b) * 16 + li];
             L[b] += v[1] * __builtin_amdgcn_exp2f(v[0] - M[b]);
         }
@@ -1033,11 +1036,12 @@ DEV void few_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int 
         if (all > 1 && !some) continue;
         const float inv = some && L[b] != 0.f ? 1.f / L[b] : 0.f;
 #pragma unroll
-        for (int y = 0; y < XT / 4; y++) {
-            const int x = wave * (XT / 4) + y;
+        for (int y = 0; y < (XT + W - 1) / W; y++) {
+            const int x = wave * ((XT + W - 1) / W) + y;
+            if (XT < W && x >= XT) break;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int w = 0; w < 4; w++) {
+            for (int w = 0; w < W; w++) {
                 const float4 z = reinterpret_cast<const float4*>(lds + w * F::WAVE)[(b * XT + x) * 64 + lane];
                 v.x += z.x, v.y += z.y, v.z += z.z, v.w += z.w;
             }
@@ -1092,7 +1096,7 @@ DEV int nth_longest(const AttnArgs& A, int r) {
     return 0;
 }
 // One launch: first the prefix tasks (MODE 0: as few-row tasks, up to 16 rows; 1
-// and 2: tiles of 64 and 128 rows; 3, of a quantised cache: few-row tasks of 32), then the own tasks, one slot's rows 16 NB at
+// and 2: tiles of 64 and 128 rows; 3, of a quantised cache: few-row tasks of 32; 4: none), then the own tasks, one slot's rows 16 NB at
 // a time, so that they fill what the prefix tasks leave.  Workgroups go to the XCDs in turn; the row tiles
 // of one range of one kv head follow each other on the same XCD, so that all but
 // the first find its pages in that XCD's L2.
@@ -1107,10 +1111,10 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
         const int kvh = grp / A.prefix_parts, part = grp % A.prefix_parts, phi = A.prefix_pages << A.page_shift;
         const int* trow = A.table + (size_t)A.prefix_slot * A.table_stride;
         if constexpr (MODE == 0 && NB == 1)
-            few_task<D, NB, BUFS>(A, lds, kvh, 0, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
+            few_task<D, NB, BUFS, 4>(A, lds, kvh, 0, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
                             ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1, true);
         else if constexpr (MODE == 3)
-            few_task<D, 2, BUFS>(A, lds, kvh, tile * 32, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
+            few_task<D, 2, BUFS, 4>(A, lds, kvh, tile * 32, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part,
                             ((phi + 31) / 32 + A.prefix_parts - 1) / A.prefix_parts * part * 32 >> A.page_shift, 1, true);
         else if constexpr (MODE == 1)  // of f16
             attn_task<D, 2, 2>(A, lds, kvh, tile * 64, A.seqs * rows, 0, phi, trow, part, A.prefix_parts, part);
@@ -1128,7 +1132,7 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
     int s = b / A.kv_heads;
     if constexpr (BITS != 16)
         if (A.by_length) s = nth_longest(A, s);
-    few_task<D, NB, BUFS>(A, lds, kvh, s * rows + tile * 16 * NB, (s + 1) * rows, A.prefix_pages << A.page_shift, 0x7fffffff,
+    few_task<D, NB, BUFS, few_waves(MODE)>(A, lds, kvh, s * rows + tile * 16 * NB, (s + 1) * rows, A.prefix_pages << A.page_shift, 0x7fffffff,
                     A.table + (size_t)s * A.table_stride, part, A.own_parts, A.prefix_parts + part, A.prefix_pages, OWN_LEAST, false);
 }
 #if CIMA_KV_BITS == 16
@@ -1139,7 +1143,7 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
 #define ATTN_NAME(D, MODE, NB) cima_attn_paged_q4_d##D##_m##MODE##_n##NB
 #endif
 #define ATTN(D, MODE, NB)                                                                                            \
-    extern "C" __global__ __launch_bounds__(256, few_wgs(D, MODE, NB)) void ATTN_NAME(D, MODE, NB)(const AttnArgs A) {  \
+    extern "C" __global__ __launch_bounds__(64 * few_waves(MODE), few_wgs(D, MODE, NB)) void ATTN_NAME(D, MODE, NB)(const AttnArgs A) {  \
         extern __shared__ __align__(1024) uint8_t lds[];                                                             \
         attn_body<D, MODE, NB>(A, lds);                                                                              \
     }
@@ -1154,6 +1158,7 @@ ATTN_MODE(2)
 ATTN_MODE(1)
 #else
 ATTN_MODE(3)
+ATTN_MODE(4)
 #endif
 
 #if CIMA_KV_BITS == 16  // the partial sums are the same for every cache

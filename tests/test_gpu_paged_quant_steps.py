@@ -355,3 +355,39 @@ def test_a_captured_batch_of_slots_whose_lengths_change(hip, t):
         b.lens = b.kv.lens.tolist()
         want, tol = b.want(q.cpu().numpy(), 0.125, 0)
         assert (np.abs(out.cpu().numpy() - want) <= tol).all()
+
+
+# ------------------------------------------------ few slots: a task, a workgroup of eight waves
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("heads,n_new", [((14, 2, 64), 1), ((14, 2, 64), 5), ((12, 12, 64), 1), ((32, 8, 128), 1),
+                                         ((28, 4, 128), 5), ((16, 1, 128), 1)], ids=str)
+@pytest.mark.parametrize("longest", [240, 257, 300, 380, 450, 600, 860, 1500])
+def test_attention_of_a_few_slots(hip, t, heads, n_new, longest):
+    """Tables around the lengths at which a task has more waves or is split: without a slab
+    in one launch, with one as it is planned, behind pages that are shared, in a window."""
+    lens = [longest - n_new, 0, 31, -1, longest // 2]
+    for prefix, window, slab in ((0, 0, 0), (0, 0, 32), (0, 37, 32), (0, longest // 2, 32), (208, 0, 32)):
+        own = [n if n < 0 else max(n, prefix) for n in lens]
+        _check(hip, QBatch(t, own, n_new, heads, 16, prefix, seed=longest + n_new), window, slab)
+
+
+@pytest.mark.parametrize("t", TYPES, ids=str)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_attention_of_a_few_slots_without_some_pages(hip, t, dim):
+    """Positions that have no page are not seen, whichever wave's they are."""
+    b = QBatch(t, [700, 333], 1, (4, 2, dim), 16, seed=40)
+    q = b.r.standard_normal((2, 4, dim)).astype(np.float16)
+    gone = [(0, 3), (0, 17), (0, 18), (0, 40), (1, 0), (1, 20)]
+    for s, e in gone:
+        b.kv.table[s, e] = -1 if e % 2 else 10 ** 6
+    got = _attend(hip, b, q)
+    for s in range(2):
+        p = np.array([i for i in range(b.lens[s] + 1) if (s, i // 16) not in gone])
+        ids = b.table[s, p // 16]
+        for h in range(4):
+            k, v = (b.pool[c, ids, h // 2, p % 16].astype(np.float64) for c in range(2))
+            z = k @ q[s, h].astype(np.float64) / np.sqrt(dim)
+            w = np.exp(z - z.max())
+            want = w @ v / w.sum()
+            assert (np.abs(got[s, h] - want) <= 2 * EPS16 * np.abs(v).max() + EPS16 * np.abs(want)).all()

@@ -69,7 +69,7 @@ def test_code_objects_hold_every_kernel():
     want = {"paged": [f"cima_rope_append_paged_q{b}_d{d}" for b in (4, 8) for d in (64, 128)]
             + [f"cima_kv_pages_read{f}_b{b}_d{d}" for f in ("", "_few") for b in (4, 8, 16) for d in (64, 128)]}
     for b in (4, 8):
-        want[f"paged_attn_q{b}"] = [f"cima_attn_paged_q{b}_d{d}_m{m}_n{n}" for d in (64, 128) for m in (0, 2, 3)
+        want[f"paged_attn_q{b}"] = [f"cima_attn_paged_q{b}_d{d}_m{m}_n{n}" for d in (64, 128) for m in (0, 2, 3, 4)
                                     for n in (1, 2)]
     for name, kernels in want.items():
         blob = open(cbuild.HSACOS[name], "rb").read()
@@ -85,7 +85,7 @@ def test_quantised_kernels_do_not_spill():
     for name in ("paged", "paged_attn_q4", "paged_attn_q8", "sample"):
         notes.update(_kernel_notes(cbuild.HSACOS[name]))
     mine = {k: v for k, v in notes.items() if "paged_q" in k or "kv_pages_read" in k or "logprobs" in k}
-    assert len(mine) == 2 * 12 + 4 + 12 + 28
+    assert len(mine) == 2 * 16 + 4 + 12 + 28
     assert not {k: v for k, v in mine.items() if v[1] > 0}
 
 
