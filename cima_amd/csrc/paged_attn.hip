@@ -671,7 +671,7 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 //
 // Tasks of up to 16 NB rows (own tasks; prefix tasks of up to 16 rows): bound by
 // reading the keys and values, and short ones by the latency of their chain of
-// loads (lengths, ids, pages).  The four waves of a workgroup take 32-position
+// loads (lengths, ids, pages).  The W waves of a workgroup take 32-position
 // tiles in turn and do not wait for each other: keys go straight from memory
 // to the registers of the A operand (16 x 16 x 32 MFMA: a lane holds 16 bytes
 // of a key), values by direct copies to the wave's own LDS.  The waves' sums are
@@ -694,6 +694,7 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 // up to 12000: Q4_1 (493 MB) 99 us, 5.0 TB/s, the vector units busy 0.63 of the time; 40
 // slots of 4 heads of up to 6001, Q8_0 (131 MB) 33.  The values' loads sent before the
 // keys are decoded: 118 -> 121 us.
+
 // waves of a task: 8 where a quantised cache's has a CU to itself (mode 4): a wave alone on
 // its SIMD takes 1 us for a tile, most of it the decoding's chain
 constexpr int few_waves(int mode) { return mode == 4 ? 8 : 4; }
@@ -1096,10 +1097,11 @@ DEV int nth_longest(const AttnArgs& A, int r) {
     return 0;
 }
 // One launch: first the prefix tasks (MODE 0: as few-row tasks, up to 16 rows; 1
-// and 2: tiles of 64 and 128 rows; 3, of a quantised cache: few-row tasks of 32; 4: none), then the own tasks, one slot's rows 16 NB at
-// a time, so that they fill what the prefix tasks leave.  Workgroups go to the XCDs in turn; the row tiles
-// of one range of one kv head follow each other on the same XCD, so that all but
-// the first find its pages in that XCD's L2.
+// and 2: tiles of 64 and 128 rows; 3, of a quantised cache: few-row tasks of 32;
+// 4: none, and eight waves an own task), then the own tasks, one slot's rows 16 NB at
+// a time, so that they fill what the prefix tasks leave.  Workgroups go to the XCDs
+// in turn; the row tiles of one range of one kv head follow each other on the same
+// XCD, so that all but the first find its pages in that XCD's L2.
 template <int D, int MODE, int NB>
 DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
     constexpr int BUFS = few_bufs(D, MODE, NB);
@@ -1132,8 +1134,10 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
     int s = b / A.kv_heads;
     if constexpr (BITS != 16)
         if (A.by_length) s = nth_longest(A, s);
-    few_task<D, NB, BUFS, few_waves(MODE)>(A, lds, kvh, s * rows + tile * 16 * NB, (s + 1) * rows, A.prefix_pages << A.page_shift, 0x7fffffff,
-                    A.table + (size_t)s * A.table_stride, part, A.own_parts, A.prefix_parts + part, A.prefix_pages, OWN_LEAST, false);
+    few_task<D, NB, BUFS, few_waves(MODE)>(A, lds, kvh, s * rows + tile * 16 * NB, (s + 1) * rows,
+                                           A.prefix_pages << A.page_shift, 0x7fffffff,
+                                           A.table + (size_t)s * A.table_stride, part, A.own_parts,
+                                           A.prefix_parts + part, A.prefix_pages, OWN_LEAST, false);
 }
 #if CIMA_KV_BITS == 16
 #define ATTN_NAME(D, MODE, NB) cima_attn_paged_d##D##_m##MODE##_n##NB
@@ -1143,7 +1147,8 @@ DEV void attn_body(const AttnArgs& A, uint8_t* lds) {
 #define ATTN_NAME(D, MODE, NB) cima_attn_paged_q4_d##D##_m##MODE##_n##NB
 #endif
 #define ATTN(D, MODE, NB)                                                                                            \
-    extern "C" __global__ __launch_bounds__(64 * few_waves(MODE), few_wgs(D, MODE, NB)) void ATTN_NAME(D, MODE, NB)(const AttnArgs A) {  \
+    extern "C" __global__ __launch_bounds__(64 * few_waves(MODE), few_wgs(D, MODE, NB)) void ATTN_NAME(D, MODE, NB)(  \
+        const AttnArgs A) {                                                                                          \
         extern __shared__ __align__(1024) uint8_t lds[];                                                             \
         attn_body<D, MODE, NB>(A, lds);                                                                              \
     }
