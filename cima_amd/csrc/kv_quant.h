@@ -129,7 +129,7 @@ DEV uint32_t kv_encode(const uint32_t (&x)[4], uint32_t (&w)[KvQ<BITS>::WORDS]) 
     hi = quad_max(hi), lo = -quad_max(-lo);
     bad = quad_max(bad ? 1.f : 0.f) > 0.f;
     constexpr float STEPS = BITS == 4 ? 15.f : 127.f;
-    const float m = BITS == 4 ? lo : 0.f;
+    const float m = BITS == 4 ? lo + 0.f : 0.f;  // a least value of -0 as 0, whichever came first
     const double width = BITS == 4 ? (double)hi - (double)lo : (double)fmaxf(hi, -lo);
     const uint32_t db = bad ? 0x7e00u : scale_up(width, STEPS);
     const float d = h2f(db), inv = d > 0.f ? __builtin_amdgcn_rcpf(d) : 0.f;

@@ -20,11 +20,12 @@ HEADS = [(14, 2, 64), (32, 8, 128), (12, 12, 64), (16, 1, 128), (8, 8, 128)]
 
 
 def quantise(x, t):
-    """f16 rows [..., D] -> (codes uint8 [..., D], scales f16 [..., D / 32, 2 or 1]), in 64 bits."""
+    """f16 rows [..., D] -> (codes uint8 [..., D], scales f16 [..., D / 32, 2 or 1]), in 64 bits.
+    A least value of -0 is 0."""
     g = x.astype(np.float64).reshape(*x.shape[:-1], -1, 32)
-    low = g.min(-1, keepdims=True) if t == DType.Q4_1 else np.zeros((*g.shape[:-1], 1))
+    low = g.min(-1, keepdims=True) + 0.0 if t == DType.Q4_1 else np.zeros((*g.shape[:-1], 1))
     steps = 15 if t == DType.Q4_1 else 127
-    width = g.max(-1, keepdims=True) - low if t == DType.Q4_1 else np.abs(g).max(-1, keepdims=True)
+    width = g.max(-1, keepdims=True) - low + 0.0 if t == DType.Q4_1 else np.abs(g).max(-1, keepdims=True)
     d = (width / steps).astype(np.float16)
     d = np.where(d.astype(np.float64) * steps < width, np.nextafter(d, np.float16(np.inf)), d)
     c = np.rint(np.divide(g - low, d.astype(np.float64), out=np.zeros_like(g), where=d > 0))
@@ -324,7 +325,8 @@ def test_rope_append(hip, t, heads, n_new, theta):
 
 @pytest.mark.parametrize("t", TYPES, ids=str)
 def test_append_of_every_kind_of_group(hip, t):
-    """Ties between two codes, equal elements, zeros, f16's smallest and largest: as the definition says."""
+    """Ties between two codes, equal elements, zeros of both signs, f16's smallest and largest:
+    as the definition says."""
     b = QBatch(t, [0, 3], 40, (2, 2, 128), 16, seed=21)
     r = b.r
     x = r.standard_normal((b.rows, 6, 128))
@@ -338,6 +340,8 @@ def test_append_of_every_kind_of_group(hip, t):
     x[9] = np.where(r.random(x[9].shape) < 0.05, -30000, r.standard_normal(x[9].shape) * 2.0 ** -20)
     x[10] = -np.abs(x[10])
     x[11:20] *= 2.0 ** np.arange(-18, 9, 3)[:, None, None]
+    x[20], x[21] = np.where(r.random(x[20].shape) < 0.5, 0.0, -0.0), -0.0
+    x[22] = np.where(r.random(x[22].shape) < 0.5, -0.0, 3.5)
     qkv = x.reshape(b.rows, -1).astype(np.float16)
     q = torch.empty((b.rows, 2, 128), dtype=torch.float16, device="cuda")
     hip.rope_append_paged(b.kv, 0, torch.from_numpy(qkv).cuda(), q, 2, 40, 2, 0.0)
