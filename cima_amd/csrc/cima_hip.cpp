@@ -1876,6 +1876,19 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
         own = few           ? std::min(own_room / 256, (4LL * ctx->num_cu + own_base - 1) / own_base)
               : prefix_pages ? std::min(own_room / 750, (16LL * ctx->num_cu + own_base - 1) / own_base)
                              : std::min(own_room / 750, 2LL * wgs * ctx->num_cu / own_base);
+        // Parts in eights, up to 32: the XCDs, which take workgroups in turn, then have the
+        // same part of every slot, not the longer and the shorter slots' turn by turn; up
+        // where one round holds them.  Parts as many as that / in eights, us: 12 slots of
+        // 32/8 heads of 2500, 5000 14.2 / 12.9, 18.7 / 16.4, of 8 bits 17.7 / 15.5, 23.7 / 20.8, 48 of
+        // 14/2 of 2500 12.1 / 11.0, 2 of 32/8 of 12000 14.2 / 13.0; but with more than a round 40 of
+        // 28/4 24.2 / 25.6, 16 of 8 bits of 1700 15.7 / 16.8, and with long parts 48 of 20000
+        // 36.1 / 38.4.
+        if (few && !prefix_pages && own >= 6) {
+            const long long near = (own + 5) / 8 * 8, down = own / 8 * 8;
+            if (near <= own || own_base * near <= (long long)wgs * ctx->num_cu) own = near;
+            else if (down && own_room <= 1536 * down) own = down;
+            own = std::min(own, 32LL);
+        }
         if (prefix_pages ? own_room <= brief || own_base * 1024 >= own_room * ctx->num_cu
                          : own_room <= once || own_base * (wide ? 2 : nb) * 1024 >= own_room * ctx->num_cu)
             own = 1;
