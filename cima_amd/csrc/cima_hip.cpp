@@ -1858,8 +1858,10 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
     while (own > 1 && own_base * own > 2LL * wgs * ctx->num_cu) own = (own + 1) / 2;
     if (kv->ggml_type) {
         // Quantised: the tasks are shorter, their joins not, and taken by their lengths
-        // (below) few parts do.  Parts of 256 positions up to four to a CU; where the tasks
-        // alone are more than one to a CU of 750 up to two rounds of the chip, behind a
+        // (below) few parts do.  Parts of 256 positions up to four to a CU (no more than
+        // that: 24 slots of 32/8 heads of 5000 in 5 / 6 parts 22.9 / 25.4, 40 of 28/4 of 8 bits of
+        // 6001 in 6 / 7 36.4 / 38.4; behind a prefix rounded up); where the tasks alone are
+        // more than one to a CU of 750 up to two rounds of the chip, behind a
         // prefix up to sixteen to a CU; one where they are one for each 1024 positions, for
         // each 2048 where eight waves take them or, without a prefix, 32 rows: 32 slots of
         // 8 heads of 128 of 1000, 1600, 2400 11.2 / 13.8, 14.6 / 16.5, 19.3 / 18.6, of 8 bits 13.6 / 18.2,
@@ -1873,16 +1875,16 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
         // prefix of 4096, 1 / 2 / 4 / 8: 8 slots of 1000 20.5 / 16.3 / 14.4 / 16.3, 128 of 1000 49 /
         // 51 / 60 / 88.
         const bool few = own_base <= ctx->num_cu;
-        own = few           ? std::min(own_room / 256, (4LL * ctx->num_cu + own_base - 1) / own_base)
+        own = few           ? std::min(own_room / 256, (4LL * ctx->num_cu + (prefix_pages ? own_base - 1 : 0)) / own_base)
               : prefix_pages ? std::min(own_room / 750, (16LL * ctx->num_cu + own_base - 1) / own_base)
                              : std::min(own_room / 750, 2LL * wgs * ctx->num_cu / own_base);
-        // Parts in eights, up to 32: the XCDs, which take workgroups in turn, then have the
-        // same part of every slot, not the longer and the shorter slots' turn by turn; up
-        // where one round holds them.  Parts as many as that / in eights, us: 12 slots of
-        // 32/8 heads of 2500, 5000 14.2 / 12.9, 18.7 / 16.4, of 8 bits 17.7 / 15.5, 23.7 / 20.8, 48 of
-        // 14/2 of 2500 12.1 / 11.0, 2 of 32/8 of 12000 14.2 / 13.0; but with more than a round 40 of
-        // 28/4 24.2 / 25.6, 16 of 8 bits of 1700 15.7 / 16.8, and with long parts 48 of 20000
-        // 36.1 / 38.4.
+        // Parts in eights, up to 32: an XCD, which take workgroups in turn, then has the same
+        // part of every slot; more of them where one round holds those, fewer where they stay
+        // short.  us: one slot of 32/8 heads of 1700 in 6 / 8 parts 9.8 / 8.9, 10 of 3500 in 12 / 8
+        // 14.8 / 14.1, 6 of 8 bits in 12 / 8, 16 16.3 / 14.7, 14.9, 48 of 14/2 of 4000 in 10 / 8 14.2 /
+        // 12.7, 2 of 32/8 of 12000 in 46 / 32 14.2 / 12.9; but more than a round, 40 of 28/4 in 7 / 8
+        // 24.2 / 25.6, 16 of 8 bits of 1700 in 6 / 8 15.7 / 16.8, and long parts, 48 of 8 bits of
+        // 20000 in 11 / 8 36.1 / 38.4.
         if (few && !prefix_pages && own >= 6) {
             const long long near = (own + 5) / 8 * 8, down = own / 8 * 8;
             if (near <= own || own_base * near <= (long long)wgs * ctx->num_cu) own = near;
