@@ -692,7 +692,7 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 // of 128 208 are the elements' (13 for 8 of Q4_1, 12 of Q8_0; all others beside the
 // softmax are addresses and the task's begin and end).  8 kv heads of 128, 64 slots of
 // up to 12000: Q4_1 (493 MB) 99 us, 5.0 TB/s, the vector units busy 0.63 of the time; 40
-// slots of 4 heads of up to 6001, Q8_0 (131 MB) 33.  The values' loads sent before the
+// slots of 4 heads of up to 6001, Q8_0 (131 MB) 32.  The values' loads sent before the
 // keys are decoded: 118 -> 121 us.
 
 // waves of a task: 8 where a quantised cache's has a CU to itself (mode 4): a wave alone on
