@@ -1860,7 +1860,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
         // Quantised: the tasks are shorter, their joins not, and taken by their lengths
         // (below) few parts do.  Parts of 256 positions up to four to a CU (no more than
         // that: 24 slots of 32/8 heads of 5000 in 5 / 6 parts 22.9 / 25.4, 40 of 28/4 of 8 bits of
-        // 6001 in 6 / 7 36.4 / 38.4; behind a prefix rounded up); where the tasks alone are
+        // 6001 in 6 / 7 36.4 / 38.4); where the tasks alone are
         // more than one to a CU of 750 up to two rounds of the chip, behind a
         // prefix up to sixteen to a CU; one where they are one for each 1024 positions, for
         // each 2048 where eight waves take them or, without a prefix, 32 rows: 32 slots of
@@ -1872,10 +1872,17 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
         // 202 / 208 / 217 / 254 / 317; Q8_0, 64 of 6000 107 / 92 / 90 / 91 / 100 / 125, 128 of 6000
         // 160 / 164 / 166 / 173 / 193 / 245; 14/2 of 64, 64 slots of 4000 28 / 19 / 18 / 15 / 15 / 19;
         // 128 slots x 5 tokens of 28/4 heads, of 4000 85 / 103 / 113 / 125 / 159 / 160.  Behind a
-        // prefix of 4096, 1 / 2 / 4 / 8: 8 slots of 1000 20.5 / 16.3 / 14.4 / 16.3, 128 of 1000 49 /
-        // 51 / 60 / 88.
+        // prefix of 4096, 1 / 2 / 4 / 8: 128 slots of 1000 49 / 51 / 60 / 88.
         const bool few = own_base <= ctx->num_cu;
-        own = few           ? std::min(own_room / 256, (4LL * ctx->num_cu + (prefix_pages ? own_base - 1 : 0)) / own_base)
+        // Behind a prefix, whose tasks have a CU each beside them, up to three to a CU, of 256
+        // to 512 positions or two.  us, four to a CU of 256 (of 64-wide heads one up to 768) / this:
+        // behind 6016 2, 8, 64 slots of 14/2 heads of 700 12.8 / 10.3, 13.2 / 11.1, 16.7 / 15.3, 32 of
+        // 4000 16.6 / 15.3, behind 8192 16 of 32/8 of 700 18.0 / 15.8, 24 of 1000 25.5 / 23.7, behind
+        // 4096 16 x 4 tokens of 28/4 of 1500 24.9 / 21.7; but 64 of 14/2 of 4000 21.6 / 22.4.
+        const long long least = (nb == 1 ? 4 : 8) * own_base <= ctx->num_cu ? 256 : 2 * own_base <= ctx->num_cu ? 384 : 512;
+        own = few && prefix_pages
+                  ? std::min(std::min(own_room / 256, std::max(own_room / least, 2LL)), 3LL * ctx->num_cu / own_base)
+              : few          ? std::min(own_room / 256, 4LL * ctx->num_cu / own_base)
               : prefix_pages ? std::min(own_room / 750, (16LL * ctx->num_cu + own_base - 1) / own_base)
                              : std::min(own_room / 750, 2LL * wgs * ctx->num_cu / own_base);
         // Parts in eights, up to 32: an XCD, which take workgroups in turn, then has the same
@@ -1891,7 +1898,7 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
             else if (down && own_room <= 1536 * down) own = down;
             own = std::min(own, 32LL);
         }
-        if (prefix_pages ? own_room <= brief || own_base * 1024 >= own_room * ctx->num_cu
+        if (prefix_pages ? (!few && own_room <= brief) || own_base * 1024 >= own_room * ctx->num_cu
                          : own_room <= once || own_base * (wide ? 2 : nb) * 1024 >= own_room * ctx->num_cu)
             own = 1;
     } else if (prefix_pages ? (own_room <= (dim == 64 ? 640 : 512) && 3 * own_base >= ctx->num_cu) || (mode && own_room <= 256)
