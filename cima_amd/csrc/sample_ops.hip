@@ -542,17 +542,56 @@ DEV float lp_f(float x, float cap) {
     const float e = __builtin_amdgcn_exp2f(x * (2.88539008177792681472f / cap));
     return __builtin_isinf(x) ? x : fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + e), cap);
 }
+// The token that is left at T <= 0 under a cap: of the largest f(x) the first, as softmax_rows
+// finds it, by its sm_f.  Several logits may have that f, the largest logit not the first
+// of them.
+struct LpBest {
+    float f = -INFINITY;
+    int at = 0x7fffffff;
+    DEV void take(float y, int i) {
+        if (y > f || (y == f && i < at)) f = y, at = i;
+    }
+    DEV void wave() {
+#pragma unroll
+        for (int o = 32; o; o >>= 1) take(__shfl_xor(f, o), __shfl_xor(at, o));
+    }
+    DEV int id() const { return f == -INFINITY ? -1 : at; }
+};
+// of logits [lo, hi) of a row of n, by the workgroup (one call in a kernel); the result in
+// every thread
+template <int NT, bool F32, int V>
+DEV LpBest lp_best(const void* x, size_t row0, int lo, int hi, int n, float cap) {
+    __shared__ float most[NT / 64];
+    __shared__ int place[NT / 64];
+    LpBest b;
+#pragma unroll 1
+    for (int i = lo + threadIdx.x * V; i < hi; i += NT * V) {
+        uint32_t v[F32 ? V : V / 2];
+        sm_load<F32, V>(x, row0, i, n, v);
+#pragma unroll
+        for (int j = 0; j < V; j++) b.take(sm_f(sm_get<F32, V>(v, j), cap), i + j);
+    }
+    b.wave();
+    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = b.f, place[threadIdx.x >> 6] = b.at;
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < NT / 64; k++) b.take(most[k], place[k]);
+    return b;
+}
+// alternatives that are looked for: where T <= 0 and there is no cap, the one token
+DEV int lp_kept(const LpArgs& A, float T, bool cap) { return A.n_top ? A.n_top : T > 0.f || cap ? 0 : 1; }
 // a row's results: largest f(x) m, sums L (and its logarithm) and H as in LpArgs, the
-// best keys in top
+// best keys in top; under a cap at T <= 0 the token that is left (LpBest::id), without one
+// the first of top
 DEV void lp_finish(const LpArgs& A, int row, float T, float m, double ln, double L, double H,
-                   const unsigned long long* top, float xt, bool cap) {
+                   const unsigned long long* top, float xt, bool cap, int left) {
     auto logprob = [&](float x) -> float {
         if (x == -INFINITY) return -INFINITY;
         const float f = cap ? lp_f(x, A.cap) : x;
         return (float)((double)(f - m) / (double)T - ln);
     };
     const bool one = !(T > 0.f);  // the largest logit alone
-    const int first = one && top[0] ? lp_id(top[0]) : -1;
+    const int first = !one ? -1 : cap ? left : top[0] ? lp_id(top[0]) : -1;
     const int t = threadIdx.x;
     if (t == 0) {
         const int id = A.tokens ? A.tokens[row] : -1;
@@ -561,7 +600,12 @@ DEV void lp_finish(const LpArgs& A, int row, float T, float m, double ln, double
         if (A.entropy) A.entropy[row] = one || L == 0. ? 0.f : (float)(ln - 0.69314718055994530942 * H / L);
     }
     if (t < A.n_top) {
-        const unsigned long long k = top[t];
+        unsigned long long k = top[t];
+        if (one && cap && first >= 0) {  // it comes before those with larger logits
+            bool behind = false;
+            for (int i = 0; i < t; i++) behind |= lp_id(top[i]) == first;
+            if (!behind) k = t ? top[t - 1] : lp_key(0, first);
+        }
         A.top_ids[(size_t)row * A.n_top + t] = k ? lp_id(k) : -1;
         A.top_logprobs[(size_t)row * A.n_top + t] =
             !k ? -INFINITY : one ? (t ? -INFINITY : 0.f) : logprob(lp_value((uint32_t)(k >> 32)));
@@ -691,7 +735,7 @@ DEV void lp_whole(const LpArgs& A) {
     P.template add<false>(v, mine, A.cap, s);
     float m;
     P.template join<NT, false>(&m, A.cap, s);
-    const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
+    const int kept = lp_kept(A, T, CAP);
     if (kept)
         lp_select<NT, F32>(
             S, kept, A.x, row0, A.n, mine,
@@ -708,7 +752,10 @@ DEV void lp_whole(const LpArgs& A) {
                 }
             },
             [&](auto f) { f(mine); }, [] {});
-    lp_finish(A, row, T, m, log((double)P.l), P.l, P.h, S.top, xt, CAP);
+    int left = -1;
+    if constexpr (CAP)
+        if (!(T > 0.f)) left = lp_best<NT, F32, V>(A.x, row0, 0, A.n, A.n, A.cap).id();
+    lp_finish(A, row, T, m, log((double)P.l), P.l, P.h, S.top, xt, CAP, left);
 }
 
 // Parts of rows: 256 threads, 2^chunk_shift chunks of 32 logits a thread (SMALL: one
@@ -732,7 +779,7 @@ DEV void lp_part(const LpArgs& A) {
     const int first = part << A.chunk_shift, all = (A.n - 1) / P::CHUNK + 1, last = min(first + (1 << A.chunk_shift), all);
     const size_t row0 = (size_t)row * A.n;
     const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
-    const bool kept = A.n_top || !(T > 0.f);
+    const bool kept = lp_kept(A, T, CAP);
     typename P::Largest* to = (typename P::Largest*)A.largest + (size_t)row * all * P::GROUPS;
     LpSums<F32, CAP, P::R, P::V> S;
     using Words = typename decltype(S)::Words;
@@ -789,6 +836,13 @@ DEV void lp_part(const LpArgs& A) {
         S.template join<256, fast>(&m, A.cap, s);
         if (t == 0) A.stats[blockIdx.x] = make_float4(m, S.l, S.h, 0.f);
     };
+    if constexpr (CAP)
+        if (!(T > 0.f)) {  // no sums are asked for, but the token that is left: {f, id, 0, 0}
+            const LpBest b = lp_best<256, F32, P::V>(A.x, row0, first * P::CHUNK, min(last * P::CHUNK, A.n), A.n, A.cap);
+            if (A.n_top) all_chunks(std::false_type{});
+            if (t == 0) A.stats[blockIdx.x] = make_float4(b.f, __builtin_bit_cast(float, b.at), 0.f, 0.f);
+            return;
+        }
     if constexpr (F32 || CAP) all_chunks(std::false_type{});
     else if (s <= LP_FAST) all_chunks(std::true_type{});
     else all_chunks(std::false_type{});
@@ -804,13 +858,25 @@ DEV void lp_join(const LpArgs& A) {
     const size_t row0 = (size_t)row * A.n;
     const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
     const float xt = lp_load<F32>(A.x, row0, A.tokens ? A.tokens[row] : -1, A.n);
-    const int kept = A.n_top ? A.n_top : T > 0.f ? 0 : 1;
+    const int kept = lp_kept(A, T, CAP);
     __shared__ double sums[3];
     __shared__ float largest;
+    __shared__ int left;
     // the sums, by one wave
     const float4* st = A.stats + (size_t)row * A.parts;
     const float4 first = st[min(lane, A.parts - 1)];
     auto join = [&] {
+        if constexpr (CAP)
+            if (!(T > 0.f)) {
+                LpBest b;
+                for (int p = lane; p < A.parts; p += 64) {
+                    const float4 q = p < 64 ? first : st[p];
+                    b.take(q.x, __builtin_bit_cast(int, q.y));
+                }
+                b.wave();
+                left = b.id();
+                return;
+            }
         float m = -INFINITY;
         for (int p = lane; p < A.parts; p += 64) m = fmaxf(m, p < 64 ? first.x : st[p].x);
         m = wave_max_u(m);
@@ -870,7 +936,7 @@ DEV void lp_join(const LpArgs& A) {
             [&](auto f) { each_group([&](float x, int) { f(x); }); }, join);
         if (t >= 64) return;
     }
-    lp_finish(A, row, T, largest, sums[0], sums[1], sums[2], S.top, xt, CAP);
+    lp_finish(A, row, T, largest, sums[0], sums[1], sums[2], S.top, xt, CAP, left);
 }
 #define LOGPROBS_WHOLE(NAME, F32, CAP, NT, R)                                                             \
     extern "C" __global__ __launch_bounds__(NT) void cima_logprobs_t##NT##_w##R##_##NAME(const LpArgs A) { \

@@ -563,8 +563,9 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
  * An id outside [0, n) has -inf, as has a token whose logit is -inf; such tokens are
  * not among the likeliest, nor is NaN: entries that no token is left for are -1 and
  * -inf.  A row that softmax_rows makes NaN has NaN for its entropy and its other log
- * probabilities, one of -inf alone an entropy of 0.  Where temp <= 0 or NaN the largest
- * logit has 0, all others -inf.
+ * probabilities, one of -inf alone an entropy of 0.  Where temp <= 0 or NaN the token
+ * that softmax_rows gives 1 (the first of the largest capped logits, which need not be the
+ * largest logit) has 0 and comes first, all others have -inf.
  * tokens, logprob and entropy may be NULL (not wanted), as top_ids and top_logprobs
  * with n_top 0; n_top at most 32, less than 2^22 rows.  slab (16-byte aligned): 528
  * bytes (f32 1040) for each 8192 logits of a row (rounded up) and row; none is needed
