@@ -628,6 +628,24 @@ DEV uint32_t lp_largest(const uint32_t* v) {
     }
     return p;
 }
+// Signalling NaN hides what a maximum had before it.  Where a thread's sum says that one of
+// its logits is NaN, the largest of V from element i on is found anew, NaN as -inf; from
+// memory, so that no register is held for it.
+template <bool F32>
+DEV uint32_t lp_number(uint32_t v) {
+    if constexpr (F32) return (v & 0x7fffffffu) > 0x7f800000u ? 0xff800000u : v;
+    const uint32_t lo = v & 0xffffu, hi = v >> 16;
+    return ((lo & 0x7fffu) > 0x7c00u ? 0xfc00u : lo) | ((hi & 0x7fffu) > 0x7c00u ? 0xfc00u : hi) << 16;
+}
+template <bool F32, int V>
+DEV uint32_t lp_largest_number(const void* x, size_t row0, int i, int n) {
+    constexpr int W = F32 ? V : V / 2;
+    uint32_t v[W];
+    sm_load<F32, V>(x, row0, i, n, v);
+#pragma unroll
+    for (int k = 0; k < W; k++) v[k] = lp_number<F32>(v[k]);
+    return lp_largest<F32, W>(v);
+}
 // (NaN alone: -inf)
 template <bool F32>
 DEV float lp_of(uint32_t p) {
@@ -731,8 +749,14 @@ DEV void lp_whole(const LpArgs& A) {
     for (int r = 0; r < R; r++) sm_load<F32, V>(A.x, row0, t * V + r * NT * V, A.n, v[r]);
     const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
     const float xt = lp_load<F32>(A.x, row0, A.tokens ? A.tokens[row] : -1, A.n);
-    const float mine = lp_of<F32>(lp_largest<F32, R * P.W>(&v[0][0]));
+    float mine = lp_of<F32>(lp_largest<F32, R * P.W>(&v[0][0]));
     P.template add<false>(v, mine, A.cap, s);
+    if (__any(P.l != P.l)) {
+        mine = -INFINITY;
+#pragma unroll 1
+        for (int r = 0; r < R; r++)
+            mine = fmaxf(mine, lp_of<F32>(lp_largest_number<F32, V>(A.x, row0, t * V + r * NT * V, A.n)));
+    }
     float m;
     P.template join<NT, false>(&m, A.cap, s);
     const int kept = lp_kept(A, T, CAP);
@@ -801,6 +825,12 @@ DEV void lp_part(const LpArgs& A) {
             for (int r = 0; r < P::R; r++) sm_load<F32, P::V>(A.x, row0, k * P::CHUNK + t * P::V + r * 256 * P::V, A.n, v[r]);
         }
     };
+    // the largest of the group that word r of this thread is in
+    auto put = [&](int k, int r, uint32_t g) {
+        typename P::Largest* o = to + k * P::GROUPS + t / P::LANES * P::R + r;
+        if constexpr (F32) *o = lp_of<F32>(g);
+        else *o = (uint16_t)f2h(lp_of<F32>(g));
+    };
     auto all_chunks = [&](auto fast) {
         auto add = [&](int k, const Words& v) {
             uint32_t word[P::R];
@@ -815,11 +845,7 @@ DEV void lp_part(const LpArgs& A) {
                     const uint32_t p = lp_lanes<F32, P::LANES>(word[r]);
                     g = i == r ? p : g;
                 }
-                typename P::Largest* o = to + k * P::GROUPS + t / P::LANES * P::R + i;
-                if (i < P::R) {
-                    if constexpr (F32) *o = lp_of<F32>(g);
-                    else *o = (uint16_t)f2h(lp_of<F32>(g));
-                }
+                if (i < P::R) put(k, i, g);
             }
             S.template add<fast>(v, m, A.cap, s);
         };
@@ -832,6 +858,13 @@ DEV void lp_part(const LpArgs& A) {
             if (k + 2 < last) load(k + 2, v);
             add(k + 1, next);
         }
+        if (kept && __any(S.l != S.l))
+#pragma unroll 1
+            for (int i = first * P::R; i < last * P::R; i++) {
+                const int k = i / P::R, r = i % P::R, at = k * P::CHUNK + t * P::V + r * 256 * P::V;
+                const uint32_t p = lp_lanes<F32, P::LANES>(lp_largest_number<F32, P::V>(A.x, row0, at, A.n));
+                if (t % P::LANES == r) put(k, r, p);  // the lane that wrote it before
+            }
         float m;
         S.template join<256, fast>(&m, A.cap, s);
         if (t == 0) A.stats[blockIdx.x] = make_float4(m, S.l, S.h, 0.f);

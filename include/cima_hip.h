@@ -570,8 +570,7 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
  * with n_top 0; n_top at most 32, less than 2^22 rows.  slab (16-byte aligned): 528
  * bytes (f32 1040) for each 8192 logits of a row (rounded up) and row; none is needed
  * up to 32768 logits, where it makes some hundreds of rows faster.  One of 280 KB or
- * more makes few long rows faster.  A signalling NaN may hide other tokens of its row
- * from the likeliest. */
+ * more makes few long rows faster. */
 int cima_hip_logprobs_rows(cima_hip_ctx* ctx, const void* x, int rows, int n, const int* tokens, float* logprob,
                            float* entropy, int n_top, int* top_ids, float* top_logprobs, const float* temp,
                            int rows_per_temp, float cap, int x_dtype, void* slab, unsigned long long slab_bytes);
