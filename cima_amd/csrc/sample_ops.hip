@@ -557,25 +557,42 @@ struct LpBest {
     }
     DEV int id() const { return f == -INFINITY ? -1 : at; }
 };
-// of logits [lo, hi) of a row of n, by the workgroup (one call in a kernel); the result in
-// every thread
+// Below this no logit's sm_f is as large as that of `most`.  sm_f is off by 2^-21 of itself at
+// most (the quotient, tanhf, the product); from 0 on tanh rises by its slope at the end
+// of a stretch or more, 1 - tanh^2, and from 6.5 to 8 by 4.3e-6.
+DEV float lp_as_large(float most, float cap) {
+    if (!(most > 0.f)) return -INFINITY;
+    if (__builtin_isinf(most)) return most;
+    const float u = most / cap;
+    if (u >= 8.f) return 6.5f * cap;
+    const float th = tanhf(u);
+    return most - cap * th * 0x1p-19f / ((1.f - th) * (1.f + th));
+}
+// of logits [lo, hi) of a row of n, by the workgroup (one call in a kernel), the largest of
+// which that a thread looked at is `most`; the result in every thread
 template <int NT, bool F32, int V>
-DEV LpBest lp_best(const void* x, size_t row0, int lo, int hi, int n, float cap) {
-    __shared__ float most[NT / 64];
+DEV LpBest lp_best(const void* x, size_t row0, int lo, int hi, int n, float cap, float most) {
+    __shared__ float best[NT / 64];
     __shared__ int place[NT / 64];
     LpBest b;
-#pragma unroll 1
+    const float least = lp_as_large(wave_max_u(most), cap);
+#pragma unroll 4
     for (int i = lo + threadIdx.x * V; i < hi; i += NT * V) {
         uint32_t v[F32 ? V : V / 2];
         sm_load<F32, V>(x, row0, i, n, v);
+        uint32_t near = 0;  // bit j: logit j may be it
 #pragma unroll
-        for (int j = 0; j < V; j++) b.take(sm_f(sm_get<F32, V>(v, j), cap), i + j);
+        for (int j = 0; j < V; j++) near |= sm_get<F32, V>(v, j) >= least ? 1u << j : 0;
+        for (; near; near &= near - 1) {
+            const int j = __builtin_ctz(near);
+            b.take(sm_f(lp_load<F32>(x, row0, i + j, n), cap), i + j);
+        }
     }
     b.wave();
-    if ((threadIdx.x & 63) == 0) most[threadIdx.x >> 6] = b.f, place[threadIdx.x >> 6] = b.at;
+    if ((threadIdx.x & 63) == 0) best[threadIdx.x >> 6] = b.f, place[threadIdx.x >> 6] = b.at;
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < NT / 64; k++) b.take(most[k], place[k]);
+    for (int k = 0; k < NT / 64; k++) b.take(best[k], place[k]);
     return b;
 }
 // alternatives that are looked for: where T <= 0 and there is no cap, the one token
@@ -749,16 +766,19 @@ DEV void lp_whole(const LpArgs& A) {
     for (int r = 0; r < R; r++) sm_load<F32, V>(A.x, row0, t * V + r * NT * V, A.n, v[r]);
     const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
     const float xt = lp_load<F32>(A.x, row0, A.tokens ? A.tokens[row] : -1, A.n);
-    float mine = lp_of<F32>(lp_largest<F32, R * P.W>(&v[0][0]));
-    P.template add<false>(v, mine, A.cap, s);
-    if (__any(P.l != P.l)) {
+    const bool one = CAP && !(T > 0.f);  // no sums are asked for, but the token that is left
+    float mine = -INFINITY, m = 0.f;
+    if (!one) {
+        mine = lp_of<F32>(lp_largest<F32, R * P.W>(&v[0][0]));
+        P.template add<false>(v, mine, A.cap, s);
+    }
+    if (one || __any(P.l != P.l)) {
         mine = -INFINITY;
 #pragma unroll 1
         for (int r = 0; r < R; r++)
             mine = fmaxf(mine, lp_of<F32>(lp_largest_number<F32, V>(A.x, row0, t * V + r * NT * V, A.n)));
     }
-    float m;
-    P.template join<NT, false>(&m, A.cap, s);
+    if (!one) P.template join<NT, false>(&m, A.cap, s);
     const int kept = lp_kept(A, T, CAP);
     if (kept)
         lp_select<NT, F32>(
@@ -778,7 +798,7 @@ DEV void lp_whole(const LpArgs& A) {
             [&](auto f) { f(mine); }, [] {});
     int left = -1;
     if constexpr (CAP)
-        if (!(T > 0.f)) left = lp_best<NT, F32, V>(A.x, row0, 0, A.n, A.n, A.cap).id();
+        if (one) left = lp_best<NT, F32, V>(A.x, row0, 0, A.n, A.n, A.cap, mine).id();
     lp_finish(A, row, T, m, log((double)P.l), P.l, P.h, S.top, xt, CAP, left);
 }
 
@@ -831,6 +851,19 @@ DEV void lp_part(const LpArgs& A) {
         if constexpr (F32) *o = lp_of<F32>(g);
         else *o = (uint16_t)f2h(lp_of<F32>(g));
     };
+    // the groups alone, NaN as -inf; the largest of this thread's logits
+    auto find_groups = [&] {
+        float most = -INFINITY;
+#pragma unroll P::R
+        for (int i = first * P::R; i < last * P::R; i++) {
+            const int k = i / P::R, r = i % P::R, at = k * P::CHUNK + t * P::V + r * 256 * P::V;
+            uint32_t p = lp_largest_number<F32, P::V>(A.x, row0, at, A.n);
+            most = fmaxf(most, lp_of<F32>(p));
+            p = lp_lanes<F32, P::LANES>(p);
+            if (kept && t % P::LANES == r) put(k, r, p);  // by the same lane as add's
+        }
+        return most;
+    };
     auto all_chunks = [&](auto fast) {
         auto add = [&](int k, const Words& v) {
             uint32_t word[P::R];
@@ -858,21 +891,15 @@ DEV void lp_part(const LpArgs& A) {
             if (k + 2 < last) load(k + 2, v);
             add(k + 1, next);
         }
-        if (kept && __any(S.l != S.l))
-#pragma unroll 1
-            for (int i = first * P::R; i < last * P::R; i++) {
-                const int k = i / P::R, r = i % P::R, at = k * P::CHUNK + t * P::V + r * 256 * P::V;
-                const uint32_t p = lp_lanes<F32, P::LANES>(lp_largest_number<F32, P::V>(A.x, row0, at, A.n));
-                if (t % P::LANES == r) put(k, r, p);  // the lane that wrote it before
-            }
+        if (kept && __any(S.l != S.l)) find_groups();
         float m;
         S.template join<256, fast>(&m, A.cap, s);
         if (t == 0) A.stats[blockIdx.x] = make_float4(m, S.l, S.h, 0.f);
     };
     if constexpr (CAP)
         if (!(T > 0.f)) {  // no sums are asked for, but the token that is left: {f, id, 0, 0}
-            const LpBest b = lp_best<256, F32, P::V>(A.x, row0, first * P::CHUNK, min(last * P::CHUNK, A.n), A.n, A.cap);
-            if (A.n_top) all_chunks(std::false_type{});
+            const float most = find_groups();
+            const LpBest b = lp_best<256, F32, P::V>(A.x, row0, first * P::CHUNK, min(last * P::CHUNK, A.n), A.n, A.cap, most);
             if (t == 0) A.stats[blockIdx.x] = make_float4(b.f, __builtin_bit_cast(float, b.at), 0.f, 0.f);
             return;
         }
