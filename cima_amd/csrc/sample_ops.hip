@@ -536,11 +536,63 @@ DEV void lp_select(LpTop<NT>& S, int kept, const void* x, size_t row0, int n, fl
     }
     __syncthreads();
 }
-// f of a logit as sm_f, cap - 2 cap / (1 + e^(2 x / cap)): off by cap 2^-21 at most, which
-// is all that a log probability asks of it (384 rows of 128256 48.6 -> 35.6 us)
-DEV float lp_f(float x, float cap) {
-    const float e = __builtin_amdgcn_exp2f(x * (2.88539008177792681472f / cap));
-    return __builtin_isinf(x) ? x : fmaf(-2.f * cap, __builtin_amdgcn_rcpf(1.f + e), cap);
+// f of a logit, cap tanh(x / cap), by two forms that are off by 2^-22 of it at most (as tanhf
+// is), whatever the cap.  Up to the cap, u = x / cap: x (1 + t P(t)), t = u^2, P fitted to
+// (tanh(u) / u - 1) / t for the least relative error, 5.5e-8; its highest coefficient is positive,
+// so that infinities stay.  Above it cap - 2 cap / (1 + e^(2 |u|)), which cancels no
+// more there: the quotient is 0.24 or less.  A wave takes the first for words of which no
+// logit is above the cap, ten instructions at the full rate a logit.
+struct LpCap {
+    float cap, inv, s;  // 1 / cap; 2 log2(e) / cap
+    uint32_t least, span;  // as bits, of f16 logits twice: above these finite logits may be above the cap; how far
+};
+template <bool F32>
+DEV LpCap lp_cap(float cap) {
+    LpCap C;
+    C.cap = cap;
+    C.inv = fminf(1.f / cap, 1e38f);
+    C.s = 2.88539008177792681472f * C.inv;
+    const float least = cap * 0.999999f;  // the rounding of u
+    if constexpr (F32) {
+        C.least = __builtin_bit_cast(uint32_t, least) + 1;
+        C.span = 0x7f800000u - C.least;
+    } else {
+        uint32_t h = least < 65504.f ? f2h(least) : 0x7bffu;
+        if (h2f(h) > least) h--;
+        C.least = (h + 1) * 0x10001u, C.span = 0x7c00u - (h + 1);
+    }
+    return C;
+}
+DEV float lp_low(float x, const LpCap& C) {
+    const float u = x * C.inv, t = u * u;
+    float p = fmaf(t, 0.0010582645928059005f, -0.006259339200112074f);
+    p = fmaf(t, p, 0.020359759264195577f);
+    p = fmaf(t, p, -0.053498707589033995f);
+    p = fmaf(t, p, 0.13326408874426884f);
+    p = fmaf(t, p, -0.3333298677943413f);
+    return fmaf(x * t, p, x);
+}
+DEV float lp_f(float x, const LpCap& C) {
+    const float e = __builtin_amdgcn_exp2f(fabsf(x) * C.s);
+    const float high = copysignf(fmaf(-2.f * __builtin_amdgcn_rcpf(1.f + e), C.cap, C.cap), x);
+    return __builtin_isinf(x) ? x : fabsf(x * C.inv) <= 1.f ? lp_low(x, C) : high;
+}
+// whether any finite logit of a wave's words may be above the cap
+template <bool F32, int W>
+DEV bool lp_any_high(const uint32_t (&v)[W], const LpCap& C) {
+    if constexpr (F32) {
+        uint32_t m = 0xffffffffu;
+#pragma unroll
+        for (int i = 0; i < W; i++) m = min(m, (v[i] & 0x7fffffffu) - C.least);
+        return __any(m < C.span);
+    } else {
+        typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+        us2 m = {0xffff, 0xffff};
+#pragma unroll
+        for (int i = 0; i < W; i++)
+            m = __builtin_elementwise_min(m, __builtin_bit_cast(us2, v[i] & 0x7fff7fffu) - __builtin_bit_cast(us2, C.least));
+        return __any(m[0] < C.span || m[1] < C.span);
+    }
 }
 // The token that is left at T <= 0 under a cap: of the largest f(x) the first, as softmax_rows
 // finds it, by its sm_f.  Several logits may have that f, the largest logit not the first
@@ -602,9 +654,10 @@ DEV int lp_kept(const LpArgs& A, float T, bool cap) { return A.n_top ? A.n_top :
 // the first of top
 DEV void lp_finish(const LpArgs& A, int row, float T, float m, double ln, double L, double H,
                    const unsigned long long* top, float xt, bool cap, int left) {
+    const LpCap C = lp_cap<true>(A.cap);
     auto logprob = [&](float x) -> float {
         if (x == -INFINITY) return -INFINITY;
-        const float f = cap ? lp_f(x, A.cap) : x;
+        const float f = cap ? lp_f(x, C) : x;
         return (float)((double)(f - m) / (double)T - ln);
     };
     const bool one = !(T > 0.f);  // the largest logit alone
@@ -702,22 +755,19 @@ struct LpSums {
     }
     // words whose largest is m
     template <bool FAST>
-    DEV void add(const Words& v, float m, float cap, float s) {
+    DEV void add(const Words& v, float m, const LpCap& C, float s) {
         if (m > mine) {
-            bring<FAST>(CAP ? lp_f(m, cap) : m, s);
+            bring<FAST>(CAP ? lp_f(m, C) : m, s);
             mine = m;
         }
         const float least = -1e30f;  // for a product with 0
-#pragma unroll
-        for (int r = 0; r < R; r++) {
+        // z of logit j of word r: of(r, j)
+        auto word = [&](int r, auto of) {
             float pl, ph;
 #pragma unroll
             for (int j = 0; j < V; j++) {
-                float z, y;
-                if constexpr (FAST) z = mix_fma(v[r][j / 2], j & 1, s, b);
-                else if constexpr (CAP) z = (lp_f(sm_get<F32, V>(v[r], j), cap) - c) * s;
-                else if constexpr (F32) z = (sm_get<F32, V>(v[r], j) - c) * s;
-                else z = mix_less(v[r][j / 2], j & 1, c) * s;
+                const float z = of(r, j);
+                float y;
                 const float e = __builtin_amdgcn_exp2f(z);
                 // (fmaxf of what an asm returns is two instructions, the first for NaN, which e has)
                 __asm__("v_max_f32 %0, %1, %2" : "=v"(y) : "s"(least), "v"(z));
@@ -725,11 +775,24 @@ struct LpSums {
                 ph = j ? fmaf(e, y, ph) : e * y;
             }
             l += pl, h += ph;
+        };
+#pragma unroll
+        for (int r = 0; r < R; r++) {
+            if constexpr (CAP) {
+                if (lp_any_high<F32>(v[r], C)) word(r, [&](int r, int j) { return (lp_f(sm_get<F32, V>(v[r], j), C) - c) * s; });
+                else word(r, [&](int r, int j) { return (lp_low(sm_get<F32, V>(v[r], j), C) - c) * s; });
+            } else {
+                word(r, [&](int r, int j) {
+                    if constexpr (FAST) return mix_fma(v[r][j / 2], j & 1, s, b);
+                    else if constexpr (F32) return (sm_get<F32, V>(v[r], j) - c) * s;
+                    else return mix_less(v[r][j / 2], j & 1, c) * s;
+                });
+            }
         }
     }
     // the workgroup's: *m is f of its largest
     template <int NT, bool FAST>
-    DEV void join(float* m, float cap, float s) {
+    DEV void join(float* m, const LpCap& C, float s) {
         __shared__ float red[3][NT / 64];
         const int w = threadIdx.x >> 6;
         const float a = wave_max_u(mine);
@@ -738,7 +801,7 @@ struct LpSums {
         float g = red[0][0];
 #pragma unroll
         for (int k = 1; k < NT / 64; k++) g = fmaxf(g, red[0][k]);
-        *m = uniform(CAP ? lp_f(g, cap) : g);
+        *m = uniform(CAP ? lp_f(g, C) : g);
         bring<FAST>(*m, s);
         l = wave_sum_u(l), h = wave_sum_u(h);
         if ((threadIdx.x & 63) == 0) red[1][w] = l, red[2][w] = h;
@@ -760,6 +823,7 @@ DEV void lp_whole(const LpArgs& A) {
     __shared__ LpTop<NT> S;
     const int row = blockIdx.x, t = threadIdx.x;
     const size_t row0 = (size_t)row * A.n;
+    const LpCap C = lp_cap<F32>(A.cap);
     LpSums<F32, CAP, R, V> P;
     typename decltype(P)::Words v;
 #pragma unroll
@@ -770,7 +834,7 @@ DEV void lp_whole(const LpArgs& A) {
     float mine = -INFINITY, m = 0.f;
     if (!one) {
         mine = lp_of<F32>(lp_largest<F32, R * P.W>(&v[0][0]));
-        P.template add<false>(v, mine, A.cap, s);
+        P.template add<false>(v, mine, C, s);
     }
     if (one || __any(P.l != P.l)) {
         mine = -INFINITY;
@@ -778,7 +842,7 @@ DEV void lp_whole(const LpArgs& A) {
         for (int r = 0; r < R; r++)
             mine = fmaxf(mine, lp_of<F32>(lp_largest_number<F32, V>(A.x, row0, t * V + r * NT * V, A.n)));
     }
-    if (!one) P.template join<NT, false>(&m, A.cap, s);
+    if (!one) P.template join<NT, false>(&m, C, s);
     const int kept = lp_kept(A, T, CAP);
     if (kept)
         lp_select<NT, F32>(
@@ -825,6 +889,7 @@ DEV void lp_part(const LpArgs& A) {
     const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
     const bool kept = lp_kept(A, T, CAP);
     typename P::Largest* to = (typename P::Largest*)A.largest + (size_t)row * all * P::GROUPS;
+    const LpCap C = lp_cap<F32>(A.cap);
     LpSums<F32, CAP, P::R, P::V> S;
     using Words = typename decltype(S)::Words;
     auto load = [&](int k, Words& v) {
@@ -880,7 +945,7 @@ DEV void lp_part(const LpArgs& A) {
                 }
                 if (i < P::R) put(k, i, g);
             }
-            S.template add<fast>(v, m, A.cap, s);
+            S.template add<fast>(v, m, C, s);
         };
         Words v, next;
         load(first, v);
@@ -893,7 +958,7 @@ DEV void lp_part(const LpArgs& A) {
         }
         if (kept && __any(S.l != S.l)) find_groups();
         float m;
-        S.template join<256, fast>(&m, A.cap, s);
+        S.template join<256, fast>(&m, C, s);
         if (t == 0) A.stats[blockIdx.x] = make_float4(m, S.l, S.h, 0.f);
     };
     if constexpr (CAP)

@@ -560,6 +560,7 @@ int cima_hip_softmax_rows(cima_hip_ctx* ctx, const void* x, float* y, int rows, 
  * gives of x, temp, rows_per_temp and cap, entropy[r] = -sum p ln p, and
  * top_ids, top_logprobs [rows, n_top] the n_top likeliest tokens of a row and their
  * log probabilities, the largest logit first, equal ones by the lower id.  All fp32.
+ * A capped logit is off by 2^-21 of itself at most, whatever the cap.
  * An id outside [0, n) has -inf, as has a token whose logit is -inf; such tokens are
  * not among the likeliest, nor is NaN: entries that no token is left for are -1 and
  * -inf.  A row that softmax_rows makes NaN has NaN for its entropy and its other log
