@@ -658,7 +658,7 @@ DEV void lp_finish(const LpArgs& A, int row, float T, float m, double ln, double
     auto logprob = [&](float x) -> float {
         if (x == -INFINITY) return -INFINITY;
         const float f = cap ? lp_f(x, C) : x;
-        return (float)((double)(f - m) / (double)T - ln);
+        return (float)(((double)f - m) / T - ln);
     };
     const bool one = !(T > 0.f);  // the largest logit alone
     const int first = !one ? -1 : cap ? left : top[0] ? lp_id(top[0]) : -1;
@@ -734,8 +734,25 @@ DEV uint32_t lp_lanes(uint32_t p) {
     if constexpr (LANES == 8) other(__builtin_amdgcn_mov_dpp(p, 0x141, 0xf, 0xf, false));
     return p;
 }
+// a row's temperature: 2^-127 where it is positive and less, whose reciprocal is none
+DEV float lp_temp(const LpArgs& A, int row) {
+    const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f;
+    return T > 0.f ? fmaxf(T, 0x1p-127f) : T;
+}
+// z = (half y - half c) s, s = log2(e) / (half T): the halves of two fp32 logits differ by a
+// number, they themselves may not; at low temperatures, where halving could round, they
+// are near each other or z is far below 0.  At an infinite one s is the least number, so that
+// -inf stays what it is.
+struct LpScale {
+    float s, half;
+};
+template <bool F32>
+DEV LpScale lp_scale(float T) {
+    const float half = F32 && T >= 1.f ? 0.5f : 1.f;
+    return {T > 0.f ? fmaxf(1.44269504088896340736f / T, 0x1p-149f) / half : 1.f, half};
+}
 // A thread's running sums of 2^z and 2^z z, R words of V logits at a time: z = (f(x) -
-// c) s, c f of the largest so far (0: none); FAST, of f16 logits, z = x s - b in one
+// c) s, c f of the largest so far (0: none), half of it as LpScale says; FAST, of f16 logits, z = x s - b in one
 // instruction, b = c s as fp32 holds it, which the end puts right.  It takes |c s| up
 // to 2^20, so that b is near enough: s up to LP_FAST.
 constexpr float LP_FAST = 16.f;
@@ -747,20 +764,22 @@ struct LpSums {
 
     // to another largest
     template <bool FAST>
-    DEV void bring(float to, float s) {
-        const float nb = to * s, z = mine == -INFINITY ? 0.f : FAST ? b - nb : (c - to) * s;
+    DEV void bring(float to, const LpScale& Z) {
+        const float nc = F32 ? to * Z.half : to, nb = to * Z.s, z = mine == -INFINITY ? 0.f : FAST ? b - nb : (c - nc) * Z.s;
         const float a = __builtin_amdgcn_exp2f(z);
         h = a * fmaf(fmaxf(z, -1e30f), l, h), l *= a;
-        c = to, b = nb;
+        c = nc, b = nb;
     }
     // words whose largest is m
     template <bool FAST>
-    DEV void add(const Words& v, float m, const LpCap& C, float s) {
+    DEV void add(const Words& v, float m, const LpCap& C, const LpScale& Z) {
         if (m > mine) {
-            bring<FAST>(CAP ? lp_f(m, C) : m, s);
+            bring<FAST>(CAP ? lp_f(m, C) : m, Z);
             mine = m;
         }
         const float least = -1e30f;  // for a product with 0
+        const float s = Z.s;
+        auto less = [&](float y) { return F32 ? fmaf(y, Z.half, -c) : y - c; };
         // z of logit j of word r: of(r, j)
         auto word = [&](int r, auto of) {
             float pl, ph;
@@ -779,12 +798,12 @@ struct LpSums {
 #pragma unroll
         for (int r = 0; r < R; r++) {
             if constexpr (CAP) {
-                if (lp_any_high<F32>(v[r], C)) word(r, [&](int r, int j) { return (lp_f(sm_get<F32, V>(v[r], j), C) - c) * s; });
-                else word(r, [&](int r, int j) { return (lp_low(sm_get<F32, V>(v[r], j), C) - c) * s; });
+                if (lp_any_high<F32>(v[r], C)) word(r, [&](int r, int j) { return less(lp_f(sm_get<F32, V>(v[r], j), C)) * s; });
+                else word(r, [&](int r, int j) { return less(lp_low(sm_get<F32, V>(v[r], j), C)) * s; });
             } else {
                 word(r, [&](int r, int j) {
                     if constexpr (FAST) return mix_fma(v[r][j / 2], j & 1, s, b);
-                    else if constexpr (F32) return (sm_get<F32, V>(v[r], j) - c) * s;
+                    else if constexpr (F32) return less(sm_get<F32, V>(v[r], j)) * s;
                     else return mix_less(v[r][j / 2], j & 1, c) * s;
                 });
             }
@@ -792,7 +811,7 @@ struct LpSums {
     }
     // the workgroup's: *m is f of its largest
     template <int NT, bool FAST>
-    DEV void join(float* m, const LpCap& C, float s) {
+    DEV void join(float* m, const LpCap& C, const LpScale& Z) {
         __shared__ float red[3][NT / 64];
         const int w = threadIdx.x >> 6;
         const float a = wave_max_u(mine);
@@ -802,7 +821,7 @@ struct LpSums {
 #pragma unroll
         for (int k = 1; k < NT / 64; k++) g = fmaxf(g, red[0][k]);
         *m = uniform(CAP ? lp_f(g, C) : g);
-        bring<FAST>(*m, s);
+        bring<FAST>(*m, Z);
         l = wave_sum_u(l), h = wave_sum_u(h);
         if ((threadIdx.x & 63) == 0) red[1][w] = l, red[2][w] = h;
         __syncthreads();
@@ -810,12 +829,11 @@ struct LpSums {
 #pragma unroll
         for (int k = 1; k < NT / 64; k++) l += red[1][k], h += red[2][k];
         if (FAST && *m != -INFINITY) {  // z less what b was rounded by
-            const float off = -fmaf(*m, s, -b), e = __builtin_amdgcn_exp2f(off);
+            const float off = -fmaf(*m, Z.s, -b), e = __builtin_amdgcn_exp2f(off);
             h = e * fmaf(off, l, h), l *= e;
         }
     }
 };
-DEV float lp_scale(float T) { return sm_scale(1.44269504088896340736f, T > 0.f ? T : 1.f); }
 
 // a row in R words of V logits a thread
 template <bool F32, bool CAP, int NT, int R, int V>
@@ -828,13 +846,14 @@ DEV void lp_whole(const LpArgs& A) {
     typename decltype(P)::Words v;
 #pragma unroll
     for (int r = 0; r < R; r++) sm_load<F32, V>(A.x, row0, t * V + r * NT * V, A.n, v[r]);
-    const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
+    const float T = lp_temp(A, row);
+    const LpScale Z = lp_scale<F32>(T);
     const float xt = lp_load<F32>(A.x, row0, A.tokens ? A.tokens[row] : -1, A.n);
     const bool one = CAP && !(T > 0.f);  // no sums are asked for, but the token that is left
     float mine = -INFINITY, m = 0.f;
     if (!one) {
         mine = lp_of<F32>(lp_largest<F32, R * P.W>(&v[0][0]));
-        P.template add<false>(v, mine, C, s);
+        P.template add<false>(v, mine, C, Z);
     }
     if (one || __any(P.l != P.l)) {
         mine = -INFINITY;
@@ -842,7 +861,7 @@ DEV void lp_whole(const LpArgs& A) {
         for (int r = 0; r < R; r++)
             mine = fmaxf(mine, lp_of<F32>(lp_largest_number<F32, V>(A.x, row0, t * V + r * NT * V, A.n)));
     }
-    if (!one) P.template join<NT, false>(&m, C, s);
+    if (!one) P.template join<NT, false>(&m, C, Z);
     const int kept = lp_kept(A, T, CAP);
     if (kept)
         lp_select<NT, F32>(
@@ -886,7 +905,8 @@ DEV void lp_part(const LpArgs& A) {
     const int row = blockIdx.x / A.parts, part = blockIdx.x % A.parts, t = threadIdx.x;
     const int first = part << A.chunk_shift, all = (A.n - 1) / P::CHUNK + 1, last = min(first + (1 << A.chunk_shift), all);
     const size_t row0 = (size_t)row * A.n;
-    const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
+    const float T = lp_temp(A, row);
+    const LpScale Z = lp_scale<F32>(T);
     const bool kept = lp_kept(A, T, CAP);
     typename P::Largest* to = (typename P::Largest*)A.largest + (size_t)row * all * P::GROUPS;
     const LpCap C = lp_cap<F32>(A.cap);
@@ -945,7 +965,7 @@ DEV void lp_part(const LpArgs& A) {
                 }
                 if (i < P::R) put(k, i, g);
             }
-            S.template add<fast>(v, m, C, s);
+            S.template add<fast>(v, m, C, Z);
         };
         Words v, next;
         load(first, v);
@@ -958,7 +978,7 @@ DEV void lp_part(const LpArgs& A) {
         }
         if (kept && __any(S.l != S.l)) find_groups();
         float m;
-        S.template join<256, fast>(&m, C, s);
+        S.template join<256, fast>(&m, C, Z);
         if (t == 0) A.stats[blockIdx.x] = make_float4(m, S.l, S.h, 0.f);
     };
     if constexpr (CAP)
@@ -969,7 +989,7 @@ DEV void lp_part(const LpArgs& A) {
             return;
         }
     if constexpr (F32 || CAP) all_chunks(std::false_type{});
-    else if (s <= LP_FAST) all_chunks(std::true_type{});
+    else if (Z.s <= LP_FAST && Z.s >= 1e-30f) all_chunks(std::true_type{});
     else all_chunks(std::false_type{});
 }
 
@@ -981,7 +1001,8 @@ DEV void lp_join(const LpArgs& A) {
     __shared__ LpTop<NT> S;
     const int row = blockIdx.x, t = threadIdx.x, lane = t & 63;
     const size_t row0 = (size_t)row * A.n;
-    const float T = A.temp ? A.temp[row / A.rows_per_temp] : 1.f, s = lp_scale(T);
+    const float T = lp_temp(A, row);
+    const double s = 1.44269504088896340736 / T;
     const float xt = lp_load<F32>(A.x, row0, A.tokens ? A.tokens[row] : -1, A.n);
     const int kept = lp_kept(A, T, CAP);
     __shared__ double sums[3];
@@ -1009,7 +1030,7 @@ DEV void lp_join(const LpArgs& A) {
         double L = 0, H = 0;
         for (int p = lane; p < A.parts; p += 64) {
             const float4 q = p < 64 ? first : st[p];
-            const float z = (q.x - c) * s, a = q.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(z);
+            const float z = (float)(((double)q.x - c) * s), a = q.x == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(z);
             L += (double)q.y * a;
             H += a != 0.f ? a * ((double)q.z + (double)q.y * (q.x == -INFINITY ? 0.f : z)) : 0.;
         }
