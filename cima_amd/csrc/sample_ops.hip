@@ -135,6 +135,13 @@ struct SmRow {
             for (int r = 0; r < R; r++)
 #pragma unroll
                 for (int j = 0; j < V; j++) m = fmaxf(m, get(r, j));
+            if (!(T > 0.f)) {  // by comparisons: a maximum loses what it had at a signalling NaN
+                m = -INFINITY;
+#pragma unroll
+                for (int r = 0; r < R; r++)
+#pragma unroll
+                    for (int j = 0; j < V; j++) m = get(r, j) > m ? get(r, j) : m;
+            }
         } else {  // two f16 at a time, exact
             typedef _Float16 hp __attribute__((ext_vector_type(2)));
             hp h = {(_Float16)-INFINITY, (_Float16)-INFINITY};
