@@ -5,8 +5,9 @@
 // Q4_1: codes 0 to 15, f16 scale d and least value m; value f16(c d + m).  d is the
 // least f16 that is not below (max - m) / 15, so that no code is cut off and a value
 // is off by at most d / 2 (and its rounding to f16).  Q8_0: codes -127 to 127, kept
-// with 128 added, f16 scale d, the least not below max|x| / 127; value f16(c d).  A
-// code is the nearest to the quotient, half to even.
+// with 128 added, f16 scale d, the least not below max|x| / 127 but at most 515.5, above
+// which 127 d would pass f16; value f16(c d).  A code is the nearest to the quotient, half
+// to even.
 //
 // A head's page is its rows' codes, then its rows' scales ({d, m} or d, in the
 // groups' order).  Eight elements of Q4_1 are a 32-bit word: element 2 k in nibble
@@ -131,7 +132,9 @@ DEV uint32_t kv_encode(const uint32_t (&x)[4], uint32_t (&w)[KvQ<BITS>::WORDS]) 
     constexpr float STEPS = BITS == 4 ? 15.f : 127.f;
     const float m = BITS == 4 ? lo + 0.f : 0.f;  // a least value of -0 as 0, whichever came first
     const double width = BITS == 4 ? (double)hi - (double)lo : (double)fmaxf(hi, -lo);
-    const uint32_t db = bad ? 0x7e00u : scale_up(width, STEPS);
+    uint32_t db = bad ? 0x7e00u : scale_up(width, STEPS);
+    // of 65472 and 65504 516, whose 127th multiple is no f16: 515.5, the nearest code still 127
+    if (BITS == 8 && db == 0x6008u) db = 0x6007u;
     const float d = h2f(db), inv = d > 0.f ? __builtin_amdgcn_rcpf(d) : 0.f;
     // the quotient's fp32 roundings (the reciprocal's 2^-23) at its largest, 15 or 127
     constexpr float NEAR = BITS == 4 ? 1e-5f : 1e-4f;

@@ -434,9 +434,9 @@ int cima_hip_decode_step(cima_hip_ctx* ctx, const cima_decoder* d);
  * quantised as they are written, a row's head_dim in groups of 32 as in the GGUF
  * block of that type, and stand for the f16 nearest to c d + m (codes c from 0 to
  * 15, f16 scale d and least value m) or c d (codes from -127 to 127).  d is the
- * least f16 that is not below (max - m) / 15 or max|x| / 127, c the code nearest to
- * the quotient (half to even): a value is off by at most d / 2 and its own rounding
- * (-0 may be 0).
+ * least f16 that is not below (max - m) / 15 or max|x| / 127 (at most 515.5, so that
+ * f16's largest read back finite), c the code nearest to the quotient (half to even): a
+ * value is off by at most d / 2 and its own rounding (-0 may be 0).
  * What is written has to be finite (a group that is not reads back as NaN), and of
  * Q4_1 at most 65000, which the sum may pass by.  A head's page is 20 / 32 or 34 /
  * 32 bytes an element: the codes of its rows, [page, head_dim], then the groups'
