@@ -1873,16 +1873,16 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
         // 160 / 164 / 166 / 173 / 193 / 245; 14/2 of 64, 64 slots of 4000 28 / 19 / 18 / 15 / 15 / 19;
         // 128 slots x 5 tokens of 28/4 heads, of 4000 85 / 103 / 113 / 125 / 159 / 160.  Behind a
         // prefix of 4096, 1 / 2 / 4 / 8: 128 slots of 1000 49 / 51 / 60 / 88.
-        const bool few = own_base <= ctx->num_cu;
+        const bool sparse = own_base <= ctx->num_cu;
         // Behind a prefix, whose tasks have a CU each beside them, up to three to a CU, of 256
         // to 512 positions or two.  us, four to a CU of 256 (of 64-wide heads one up to 768) / this:
         // behind 6016 2, 8, 64 slots of 14/2 heads of 700 12.8 / 10.3, 13.2 / 11.1, 16.7 / 15.3, 32 of
         // 4000 16.6 / 15.3, behind 8192 16 of 32/8 of 700 18.0 / 15.8, 24 of 1000 25.5 / 23.7, behind
         // 4096 16 x 4 tokens of 28/4 of 1500 24.9 / 21.7; but 64 of 14/2 of 4000 21.6 / 22.4.
         const long long least = (nb == 1 ? 4 : 8) * own_base <= ctx->num_cu ? 256 : 2 * own_base <= ctx->num_cu ? 384 : 512;
-        own = few && prefix_pages
+        own = sparse && prefix_pages
                   ? std::min(std::min(own_room / 256, std::max(own_room / least, 2LL)), 3LL * ctx->num_cu / own_base)
-              : few          ? std::min(own_room / 256, 4LL * ctx->num_cu / own_base)
+              : sparse       ? std::min(own_room / 256, 4LL * ctx->num_cu / own_base)
               : prefix_pages ? std::min(own_room / 750, (16LL * ctx->num_cu + own_base - 1) / own_base)
                              : std::min(own_room / 750, 2LL * wgs * ctx->num_cu / own_base);
         // Parts in eights, up to 32: an XCD, which take workgroups in turn, then has the same
@@ -1892,13 +1892,13 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
         // 12.7, 2 of 32/8 of 12000 in 46 / 32 14.2 / 12.9; but more than a round, 40 of 28/4 in 7 / 8
         // 24.2 / 25.6, 16 of 8 bits of 1700 in 6 / 8 15.7 / 16.8, and long parts, 48 of 8 bits of
         // 20000 in 11 / 8 36.1 / 38.4.
-        if (few && !prefix_pages && own >= 6) {
+        if (sparse && !prefix_pages && own >= 6) {
             const long long near = (own + 5) / 8 * 8, down = own / 8 * 8;
             if (near <= own || own_base * near <= (long long)wgs * ctx->num_cu) own = near;
             else if (down && own_room <= 1536 * down) own = down;
             own = std::min(own, 32LL);
         }
-        if (prefix_pages ? (!few && own_room <= brief) || own_base * 1024 >= own_room * ctx->num_cu
+        if (prefix_pages ? (!sparse && own_room <= brief) || own_base * 1024 >= own_room * ctx->num_cu
                          : own_room <= once || own_base * (wide ? 2 : nb) * 1024 >= own_room * ctx->num_cu)
             own = 1;
     } else if (prefix_pages ? (own_room <= (dim == 64 ? 640 : 512) && 3 * own_base >= ctx->num_cu) || (mode && own_room <= 256)

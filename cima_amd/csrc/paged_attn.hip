@@ -669,9 +669,10 @@ DEV void attn_task(const AttnArgs& A, uint8_t* lds, int kvh, int r0, int rb, int
 
 // ------------------------------------------------------------- few rows
 //
-// Tasks of up to 16 NB rows (own tasks; prefix tasks of up to 16 rows): bound by
-// reading the keys and values, and short ones by the latency of their chain of
-// loads (lengths, ids, pages).  The W waves of a workgroup take 32-position
+// Tasks of up to 16 NB rows (own tasks; prefix tasks of up to 16 rows, over quantised pages
+// of up to 64 rows of 128 or 256 of 64 elements, 32 at a time): bound by reading the
+// keys and values, and short ones by the latency of their chain of loads (lengths,
+// ids, pages).  The W waves of a workgroup take 32-position
 // tiles in turn and do not wait for each other: keys go straight from memory
 // to the registers of the A operand (16 x 16 x 32 MFMA: a lane holds 16 bytes
 // of a key), values by direct copies to the wave's own LDS.  The waves' sums are

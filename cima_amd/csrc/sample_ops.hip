@@ -331,8 +331,8 @@ DEV double lane_d(double v, int lane) {
 // Rows up to 32768 logits go to a workgroup each, in one launch; of longer ones the
 // parts leave their sums and groups' largest, and a second launch joins them (in
 // fp64) and finds the likeliest: looked for in each part they took as long as the
-// sums did.  Measured on MI355X: 384 rows of 128256 f16 with 20 alternatives 21 us (4.7
-// TB/s) and 8.4 for the join; 777 rows of 151936 without 41.5 (5.7 TB/s) and 4.6; one of
+// sums did.  Measured on MI355X: 384 rows of 128256 f16 with 20 alternatives 21.5 us (4.6
+// TB/s) and 8.4 for the join, capped 37.4 and 8.6, f32 35.9 and 8.1, both 43.6 and 8.2; 777 rows of 151936 without 41.5 (5.7 TB/s) and 4.6; one of
 // them with 5 3.3 and 6.8, a chain of three loads, a search by bits and a ranking; 384
 // rows of 2000 in one launch 6.8.  Bound by vector instructions: a logit is a fused
 // multiply-add, an exponential at half rate, a maximum, an addition and another
@@ -1049,7 +1049,9 @@ DEV void lp_join(const LpArgs& A) {
         if (t >= 64) return;
         join();
     } else {
-        constexpr int K = 4;  // loads that a thread keeps: rows up to 1048576 / VG logits
+        // loads that a thread keeps, of rows up to 32768 VG logits (f16 262144, f32 131072);
+        // those behind are read again
+        constexpr int K = 4;
         const int loads = ((A.n - 1) / P::CHUNK + 1) * P::GROUPS / VG;
         const uint4* from = (const uint4*)((const typename P::Largest*)A.largest + (size_t)row * loads * VG);
         uint4 q[K];

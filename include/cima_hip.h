@@ -451,7 +451,8 @@ typedef struct cima_kv_pages {
     int* table;             /* [max_seqs, table_stride] */
     int* lens;              /* [max_seqs] */
     int n_planes, n_pages, kv_heads, page, head_dim, max_seqs, table_stride;
-    int ggml_type;          /* 0 (f16), CIMA_GGML_Q4_1 or CIMA_GGML_Q8_0 */
+    int ggml_type;          /* 0 (f16), CIMA_GGML_Q4_1 or CIMA_GGML_Q8_0.  It lies where the struct had
+                             * padding: one filled member by member is cleared first */
 } cima_kv_pages;
 
 /* RoPE of a step's queries and keys, and the append of its keys and values:
@@ -501,7 +502,8 @@ int cima_hip_attn_paged(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, c
  * cima_hip_attn_decode.  slots NULL: slots 0, 1, ...; first NULL: from position 0.
  * A position without a page, a negative one, or any of a slot outside [0, max_seqs),
  * is zeros; lens is not looked at: a position that has a page is what the page holds.
- * n <= max_seq; k and v 16-byte aligned, not overlapping. */
+ * n <= max_seq, at most 2^30, and less than 2^24 pieces of 64 rows (head_dim 64: 128)
+ * of a head; k and v 16-byte aligned, not overlapping. */
 int cima_hip_kv_pages_read(cima_hip_ctx* ctx, const cima_kv_pages* kv, int layer, const int* slots, const int* first,
                            void* k, void* v, int n_slots, int n, int max_seq);
 
