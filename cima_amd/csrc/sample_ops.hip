@@ -332,9 +332,10 @@ DEV double lane_d(double v, int lane) {
 // parts leave their sums and groups' largest, and a second launch joins them (in
 // fp64) and finds the likeliest: looked for in each part they took as long as the
 // sums did.  Measured on MI355X: 384 rows of 128256 f16 with 20 alternatives 21.5 us (4.6
-// TB/s) and 8.4 for the join, capped 37.4 and 8.6, f32 35.9 and 8.1, both 43.6 and 8.2; 777 rows of 151936 without 41.5 (5.7 TB/s) and 4.6; one of
-// them with 5 3.3 and 6.8, a chain of three loads, a search by bits and a ranking; 384
-// rows of 2000 in one launch 6.8.  Bound by vector instructions: a logit is a fused
+// TB/s) and 8.4 for the join, capped 37.4 and 8.6, f32 35.9 and 8.1, both 43.6 and 8.2;
+// 777 rows of 151936 without 41.5 (5.7 TB/s) and 4.6; one of them with 5 3.3 and 6.8, a
+// chain of three loads, a search by bits and a ranking; 384 rows of 2000 in one launch
+// 6.8.  Bound by vector instructions: a logit is a fused
 // multiply-add, an exponential at half rate, a maximum, an addition and another
 // multiply-add, and a share of finding its group's largest.
 
@@ -617,15 +618,16 @@ struct LpBest {
     DEV int id() const { return f == -INFINITY ? -1 : at; }
 };
 // Below this no logit's sm_f is as large as that of `most`.  sm_f is off by 2^-21 of itself at
-// most (the quotient, tanhf, the product); from 0 on tanh rises by its slope at the end
-// of a stretch or more, 1 - tanh^2, and from 6.5 to 8 by 4.3e-6.
+// most (the quotient, tanhf, the product), and by cap 2^-149 where the quotient is next to
+// nothing; from 0 on tanh rises by its slope at the end of a stretch or more, 1 - tanh^2,
+// and from 6.5 to 8 by 4.3e-6.
 DEV float lp_as_large(float most, float cap) {
     if (!(most > 0.f)) return -INFINITY;
     if (__builtin_isinf(most)) return most;
     const float u = most / cap;
     if (u >= 8.f) return 6.5f * cap;
     const float th = tanhf(u);
-    return most - cap * th * 0x1p-19f / ((1.f - th) * (1.f + th));
+    return most - cap * (th * 0x1p-19f / ((1.f - th) * (1.f + th)) + 0x1p-147f);
 }
 // of logits [lo, hi) of a row of n, by the workgroup (one call in a kernel), the largest of
 // which that a thread looked at is `most`; the result in every thread
@@ -759,9 +761,9 @@ DEV LpScale lp_scale(float T) {
     return {T > 0.f ? fmaxf(1.44269504088896340736f / T, 0x1p-149f) / half : 1.f, half};
 }
 // A thread's running sums of 2^z and 2^z z, R words of V logits at a time: z = (f(x) -
-// c) s, c f of the largest so far (0: none), half of it as LpScale says; FAST, of f16 logits, z = x s - b in one
-// instruction, b = c s as fp32 holds it, which the end puts right.  It takes |c s| up
-// to 2^20, so that b is near enough: s up to LP_FAST.
+// c) s, c f of the largest so far (0: none), half of it as LpScale says; FAST, of f16
+// logits, z = x s - b in one instruction, b = c s as fp32 holds it, which the end puts
+// right.  It takes |c s| up to 2^20, so that b is near enough: s up to LP_FAST.
 constexpr float LP_FAST = 16.f;
 template <bool F32, bool CAP, int R, int V>
 struct LpSums {

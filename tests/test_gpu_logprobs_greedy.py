@@ -80,3 +80,20 @@ def test_the_token_that_is_left(hip, dtype, cap, rows, n):
                 want = np.full(top, -np.inf)
                 want[:1] = 0 if len(order) else -np.inf
                 assert np.array_equal(alt[i], want)
+
+
+@pytest.mark.parametrize("cap", [2e38, 3e37, 1.0, 1e-37])
+@pytest.mark.parametrize("size", [0.01, 1e-5, 1e-30, 1e-38, 1e-41])
+@pytest.mark.parametrize("rows,n", FORMS)
+def test_quotients_next_to_nothing(hip, cap, size, rows, n):
+    """x / cap among the numbers below 2^-126, which are far apart: logits whose capped values are
+    the same though they differ by more than roundings do elsewhere."""
+    r = np.random.default_rng(n)
+    x = (size * (1 - 1e-3 * r.random((rows, n)) ** 8)).astype(np.float32)
+    x[1::2] = np.sort(x[1::2], 1)
+    temp = np.zeros(rows, np.float32)
+    p = _probabilities(hip, x, temp, cap)
+    best = np.where(p.max(1) == 1, p.argmax(1), -1)
+    lp, _, ids, alt = _run(hip, x, temp, cap, best, 3, 4 << 20)
+    assert np.array_equal(lp, np.where(best >= 0, 0, -np.inf))
+    assert np.array_equal(ids[:, 0], best) and (alt[:, 0] == 0).all()
